@@ -23,6 +23,54 @@
  * M, N, K come from the push constants of the enclosing nf_task_desc
  * (bytes 20, 24, 28), recovered through the offsetof bridge
  * (metal_provider.mm:2301-2307).
+ *
+ * Serving ops (no counterpart in the reference): a batch of sequences over a
+ * paged key / value cache, and sampling of the next token.
+ *   paged_kv_append     K_new, V_new, TABLES, STARTS, LENS -> K_pool, V_pool
+ *   paged_kv_gather     K_pool, V_pool, TABLES, STARTS, LENS -> K, V
+ *   flash_attention_paged_chunk   Q, K_pool, V_pool, TABLES, STARTS, LENS -> O
+ *     The batch is K = n_seqs sequences.  Rows STARTS[s] .. STARTS[s+1]-1
+ *     (int32[n_seqs+1], not decreasing) of the dense operands are the last
+ *     positions of sequence s, which has LENS[s] (int32[n_seqs]) of them, those
+ *     rows included.  Position p lies in block TABLES[s][p / block_size]
+ *     (uint32[n_seqs][N]), slot p % block_size.  K_new, V_new, K, V are
+ *     [seq_len, M, head_dim], Q and O [seq_len, n_heads, head_dim], F32 or F16;
+ *     seq_len counts every row, M the KV heads (M = 0 in the attention: one per
+ *     query head).  Push constants: seq_len, n_heads (attention), head_dim (at
+ *     most 256), M, N, K, window_size = block_size (0: 16), max_seq_len = a
+ *     bound on LENS (0: N * block_size; longer sequences are cut off there).  A
+ *     tight bound lets the attention launch fewer workgroups.
+ *     Pools are [block][M][block_size][head_dim] of the rows' dtype, or I8: the
+ *     page of one KV head in a block is then block_size * head_dim int8 codes
+ *     followed by block_size * head_dim / 32 fp16 scales (head_dim % 32 == 0).
+ *     A group of 32 elements x of a row is held as scale = fp16(fp32(max|x| /
+ *     127)) and codes x / scale to nearest, ties to even; it stands for code *
+ *     scale.  Codes saturate, NaN is held as 0.
+ *     Attention: the row at position p attends to positions 0 .. p with the
+ *     scale 1 / sqrt(head_dim); query head h reads KV head h * M / n_heads.
+ *     The chunk's own keys have to be in the cache (paged_kv_append before it).
+ *     O may be Q's buffer; other overlaps of outputs with operands are not
+ *     allowed.  Tables, starts and lengths are read when the op runs, so a
+ *     captured op follows their contents at each replay.  A position below 0 or
+ *     past the bound, or in a block that the pools do not hold, has no storage:
+ *     append skips it, gather gives zeros for it, attention counts no key; a row
+ *     without any key gives zeros.  Rows of no sequence are left as they are.  A
+ *     slot that several rows of one append name ends with any of their values.
+ *   sample_token        LOGITS, U, PARAMS, TOP_K -> TOKEN, PROB
+ *     LOGITS [seq_len, N] F32 or F16; U f32[seq_len], random numbers of [0, 1);
+ *     PARAMS f32[seq_len][3] = temperature, top_p, min_p; TOP_K int32[seq_len];
+ *     TOKEN int32[seq_len]; PROB f32[seq_len].  With x a row's logits and T its
+ *     temperature, token i has the weight w = rint(2^40 exp((x_i - max x) / T)).
+ *     In the order of x descending, index ascending, the first TOP_K tokens stay
+ *     (<= 0 or >= N: all); of those the shortest prefix whose weights sum to at
+ *     least top_p of theirs (>= 1: all; at least one token); of those the ones
+ *     with w >= min_p 2^40.  With S the sum of what stays, TOKEN is the first in
+ *     index order whose running sum exceeds floor(U S), and PROB = w / S.  T <= 0
+ *     takes the first largest logit.  +inf counts as the largest finite value;
+ *     NaN and -inf are never drawn; a row of nothing else gives -1 and 0.  N is
+ *     at most 2^22.
+ * These ops may use the provider's workspace: replays of graphs that hold them
+ * must not overlap each other or later dispatches (one stream does that).
  */
 #ifndef NF_HIP_PLUGIN_H
 #define NF_HIP_PLUGIN_H

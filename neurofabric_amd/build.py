@@ -40,6 +40,9 @@ HIP_SOURCES = [
     CSRC / "kernels" / "dense.hip",
     CSRC / "kernels" / "layer.hip",
     CSRC / "kernels" / "attention.hip",
+    CSRC / "kernels" / "paged.hip",
+    CSRC / "kernels" / "paged_attention.hip",
+    CSRC / "kernels" / "sample.hip",
 ]
 CXX_SOURCES = [CSRC / "plan.cpp", CSRC / "plan_layer.cpp", CSRC / "model_ops.cpp"]
 

@@ -144,4 +144,25 @@ struct AttnArgs {
 };
 hipError_t launch_attention(EType t, const AttnArgs& a, hipStream_t s);
 
+// ---- serving: a batch of sequences over a paged cache (kernels/paged*.hip) ----
+struct PagedBatch {
+  const uint32_t* table = nullptr;  // [n_seqs, width] physical blocks
+  const int32_t* starts = nullptr;  // [n_seqs + 1] first row of each sequence
+  const int32_t* lens = nullptr;    // [n_seqs] positions of each, its rows included
+  uint32_t n_seqs = 0, width = 0, rows = 0, n_kv = 0, dim = 0, block_size = 0;
+  uint32_t limit = 0;   // positions a sequence may hold
+  uint32_t blocks = 0;  // whole blocks in the pools
+};
+hipError_t launch_paged_append(EType t, PoolType pool, const PagedBatch& b, const void* k, const void* v, void* k_pool,
+                               void* v_pool, hipStream_t s);
+hipError_t launch_paged_gather(EType t, PoolType pool, const PagedBatch& b, const void* k_pool, const void* v_pool,
+                               void* k, void* v, hipStream_t s);
+// Attention of the batch's rows; `ws` holds the partials of keys split over workgroups.
+hipError_t launch_paged_chunk(EType t, PoolType pool, const PagedBatch& b, uint32_t n_heads, const void* q,
+                              const void* k_pool, const void* v_pool, void* out, const Workspace& ws, hipStream_t s);
+
+// ---- sampling (kernels/sample.hip) ---------------------------------------------
+hipError_t launch_sample(EType t, const void* logits, const float* u, const float* params, const int32_t* top_k,
+                         int32_t* token, float* prob, uint32_t rows, uint32_t n, const Workspace& ws, hipStream_t s);
+
 }  // namespace nfhip

@@ -37,8 +37,17 @@ enum class Path {
   Argmax,
   Attention,   // every attention op (causal, cached, flash, gqa, paged)
   MoeGate,     // moe_top_k_gating
-  MoeScatter   // moe_scatter_gather
+  MoeScatter,  // moe_scatter_gather
+  // serving: a batch of sequences over a paged cache, and sampling
+  PagedAppend,  // paged_kv_append
+  PagedGather,  // paged_kv_gather
+  PagedChunk,   // flash_attention_paged_chunk
+  Sample        // sample_token
 };
+
+// Element type of a paged cache's pools.  I8: a page (one KV head of a block)
+// is block_size * head_dim int8 codes, then one fp16 scale per 32 codes.
+enum class PoolType { F32, F16, I8 };
 
 // Element-wise functions of the Binary / Unary paths.
 enum class EwFn { Add, Mul, Silu, Gelu, Relu };
@@ -63,6 +72,8 @@ struct LayerParams {
   uint32_t step = 0, max_seq = 0, window = 0;
   uint32_t n_blocks = 0, block_size = 0, q_offset = 0;  // paged attention
   uint32_t n_experts = 0, top_k = 0;                     // MoE gating / scatter-gather
+  PoolType pool = PoolType::F32;  // serving ops: rows = sequences, dim = block table width,
+                                  // max_seq = positions a sequence may hold, count2 = blocks of the pools
   uint64_t count2 = 0;  // attention_prefill: elements of the second output
   float eps = 0.f, theta = 0.f;
   bool decode = false;  // attention with step_idx > 0 (one query token)
@@ -155,6 +166,10 @@ inline uint32_t block_elems(QFmt q) {
              : 32u;
 }
 inline uint32_t elt_bytes(EType t) { return t == EType::F16 ? 2u : 4u; }
+// Bytes of a page of `elems` elements (block_size * head_dim).
+constexpr uint64_t page_bytes(PoolType t, uint64_t elems) {
+  return t == PoolType::I8 ? elems + elems / 16 : elems * (t == PoolType::F16 ? 2u : 4u);
+}
 
 // Validates and plans one dispatch.  `ins`/`outs` are descriptor pointers
 // (may be null when n == 0).  `pc` points at the task's push-constant bytes

@@ -1,9 +1,11 @@
 // plan_layer.cpp — validation and planning of the layer ops that sit around
 // the linears in a transformer block: element-wise (metal_vector_add,
 // elementwise_mul, silu, gelu, mock_relu, attention_prefill), rms_norm, rope,
-// rope_batch, softmax, embedding_lookup, argmax and the attention family
+// rope_batch, softmax, embedding_lookup, argmax, the attention family
 // (causal_attention, causal_attention_cached, flash_attention_cached,
-// flash_attention_gqa, flash_attention_paged).
+// flash_attention_gqa, flash_attention_paged), and the serving ops, which have
+// no counterpart in the reference: paged_kv_append, paged_kv_gather,
+// flash_attention_paged_chunk and sample_token.
 //
 // Semantics follow the reference's Metal host code (metal_provider.mm:2313-2990,
 // 3034-3079): the f16 variant is picked from the OUTPUT dtype, element counts
@@ -58,6 +60,10 @@ const std::unordered_map<std::string, LayerInfo>& layer_table() {
       {"flash_attention_paged", {Path::Attention, EwFn::Add, AttnMode::Paged, true, false, false}},
       {"moe_top_k_gating", {Path::MoeGate, EwFn::Add, AttnMode::Plain, true, false, false}},
       {"moe_scatter_gather", {Path::MoeScatter, EwFn::Add, AttnMode::Plain, true, false, false}},
+      {"paged_kv_append", {Path::PagedAppend, EwFn::Add, AttnMode::Paged, true, false, false}},
+      {"paged_kv_gather", {Path::PagedGather, EwFn::Add, AttnMode::Paged, true, true, false}},
+      {"flash_attention_paged_chunk", {Path::PagedChunk, EwFn::Add, AttnMode::Paged, true, true, false}},
+      {"sample_token", {Path::Sample, EwFn::Add, AttnMode::Plain, true, false, false}},
   };
   return t;
 }
@@ -179,6 +185,131 @@ nf_status plan_attention(const LayerInfo& info, const char* op_name, const nf_te
               (info.attn == AttnMode::Plain ? "plain" : info.attn == AttnMode::Cached ? "cached"
                                                         : info.attn == AttnMode::Gqa  ? "gqa" : "paged") +
               (lp.decode ? "_decode_" : "_prefill_") + tname(p->c);
+  return NF_OK;
+}
+
+bool float_type(nf_dtype d, EType* t) {
+  if (d != NF_DTYPE_F32 && d != NF_DTYPE_F16) return false;
+  *t = d == NF_DTYPE_F16 ? EType::F16 : EType::F32;
+  return true;
+}
+
+// The batch of a serving op: `rows` rows (tokens) of the op's dense operand `x`
+// and of `y` when it has a second, the pools of `act` or I8 elements, and the
+// block tables, row starts and lengths in batch[0..2].
+nf_status plan_paged_batch(const nf_tensor_desc* const* dense, uint32_t n_dense, const nf_tensor_desc* const* pools,
+                           const nf_tensor_desc* const* batch, const Pc& pc, Plan* p, std::string* why) {
+  LayerParams& lp = p->lp;
+  for (uint32_t i = 0; i < n_dense; ++i)
+    if (!dense[i]) return fail(why, "null descriptor");
+  for (int i = 0; i < 3; ++i)
+    if ((i < 2 && !pools[i]) || !batch[i]) return fail(why, "null descriptor");
+  if (!pc.present) return fail(why, "serving ops need push constants");
+  lp.seq_len = pc.seq_len;
+  lp.head_dim = pc.head_dim;
+  lp.n_kv = pc.M;
+  lp.dim = pc.N;
+  lp.rows = pc.K;
+  lp.block_size = pc.window ? pc.window : 16;
+  if (lp.head_dim == 0 || lp.head_dim > 256) return fail(why, "head_dim must be 1 to 256");
+  if (lp.n_kv == 0) return fail(why, "M (KV heads) must be non-zero");
+  if (lp.n_kv > 65535 || lp.rows > 65535 || lp.block_size > 65536)
+    return fail(why, "more than 65535 KV heads or sequences, or 65536 positions a block");
+  EType act;
+  if (!float_type(dense[0]->dtype, &act)) return fail(why, "rows must be F32 or F16");
+  for (uint32_t i = 1; i < n_dense; ++i)
+    if (dense[i]->dtype != dense[0]->dtype) return fail(why, "rows must have one dtype");
+  if (pools[0]->dtype != pools[1]->dtype) return fail(why, "the K and V pools must have one dtype");
+  if (pools[0]->dtype == NF_DTYPE_I8) {
+    lp.pool = PoolType::I8;
+    if (lp.head_dim % 32 != 0) return fail(why, "I8 pools need head_dim % 32 == 0");
+  } else if (pools[0]->dtype == dense[0]->dtype) {
+    lp.pool = act == EType::F16 ? PoolType::F16 : PoolType::F32;
+  } else {
+    return fail(why, "pools must have the rows' dtype or I8");
+  }
+  p->a = p->b = p->c = act;
+  const uint64_t S = lp.rows;
+  if (!fits(batch[0], S * lp.dim, 4)) return fail(why, "block tables hold fewer than K * N entries");
+  if (!fits(batch[1], S + 1, 4)) return fail(why, "row starts hold fewer than K + 1 entries");
+  if (!fits(batch[2], S, 4)) return fail(why, "lengths hold fewer than K entries");
+  // Positions a sequence may hold: the tables' capacity, or max_seq_len when
+  // it is given and smaller; lengths are int32.
+  uint64_t limit = std::min<uint64_t>((uint64_t)lp.dim * lp.block_size, 0x7FFFFFFFu);
+  if (pc.max_seq) limit = std::min<uint64_t>(limit, pc.max_seq);
+  lp.max_seq = (uint32_t)limit;
+  const uint64_t block = page_bytes(lp.pool, (uint64_t)lp.block_size * lp.head_dim) * lp.n_kv;
+  lp.count2 = std::min<uint64_t>(std::min(pools[0]->size_bytes, pools[1]->size_bytes) / block, 0xFFFFFFFFu);
+  return NF_OK;
+}
+
+const char* pname(PoolType t) { return t == PoolType::I8 ? "i8" : t == PoolType::F16 ? "f16" : "f32"; }
+
+// paged_kv_append / paged_kv_gather: dense rows [seq_len, n_kv, head_dim] of K
+// and V on one side, the pools on the other.
+nf_status plan_paged_rows(bool append, const nf_tensor_desc* const* ins, uint32_t n_in,
+                          const nf_tensor_desc* const* outs, uint32_t n_out, const Pc& pc, Plan* p, std::string* why) {
+  if (n_in < 5 || n_out < 2) return fail(why, "takes 5 inputs and 2 outputs");
+  nf_status st = plan_paged_batch(append ? ins : outs, 2, append ? outs : ins, ins + 2, pc, p, why);
+  if (st != NF_OK) return st;
+  const uint64_t n = (uint64_t)p->lp.seq_len * p->lp.n_kv * p->lp.head_dim, elt = elt_bytes(p->a);
+  if (n >= kMaxElems) return fail(why, "too many rows");
+  const nf_tensor_desc* const* dense = append ? ins : outs;
+  if (!fits(dense[0], n, elt) || !fits(dense[1], n, elt))
+    return fail(why, "K and V rows hold fewer than seq_len * M * head_dim elements");
+  p->count = n;
+  const uint64_t cells = 2 * page_bytes(p->lp.pool, n);
+  p->act_bytes = append ? 2 * n * elt : cells;
+  p->out_bytes = append ? cells : 2 * n * elt;
+  p->kernel = std::string(append ? "paged_append_" : "paged_gather_") + tname(p->a) + "_" + pname(p->lp.pool);
+  return NF_OK;
+}
+
+nf_status plan_paged_chunk(const nf_tensor_desc* const* ins, uint32_t n_in, const nf_tensor_desc* const* outs,
+                           uint32_t n_out, const Pc& pc, Plan* p, std::string* why) {
+  if (n_in < 6 || n_out < 1) return fail(why, "takes 6 inputs and 1 output");
+  const nf_tensor_desc* dense[2] = {ins[0], outs[0]};
+  Pc c = pc;
+  c.M = pc.M ? pc.M : pc.n_heads;
+  nf_status st = plan_paged_batch(dense, 2, ins + 1, ins + 3, c, p, why);
+  if (st != NF_OK) return st;
+  LayerParams& lp = p->lp;
+  lp.n_heads = pc.n_heads;
+  if (lp.n_heads < lp.n_kv) return fail(why, "n_heads must be at least M (KV heads)");
+  if (lp.n_heads > 65535) return fail(why, "more than 65535 heads");
+  const uint64_t n = (uint64_t)lp.seq_len * lp.n_heads * lp.head_dim, elt = elt_bytes(p->a);
+  if (n >= kMaxElems) return fail(why, "attention problem too large");
+  if (!fits(ins[0], n, elt)) return fail(why, "Q holds fewer than seq_len * n_heads * head_dim elements");
+  if (!fits(outs[0], n, elt)) return fail(why, "output holds fewer than seq_len * n_heads * head_dim elements");
+  p->count = (uint64_t)lp.seq_len * lp.n_heads;
+  p->act_bytes = n * elt;
+  p->out_bytes = n * elt;
+  p->kernel = std::string("attention_paged_chunk_") + tname(p->a) + "_" + pname(lp.pool);
+  return NF_OK;
+}
+
+nf_status plan_sample(const nf_tensor_desc* const* ins, uint32_t n_in, const nf_tensor_desc* const* outs,
+                      uint32_t n_out, const Pc& pc, Plan* p, std::string* why) {
+  if (n_in < 4 || n_out < 2) return fail(why, "takes 4 inputs and 2 outputs");
+  for (int i = 0; i < 4; ++i)
+    if (!ins[i] || (i < 2 && !outs[i])) return fail(why, "null descriptor");
+  if (!pc.present) return fail(why, "sample_token needs push constants");
+  LayerParams& lp = p->lp;
+  lp.rows = pc.seq_len;
+  lp.dim = pc.N;
+  if (!float_type(ins[0]->dtype, &p->a)) return fail(why, "logits must be F32 or F16");
+  if (lp.dim == 0 || lp.dim > (1u << 22)) return fail(why, "N (logits a row) must be 1 to 2^22");
+  if (lp.rows > 65535) return fail(why, "more than 65535 rows");
+  const uint64_t n = (uint64_t)lp.rows * lp.dim;
+  if (!fits(ins[0], n, elt_bytes(p->a))) return fail(why, "logits hold fewer than seq_len * N elements");
+  if (!fits(ins[1], lp.rows, 4)) return fail(why, "random numbers hold fewer than seq_len floats");
+  if (!fits(ins[2], 3ull * lp.rows, 4)) return fail(why, "parameters hold fewer than seq_len * 3 floats");
+  if (!fits(ins[3], lp.rows, 4)) return fail(why, "top_k holds fewer than seq_len int32");
+  if (!fits(outs[0], lp.rows, 4) || !fits(outs[1], lp.rows, 4)) return fail(why, "outputs hold fewer than seq_len entries");
+  p->count = lp.rows;
+  p->act_bytes = n * elt_bytes(p->a) + 20ull * lp.rows;
+  p->out_bytes = 8ull * lp.rows;
+  p->kernel = std::string("sample_token_") + tname(p->a);
   return NF_OK;
 }
 
@@ -373,6 +504,22 @@ nf_status make_layer_plan(const char* op_name, const nf_tensor_desc* const* ins,
     }
     case Path::Attention: {
       nf_status st = plan_attention(info, op_name, ins, n_in, outs, n_out, pc, &p, why);
+      if (st != NF_OK) return st;
+      break;
+    }
+    case Path::PagedAppend:
+    case Path::PagedGather: {
+      nf_status st = plan_paged_rows(info.path == Path::PagedAppend, ins, n_in, outs, n_out, pc, &p, why);
+      if (st != NF_OK) return st;
+      break;
+    }
+    case Path::PagedChunk: {
+      nf_status st = plan_paged_chunk(ins, n_in, outs, n_out, pc, &p, why);
+      if (st != NF_OK) return st;
+      break;
+    }
+    case Path::Sample: {
+      nf_status st = plan_sample(ins, n_in, outs, n_out, pc, &p, why);
       if (st != NF_OK) return st;
       break;
     }

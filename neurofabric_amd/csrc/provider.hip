@@ -564,6 +564,23 @@ const nf_task_desc* enclosing_task(const nf_buffer* inputs) {
   return reinterpret_cast<const nf_task_desc*>(base);
 }
 
+// The batch of a serving op from its block tables, row starts and lengths.
+PagedBatch paged_batch(const Plan& pl, Buffer* const* batch) {
+  PagedBatch b;
+  b.table = static_cast<const uint32_t*>(batch[0]->dev);
+  b.starts = static_cast<const int32_t*>(batch[1]->dev);
+  b.lens = static_cast<const int32_t*>(batch[2]->dev);
+  b.n_seqs = pl.lp.rows;
+  b.width = pl.lp.dim;
+  b.rows = pl.lp.seq_len;
+  b.n_kv = pl.lp.n_kv;
+  b.dim = pl.lp.head_dim;
+  b.block_size = pl.lp.block_size;
+  b.limit = pl.lp.max_seq;
+  b.blocks = (uint32_t)pl.lp.count2;
+  return b;
+}
+
 hipError_t run_plan(const Plan& pl, Buffer* const* in, Buffer* const* out, int gemm_tile, const Workspace& ws,
                     hipStream_t s) {
   switch (pl.path) {
@@ -619,6 +636,20 @@ hipError_t run_plan(const Plan& pl, Buffer* const* in, Buffer* const* out, int g
                                 pl.lp.top_k, pl.lp.dim, s);
     case Path::Argmax:
       return launch_argmax(in[0]->dev, out[0]->dev, pl.lp.rows, pl.lp.dim, ws.part, ws.part_floats, s);
+    case Path::PagedAppend:
+      return launch_paged_append(pl.a, pl.lp.pool, paged_batch(pl, in + 2), in[0]->dev, in[1]->dev, out[0]->dev,
+                                 out[1]->dev, s);
+    case Path::PagedGather:
+      return launch_paged_gather(pl.a, pl.lp.pool, paged_batch(pl, in + 2), in[0]->dev, in[1]->dev, out[0]->dev,
+                                 out[1]->dev, s);
+    case Path::PagedChunk:
+      return launch_paged_chunk(pl.a, pl.lp.pool, paged_batch(pl, in + 3), pl.lp.n_heads, in[0]->dev, in[1]->dev,
+                                in[2]->dev, out[0]->dev, ws, s);
+    case Path::Sample:
+      return launch_sample(pl.a, in[0]->dev, static_cast<const float*>(in[1]->dev),
+                           static_cast<const float*>(in[2]->dev), static_cast<const int32_t*>(in[3]->dev),
+                           static_cast<int32_t*>(out[0]->dev), static_cast<float*>(out[1]->dev), pl.lp.rows, pl.lp.dim,
+                           ws, s);
     case Path::Attention: {
       AttnArgs a;
       a.q = in[0]->dev;
