@@ -6,7 +6,8 @@
 // block_size; a block holds one page per KV head.  Starts, lengths and tables
 // are device data that the host never sees, so every index made from them is
 // checked here: a row before starts[0] or behind the last start belongs to no
-// sequence, and a position below 0, at or past `limit`, or in a block past the
+// sequence, nor does one of a sequence whose rows are not all rows of the batch,
+// and a position below 0, at or past `limit`, or in a block past the
 // pools has no storage.
 #pragma once
 
@@ -27,9 +28,11 @@ __device__ __forceinline__ bool find_row(const PagedBatch& b, uint32_t row, uint
     if ((int64_t)b.starts[mid + 1] <= (int64_t)row) lo = mid + 1;
     else hi = mid;
   }
-  if (lo >= b.n_seqs || (int64_t)b.starts[lo] > (int64_t)row) return false;
+  if (lo >= b.n_seqs) return false;
+  const int64_t a = b.starts[lo], e = b.starts[lo + 1];
+  if (a < 0 || a > (int64_t)row || e > (int64_t)b.rows) return false;
   seq = lo;
-  pos = (int64_t)b.lens[lo] - ((int64_t)b.starts[lo + 1] - (int64_t)row);
+  pos = (int64_t)b.lens[lo] - (e - (int64_t)row);
   return true;
 }
 

@@ -108,9 +108,818 @@ __global__ __launch_bounds__(256) void chunk_any_kernel(PagedBatch b, uint32_t n
   }
 }
 
+// ---- shared by the MFMA kernels --------------------------------------------------
+
+// Row tiles of the batch.  A sequence of n rows (tokens) has n G query rows per
+// KV head (G query heads read it), row r being token r / G, head kvh G + r % G:
+// all of them share the KV head's keys.  Sequences with `lo` < n G <= `hi` query
+// rows are cut into tiles of `per`; tile `idx` of KV head and batch is found by a
+// scan over the sequences, 64 at a time.
+struct RowTile {
+  uint32_t seq, first, rows;  // sequence, first query row, query rows of the sequence
+  uint32_t start;             // the sequence's first token
+  int64_t pos0;               // position of that token
+  int64_t len;                // positions of the sequence, at most `limit`
+};
+
+__device__ __forceinline__ bool find_tile(const PagedBatch& b, uint32_t idx, uint32_t G, uint32_t per, uint64_t lo,
+                                          uint64_t hi, RowTile& t) {
+  const int lane = threadIdx.x & 63;
+  for (uint32_t s0 = 0; s0 < b.n_seqs; s0 += 64) {
+    const uint32_t s = s0 + lane;
+    uint32_t n = 0, start = 0;
+    int32_t len = 0;
+    if (s < b.n_seqs) {
+      const int64_t a = b.starts[s], e = b.starts[s + 1];
+      len = b.lens[s];
+      if (a >= 0 && e > a && e <= (int64_t)b.rows) {
+        n = (uint32_t)(e - a);
+        start = (uint32_t)a;
+      }
+    }
+    const uint64_t rows = (uint64_t)n * G;
+    const uint32_t tiles = rows > lo && rows <= hi ? (uint32_t)((rows + per - 1) / per) : 0;
+    uint32_t up = tiles;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t v = __shfl_up(up, o);
+      if (lane >= o) up += v;
+    }
+    const uint32_t total = __shfl(up, 63);
+    if (idx < total) {
+      const int at = __builtin_ctzll(__ballot(up > idx));
+      t.seq = s0 + at;
+      t.first = (idx - __shfl(up - tiles, at)) * per;
+      t.rows = __shfl((uint32_t)rows, at);
+      t.start = __shfl(start, at);
+      const int64_t l = __shfl(len, at);
+      t.pos0 = l - (int64_t)(t.rows / G);
+      t.len = l < (int64_t)b.limit ? l : (int64_t)b.limit;
+      return true;
+    }
+    idx -= total;
+  }
+  return false;
+}
+
+// What every kernel of an attention launch is given.
+struct Chunk {
+  PagedBatch b;
+  const void* q;
+  const uint8_t* k;
+  const uint8_t* v;
+  void* out;
+  float* ml;   // partials: (maximum, sum) of split sp of query row (token, head) at 2 ((token H + head) splits + sp)
+  float* acc;  // and its unscaled output row
+  uint32_t n_heads, group, splits, keys_per_split;
+  uint32_t tiles;  // grid size: row tiles per KV head
+  uint64_t lo, hi; // query rows of the sequences that this launch takes
+  float scale_log2;  // scale * log2(e): softmax in base 2
+};
+
+// Splits that a sequence of `len` positions takes.
+__device__ __forceinline__ uint32_t splits_of(const Chunk& c, int64_t len) {
+  return len <= 0 ? 1u : (uint32_t)((len + c.keys_per_split - 1) / c.keys_per_split);
+}
+
+// Byte offset of the row of position `pos` in a pool (kNoRow without one), and
+// for I8 the distance from it to the row's scales.
+constexpr uint64_t kNoRow = ~0ull;
+template <PoolType PT, int DD>
+__device__ __forceinline__ uint64_t row_offset(const PagedBatch& b, uint32_t seq, uint32_t kvh, int64_t pos, int64_t end,
+                                               uint32_t& to_scales) {
+  to_scales = 0;
+  if (pos >= end) return kNoRow;
+  const uint32_t blk = (uint32_t)pos / b.block_size, slot = (uint32_t)pos - blk * b.block_size;
+  const uint32_t phys = b.table[(uint64_t)seq * b.width + blk];
+  if (phys >= b.blocks) return kNoRow;
+  if constexpr (PT == PoolType::I8) to_scales = (b.block_size - slot) * DD + slot * (DD / 16);
+  constexpr uint32_t row_bytes = PT == PoolType::I8 ? DD : PT == PoolType::F16 ? 2 * DD : 4 * DD;
+  return ((uint64_t)phys * b.n_kv + kvh) * nfhip::page_bytes(PT, (uint64_t)b.block_size * DD) + (uint64_t)slot * row_bytes;
+}
+
+__device__ __forceinline__ uint64_t shfl64(uint64_t v, int src) {
+  return (uint64_t)(uint32_t)__shfl((int)(uint32_t)v, src) | (uint64_t)(uint32_t)__shfl((int)(uint32_t)(v >> 32), src) << 32;
+}
+
+// Eight codes as f16: 0x64cc is 1024 + cc, so (code + 128) goes into the low byte
+// and 1152 off again (exact); times the scale, rounded once to f16.
+__device__ __forceinline__ half8 dequant8(uint2 w, half_t d) {
+  const half2v off = {(half_t)1152.0f, (half_t)1152.0f}, dd = {d, d};
+  half8 r;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t x = (i ? w.y : w.x) ^ 0x80808080u;
+    const half2v lo = (__builtin_bit_cast(half2v, __builtin_amdgcn_perm(x, 0x64646464u, 0x00050004u)) - off) * dd;
+    const half2v hi = (__builtin_bit_cast(half2v, __builtin_amdgcn_perm(x, 0x64646464u, 0x00070006u)) - off) * dd;
+    r[4 * i] = lo[0];
+    r[4 * i + 1] = lo[1];
+    r[4 * i + 2] = hi[0];
+    r[4 * i + 3] = hi[1];
+  }
+  return r;
+}
+__device__ __forceinline__ bool any_not_finite(half8 x) {
+  const u32x4 u = __builtin_bit_cast(u32x4, x);
+  uint32_t bad = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bad |= (uint32_t)((u[i] & 0x7C00u) == 0x7C00u) | (uint32_t)((u[i] & 0x7C000000u) == 0x7C000000u);
+  return bad != 0;
+}
+
+// Sum / max over the 4 lanes of a column (lanes n, n + 16, n + 32, n + 48) or the
+// 2 of one (n, n + 32) with the swaps of lane rows; s_nop covers the wait states
+// between a VALU write and a permlane read.
+template <bool ROW32>
+__device__ __forceinline__ float2s lane_swap(float v) {
+  float a = v, b = v;
+  if constexpr (ROW32) asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+  else asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+  return float2s{a, b};
+}
+__device__ __forceinline__ float max2(float v) {
+  const float2s r = lane_swap<true>(v);
+  return fmaxf(r[0], r[1]);
+}
+__device__ __forceinline__ float sum2(float v) {
+  const float2s r = lane_swap<true>(v);
+  return r[0] + r[1];
+}
+__device__ __forceinline__ float max4(float v) {
+  const float2s r = lane_swap<false>(v);
+  return max2(fmaxf(r[0], r[1]));
+}
+__device__ __forceinline__ float sum4(float v) {
+  const float2s r = lane_swap<false>(v);
+  return sum2(r[0] + r[1]);
+}
+
+// The f16 weights carry 2^kWeightLog2, which keeps the small ones out of the
+// subnormal range (it is divided out with the sum); the reference maximum may lag
+// the running one by 2^kLagLog2 before the sums are rescaled, so weights stay
+// below 2^15.
+constexpr float kWeightLog2 = 7.f, kLagLog2 = 8.f;
+
+typedef short short4v __attribute__((ext_vector_type(4)));
+// ds_read_b64_tr_b16: among each 16 lanes, lane i receives element i % 4 of the 8
+// bytes that lane 4e + i / 4 addresses, as its element e.
+__device__ __forceinline__ uint2 read_tr(const half_t* p) {
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)p));
+}
+
+// ---- few query rows: keys split over the waves, f16 ----------------------------------
+//
+// Single tokens and short chunks, where the cache is read once and the time is
+// that of reading it.  A workgroup takes up to 16 NT query rows of one KV head
+// and one split of the keys; its four waves take 32-key tiles in turn, each on
+// its own, and merge at the end.  Per tile:
+//  * S^T[key][row] = K . Q^T on v_mfma_f32_16x16x32_f16: a lane loads the 8 dims
+//    of its key that are its A operand straight from the cache (16 bytes; I8: 16
+//    codes are the operands of two steps, the order of the dims being free);
+//  * base-2 online softmax per row;
+//  * O^T[dim][row] += V^T . P^T: the weights are the B operand as S^T leaves them,
+//    rounded to f16 (2^-11 of each, the size of the output's own rounding); V
+//    goes through the wave's own part of LDS (no workgroup barrier), from where
+//    transposing reads fetch the A operand.
+// An 8-bit cache becomes f16 in registers, code * scale rounded once, as a gather
+// into f16 rows would.
+// A weight of 0 times a value that is not finite is NaN inside the MFMA, so values
+// that no row sees are stored as zeros, and a tile that has a value that is not
+// finite and a row that does not see some key of it takes the vector ALU, which
+// skips the pairs that are masked.
+template <PoolType PT, int DD, int NT>
+__global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
+  constexpr bool I8 = PT == PoolType::I8;
+  constexpr int KSTEP = DD / 32, DB = DD / 16;
+  constexpr int VP = DD + 8;                         // LDS row (halves)
+  constexpr int VC = I8 ? 16 : 8;                    // elements per 16-byte chunk
+  constexpr int CPR = DD / VC, NV = 32 * CPR / 64;   // chunks per row, per lane and tile
+  constexpr int NP = KSTEP / 2;                      // I8: 16-code loads per key row
+  __shared__ __attribute__((aligned(16))) half_t vs[4][32 * VP];
+  __shared__ __attribute__((aligned(16))) float ps[4][32][16];
+  __shared__ float wm[4][16 * NT], wl[4][16 * NT];
+  static_assert(sizeof(float) * 16 * DD <= sizeof(half_t) * 32 * VP, "a wave's rows merge in its part of vs");
+
+  const uint32_t sp = blockIdx.x % c.splits, kvh = blockIdx.y;
+  RowTile t;
+  if (!find_tile(c.b, blockIdx.x / c.splits, c.group, 16 * NT, c.lo, c.hi, t)) return;
+  const uint32_t ns = splits_of(c, t.len);
+  if (sp >= ns) return;
+  const uint32_t G = c.group, H = c.n_heads;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t live = t.rows - t.first < 16u * NT ? t.rows - t.first : 16u * NT;
+  // positions of the tile's rows, first to last
+  const int64_t pos_lo = t.pos0 + t.first / G, pos_hi = t.pos0 + (t.first + live - 1) / G;
+  int64_t end = pos_hi + 1 < t.len ? pos_hi + 1 : t.len;  // keys below it
+  const int64_t begin = (int64_t)sp * c.keys_per_split;
+  if (end > begin + c.keys_per_split) end = begin + c.keys_per_split;
+
+  half8 qb[NT][KSTEP];
+  int64_t pos[NT];
+#pragma unroll
+  for (int u = 0; u < NT; ++u) {
+    const uint32_t r = t.first + 16 * u + n < t.rows ? t.first + 16 * u + n : t.rows - 1;
+    pos[u] = t.pos0 + r / G;
+    const half_t* qr = static_cast<const half_t*>(c.q) + ((uint64_t)(t.start + r / G) * H + kvh * G + r % G) * DD;
+#pragma unroll
+    for (int s = 0; s < KSTEP; ++s) {
+      const int d = !I8 || s >= 2 * NP ? 32 * s + 8 * g : 64 * (s / 2) + 16 * g + 8 * (s % 2);
+      qb[u][s] = *reinterpret_cast<const half8*>(qr + d);
+    }
+  }
+  float4v ot[NT][DB];
+  float m[NT], l[NT];
+#pragma unroll
+  for (int u = 0; u < NT; ++u) {
+    m[u] = -INFINITY;
+    l[u] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) ot[u][d] = float4v{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // loads of a tile: lane j < 32 finds the row of key t0 + j, the others ask it
+  u32x4 kraw[2][I8 ? (NP > 0 ? NP : 1) : KSTEP];
+  uint2 kodd[2];       // I8, odd KSTEP: the last 32 dims
+  half_t kd[2][KSTEP]; // I8: scales
+  u32x4 vraw[NV];
+  half_t vd[NV];
+  uint32_t have = 0;   // keys of the tile that have a row
+  uint64_t off = kNoRow;
+  uint32_t to_s = 0;
+  auto find = [&](int64_t t0) { off = row_offset<PT, DD>(c.b, t.seq, kvh, t0 + (lane & 31), end, to_s); };
+  auto fetch = [&]() {
+    have = (uint32_t)__ballot(off != kNoRow);
+    const uint64_t o = off != kNoRow ? off : 0;  // row 0 of the pool stands in
+    const uint32_t ts = off != kNoRow ? to_s : 0;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint64_t ko = shfl64(o, 16 * j + n);
+      const uint8_t* kr = c.k + ko;
+      if constexpr (I8) {
+        const half_t* sc = reinterpret_cast<const half_t*>(kr + __shfl((int)ts, 16 * j + n));
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          kraw[j][p] = *reinterpret_cast<const u32x4*>(kr + 64 * p + 16 * g);
+          kd[j][2 * p] = sc[2 * p + (g >> 1)];
+        }
+        if constexpr (KSTEP % 2) {
+          kodd[j] = *reinterpret_cast<const uint2*>(kr + 64 * NP + 8 * g);
+          kd[j][KSTEP - 1] = sc[KSTEP - 1];
+        }
+      } else {
+#pragma unroll
+        for (int s = 0; s < KSTEP; ++s) kraw[j][s] = *reinterpret_cast<const u32x4*>(kr + 64 * s + 16 * g);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      const int ch = lane + 64 * u, r = ch / CPR, col = ch % CPR;
+      const uint64_t vo = shfl64(o, r);
+      vraw[u] = *reinterpret_cast<const u32x4*>(c.v + vo + 16 * col);
+      if constexpr (I8)
+        vd[u] = reinterpret_cast<const half_t*>(c.v + vo + __shfl((int)ts, r))[col / 2];
+    }
+  };
+
+  half_t* const vw = vs[w];
+  const half_t* const vtr = vw + (4 * g + n / 4) * VP + 4 * (n % 4);
+  int64_t t0 = begin + 32 * w;
+  if (t0 < end) {
+    find(t0);
+    fetch();
+    if (t0 + 128 < end) find(t0 + 128);
+  }
+  for (; t0 < end; t0 += 128) {
+    // scores
+    float4v sc[NT][2];
+    {
+      half8 ka[2][KSTEP];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if constexpr (I8) {
+#pragma unroll
+          for (int p = 0; p < NP; ++p) {
+            ka[j][2 * p] = dequant8(uint2{kraw[j][p][0], kraw[j][p][1]}, kd[j][2 * p]);
+            ka[j][2 * p + 1] = dequant8(uint2{kraw[j][p][2], kraw[j][p][3]}, kd[j][2 * p]);
+          }
+          if constexpr (KSTEP % 2) ka[j][KSTEP - 1] = dequant8(kodd[j], kd[j][KSTEP - 1]);
+        } else {
+#pragma unroll
+          for (int s = 0; s < KSTEP; ++s) ka[j][s] = __builtin_bit_cast(half8, kraw[j][s]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < NT; ++u)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          sc[u][j] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int s = 0; s < KSTEP; ++s)
+            sc[u][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[j][s], qb[u][s], sc[u][j], 0, 0, 0);
+        }
+    }
+    // values into the wave's part of LDS, rows without storage as zeros
+    const uint32_t seen = have;
+    const bool open = seen == ~0u && t0 + 31 <= pos_lo;  // every row sees every key (uniform)
+    bool bad = false;
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      const int ch = lane + 64 * u, r = ch / CPR, col = ch % CPR;
+      half8 x[I8 ? 2 : 1];
+      if constexpr (I8) {
+        x[0] = dequant8(uint2{vraw[u][0], vraw[u][1]}, vd[u]);
+        x[1] = dequant8(uint2{vraw[u][2], vraw[u][3]}, vd[u]);
+      } else {
+        x[0] = __builtin_bit_cast(half8, vraw[u]);
+      }
+#pragma unroll
+      for (int e = 0; e < VC / 8; ++e) {
+        if (!open) {
+          if (!((seen >> r) & 1)) x[e] = half8{};
+          bad = bad || any_not_finite(x[e]);
+        }
+        *reinterpret_cast<half8*>(vw + r * VP + VC * col + 8 * e) = x[e];
+      }
+    }
+    const bool alu = !open && __ballot(bad) != 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's LDS accesses stay in order
+    __builtin_amdgcn_wave_barrier();
+    if (t0 + 128 < end) {
+      fetch();
+      if (t0 + 256 < end) find(t0 + 256);
+    }
+    half8 pb[NT];
+    float pv[NT][2][4];
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int k = 16 * j + 4 * g + i;
+          if (!open && (!((seen >> k) & 1) || t0 + k > pos[u])) sc[u][j][i] = -INFINITY;
+          top = fmaxf(top, sc[u][j][i]);
+        }
+      top = max4(top) * c.scale_log2;
+      if (__ballot(top > m[u] + kLagLog2) != 0) {  // uniform
+        const float mn = fmaxf(m[u], top);
+        const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[u] - mn);
+        l[u] *= corr;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) ot[u][d] *= corr;
+        m[u] = mn;
+      }
+      const float mb = m[u] - kWeightLog2;
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float s = sc[u][j][i];
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s, c.scale_log2, -mb));
+          pv[u][j][i] = !open && s == -INFINITY ? 0.f : e;
+          sum += pv[u][j][i];
+          pb[u][4 * j + i] = (half_t)pv[u][j][i];
+        }
+      l[u] += sum4(sum);
+    }
+    if (!alu) {
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const uint2 lo = read_tr(vtr + 16 * d), hi = read_tr(vtr + 16 * VP + 16 * d);
+        const half8 av = __builtin_bit_cast(half8, u32x4{lo.x, lo.y, hi.x, hi.y});
+#pragma unroll
+        for (int u = 0; u < NT; ++u) ot[u][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, pb[u], ot[u][d], 0, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) ps[w][16 * j + 4 * g + i][n] = pv[u][j][i];
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (int k = 0; k < 32; ++k) {
+          if (!((seen >> k) & 1) || t0 + k > pos[u]) continue;
+          const float p = ps[w][k][n];
+#pragma unroll
+          for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ot[u][d][i] += p * (float)vw[k * VP + 16 * d + 4 * g + i];
+        }
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the next tile's values come after these reads
+    __builtin_amdgcn_wave_barrier();
+  }
+
+  // merge the waves, 16 rows at a time; write the output (a lone split) or the partial
+#pragma unroll
+  for (int u = 0; u < NT; ++u)
+    if (g == 0) {
+      wm[w][16 * u + n] = m[u];
+      wl[w][16 * u + n] = l[u];
+    }
+#pragma unroll
+  for (int u = 0; u < NT; ++u) {
+    if (u > 0) __syncthreads();
+    float* mine = reinterpret_cast<float*>(vw);
+#pragma unroll
+    for (int d = 0; d < DB; ++d) *reinterpret_cast<float4v*>(mine + n * DD + 16 * d + 4 * g) = ot[u][d];
+    __syncthreads();
+    for (int idx = tid; idx < 16 * DD / 4; idx += 256) {
+      const int r = idx / (DD / 4), d = idx % (DD / 4) * 4;
+      const uint32_t row = t.first + 16 * u + r;
+      if (row >= t.rows) break;
+      float M = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int v = 0; v < 4; ++v) M = fmaxf(M, wm[v][16 * u + r]);
+      float4v A = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const float mv = wm[v][16 * u + r];
+        const float f = mv == M ? 1.f : __builtin_amdgcn_exp2f(mv - M);
+        L += f * wl[v][16 * u + r];
+        A += f * *reinterpret_cast<const float4v*>(reinterpret_cast<const float*>(vs[v]) + r * DD + d);
+      }
+      const uint64_t o = (uint64_t)(t.start + row / G) * H + kvh * G + row % G;
+      if (ns == 1) {
+        const float inv = L == 0.f ? 0.f : 1.0f / L;
+        half2v a = {(half_t)(A[0] * inv), (half_t)(A[1] * inv)}, bb = {(half_t)(A[2] * inv), (half_t)(A[3] * inv)};
+        *reinterpret_cast<uint2*>(static_cast<half_t*>(c.out) + o * DD + d) =
+            uint2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, bb)};
+      } else {
+        const uint64_t p = o * c.splits + sp;
+        if (d == 0) *reinterpret_cast<float2s*>(c.ml + 2 * p) = float2s{M, L};
+        *reinterpret_cast<float4v*>(c.acc + p * DD + d) = A;
+      }
+    }
+  }
+}
+
+// The splits of every query row whose sequence has more than one: a wave per row.
+template <typename T, int DD>
+__global__ __launch_bounds__(256) void chunk_combine_kernel(Chunk c) {
+  const uint64_t o = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (o >= (uint64_t)c.b.rows * c.n_heads) return;
+  uint32_t seq;
+  int64_t pos;
+  if (!find_row(c.b, (uint32_t)(o / c.n_heads), seq, pos)) return;
+  const int64_t l = c.b.lens[seq];
+  const uint32_t ns = splits_of(c, l < (int64_t)c.b.limit ? l : (int64_t)c.b.limit);
+  if (ns == 1) return;
+  float M = -INFINITY;
+  for (uint32_t s = lane; s < ns; s += 64) M = fmaxf(M, c.ml[2 * (o * c.splits + s)]);
+#pragma unroll
+  for (int k = 32; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor(M, k));
+  float L = 0.f, A[(DD + 63) / 64] = {};
+  for (uint32_t s = 0; s < ns; ++s) {
+    const float2s ml = *reinterpret_cast<const float2s*>(c.ml + 2 * (o * c.splits + s));
+    if (ml[1] == 0.f) continue;  // no key
+    const float f = ml[0] == M ? 1.f : __builtin_amdgcn_exp2f(ml[0] - M);
+    L += f * ml[1];
+    const float* a = c.acc + (o * c.splits + s) * DD;
+#pragma unroll
+    for (int r = 0; r < (DD + 63) / 64; ++r)
+      if (lane + 64 * r < DD) A[r] += f * a[lane + 64 * r];
+  }
+  const float inv = L == 0.f ? 0.f : 1.0f / L;
+#pragma unroll
+  for (int r = 0; r < (DD + 63) / 64; ++r)
+    if (lane + 64 * r < DD) static_cast<T*>(c.out)[o * DD + lane + 64 * r] = (T)(A[r] * inv);
+}
+
+// ---- many query rows, f16 --------------------------------------------------------------
+//
+// A workgroup takes 128 query rows of one KV head, 32 per wave (and one split of
+// the keys); 64-key tiles of K and V are staged row-major in LDS for all of them
+// (an 8-bit cache becomes f16 there), the next tile's loads in flight meanwhile.
+// The matrices are transposed as in the narrow kernel, on
+// v_mfma_f32_32x32x16_f16: S^T[key][row] = K . Q^T with the queries held in
+// registers; a lane then has half of its row's scores, and the weights, rounded to
+// f16, are the B operand of O^T[dim][row] += V^T . P^T as they are.
+// Masking, the lazy rescale and values that are not finite: as above; tiles that
+// every row of the workgroup sees whole skip all of it.
+template <PoolType PT, int DD>
+__global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
+  constexpr bool I8 = PT == PoolType::I8;
+  constexpr int KS = DD / 16, DB = DD / 32, KP = DD + 8;
+  constexpr int VC = I8 ? 16 : 8;
+  constexpr int CPR = DD / VC, NL = 64 * CPR / 256;
+  static_assert(64 * CPR % 256 == 0 || I8, "chunks");
+  constexpr int NU = (64 * CPR + 255) / 256;
+  __shared__ __attribute__((aligned(16))) half_t ks[64 * KP];
+  __shared__ __attribute__((aligned(16))) half_t vs[64 * KP];
+  __shared__ __attribute__((aligned(16))) float ps[4][32][32];
+  __shared__ int tile_bad[2];
+  (void)NL;
+
+  // Workgroup L runs on XCD L % 8, which has its own L2: each XCD gets the tiles of
+  // whole KV heads, late tiles (most keys) first.
+  const uint32_t X = gridDim.x, i0 = (blockIdx.x % 8) * (X / 8) + blockIdx.x / 8;
+  if (i0 >= c.tiles * c.b.n_kv) return;
+  const uint32_t kvh = i0 / c.tiles, sp = blockIdx.y;
+  RowTile t;
+  if (!find_tile(c.b, c.tiles - 1 - i0 % c.tiles, c.group, 128, c.lo, c.hi, t)) return;
+  const uint32_t ns = splits_of(c, t.len);
+  if (sp >= ns) return;
+  const uint32_t G = c.group, H = c.n_heads;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, hf = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t last = (t.first + 128 < t.rows ? t.first + 128 : t.rows) - 1;
+  const int64_t pos_lo = t.pos0 + t.first / G, pos_hi = t.pos0 + last / G;
+  int64_t end = pos_hi + 1 < t.len ? pos_hi + 1 : t.len;
+  const int64_t begin = (int64_t)sp * c.keys_per_split;
+  if (end > begin + c.keys_per_split) end = begin + c.keys_per_split;
+
+  const uint32_t r0 = t.first + 32 * w;
+  const bool wave_live = r0 < t.rows;
+  const uint32_t row = r0 + n < t.rows ? r0 + n : t.rows - 1;
+  const uint64_t orow = (uint64_t)(t.start + row / G) * H + kvh * G + row % G;
+  const int64_t pos = t.pos0 + row / G;
+  const int64_t w_lo = t.pos0 + (wave_live ? r0 : t.rows - 1) / G;
+  const int64_t w_hi = t.pos0 + (r0 + 31 < t.rows ? r0 + 31 : t.rows - 1) / G;
+  half8 qb[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+    qb[s] = *reinterpret_cast<const half8*>(static_cast<const half_t*>(c.q) + orow * DD + 16 * s + 8 * hf);
+  f32x16 ot[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) ot[d][i] = 0.f;
+  float m = -INFINITY, l = 0.f;
+
+  u32x4 kraw[NU], vraw[NU];
+  half_t kd[NU], vd[NU];
+  uint64_t off = kNoRow, have = 0;
+  uint32_t to_s = 0;
+  auto find = [&](int64_t t0) { off = row_offset<PT, DD>(c.b, t.seq, kvh, t0 + lane, end, to_s); };
+  auto fetch = [&]() {
+    have = __ballot(off != kNoRow);
+    const uint64_t o = off != kNoRow ? off : 0;
+    const uint32_t ts = off != kNoRow ? to_s : 0;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int ch = tid + 256 * u < 64 * CPR ? tid + 256 * u : 64 * CPR - 1;
+      const int r = ch / CPR, col = ch % CPR;
+      const uint64_t ro = shfl64(o, r);
+      kraw[u] = *reinterpret_cast<const u32x4*>(c.k + ro + 16 * col);
+      vraw[u] = *reinterpret_cast<const u32x4*>(c.v + ro + 16 * col);
+      if constexpr (I8) {
+        const uint32_t s = __shfl((int)ts, r);
+        kd[u] = reinterpret_cast<const half_t*>(c.k + ro + s)[col / 2];
+        vd[u] = reinterpret_cast<const half_t*>(c.v + ro + s)[col / 2];
+      }
+    }
+  };
+  auto stage = [&](uint64_t seen, bool open, int par) {
+    bool bad = false;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int ch = tid + 256 * u;
+      if (64 * CPR % 256 != 0 && ch >= 64 * CPR) break;
+      const int r = ch / CPR, col = ch % CPR;
+      half8 kx[VC / 8], vx[VC / 8];
+      if constexpr (I8) {
+        kx[0] = dequant8(uint2{kraw[u][0], kraw[u][1]}, kd[u]);
+        kx[1] = dequant8(uint2{kraw[u][2], kraw[u][3]}, kd[u]);
+        vx[0] = dequant8(uint2{vraw[u][0], vraw[u][1]}, vd[u]);
+        vx[1] = dequant8(uint2{vraw[u][2], vraw[u][3]}, vd[u]);
+      } else {
+        kx[0] = __builtin_bit_cast(half8, kraw[u]);
+        vx[0] = __builtin_bit_cast(half8, vraw[u]);
+      }
+#pragma unroll
+      for (int e = 0; e < VC / 8; ++e) {
+        if (!open) {
+          if (!((seen >> r) & 1)) vx[e] = half8{};
+          bad = bad || any_not_finite(vx[e]);
+        }
+        *reinterpret_cast<half8*>(ks + r * KP + VC * col + 8 * e) = kx[e];
+        *reinterpret_cast<half8*>(vs + r * KP + VC * col + 8 * e) = vx[e];
+      }
+    }
+    if (bad) tile_bad[par] = 1;
+  };
+  const half_t* const vtr = vs + (4 * hf + (lane & 15) / 4) * KP + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+
+  auto tile = [&](int64_t t0, uint64_t seen, int par, auto open_c) {
+    constexpr bool OPEN = decltype(open_c)::value;
+    f32x16 sc[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[j][i] = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const half8 a = *reinterpret_cast<const half8*>(ks + (32 * j + n) * KP + 16 * s + 8 * hf);
+        sc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qb[s], sc[j], 0, 0, 0);
+      }
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        if constexpr (!OPEN) {
+          const int k = 32 * j + 8 * (i / 4) + 4 * hf + i % 4;
+          if (!((seen >> k) & 1) || t0 + k > pos) sc[j][i] = -INFINITY;
+        }
+        top = fmaxf(top, sc[j][i]);
+      }
+    top = max2(top) * c.scale_log2;
+    if (__ballot(top > m + kLagLog2) != 0) {  // uniform
+      const float mn = fmaxf(m, top);
+      const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      l *= corr;
+#pragma unroll
+      for (int d = 0; d < DB; ++d) ot[d] *= corr;
+      m = mn;
+    }
+    const float mb = m - kWeightLog2;
+    float sum = 0.f;
+    half8 pb[2][2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][i], c.scale_log2, -mb));
+        if constexpr (!OPEN) e = sc[j][i] == -INFINITY ? 0.f : e;
+        sum += e;
+        pb[j][i / 8][i % 8] = (half_t)e;
+        if constexpr (!OPEN) sc[j][i] = e;
+      }
+    l += sum2(sum);
+    if (OPEN || !tile_bad[par]) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int d = 0; d < DB; ++d) {
+            const uint2 lo = read_tr(vtr + (32 * j + 16 * k) * KP + 32 * d);
+            const uint2 hi = read_tr(vtr + (32 * j + 16 * k + 8) * KP + 32 * d);
+            const half8 av = __builtin_bit_cast(half8, u32x4{lo.x, lo.y, hi.x, hi.y});
+            ot[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, pb[j][k], ot[d], 0, 0, 0);
+          }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int i = 0; i < 16; ++i) ps[w][8 * (i / 4) + 4 * hf + i % 4][n] = sc[j][i];
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (int k = 0; k < 32; ++k) {
+          if (!((seen >> (32 * j + k)) & 1) || t0 + 32 * j + k > pos) continue;
+          const float p = ps[w][k][n];
+#pragma unroll
+          for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              ot[d][i] += p * (float)vs[(32 * j + k) * KP + 32 * d + 8 * (i / 4) + 4 * hf + i % 4];
+        }
+      }
+    }
+  };
+
+  if (tid == 0) tile_bad[0] = tile_bad[1] = 0;
+  int64_t t0 = begin;
+  if (t0 < end) {
+    find(t0);
+    fetch();
+    if (t0 + 64 < end) find(t0 + 64);
+  }
+  for (int par = 0; t0 < end; t0 += 64, par ^= 1) {
+    __syncthreads();  // the previous tile's readers are done
+    // the other parity's flag was last read before this barrier and is set again
+    // only behind the next tile's first barrier
+    if (tid == 0) tile_bad[par ^ 1] = 0;
+    const uint64_t seen = have;
+    const bool open = seen == ~0ull && t0 + 63 <= pos_lo;  // uniform
+    stage(seen, open, par);
+    __syncthreads();
+    if (t0 + 64 < end) {
+      fetch();
+      if (t0 + 128 < end) find(t0 + 128);
+    }
+    if (!wave_live || t0 > w_hi) continue;  // no key of this tile for the wave (uniform)
+    if (seen == ~0ull && t0 + 63 <= w_lo) tile(t0, seen, par, std::true_type{});
+    else tile(t0, seen, par, std::false_type{});
+  }
+
+  if (!wave_live || r0 + n >= t.rows) return;
+  if (ns == 1) {
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    half_t* o = static_cast<half_t*>(c.out) + orow * DD;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        half2v a = {(half_t)(ot[d][4 * q] * inv), (half_t)(ot[d][4 * q + 1] * inv)};
+        half2v b = {(half_t)(ot[d][4 * q + 2] * inv), (half_t)(ot[d][4 * q + 3] * inv)};
+        *reinterpret_cast<uint2*>(o + 32 * d + 8 * q + 4 * hf) =
+            uint2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
+      }
+  } else {
+    const uint64_t p = orow * c.splits + sp;
+    if (hf == 0) *reinterpret_cast<float2s*>(c.ml + 2 * p) = float2s{m, l};
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<float4v*>(c.acc + p * DD + 32 * d + 8 * q + 4 * hf) =
+            float4v{ot[d][4 * q], ot[d][4 * q + 1], ot[d][4 * q + 2], ot[d][4 * q + 3]};
+  }
+}
+
+// ---- launch ------------------------------------------------------------------------------
+
+// Query rows of a sequence up to which the narrow kernel takes it where the wide
+// kernel runs too.
+constexpr uint32_t kNarrowRows = 32;
+
+template <typename T, PoolType PT, int DD>
+hipError_t chunk_mfma(const PagedBatch& b, uint32_t n_heads, const void* q, const void* kp, const void* vp, void* out,
+                      const nfhip::Workspace& ws, hipStream_t s) {
+  Chunk c{};
+  c.b = b;
+  c.q = q;
+  c.k = static_cast<const uint8_t*>(kp);
+  c.v = static_cast<const uint8_t*>(vp);
+  c.out = out;
+  c.n_heads = n_heads;
+  c.group = n_heads / b.n_kv;
+  c.scale_log2 = 1.4426950408889634f / sqrtf((float)DD);
+  const uint64_t rows = (uint64_t)b.rows * c.group;  // query rows per KV head
+  // The wide kernel where sequences have more than kNarrowRows query rows on
+  // average; the narrow one for all of them, or for the short ones among them.
+  // (Lengths are known on the device only: each kernel skips the sequences that
+  // are the other's.)
+  const bool wide = rows > (uint64_t)kNarrowRows * b.n_seqs;
+  const bool narrow = !wide || b.n_seqs > 1;
+  const uint32_t nt = rows > 16ull * b.n_seqs ? 2 : 1;
+  const uint64_t tiles = wide ? rows / 128 + b.n_seqs : rows / (16 * nt) + b.n_seqs;
+  // Splits of the keys: enough workgroups for the chip, at least kMinKeys keys each,
+  // and partials that fit the workspace.
+  const uint64_t units = (wide ? rows / 128 + b.n_seqs : rows / (16 * nt) > b.n_seqs ? rows / (16 * nt) : b.n_seqs) * b.n_kv;
+  const uint32_t target = wide ? 512 : 2048, min_keys = wide ? 512 : 128;
+  uint64_t splits = (target + units - 1) / units;
+  const uint64_t most = ws.part ? ws.part_floats / ((uint64_t)b.rows * n_heads * (DD + 4)) : 1;
+  if (splits > most) splits = most ? most : 1;
+  uint64_t keys = splits > 1 ? (b.limit + splits - 1) / splits : b.limit;
+  keys = keys < min_keys ? min_keys : keys;
+  keys = (keys + 127) / 128 * 128;
+  c.keys_per_split = (uint32_t)keys;
+  c.splits = (uint32_t)((b.limit + keys - 1) / keys);
+  if (c.splits == 0) c.splits = 1;
+  c.ml = ws.part;
+  c.acc = ws.part + ((uint64_t)b.rows * n_heads * c.splits * 2 + 3) / 4 * 4;
+  if (wide) {
+    c.tiles = (uint32_t)tiles;
+    c.lo = narrow ? kNarrowRows : 0;
+    c.hi = ~0ull;
+    const uint64_t x = (tiles * b.n_kv + 7) / 8 * 8;
+    chunk_wide_kernel<PT, DD><<<dim3((unsigned)x, c.splits), 256, 0, s>>>(c);
+  }
+  if (narrow) {
+    c.tiles = (uint32_t)(wide ? b.n_seqs : tiles);
+    c.lo = 0;
+    c.hi = wide ? kNarrowRows : ~0ull;
+    const dim3 grid(c.splits * c.tiles, b.n_kv);
+    if (wide || nt == 2) chunk_narrow_kernel<PT, DD, 2><<<grid, 256, 0, s>>>(c);
+    else chunk_narrow_kernel<PT, DD, 1><<<grid, 256, 0, s>>>(c);
+  }
+  if (c.splits > 1) {
+    const uint64_t n = (uint64_t)b.rows * n_heads;
+    chunk_combine_kernel<T, DD><<<dim3((unsigned)((n + 3) / 4)), 256, 0, s>>>(c);
+  }
+  return hipGetLastError();
+}
+
 template <typename T, PoolType PT>
 hipError_t chunk(const PagedBatch& b, uint32_t n_heads, const void* q, const void* kp, const void* vp, void* out,
-                 const nfhip::Workspace&, hipStream_t s) {
+                 const nfhip::Workspace& ws, hipStream_t s) {
+  if constexpr (std::is_same<T, half_t>::value) {
+    const uintptr_t all = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(kp) |
+                          reinterpret_cast<uintptr_t>(vp) | reinterpret_cast<uintptr_t>(out);
+    // 16-byte rows: an I8 page of block_size head_dim 17/16 bytes has to be whole chunks
+    if (all % 16 == 0 && n_heads % b.n_kv == 0 && b.blocks > 0 && b.limit > 0 &&
+        (PT != PoolType::I8 || b.block_size * b.dim % 256 == 0)) {
+      if (b.dim == 128) return chunk_mfma<T, PT, 128>(b, n_heads, q, kp, vp, out, ws, s);
+      if (b.dim == 96) return chunk_mfma<T, PT, 96>(b, n_heads, q, kp, vp, out, ws, s);
+      if (b.dim == 64) return chunk_mfma<T, PT, 64>(b, n_heads, q, kp, vp, out, ws, s);
+    }
+  }
   const float scale = 1.0f / sqrtf((float)b.dim);
   chunk_any_kernel<T, PT><<<dim3(b.rows, n_heads), 256, 0, s>>>(b, n_heads, scale, (const T*)q, (const uint8_t*)kp,
                                                                 (const uint8_t*)vp, (T*)out);
