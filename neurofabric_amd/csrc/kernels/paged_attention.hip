@@ -842,6 +842,489 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
   }
 }
 
+// ---- f32 rows -----------------------------------------------------------------------
+//
+// The same two kernels on v_mfma_f32_16x16x4_f32, whose products and sums are
+// those of f32 arithmetic; 8-bit codes become f32 exactly.  The MFMA takes one
+// value per lane and operand, so the order in which dims (scores) and keys (P.V)
+// are summed is free and every operand comes in 16-byte pieces:
+//  * scores: k-step s of lane group g is dim DD/4 g + s, a lane's operand DD/4
+//    consecutive elements of its key's row;
+//  * P.V: the k-step over keys 16j + 4g + i takes the weight that the scores left
+//    in lane (row, g) as element (j, i); row m of output block 4h + e is dim 64h +
+//    4m + e, so a lane's operands are 4 consecutive elements of one value row, and
+//    it ends with 16 consecutive dims per h.  (DD = 96: half of the second h is
+//    not there; its columns are computed and dropped.)
+
+// Eight codes and four codes as f32.
+__device__ __forceinline__ void codes8_f32(uint2 w, float d, float* x) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = d * (float)(int)(int8_t)((e < 4 ? w.x : w.y) >> (8 * (e & 3)));
+}
+__device__ __forceinline__ float4v codes4_f32(uint32_t w, float d) {
+  return float4v{d * (float)(int)(int8_t)w, d * (float)(int)(int8_t)(w >> 8), d * (float)(int)(int8_t)(w >> 16),
+                 d * (float)(int)(int8_t)(w >> 24)};
+}
+
+// One row's output or partial, from the layout above.
+template <int DD>
+__device__ __forceinline__ void store_f32(const Chunk& c, uint64_t orow, uint32_t sp, uint32_t ns, int g, float m, float l,
+                                          const float4v* ot) {
+  float* dst = ns == 1 ? static_cast<float*>(c.out) + orow * DD : c.acc + (orow * c.splits + sp) * DD;
+  const float f = ns > 1 ? 1.0f : l == 0.f ? 0.f : 1.0f / l;
+  if (ns > 1 && g == 0) *reinterpret_cast<float2s*>(c.ml + 2 * (orow * c.splits + sp)) = float2s{m, l};
+#pragma unroll
+  for (int h = 0; h < (DD + 63) / 64; ++h)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (64 * h + 16 * g < DD)
+        *reinterpret_cast<float4v*>(dst + 64 * h + 16 * g + 4 * r) =
+            float4v{ot[4 * h][r] * f, ot[4 * h + 1][r] * f, ot[4 * h + 2][r] * f, ot[4 * h + 3][r] * f};
+}
+
+// Few query rows: 16 a workgroup, its waves take 32-key tiles in turn; K and V go
+// from the cache straight into the operands, no LDS before the merge.  A tile
+// with a masked pair and a value that is not finite reads the values again, row by
+// row, for the pairs that count.
+template <PoolType PT, int DD>
+__global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
+  constexpr bool I8 = PT == PoolType::I8;
+  constexpr int DG = DD / 4, NH = (DD + 63) / 64, NB = 4 * NH;
+  __shared__ __attribute__((aligned(16))) float merge[4][16 * 64 * NH];
+  __shared__ float wm[4][16], wl[4][16];
+  const uint32_t sp = blockIdx.x % c.splits, kvh = blockIdx.y;
+  RowTile t;
+  if (!find_tile(c.b, blockIdx.x / c.splits, c.group, 16, c.lo, c.hi, t)) return;
+  const uint32_t ns = splits_of(c, t.len);
+  if (sp >= ns) return;
+  const uint32_t G = c.group, H = c.n_heads;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t last = (t.first + 16 < t.rows ? t.first + 16 : t.rows) - 1;
+  const int64_t pos_lo = t.pos0 + t.first / G, pos_hi = t.pos0 + last / G;
+  int64_t end = pos_hi + 1 < t.len ? pos_hi + 1 : t.len;
+  const int64_t begin = (int64_t)sp * c.keys_per_split;
+  if (end > begin + c.keys_per_split) end = begin + c.keys_per_split;
+  const uint32_t row = t.first + n < t.rows ? t.first + n : t.rows - 1;
+  const uint64_t orow = (uint64_t)(t.start + row / G) * H + kvh * G + row % G;
+  const int64_t pos = t.pos0 + row / G;
+
+  float qb[DG];
+#pragma unroll
+  for (int s = 0; s < DG / 4; ++s) {
+    const float4v x = *reinterpret_cast<const float4v*>(static_cast<const float*>(c.q) + orow * DD + DG * g + 4 * s);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) qb[4 * s + e] = x[e];
+  }
+  float4v ot[NB];
+#pragma unroll
+  for (int d = 0; d < NB; ++d) ot[d] = float4v{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+
+  float4v kf[2][I8 ? 1 : DG / 4], vf[2][4][I8 ? 1 : NH];
+  uint2 kc[2][I8 ? DG / 8 : 1];
+  half_t kd[2][I8 ? DG / 8 : 1], vd[2][4][NH];
+  uint32_t vc[2][4][NH];
+  uint32_t have = 0, to_s = 0;
+  uint64_t off = kNoRow, cur = 0;  // rows of the tile after the next, and of the next
+  auto find = [&](int64_t t0) { off = row_offset<PT, DD>(c.b, t.seq, kvh, t0 + (lane & 31), end, to_s); };
+  uint32_t cur_s = 0;
+  auto fetch_k = [&]() {
+    have = (uint32_t)__ballot(off != kNoRow);
+    cur = off != kNoRow ? off : 0;
+    cur_s = off != kNoRow ? to_s : 0;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint8_t* kr = c.k + shfl64(cur, 16 * j + n);
+      if constexpr (I8) {
+        const half_t* sc = reinterpret_cast<const half_t*>(kr + __shfl((int)cur_s, 16 * j + n));
+#pragma unroll
+        for (int p = 0; p < DG / 8; ++p) {
+          kc[j][p] = *reinterpret_cast<const uint2*>(kr + DG * g + 8 * p);
+          kd[j][p] = sc[(DG * g + 8 * p) / 32];
+        }
+      } else {
+#pragma unroll
+        for (int p = 0; p < DG / 4; ++p) kf[j][p] = *reinterpret_cast<const float4v*>(kr + 4 * (DG * g + 4 * p));
+      }
+    }
+  };
+  auto fetch_v = [&]() {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = 16 * j + 4 * g + i;
+        const uint8_t* vr = c.v + shfl64(cur, k);
+        const uint32_t s = I8 ? (uint32_t)__shfl((int)cur_s, k) : 0u;
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          const int d = 64 * h + 4 * n < DD ? 64 * h + 4 * n : 0;
+          if constexpr (I8) {
+            vc[j][i][h] = *reinterpret_cast<const uint32_t*>(vr + d);
+            vd[j][i][h] = reinterpret_cast<const half_t*>(vr + s)[d / 32];
+          } else {
+            vf[j][i][h] = *reinterpret_cast<const float4v*>(vr + 4 * d);
+          }
+        }
+      }
+  };
+
+  int64_t t0 = begin + 32 * w;
+  if (t0 < end) {
+    find(t0);
+    fetch_k();
+    fetch_v();
+    if (t0 + 128 < end) find(t0 + 128);
+  }
+  for (; t0 < end; t0 += 128) {
+    float4v sc[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      sc[j] = float4v{0.f, 0.f, 0.f, 0.f};
+      float a[DG];
+      if constexpr (I8) {
+#pragma unroll
+        for (int p = 0; p < DG / 8; ++p) codes8_f32(kc[j][p], (float)kd[j][p], a + 8 * p);
+      } else {
+#pragma unroll
+        for (int p = 0; p < DG; ++p) a[p] = kf[j][p / 4][p % 4];
+      }
+#pragma unroll
+      for (int s = 0; s < DG; ++s) sc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], qb[s], sc[j], 0, 0, 0);
+    }
+    const uint32_t seen = have;
+    const uint64_t rows = cur;
+    const bool open = seen == ~0u && t0 + 31 <= pos_lo;  // uniform
+    float4v va[2][4][NH];
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          if constexpr (I8) va[j][i][h] = codes4_f32(vc[j][i][h], (float)vd[j][i][h]);
+          else va[j][i][h] = vf[j][i][h];
+          if (!open) {
+            if (!((seen >> (16 * j + 4 * g + i)) & 1)) va[j][i][h] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) bad = bad || !__builtin_isfinite(va[j][i][h][e]);
+          }
+        }
+    const bool alu = !open && __ballot(bad) != 0;
+    __builtin_amdgcn_sched_barrier(0);
+    if (t0 + 128 < end) {
+      fetch_k();
+      if (t0 + 256 < end) find(t0 + 256);
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = 16 * j + 4 * g + i;
+        if (!open && (!((seen >> k) & 1) || t0 + k > pos)) sc[j][i] = -INFINITY;
+        top = fmaxf(top, sc[j][i]);
+      }
+    top = max4(top) * c.scale_log2;
+    if (__ballot(top > m + kLagLog2) != 0) {  // uniform
+      const float mn = fmaxf(m, top);
+      const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      l *= corr;
+#pragma unroll
+      for (int d = 0; d < NB; ++d) ot[d] *= corr;
+      m = mn;
+    }
+    float pv[2][4], sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][i], c.scale_log2, -m));
+        pv[j][i] = !open && sc[j][i] == -INFINITY ? 0.f : e;
+        sum += pv[j][i];
+      }
+    l += sum4(sum);
+    if (!alu) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int d = 0; d < NB; ++d)
+            ot[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(va[j][i][d / 4][d % 4], pv[j][i], ot[d], 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          for (int gk = 0; gk < 4; ++gk) {
+            const int k = 16 * j + 4 * gk + i;
+            const float p = __shfl(pv[j][i], 16 * gk + n);
+            const uint64_t ro = shfl64(rows, k);
+            if (!((seen >> k) & 1)) continue;  // uniform
+            const uint32_t slot = (uint32_t)(t0 + k) % c.b.block_size;
+            const uint8_t* page = c.v + ro - (uint64_t)slot * (I8 ? DD : 4 * DD);
+            if (t0 + k > pos) continue;
+#pragma unroll
+            for (int d = 0; d < NB; ++d)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const uint32_t dim = 64 * (d / 4) + 16 * g + 4 * r + d % 4;
+                if (dim < DD) ot[d][r] += p * page_value<PT>(c.b, page, slot, dim);
+              }
+          }
+    }
+    // a tile of values and the next one's do not fit the registers together
+    __builtin_amdgcn_sched_barrier(0);
+    if (t0 + 128 < end) fetch_v();
+  }
+
+  if (g == 0) {
+    wm[w][n] = m;
+    wl[w][n] = l;
+  }
+  // row n of the wave: dim order of the registers, 4 floats (d = 4h .. 4h + 3, r) at a time
+#pragma unroll
+  for (int h = 0; h < NH; ++h)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      *reinterpret_cast<float4v*>(&merge[w][(n * NH + h) * 64 + 16 * g + 4 * r]) =
+          float4v{ot[4 * h][r], ot[4 * h + 1][r], ot[4 * h + 2][r], ot[4 * h + 3][r]};
+  __syncthreads();
+  for (int idx = tid; idx < 16 * DD / 4; idx += 256) {
+    const int r = idx / (DD / 4), d = idx % (DD / 4) * 4;
+    const uint32_t qr = t.first + r;
+    if (qr >= t.rows) break;
+    float M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) M = fmaxf(M, wm[v][r]);
+    float4v A = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const float f = wm[v][r] == M ? 1.f : __builtin_amdgcn_exp2f(wm[v][r] - M);
+      L += f * wl[v][r];
+      A += f * *reinterpret_cast<const float4v*>(&merge[v][r * NH * 64 + d]);
+    }
+    const uint64_t o = (uint64_t)(t.start + qr / G) * H + kvh * G + qr % G;
+    if (ns == 1) {
+      const float inv = L == 0.f ? 0.f : 1.0f / L;
+      *reinterpret_cast<float4v*>(static_cast<float*>(c.out) + o * DD + d) = A * inv;
+    } else {
+      const uint64_t p = o * c.splits + sp;
+      if (d == 0) *reinterpret_cast<float2s*>(c.ml + 2 * p) = float2s{M, L};
+      *reinterpret_cast<float4v*>(c.acc + p * DD + d) = A;
+    }
+  }
+}
+
+// Many query rows: 64 a workgroup, 16 per wave, 32-key tiles of K and V in LDS.
+template <PoolType PT, int DD>
+__global__ __launch_bounds__(256, 2) void chunk_wide_f32_kernel(Chunk c) {
+  constexpr bool I8 = PT == PoolType::I8;
+  constexpr int TK = 32, DP = DD + 4, DG = DD / 4, NH = (DD + 63) / 64, NB = 4 * NH;
+  constexpr int EC = I8 ? 8 : 4;                  // elements per chunk (8 or 16 bytes)
+  constexpr int CPR = DD / EC, NU = (TK * CPR + 255) / 256;
+  __shared__ __attribute__((aligned(16))) float ks[TK * DP];
+  __shared__ __attribute__((aligned(16))) float vs[TK * DP + 64 * NH - DD];
+  __shared__ __attribute__((aligned(16))) float ps[4][TK][16];
+  __shared__ int tile_bad[2];
+  const uint32_t X = gridDim.x, i0 = (blockIdx.x % 8) * (X / 8) + blockIdx.x / 8;
+  if (i0 >= c.tiles * c.b.n_kv) return;
+  const uint32_t kvh = i0 / c.tiles, sp = blockIdx.y;
+  RowTile t;
+  if (!find_tile(c.b, c.tiles - 1 - i0 % c.tiles, c.group, 64, c.lo, c.hi, t)) return;
+  const uint32_t ns = splits_of(c, t.len);
+  if (sp >= ns) return;
+  const uint32_t G = c.group, H = c.n_heads;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t last = (t.first + 64 < t.rows ? t.first + 64 : t.rows) - 1;
+  const int64_t pos_lo = t.pos0 + t.first / G, pos_hi = t.pos0 + last / G;
+  int64_t end = pos_hi + 1 < t.len ? pos_hi + 1 : t.len;
+  const int64_t begin = (int64_t)sp * c.keys_per_split;
+  if (end > begin + c.keys_per_split) end = begin + c.keys_per_split;
+  const uint32_t r0 = t.first + 16 * w;
+  const bool wave_live = r0 < t.rows;
+  const uint32_t row = r0 + n < t.rows ? r0 + n : t.rows - 1;
+  const uint64_t orow = (uint64_t)(t.start + row / G) * H + kvh * G + row % G;
+  const int64_t pos = t.pos0 + row / G;
+  const int64_t w_lo = t.pos0 + (wave_live ? r0 : t.rows - 1) / G;
+  const int64_t w_hi = t.pos0 + (r0 + 15 < t.rows ? r0 + 15 : t.rows - 1) / G;
+  float qb[DG];
+#pragma unroll
+  for (int s = 0; s < DG / 4; ++s) {
+    const float4v x = *reinterpret_cast<const float4v*>(static_cast<const float*>(c.q) + orow * DD + DG * g + 4 * s);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) qb[4 * s + e] = x[e];
+  }
+  float4v ot[NB];
+#pragma unroll
+  for (int d = 0; d < NB; ++d) ot[d] = float4v{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+
+  float4v kf[I8 ? 1 : NU], vf[I8 ? 1 : NU];
+  uint2 kc[I8 ? NU : 1], vc[I8 ? NU : 1];
+  half_t kd[NU], vd[NU];
+  uint32_t have = 0, to_s = 0;
+  uint64_t off = kNoRow;
+  auto find = [&](int64_t t0) { off = row_offset<PT, DD>(c.b, t.seq, kvh, t0 + (lane & 31), end, to_s); };
+  auto fetch = [&]() {
+    have = (uint32_t)__ballot(off != kNoRow);
+    const uint64_t o = off != kNoRow ? off : 0;
+    const uint32_t ts = off != kNoRow ? to_s : 0;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int ch = tid + 256 * u < TK * CPR ? tid + 256 * u : TK * CPR - 1;
+      const int r = ch / CPR, col = ch % CPR;
+      const uint64_t ro = shfl64(o, r);
+      if constexpr (I8) {
+        const uint32_t s = __shfl((int)ts, r);
+        kc[u] = *reinterpret_cast<const uint2*>(c.k + ro + 8 * col);
+        vc[u] = *reinterpret_cast<const uint2*>(c.v + ro + 8 * col);
+        kd[u] = reinterpret_cast<const half_t*>(c.k + ro + s)[col / 4];
+        vd[u] = reinterpret_cast<const half_t*>(c.v + ro + s)[col / 4];
+      } else {
+        kf[u] = *reinterpret_cast<const float4v*>(c.k + ro + 16 * col);
+        vf[u] = *reinterpret_cast<const float4v*>(c.v + ro + 16 * col);
+      }
+    }
+  };
+  auto stage = [&](uint32_t seen, bool open, int par) {
+    bool bad = false;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int ch = tid + 256 * u;
+      if (TK * CPR % 256 != 0 && ch >= TK * CPR) break;
+      const int r = ch / CPR, col = ch % CPR;
+      float kx[EC], vx[EC];
+      if constexpr (I8) {
+        codes8_f32(kc[u], (float)kd[u], kx);
+        codes8_f32(vc[u], (float)vd[u], vx);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          kx[e] = kf[u][e];
+          vx[e] = vf[u][e];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < EC; ++e)
+        if (!open) {
+          if (!((seen >> r) & 1)) vx[e] = 0.f;
+          bad = bad || !__builtin_isfinite(vx[e]);
+        }
+#pragma unroll
+      for (int e = 0; e < EC; e += 4) {
+        *reinterpret_cast<float4v*>(ks + r * DP + EC * col + e) = float4v{kx[e], kx[e + 1], kx[e + 2], kx[e + 3]};
+        *reinterpret_cast<float4v*>(vs + r * DP + EC * col + e) = float4v{vx[e], vx[e + 1], vx[e + 2], vx[e + 3]};
+      }
+    }
+    if (bad) tile_bad[par] = 1;
+  };
+  auto tile = [&](int64_t t0, uint32_t seen, int par, auto open_c) {
+    constexpr bool OPEN = decltype(open_c)::value;
+    float4v sc[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      sc[j] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int p = 0; p < DG / 4; ++p) {
+        const float4v a = *reinterpret_cast<const float4v*>(ks + (16 * j + n) * DP + DG * g + 4 * p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], qb[4 * p + e], sc[j], 0, 0, 0);
+      }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (!OPEN) {
+          const int k = 16 * j + 4 * g + i;
+          if (!((seen >> k) & 1) || t0 + k > pos) sc[j][i] = -INFINITY;
+        }
+        top = fmaxf(top, sc[j][i]);
+      }
+    top = max4(top) * c.scale_log2;
+    if (__ballot(top > m + kLagLog2) != 0) {  // uniform
+      const float mn = fmaxf(m, top);
+      const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      l *= corr;
+#pragma unroll
+      for (int d = 0; d < NB; ++d) ot[d] *= corr;
+      m = mn;
+    }
+    float pv[2][4], sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][i], c.scale_log2, -m));
+        pv[j][i] = !OPEN && sc[j][i] == -INFINITY ? 0.f : e;
+        sum += pv[j][i];
+      }
+    l += sum4(sum);
+    if (OPEN || !tile_bad[par]) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int h = 0; h < NH; ++h) {
+            const float4v a = *reinterpret_cast<const float4v*>(vs + (16 * j + 4 * g + i) * DP + 4 * n + 64 * h);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              ot[4 * h + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], pv[j][i], ot[4 * h + e], 0, 0, 0);
+          }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ps[w][16 * j + 4 * g + i][n] = pv[j][i];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      for (int k = 0; k < TK; ++k) {
+        if (!((seen >> k) & 1) || t0 + k > pos) continue;
+        const float p = ps[w][k][n];
+#pragma unroll
+        for (int d = 0; d < NB; ++d)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int dim = 64 * (d / 4) + 16 * g + 4 * r + d % 4;
+            if (dim < DD) ot[d][r] += p * vs[k * DP + dim];
+          }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+  };
+
+  if (tid == 0) tile_bad[0] = tile_bad[1] = 0;
+  int64_t t0 = begin;
+  if (t0 < end) {
+    find(t0);
+    fetch();
+    if (t0 + TK < end) find(t0 + TK);
+  }
+  for (int par = 0; t0 < end; t0 += TK, par ^= 1) {
+    __syncthreads();  // the previous tile's readers are done
+    if (tid == 0) tile_bad[par ^ 1] = 0;
+    const uint32_t seen = have;
+    stage(seen, seen == ~0u && t0 + TK - 1 <= pos_lo, par);
+    __syncthreads();
+    if (t0 + TK < end) {
+      fetch();
+      if (t0 + 2 * TK < end) find(t0 + 2 * TK);
+    }
+    if (!wave_live || t0 > w_hi) continue;  // uniform
+    if (seen == ~0u && t0 + TK - 1 <= w_lo) tile(t0, seen, par, std::true_type{});
+    else tile(t0, seen, par, std::false_type{});
+  }
+  if (wave_live && r0 + n < t.rows) store_f32<DD>(c, orow, sp, ns, g, m, l, ot);
+}
+
 // ---- launch ------------------------------------------------------------------------------
 
 // Query rows of a sequence up to which the narrow kernel takes it where the wide
@@ -867,11 +1350,13 @@ hipError_t chunk_mfma(const PagedBatch& b, uint32_t n_heads, const void* q, cons
   // are the other's.)
   const bool wide = rows > (uint64_t)kNarrowRows * b.n_seqs;
   const bool narrow = !wide || b.n_seqs > 1;
-  const uint32_t nt = rows > 16ull * b.n_seqs ? 2 : 1;
-  const uint64_t tiles = wide ? rows / 128 + b.n_seqs : rows / (16 * nt) + b.n_seqs;
+  constexpr bool F16 = std::is_same<T, half_t>::value;
+  constexpr uint32_t kWideRows = F16 ? 128 : 64;  // a wide workgroup's query rows
+  const uint32_t nt = F16 && (wide || rows > 16ull * b.n_seqs) ? 2 : 1;
   // Splits of the keys: enough workgroups for the chip, at least kMinKeys keys each,
   // and partials that fit the workspace.
-  const uint64_t units = (wide ? rows / 128 + b.n_seqs : rows / (16 * nt) > b.n_seqs ? rows / (16 * nt) : b.n_seqs) * b.n_kv;
+  const uint64_t most_tiles = wide ? rows / kWideRows + b.n_seqs : rows / (16 * nt) + b.n_seqs;
+  const uint64_t units = (wide ? most_tiles : rows / (16 * nt) > b.n_seqs ? rows / (16 * nt) : b.n_seqs) * b.n_kv;
   const uint32_t target = wide ? 512 : 2048, min_keys = wide ? 512 : 128;
   uint64_t splits = (target + units - 1) / units;
   const uint64_t most = ws.part ? ws.part_floats / ((uint64_t)b.rows * n_heads * (DD + 4)) : 1;
@@ -885,18 +1370,20 @@ hipError_t chunk_mfma(const PagedBatch& b, uint32_t n_heads, const void* q, cons
   c.ml = ws.part;
   c.acc = ws.part + ((uint64_t)b.rows * n_heads * c.splits * 2 + 3) / 4 * 4;
   if (wide) {
-    c.tiles = (uint32_t)tiles;
+    c.tiles = (uint32_t)most_tiles;
     c.lo = narrow ? kNarrowRows : 0;
     c.hi = ~0ull;
-    const uint64_t x = (tiles * b.n_kv + 7) / 8 * 8;
-    chunk_wide_kernel<PT, DD><<<dim3((unsigned)x, c.splits), 256, 0, s>>>(c);
+    const dim3 grid((unsigned)((most_tiles * b.n_kv + 7) / 8 * 8), c.splits);
+    if constexpr (F16) chunk_wide_kernel<PT, DD><<<grid, 256, 0, s>>>(c);
+    else chunk_wide_f32_kernel<PT, DD><<<grid, 256, 0, s>>>(c);
   }
   if (narrow) {
-    c.tiles = (uint32_t)(wide ? b.n_seqs : tiles);
     c.lo = 0;
     c.hi = wide ? kNarrowRows : ~0ull;
+    c.tiles = (uint32_t)(!wide ? most_tiles : b.n_seqs * (F16 ? 1 : kNarrowRows / 16));
     const dim3 grid(c.splits * c.tiles, b.n_kv);
-    if (wide || nt == 2) chunk_narrow_kernel<PT, DD, 2><<<grid, 256, 0, s>>>(c);
+    if constexpr (!F16) chunk_narrow_f32_kernel<PT, DD><<<grid, 256, 0, s>>>(c);
+    else if (nt == 2) chunk_narrow_kernel<PT, DD, 2><<<grid, 256, 0, s>>>(c);
     else chunk_narrow_kernel<PT, DD, 1><<<grid, 256, 0, s>>>(c);
   }
   if (c.splits > 1) {
@@ -909,16 +1396,14 @@ hipError_t chunk_mfma(const PagedBatch& b, uint32_t n_heads, const void* q, cons
 template <typename T, PoolType PT>
 hipError_t chunk(const PagedBatch& b, uint32_t n_heads, const void* q, const void* kp, const void* vp, void* out,
                  const nfhip::Workspace& ws, hipStream_t s) {
-  if constexpr (std::is_same<T, half_t>::value) {
-    const uintptr_t all = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(kp) |
-                          reinterpret_cast<uintptr_t>(vp) | reinterpret_cast<uintptr_t>(out);
-    // 16-byte rows: an I8 page of block_size head_dim 17/16 bytes has to be whole chunks
-    if (all % 16 == 0 && n_heads % b.n_kv == 0 && b.blocks > 0 && b.limit > 0 &&
-        (PT != PoolType::I8 || b.block_size * b.dim % 256 == 0)) {
-      if (b.dim == 128) return chunk_mfma<T, PT, 128>(b, n_heads, q, kp, vp, out, ws, s);
-      if (b.dim == 96) return chunk_mfma<T, PT, 96>(b, n_heads, q, kp, vp, out, ws, s);
-      if (b.dim == 64) return chunk_mfma<T, PT, 64>(b, n_heads, q, kp, vp, out, ws, s);
-    }
+  const uintptr_t all = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(kp) |
+                        reinterpret_cast<uintptr_t>(vp) | reinterpret_cast<uintptr_t>(out);
+  // 16-byte rows: an I8 page of block_size head_dim 17/16 bytes has to be whole chunks
+  if (all % 16 == 0 && n_heads % b.n_kv == 0 && b.blocks > 0 && b.limit > 0 &&
+      (PT != PoolType::I8 || b.block_size * b.dim % 256 == 0)) {
+    if (b.dim == 128) return chunk_mfma<T, PT, 128>(b, n_heads, q, kp, vp, out, ws, s);
+    if (b.dim == 96) return chunk_mfma<T, PT, 96>(b, n_heads, q, kp, vp, out, ws, s);
+    if (b.dim == 64) return chunk_mfma<T, PT, 64>(b, n_heads, q, kp, vp, out, ws, s);
   }
   const float scale = 1.0f / sqrtf((float)b.dim);
   chunk_any_kernel<T, PT><<<dim3(b.rows, n_heads), 256, 0, s>>>(b, n_heads, scale, (const T*)q, (const uint8_t*)kp,
