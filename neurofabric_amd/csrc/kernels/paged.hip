@@ -67,8 +67,161 @@ __global__ __launch_bounds__(256) void gather_any_kernel(PagedBatch b, const uin
   (blockIdx.y ? vo : ko)[id] = (T)x;
 }
 
+// 16-byte pieces of the dense rows (4 f32, 8 f16), a wave per row: K and V of up to
+// kPieces pieces a lane are loaded before the row's place is looked up, so the two
+// latencies overlap.  I8: the 8 (f32) or 4 (f16) lanes of 32 elements find their
+// largest together.
+constexpr int kPieces = 2;
+
+template <typename T>
+struct Piece {
+  static constexpr int kElems = 16 / sizeof(T);
+  typedef T type __attribute__((ext_vector_type(kElems)));
+};
+
+template <typename T>
+__device__ __forceinline__ void put_codes(typename Piece<T>::type x, uint8_t* codes, half_t* scale, bool first) {
+  constexpr int E = Piece<T>::kElems;
+  float amax = 0.0f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) amax = fmaxf(amax, __builtin_fabsf((float)x[e]));
+#pragma unroll
+  for (int o = 1; o < 32 / E; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
+  const half_t d = scale_of(amax);
+  const float df = (float)d, inv = df > 0.0f ? 1.0f / df : 0.0f;
+  uint32_t w[E / 4] = {};
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    w[e / 4] |= (uint32_t)(uint8_t)(df > 0.0f ? code_of_value((float)x[e], df, inv) : 0) << (8 * (e % 4));
+  if constexpr (E == 8) *reinterpret_cast<uint2*>(codes) = uint2{w[0], w[1]};
+  else *reinterpret_cast<uint32_t*>(codes) = w[0];
+  if (first) *scale = d;
+}
+
+template <typename T, PoolType PT>
+__global__ __launch_bounds__(256) void append_kernel(PagedBatch b, const T* __restrict__ kn, const T* __restrict__ vn,
+                                                     uint8_t* __restrict__ kp, uint8_t* __restrict__ vp) {
+  constexpr uint32_t E = Piece<T>::kElems;
+  typedef typename Piece<T>::type vec;
+  const uint32_t row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (row >= b.rows) return;
+  const uint32_t per_head = b.dim / E, pieces = b.n_kv * per_head;
+  const vec* ks = reinterpret_cast<const vec*>(kn) + (uint64_t)row * pieces;
+  const vec* vs = reinterpret_cast<const vec*>(vn) + (uint64_t)row * pieces;
+  vec kx[kPieces], vx[kPieces];
+  auto load = [&](uint32_t u0) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const uint32_t u = u0 + 64 * i + lane < pieces ? u0 + 64 * i + lane : pieces - 1;
+      kx[i] = ks[u];
+      vx[i] = vs[u];
+    }
+  };
+  load(0);
+  uint32_t seq;
+  int64_t pos;
+  if (!find_row_wave(b, row, seq, pos)) return;  // uniform
+  const uint32_t phys = find_block(b, seq, pos);
+  if (phys == ~0u) return;
+  const uint32_t slot = (uint32_t)pos % b.block_size;
+  const uint64_t page = nfhip::page_bytes(PT, (uint64_t)b.block_size * b.dim), block = (uint64_t)phys * b.n_kv * page;
+  for (uint32_t u0 = 0; u0 < pieces; u0 += 64 * kPieces) {
+    if (u0) load(u0);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const uint32_t u = u0 + 64 * i + lane;
+      const uint32_t head = u / per_head, d = (u - head * per_head) * E;
+      const uint64_t at = block + head * page;
+      if constexpr (PT != PoolType::I8) {
+        if (u >= pieces) break;
+        const uint64_t to = at + (uint64_t)(slot * b.dim + d) * sizeof(T);
+        *reinterpret_cast<vec*>(kp + to) = kx[i];
+        *reinterpret_cast<vec*>(vp + to) = vx[i];
+      } else {
+        if (u0 + 64 * i >= pieces) break;  // uniform: groups of 32 elements are never split
+        const uint32_t el = slot * b.dim + d;
+        const uint64_t sc = at + (uint64_t)b.block_size * b.dim + el / 16;
+        if (u >= pieces) continue;
+        put_codes<T>(kx[i], kp + at + el, reinterpret_cast<half_t*>(kp + sc), d % 32 == 0);
+        put_codes<T>(vx[i], vp + at + el, reinterpret_cast<half_t*>(vp + sc), d % 32 == 0);
+      }
+    }
+  }
+}
+
+template <typename T, PoolType PT>
+__global__ __launch_bounds__(256) void gather_kernel(PagedBatch b, const uint8_t* __restrict__ kp,
+                                                     const uint8_t* __restrict__ vp, T* __restrict__ ko,
+                                                     T* __restrict__ vo) {
+  constexpr uint32_t E = Piece<T>::kElems;
+  typedef typename Piece<T>::type vec;
+  typedef typename std::conditional<E == 8, uint2, uint32_t>::type codes_t;
+  const uint32_t row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (row >= b.rows) return;
+  uint32_t seq;
+  int64_t pos;
+  if (!find_row_wave(b, row, seq, pos)) return;  // uniform
+  const uint32_t phys = find_block(b, seq, pos);
+  const uint32_t per_head = b.dim / E, pieces = b.n_kv * per_head;
+  vec* kd = reinterpret_cast<vec*>(ko) + (uint64_t)row * pieces;
+  vec* vd = reinterpret_cast<vec*>(vo) + (uint64_t)row * pieces;
+  if (phys == ~0u) {
+    for (uint32_t u = lane; u < pieces; u += 64) kd[u] = vd[u] = vec{};
+    return;
+  }
+  const uint32_t slot = (uint32_t)pos % b.block_size;
+  const uint64_t page = nfhip::page_bytes(PT, (uint64_t)b.block_size * b.dim), block = (uint64_t)phys * b.n_kv * page;
+  for (uint32_t u0 = 0; u0 < pieces; u0 += 64 * kPieces) {
+    vec x[kPieces][2];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const uint32_t u = u0 + 64 * i + lane < pieces ? u0 + 64 * i + lane : pieces - 1;
+      const uint32_t head = u / per_head, el = slot * b.dim + (u - head * per_head) * E;
+      const uint64_t at = block + head * page;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint8_t* p = (j ? vp : kp) + at;
+        if constexpr (PT != PoolType::I8) {
+          x[i][j] = *reinterpret_cast<const vec*>(p + (uint64_t)el * sizeof(T));
+        } else {
+          const codes_t c = *reinterpret_cast<const codes_t*>(p + el);
+          const float d = (float)*reinterpret_cast<const half_t*>(p + (uint64_t)b.block_size * b.dim + el / 32 * 2);
+#pragma unroll
+          for (uint32_t e = 0; e < E; ++e) {
+            uint32_t word;
+            if constexpr (E == 8) word = e < 4 ? c.x : c.y;
+            else word = c;
+            x[i][j][e] = (T)(d * (float)(int)(int8_t)(word >> (8 * (e % 4))));
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const uint32_t u = u0 + 64 * i + lane;
+      if (u < pieces) {
+        kd[u] = x[i][0];
+        vd[u] = x[i][1];
+      }
+    }
+  }
+}
+
+// Whole 16-byte pieces in rows and pages, and for I8 codes at multiples of 8 bytes.
+template <typename T, PoolType PT>
+bool pieces_fit(const PagedBatch& b, const void* k, const void* v, const void* kp, const void* vp) {
+  const uintptr_t all = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+                        reinterpret_cast<uintptr_t>(kp) | reinterpret_cast<uintptr_t>(vp);
+  return all % 16 == 0 && b.dim % Piece<T>::kElems == 0 &&
+         (PT != PoolType::I8 || nfhip::page_bytes(PT, (uint64_t)b.block_size * b.dim) % 8 == 0);
+}
+
 template <typename T, PoolType PT>
 hipError_t append(const PagedBatch& b, const void* kn, const void* vn, void* kp, void* vp, hipStream_t s) {
+  if (pieces_fit<T, PT>(b, kn, vn, kp, vp)) {
+    append_kernel<T, PT><<<dim3((b.rows + 3) / 4), 256, 0, s>>>(b, (const T*)kn, (const T*)vn, (uint8_t*)kp, (uint8_t*)vp);
+    return hipGetLastError();
+  }
   const uint64_t n = (uint64_t)b.rows * b.n_kv * (PT == PoolType::I8 ? b.dim / 32 : b.dim);
   append_any_kernel<T, PT><<<dim3((unsigned)((n + 255) / 256), 2), 256, 0, s>>>(
       b, (const T*)kn, (const T*)vn, (uint8_t*)kp, (uint8_t*)vp);
@@ -77,6 +230,10 @@ hipError_t append(const PagedBatch& b, const void* kn, const void* vn, void* kp,
 
 template <typename T, PoolType PT>
 hipError_t gather(const PagedBatch& b, const void* kp, const void* vp, void* ko, void* vo, hipStream_t s) {
+  if (pieces_fit<T, PT>(b, ko, vo, kp, vp)) {
+    gather_kernel<T, PT><<<dim3((b.rows + 3) / 4), 256, 0, s>>>(b, (const uint8_t*)kp, (const uint8_t*)vp, (T*)ko, (T*)vo);
+    return hipGetLastError();
+  }
   const uint64_t n = (uint64_t)b.rows * b.n_kv * b.dim;
   gather_any_kernel<T, PT><<<dim3((unsigned)((n + 255) / 256), 2), 256, 0, s>>>(
       b, (const uint8_t*)kp, (const uint8_t*)vp, (T*)ko, (T*)vo);

@@ -36,6 +36,25 @@ __device__ __forceinline__ bool find_row(const PagedBatch& b, uint32_t row, uint
   return true;
 }
 
+// The same for a row that is the same in all lanes: up to 64 sequences in one
+// round of loads, where the search takes one for each of its steps.
+__device__ __forceinline__ bool find_row_wave(const PagedBatch& b, uint32_t row, uint32_t& seq, int64_t& pos) {
+  if (b.n_seqs > 64) return find_row(b, row, seq, pos);
+  const uint32_t s = threadIdx.x & 63;
+  int32_t a = -1, e = -1, len = 0;
+  if (s < b.n_seqs) {
+    a = b.starts[s];
+    e = b.starts[s + 1];
+    len = b.lens[s];
+  }
+  const uint64_t mine = __ballot(a >= 0 && (int64_t)a <= (int64_t)row && (int64_t)row < (int64_t)e && (int64_t)e <= (int64_t)b.rows);
+  if (mine == 0) return false;
+  const int at = __builtin_ctzll(mine);
+  seq = at;
+  pos = (int64_t)__shfl(len, at) - ((int64_t)__shfl(e, at) - (int64_t)row);
+  return true;
+}
+
 // Physical block of position `pos` of sequence `seq`, or ~0 without storage.
 __device__ __forceinline__ uint32_t find_block(const PagedBatch& b, uint32_t seq, int64_t pos) {
   if (pos < 0 || pos >= (int64_t)b.limit) return ~0u;
