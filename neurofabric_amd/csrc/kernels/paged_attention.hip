@@ -118,8 +118,8 @@ __global__ __launch_bounds__(256) void chunk_any_kernel(PagedBatch b, uint32_t n
 struct RowTile {
   uint32_t seq, first, rows;  // sequence, first query row, query rows of the sequence
   uint32_t start;             // the sequence's first token
-  int64_t pos0;               // position of that token
-  int64_t len;                // positions of the sequence, at most `limit`
+  int pos0;                   // position of that token
+  int len;                    // positions of the sequence, at most `limit`
 };
 
 __device__ __forceinline__ bool find_tile(const PagedBatch& b, uint32_t idx, uint32_t G, uint32_t per, uint64_t lo,
@@ -145,16 +145,17 @@ __device__ __forceinline__ bool find_tile(const PagedBatch& b, uint32_t idx, uin
       const uint32_t v = __shfl_up(up, o);
       if (lane >= o) up += v;
     }
-    const uint32_t total = __shfl(up, 63);
+    const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)up, 63);
     if (idx < total) {
       const int at = __builtin_ctzll(__ballot(up > idx));
+      auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, at); };
       t.seq = s0 + at;
-      t.first = (idx - __shfl(up - tiles, at)) * per;
-      t.rows = __shfl((uint32_t)rows, at);
-      t.start = __shfl(start, at);
-      const int64_t l = __shfl(len, at);
-      t.pos0 = l - (int64_t)(t.rows / G);
-      t.len = l < (int64_t)b.limit ? l : (int64_t)b.limit;
+      t.first = (idx - of(up - tiles)) * per;
+      t.rows = of((uint32_t)rows);
+      t.start = of(start);
+      const int l = (int)of((uint32_t)len);
+      t.pos0 = l - (int)of(n);
+      t.len = l < (int)b.limit ? l : (int)b.limit;
       return true;
     }
     idx -= total;
@@ -178,29 +179,121 @@ struct Chunk {
 };
 
 // Splits that a sequence of `len` positions takes.
-__device__ __forceinline__ uint32_t splits_of(const Chunk& c, int64_t len) {
-  return len <= 0 ? 1u : (uint32_t)((len + c.keys_per_split - 1) / c.keys_per_split);
-}
-
-// Byte offset of the row of position `pos` in a pool (kNoRow without one), and
-// for I8 the distance from it to the row's scales.
-constexpr uint64_t kNoRow = ~0ull;
-template <PoolType PT, int DD>
-__device__ __forceinline__ uint64_t row_offset(const PagedBatch& b, uint32_t seq, uint32_t kvh, int64_t pos, int64_t end,
-                                               uint32_t& to_scales) {
-  to_scales = 0;
-  if (pos >= end) return kNoRow;
-  const uint32_t blk = (uint32_t)pos / b.block_size, slot = (uint32_t)pos - blk * b.block_size;
-  const uint32_t phys = b.table[(uint64_t)seq * b.width + blk];
-  if (phys >= b.blocks) return kNoRow;
-  if constexpr (PT == PoolType::I8) to_scales = (b.block_size - slot) * DD + slot * (DD / 16);
-  constexpr uint32_t row_bytes = PT == PoolType::I8 ? DD : PT == PoolType::F16 ? 2 * DD : 4 * DD;
-  return ((uint64_t)phys * b.n_kv + kvh) * nfhip::page_bytes(PT, (uint64_t)b.block_size * DD) + (uint64_t)slot * row_bytes;
+__device__ __forceinline__ uint32_t splits_of(const Chunk& c, int len) {
+  return len <= 0 ? 1u : ((uint32_t)len + c.keys_per_split - 1) / c.keys_per_split;
 }
 
 __device__ __forceinline__ uint64_t shfl64(uint64_t v, int src) {
   return (uint64_t)(uint32_t)__shfl((int)(uint32_t)v, src) | (uint64_t)(uint32_t)__shfl((int)(uint32_t)(v >> 32), src) << 32;
 }
+
+// Where the rows of a tile of 16 N keys lie.  UNI (block_size a multiple of 16): each
+// 16 keys lie in one block, whose address is the same for the wave and stays in scalar
+// registers, so a lane's address is that and an offset that never changes.  Otherwise
+// lane j looks up key j's row, and the others ask it: 18 exchanges between lanes and
+// the 64-bit additions for each 32-key tile of an I8 cache, where the time is that
+// of instructions (decode of four long sequences 214 us, with UNI 164).
+// look() finds the tile that take() then makes the current one, so that a tile's
+// table entries are read while the one before is computed.  Keys without a row have
+// that of the pool's first key, and no bit in have().
+template <PoolType PT, int DD, int N, bool UNI>
+struct Rows {
+  static constexpr uint32_t kRow = PT == PoolType::I8 ? DD : PT == PoolType::F16 ? 2 * DD : 4 * DD;
+  const PagedBatch& b;
+  const uint32_t* table;  // of the sequence
+  uint32_t kvh, page;     // bytes of a page (at most 65536 * 256 * 4)
+  int end;                // keys below it
+  uint32_t blk, slot, step_blk, step_slot;  // UNI: of the next tile's first key, and a step of tiles
+  uint32_t next_phys[N], next_slot[N];
+  uint64_t base[N];
+  uint32_t scales[N];
+  uint64_t off, next_off;  // else: the lane's key
+  uint32_t sc, next_sc;
+  uint64_t valid, next_valid;
+
+  __device__ __forceinline__ Rows(const PagedBatch& b_, uint32_t seq, uint32_t kvh_, int end_, int first, int step)
+      : b(b_), table(b_.table + (uint64_t)seq * b_.width), kvh(kvh_),
+        page((uint32_t)nfhip::page_bytes(PT, (uint64_t)b_.block_size * DD)), end(end_) {
+    if constexpr (UNI) {
+      blk = __builtin_amdgcn_readfirstlane((uint32_t)first / b.block_size);
+      slot = (uint32_t)first - blk * b.block_size;
+      step_blk = __builtin_amdgcn_readfirstlane((uint32_t)step / b.block_size);
+      step_slot = (uint32_t)step - step_blk * b.block_size;
+    }
+  }
+  __device__ __forceinline__ uint64_t place(uint32_t phys, uint32_t at) const {
+    return ((uint64_t)phys * b.n_kv + kvh) * page + at * kRow;
+  }
+  // From a key's row to its scales.
+  __device__ __forceinline__ uint32_t to_scales(uint32_t at) const {
+    return PT == PoolType::I8 ? (b.block_size - at) * DD + at * (DD / 16) : 0;
+  }
+  __device__ __forceinline__ void look(int t0) {
+    if constexpr (UNI) {
+      uint32_t k = blk, at = slot;
+      next_valid = 0;
+#pragma unroll
+      for (int h = 0; h < N; ++h) {
+        const int left = end - (t0 + 16 * h);
+        next_phys[h] = left > 0 ? table[k] : ~0u;
+        next_slot[h] = at;
+        at += 16;
+        if (at >= b.block_size) {
+          at = 0;
+          ++k;
+        }
+      }
+      blk += step_blk;
+      slot += step_slot;
+      if (slot >= b.block_size) {
+        slot -= b.block_size;
+        ++blk;
+      }
+    } else {
+      const int p = t0 + (int)(threadIdx.x & (16 * N - 1));
+      next_off = 0;
+      next_sc = 0;
+      bool ok = false;
+      if (p < end) {
+        const uint32_t k = (uint32_t)p / b.block_size, at = (uint32_t)p - k * b.block_size, phys = table[k];
+        ok = phys < b.blocks;
+        if (ok) {
+          next_off = place(phys, at);
+          next_sc = to_scales(at);
+        }
+      }
+      next_valid = __ballot(ok);
+      if constexpr (N < 4) next_valid &= (1ull << (16 * N)) - 1;
+    }
+  }
+  __device__ __forceinline__ void take(int t0) {
+    if constexpr (UNI) {
+      valid = 0;
+#pragma unroll
+      for (int h = 0; h < N; ++h) {
+        const bool ok = next_phys[h] < b.blocks;
+        base[h] = ok ? place(next_phys[h], next_slot[h]) : 0;
+        scales[h] = ok ? to_scales(next_slot[h]) : 0;
+        const int left = end - (t0 + 16 * h);
+        valid |= (uint64_t)(ok ? (left >= 16 ? 0xFFFFu : (1u << left) - 1) : 0u) << (16 * h);
+      }
+    } else {
+      off = next_off;
+      sc = next_sc;
+      valid = next_valid;
+    }
+  }
+  __device__ __forceinline__ uint64_t have() const { return valid; }
+  // The row of key 16 h + r, and its scales.
+  __device__ __forceinline__ const uint8_t* row(const uint8_t* pool, int h, uint32_t r) const {
+    if constexpr (UNI) return pool + base[h] + r * kRow;
+    else return pool + shfl64(off, 16 * h + r);
+  }
+  __device__ __forceinline__ const half_t* scale(const uint8_t* pool, int h, uint32_t r) const {
+    if constexpr (UNI) return reinterpret_cast<const half_t*>(pool + base[h] + scales[h] + r * (DD / 16));
+    else return reinterpret_cast<const half_t*>(pool + shfl64(off, 16 * h + r) + (uint32_t)__shfl((int)sc, 16 * h + r));
+  }
+};
 
 // Eight codes as f16: 0x64cc is 1024 + cc, so (code + 128) goes into the low byte
 // and 1152 off again (exact); times the scale, rounded once to f16.
@@ -287,7 +380,7 @@ __device__ __forceinline__ uint2 read_tr(const half_t* p) {
 // that no row sees are stored as zeros, and a tile that has a value that is not
 // finite and a row that does not see some key of it takes the vector ALU, which
 // skips the pairs that are masked.
-template <PoolType PT, int DD, int NT>
+template <PoolType PT, int DD, int NT, bool UNI>
 __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
   constexpr bool I8 = PT == PoolType::I8;
   constexpr int KSTEP = DD / 32, DB = DD / 16;
@@ -310,17 +403,18 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t live = t.rows - t.first < 16u * NT ? t.rows - t.first : 16u * NT;
   // positions of the tile's rows, first to last
-  const int64_t pos_lo = t.pos0 + t.first / G, pos_hi = t.pos0 + (t.first + live - 1) / G;
-  int64_t end = pos_hi + 1 < t.len ? pos_hi + 1 : t.len;  // keys below it
-  const int64_t begin = (int64_t)sp * c.keys_per_split;
-  if (end > begin + c.keys_per_split) end = begin + c.keys_per_split;
+  const int pos_lo = t.pos0 + (int)(t.first / G), pos_hi = t.pos0 + (int)((t.first + live - 1) / G);
+  const int begin = (int)(sp * c.keys_per_split);
+  int end = pos_hi + 1 < t.len ? pos_hi + 1 : t.len;  // keys below it
+  if (end > begin + (int)c.keys_per_split) end = begin + (int)c.keys_per_split;
+  end = __builtin_amdgcn_readfirstlane(end);
 
   half8 qb[NT][KSTEP];
-  int64_t pos[NT];
+  int pos[NT];
 #pragma unroll
   for (int u = 0; u < NT; ++u) {
     const uint32_t r = t.first + 16 * u + n < t.rows ? t.first + 16 * u + n : t.rows - 1;
-    pos[u] = t.pos0 + r / G;
+    pos[u] = t.pos0 + (int)(r / G);
     const half_t* qr = static_cast<const half_t*>(c.q) + ((uint64_t)(t.start + r / G) * H + kvh * G + r % G) * DD;
 #pragma unroll
     for (int s = 0; s < KSTEP; ++s) {
@@ -338,26 +432,18 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
     for (int d = 0; d < DB; ++d) ot[u][d] = float4v{0.f, 0.f, 0.f, 0.f};
   }
 
-  // loads of a tile: lane j < 32 finds the row of key t0 + j, the others ask it
   u32x4 kraw[2][I8 ? (NP > 0 ? NP : 1) : KSTEP];
   uint2 kodd[2];       // I8, odd KSTEP: the last 32 dims
   half_t kd[2][KSTEP]; // I8: scales
   u32x4 vraw[NV];
   half_t vd[NV];
-  uint32_t have = 0;   // keys of the tile that have a row
-  uint64_t off = kNoRow;
-  uint32_t to_s = 0;
-  auto find = [&](int64_t t0) { off = row_offset<PT, DD>(c.b, t.seq, kvh, t0 + (lane & 31), end, to_s); };
+  Rows<PT, DD, 2, UNI> rows(c.b, t.seq, kvh, end, begin + 32 * w, 128);
   auto fetch = [&]() {
-    have = (uint32_t)__ballot(off != kNoRow);
-    const uint64_t o = off != kNoRow ? off : 0;  // row 0 of the pool stands in
-    const uint32_t ts = off != kNoRow ? to_s : 0;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const uint64_t ko = shfl64(o, 16 * j + n);
-      const uint8_t* kr = c.k + ko;
+      const uint8_t* kr = rows.row(c.k, j, n);
       if constexpr (I8) {
-        const half_t* sc = reinterpret_cast<const half_t*>(kr + __shfl((int)ts, 16 * j + n));
+        const half_t* sc = rows.scale(c.k, j, n);
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
           kraw[j][p] = *reinterpret_cast<const u32x4*>(kr + 64 * p + 16 * g);
@@ -375,22 +461,35 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
       const int ch = lane + 64 * u, r = ch / CPR, col = ch % CPR;
-      const uint64_t vo = shfl64(o, r);
-      vraw[u] = *reinterpret_cast<const u32x4*>(c.v + vo + 16 * col);
-      if constexpr (I8)
-        vd[u] = reinterpret_cast<const half_t*>(c.v + vo + __shfl((int)ts, r))[col / 2];
+      if constexpr (16 * CPR % 64 == 0) {  // the 64 chunks of a load lie in one group of 16 keys
+        const int h = 64 * u / (16 * CPR);
+        vraw[u] = *reinterpret_cast<const u32x4*>(rows.row(c.v, h, r - 16 * h) + 16 * col);
+        if constexpr (I8) vd[u] = rows.scale(c.v, h, r - 16 * h)[col / 2];
+      } else {
+        vraw[u] = *reinterpret_cast<const u32x4*>((r < 16 ? rows.row(c.v, 0, r) : rows.row(c.v, 1, r - 16)) + 16 * col);
+        if constexpr (I8) vd[u] = (r < 16 ? rows.scale(c.v, 0, r) : rows.scale(c.v, 1, r - 16))[col / 2];
+      }
     }
   };
 
   half_t* const vw = vs[w];
   const half_t* const vtr = vw + (4 * g + n / 4) * VP + 4 * (n % 4);
-  int64_t t0 = begin + 32 * w;
+  int t0 = begin + 32 * w;
   if (t0 < end) {
-    find(t0);
+    rows.look(t0);
+    rows.take(t0);
     fetch();
-    if (t0 + 128 < end) find(t0 + 128);
+    if (t0 + 128 < end) rows.look(t0 + 128);
   }
-  for (; t0 < end; t0 += 128) {
+  auto next = [&]() {
+    if (t0 + 128 >= end) return;
+    rows.take(t0 + 128);
+    fetch();
+    if (t0 + 256 < end) rows.look(t0 + 256);
+  };
+  // One tile; OPEN: every row sees every key, and no check is needed.
+  auto tile = [&](uint32_t seen, auto open_c) {
+    constexpr bool OPEN = decltype(open_c)::value;
     // scores
     float4v sc[NT][2];
     {
@@ -419,9 +518,10 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
             sc[u][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[j][s], qb[u][s], sc[u][j], 0, 0, 0);
         }
     }
+    // (the scheduling barriers keep the compiler from starting on one phase's operands
+    // while it holds another's: they do not fit the registers together)
+    __builtin_amdgcn_sched_barrier(0);
     // values into the wave's part of LDS, rows without storage as zeros
-    const uint32_t seen = have;
-    const bool open = seen == ~0u && t0 + 31 <= pos_lo;  // every row sees every key (uniform)
     bool bad = false;
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
@@ -435,20 +535,19 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
       }
 #pragma unroll
       for (int e = 0; e < VC / 8; ++e) {
-        if (!open) {
+        if constexpr (!OPEN) {
           if (!((seen >> r) & 1)) x[e] = half8{};
           bad = bad || any_not_finite(x[e]);
         }
         *reinterpret_cast<half8*>(vw + r * VP + VC * col + 8 * e) = x[e];
       }
     }
-    const bool alu = !open && __ballot(bad) != 0;
+    const bool alu = !OPEN && __ballot(bad) != 0;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's LDS accesses stay in order
     __builtin_amdgcn_wave_barrier();
-    if (t0 + 128 < end) {
-      fetch();
-      if (t0 + 256 < end) find(t0 + 256);
-    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (OPEN) next();
+    __builtin_amdgcn_sched_barrier(0);
     half8 pb[NT];
     float pv[NT][2][4];
 #pragma unroll
@@ -459,7 +558,7 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int k = 16 * j + 4 * g + i;
-          if (!open && (!((seen >> k) & 1) || t0 + k > pos[u])) sc[u][j][i] = -INFINITY;
+          if (!OPEN && (!((seen >> k) & 1) || t0 + k > pos[u])) sc[u][j][i] = -INFINITY;
           top = fmaxf(top, sc[u][j][i]);
         }
       top = max4(top) * c.scale_log2;
@@ -479,15 +578,17 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
         for (int i = 0; i < 4; ++i) {
           const float s = sc[u][j][i];
           const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s, c.scale_log2, -mb));
-          pv[u][j][i] = !open && s == -INFINITY ? 0.f : e;
+          pv[u][j][i] = !OPEN && s == -INFINITY ? 0.f : e;
           sum += pv[u][j][i];
           pb[u][4 * j + i] = (half_t)pv[u][j][i];
         }
       l[u] += sum4(sum);
     }
+    __builtin_amdgcn_sched_barrier(0);
     if (!alu) {
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
+        if (d % 4 == 0) __builtin_amdgcn_sched_barrier(0);
         const uint2 lo = read_tr(vtr + 16 * d), hi = read_tr(vtr + 16 * VP + 16 * d);
         const half8 av = __builtin_bit_cast(half8, u32x4{lo.x, lo.y, hi.x, hi.y});
 #pragma unroll
@@ -502,13 +603,16 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
           for (int i = 0; i < 4; ++i) ps[w][16 * j + 4 * g + i][n] = pv[u][j][i];
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 1
         for (int k = 0; k < 32; ++k) {
           if (!((seen >> k) & 1) || t0 + k > pos[u]) continue;
           const float p = ps[w][k][n];
 #pragma unroll
-          for (int d = 0; d < DB; ++d)
+          for (int d = 0; d < DB; ++d) {
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < 4; ++i) ot[u][d][i] += p * (float)vw[k * VP + 16 * d + 4 * g + i];
+          }
         }
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -516,6 +620,17 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the next tile's values come after these reads
     __builtin_amdgcn_wave_barrier();
+    if (!OPEN) next();
+  };
+  // The open tiles come first: those that every row sees whole, up to the first that
+  // has a hole.  Two loops, as one with both bodies does not fit the registers.
+  while (t0 < end && (uint32_t)rows.have() == ~0u && t0 + 31 <= pos_lo) {  // uniform
+    tile(~0u, std::true_type{});
+    t0 += 128;
+  }
+  while (t0 < end) {
+    tile((uint32_t)rows.have(), std::false_type{});
+    t0 += 128;
   }
 
   // merge the waves, 16 rows at a time; write the output (a lone split) or the partial
@@ -562,37 +677,64 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
   }
 }
 
-// The splits of every query row whose sequence has more than one: a wave per row.
+// The splits of every query row whose sequence has more than one.  A workgroup per
+// row: the splits' weights exp2(m - M) are formed once, then each wave sums every
+// fourth split's row (a wave per row, which took them one after the other, needed
+// 54 us for 64 splits of 128 rows of 128).
+constexpr int kSplitsAtOnce = 256;
 template <typename T, int DD>
 __global__ __launch_bounds__(256) void chunk_combine_kernel(Chunk c) {
-  const uint64_t o = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (o >= (uint64_t)c.b.rows * c.n_heads) return;
+  constexpr int R = (DD + 63) / 64;
+  __shared__ float weight[kSplitsAtOnce];
+  __shared__ float part[4][64 * R];
+  __shared__ float wave_m[4], wave_l[4];
+  const uint32_t o = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   uint32_t seq;
   int64_t pos;
-  if (!find_row(c.b, (uint32_t)(o / c.n_heads), seq, pos)) return;
-  const int64_t l = c.b.lens[seq];
-  const uint32_t ns = splits_of(c, l < (int64_t)c.b.limit ? l : (int64_t)c.b.limit);
+  if (!find_row_wave(c.b, o / c.n_heads, seq, pos)) return;  // uniform
+  const int l = c.b.lens[seq];
+  const uint32_t ns = splits_of(c, l < (int)c.b.limit ? l : (int)c.b.limit);
   if (ns == 1) return;
-  float M = -INFINITY;
-  for (uint32_t s = lane; s < ns; s += 64) M = fmaxf(M, c.ml[2 * (o * c.splits + s)]);
+  const uint64_t first = (uint64_t)o * c.splits;
+  const float2s* ml = reinterpret_cast<const float2s*>(c.ml) + first;
+  float M = -INFINITY, L = 0.f;
+  for (uint32_t s = tid; s < ns; s += 256) M = fmaxf(M, ml[s][0]);
 #pragma unroll
   for (int k = 32; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor(M, k));
-  float L = 0.f, A[(DD + 63) / 64] = {};
-  for (uint32_t s = 0; s < ns; ++s) {
-    const float2s ml = *reinterpret_cast<const float2s*>(c.ml + 2 * (o * c.splits + s));
-    if (ml[1] == 0.f) continue;  // no key
-    const float f = ml[0] == M ? 1.f : __builtin_amdgcn_exp2f(ml[0] - M);
-    L += f * ml[1];
-    const float* a = c.acc + (o * c.splits + s) * DD;
+  if (lane == 0) wave_m[wave] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(wave_m[0], wave_m[1]), fmaxf(wave_m[2], wave_m[3]));
+  float A[R] = {};
+  for (uint32_t s0 = 0; s0 < ns; s0 += kSplitsAtOnce) {
+    if (s0) __syncthreads();
+    if (s0 + tid < ns) {
+      const float2s v = ml[s0 + tid];
+      const float f = v[0] == M ? 1.f : __builtin_amdgcn_exp2f(v[0] - M);
+      weight[tid] = v[1] == 0.f ? 0.f : f;  // no key: its row may be anything
+      L += v[1] == 0.f ? 0.f : f * v[1];
+    }
+    __syncthreads();
+    const uint32_t n = ns - s0 < (uint32_t)kSplitsAtOnce ? ns - s0 : kSplitsAtOnce;
+#pragma unroll 4
+    for (uint32_t s = wave; s < n; s += 4) {
+      const float f = weight[s];
+      const float* a = c.acc + (first + s0 + s) * DD;
 #pragma unroll
-    for (int r = 0; r < (DD + 63) / 64; ++r)
-      if (lane + 64 * r < DD) A[r] += f * a[lane + 64 * r];
+      for (int r = 0; r < R; ++r) {
+        const float x = a[lane + 64 * r < DD ? lane + 64 * r : DD - 1];
+        A[r] += f == 0.f ? 0.f : f * x;
+      }
+    }
   }
-  const float inv = L == 0.f ? 0.f : 1.0f / L;
+  L = wave_sum(L);
+  if (lane == 0) wave_l[wave] = L;
 #pragma unroll
-  for (int r = 0; r < (DD + 63) / 64; ++r)
-    if (lane + 64 * r < DD) static_cast<T*>(c.out)[o * DD + lane + 64 * r] = (T)(A[r] * inv);
+  for (int r = 0; r < R; ++r) part[wave][lane + 64 * r] = A[r];
+  __syncthreads();
+  L = (wave_l[0] + wave_l[1]) + (wave_l[2] + wave_l[3]);
+  const float inv = L == 0.f ? 0.f : 1.0f / L;
+  for (uint32_t d = tid; d < DD; d += 256)
+    static_cast<T*>(c.out)[(uint64_t)o * DD + d] = (T)(((part[0][d] + part[1][d]) + (part[2][d] + part[3][d])) * inv);
 }
 
 // ---- many query rows, f16 --------------------------------------------------------------
@@ -606,19 +748,17 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(Chunk c) {
 // f16, are the B operand of O^T[dim][row] += V^T . P^T as they are.
 // Masking, the lazy rescale and values that are not finite: as above; tiles that
 // every row of the workgroup sees whole skip all of it.
-template <PoolType PT, int DD>
+template <PoolType PT, int DD, bool UNI>
 __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
   constexpr bool I8 = PT == PoolType::I8;
   constexpr int KS = DD / 16, DB = DD / 32, KP = DD + 8;
   constexpr int VC = I8 ? 16 : 8;
-  constexpr int CPR = DD / VC, NL = 64 * CPR / 256;
-  static_assert(64 * CPR % 256 == 0 || I8, "chunks");
+  constexpr int CPR = DD / VC;
   constexpr int NU = (64 * CPR + 255) / 256;
   __shared__ __attribute__((aligned(16))) half_t ks[64 * KP];
   __shared__ __attribute__((aligned(16))) half_t vs[64 * KP];
   __shared__ __attribute__((aligned(16))) float ps[4][32][32];
   __shared__ int tile_bad[2];
-  (void)NL;
 
   // Workgroup L runs on XCD L % 8, which has its own L2: each XCD gets the tiles of
   // whole KV heads, late tiles (most keys) first.
@@ -633,18 +773,18 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, hf = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t last = (t.first + 128 < t.rows ? t.first + 128 : t.rows) - 1;
-  const int64_t pos_lo = t.pos0 + t.first / G, pos_hi = t.pos0 + last / G;
-  int64_t end = pos_hi + 1 < t.len ? pos_hi + 1 : t.len;
-  const int64_t begin = (int64_t)sp * c.keys_per_split;
-  if (end > begin + c.keys_per_split) end = begin + c.keys_per_split;
+  const int pos_lo = t.pos0 + (int)(t.first / G), pos_hi = t.pos0 + (int)(last / G);
+  const int begin = (int)(sp * c.keys_per_split);
+  int end = pos_hi + 1 < t.len ? pos_hi + 1 : t.len;
+  if (end > begin + (int)c.keys_per_split) end = begin + (int)c.keys_per_split;
+  end = __builtin_amdgcn_readfirstlane(end);
 
   const uint32_t r0 = t.first + 32 * w;
   const bool wave_live = r0 < t.rows;
   const uint32_t row = r0 + n < t.rows ? r0 + n : t.rows - 1;
   const uint64_t orow = (uint64_t)(t.start + row / G) * H + kvh * G + row % G;
-  const int64_t pos = t.pos0 + row / G;
-  const int64_t w_lo = t.pos0 + (wave_live ? r0 : t.rows - 1) / G;
-  const int64_t w_hi = t.pos0 + (r0 + 31 < t.rows ? r0 + 31 : t.rows - 1) / G;
+  const int pos = t.pos0 + (int)(row / G);
+  const int w_hi = __builtin_amdgcn_readfirstlane(t.pos0 + (int)((r0 + 31 < t.rows ? r0 + 31 : t.rows - 1) / G));
   half8 qb[KS];
 #pragma unroll
   for (int s = 0; s < KS; ++s)
@@ -658,28 +798,41 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
 
   u32x4 kraw[NU], vraw[NU];
   half_t kd[NU], vd[NU];
-  uint64_t off = kNoRow, have = 0;
-  uint32_t to_s = 0;
-  auto find = [&](int64_t t0) { off = row_offset<PT, DD>(c.b, t.seq, kvh, t0 + lane, end, to_s); };
+  Rows<PT, DD, 4, UNI> rows(c.b, t.seq, kvh, end, begin, 64);
   auto fetch = [&]() {
-    have = __ballot(off != kNoRow);
-    const uint64_t o = off != kNoRow ? off : 0;
-    const uint32_t ts = off != kNoRow ? to_s : 0;
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       const int ch = tid + 256 * u < 64 * CPR ? tid + 256 * u : 64 * CPR - 1;
       const int r = ch / CPR, col = ch % CPR;
-      const uint64_t ro = shfl64(o, r);
-      kraw[u] = *reinterpret_cast<const u32x4*>(c.k + ro + 16 * col);
-      vraw[u] = *reinterpret_cast<const u32x4*>(c.v + ro + 16 * col);
-      if constexpr (I8) {
-        const uint32_t s = __shfl((int)ts, r);
-        kd[u] = reinterpret_cast<const half_t*>(c.k + ro + s)[col / 2];
-        vd[u] = reinterpret_cast<const half_t*>(c.v + ro + s)[col / 2];
+      // a wave's 64 chunks lie in one group of 16 keys, known to be the same for it, or in two
+      const int h = 16 * CPR % 64 == 0 ? __builtin_amdgcn_readfirstlane(r / 16) : r / 16;
+      auto get = [&](int hh) {
+        kraw[u] = *reinterpret_cast<const u32x4*>(rows.row(c.k, hh, r - 16 * hh) + 16 * col);
+        vraw[u] = *reinterpret_cast<const u32x4*>(rows.row(c.v, hh, r - 16 * hh) + 16 * col);
+        if constexpr (I8) {
+          kd[u] = rows.scale(c.k, hh, r - 16 * hh)[col / 2];
+          vd[u] = rows.scale(c.v, hh, r - 16 * hh)[col / 2];
+        }
+      };
+      if constexpr (UNI && 16 * CPR == 256) {
+        get(u);  // F16, 128: the workgroup's 256
+      } else if constexpr (UNI) {
+        const uint64_t ro = h < 2 ? (h ? rows.base[1] : rows.base[0]) : (h == 2 ? rows.base[2] : rows.base[3]);
+        const uint32_t so = h < 2 ? (h ? rows.scales[1] : rows.scales[0]) : (h == 2 ? rows.scales[2] : rows.scales[3]);
+        const uint32_t rr = r - 16 * h;
+        kraw[u] = *reinterpret_cast<const u32x4*>(c.k + ro + rr * rows.kRow + 16 * col);
+        vraw[u] = *reinterpret_cast<const u32x4*>(c.v + ro + rr * rows.kRow + 16 * col);
+        if constexpr (I8) {
+          kd[u] = reinterpret_cast<const half_t*>(c.k + ro + so + rr * (DD / 16))[col / 2];
+          vd[u] = reinterpret_cast<const half_t*>(c.v + ro + so + rr * (DD / 16))[col / 2];
+        }
+      } else {
+        get(h);
       }
     }
   };
-  auto stage = [&](uint64_t seen, bool open, int par) {
+  auto stage = [&](uint64_t seen, auto open_c, int par) {
+    constexpr bool OPEN = decltype(open_c)::value;
     bool bad = false;
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
@@ -698,7 +851,7 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
       }
 #pragma unroll
       for (int e = 0; e < VC / 8; ++e) {
-        if (!open) {
+        if constexpr (!OPEN) {
           if (!((seen >> r) & 1)) vx[e] = half8{};
           bad = bad || any_not_finite(vx[e]);
         }
@@ -706,11 +859,11 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
         *reinterpret_cast<half8*>(vs + r * KP + VC * col + 8 * e) = vx[e];
       }
     }
-    if (bad) tile_bad[par] = 1;
+    if (!OPEN && bad) tile_bad[par] = 1;
   };
   const half_t* const vtr = vs + (4 * hf + (lane & 15) / 4) * KP + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
 
-  auto tile = [&](int64_t t0, uint64_t seen, int par, auto open_c) {
+  auto tile = [&](int t0, uint64_t seen, int par, auto open_c) {
     constexpr bool OPEN = decltype(open_c)::value;
     f32x16 sc[2];
 #pragma unroll
@@ -721,6 +874,7 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
     for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
+        if (s % 2 == 0 && j == 0) __builtin_amdgcn_sched_barrier(0);  // bounds the operands that are held at once
         const half8 a = *reinterpret_cast<const half8*>(ks + (32 * j + n) * KP + 16 * s + 8 * hf);
         sc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qb[s], sc[j], 0, 0, 0);
       }
@@ -765,6 +919,7 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
         for (int k = 0; k < 2; ++k)
 #pragma unroll
           for (int d = 0; d < DB; ++d) {
+            if (d == 0) __builtin_amdgcn_sched_barrier(0);
             const uint2 lo = read_tr(vtr + (32 * j + 16 * k) * KP + 32 * d);
             const uint2 hi = read_tr(vtr + (32 * j + 16 * k + 8) * KP + 32 * d);
             const half8 av = __builtin_bit_cast(half8, u32x4{lo.x, lo.y, hi.x, hi.y});
@@ -779,42 +934,57 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
         for (int i = 0; i < 16; ++i) ps[w][8 * (i / 4) + 4 * hf + i % 4][n] = sc[j][i];
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 1
         for (int k = 0; k < 32; ++k) {
           if (!((seen >> (32 * j + k)) & 1) || t0 + 32 * j + k > pos) continue;
           const float p = ps[w][k][n];
 #pragma unroll
           for (int d = 0; d < DB; ++d)
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
+            for (int i = 0; i < 16; ++i) {
+              if (i % 8 == 0) __builtin_amdgcn_sched_barrier(0);
               ot[d][i] += p * (float)vs[(32 * j + k) * KP + 32 * d + 8 * (i / 4) + 4 * hf + i % 4];
+            }
         }
       }
     }
   };
 
   if (tid == 0) tile_bad[0] = tile_bad[1] = 0;
-  int64_t t0 = begin;
+  int t0 = begin;
   if (t0 < end) {
-    find(t0);
+    rows.look(t0);
+    rows.take(t0);
     fetch();
-    if (t0 + 64 < end) find(t0 + 64);
+    if (t0 + 64 < end) rows.look(t0 + 64);
+  }
+  auto next = [&]() {
+    if (t0 + 64 >= end) return;
+    rows.take(t0 + 64);
+    fetch();
+    if (t0 + 128 < end) rows.look(t0 + 128);
+  };
+  // The open tiles come first: those that every row of the workgroup sees whole, up to
+  // the first that has a hole.  Two loops, as one with both bodies does not fit the
+  // registers.
+  while (t0 < end && rows.have() == ~0ull && t0 + 63 <= pos_lo) {  // uniform
+    __syncthreads();  // the previous tile's readers are done
+    stage(~0ull, std::true_type{}, 0);
+    __syncthreads();
+    next();
+    tile(t0, ~0ull, 0, std::true_type{});
+    t0 += 64;
   }
   for (int par = 0; t0 < end; t0 += 64, par ^= 1) {
-    __syncthreads();  // the previous tile's readers are done
+    __syncthreads();
     // the other parity's flag was last read before this barrier and is set again
     // only behind the next tile's first barrier
     if (tid == 0) tile_bad[par ^ 1] = 0;
-    const uint64_t seen = have;
-    const bool open = seen == ~0ull && t0 + 63 <= pos_lo;  // uniform
-    stage(seen, open, par);
+    const uint64_t seen = rows.have();
+    stage(seen, std::false_type{}, par);
     __syncthreads();
-    if (t0 + 64 < end) {
-      fetch();
-      if (t0 + 128 < end) find(t0 + 128);
-    }
-    if (!wave_live || t0 > w_hi) continue;  // no key of this tile for the wave (uniform)
-    if (seen == ~0ull && t0 + 63 <= w_lo) tile(t0, seen, par, std::true_type{});
-    else tile(t0, seen, par, std::false_type{});
+    if (wave_live && t0 <= w_hi) tile(t0, seen, par, std::false_type{});  // uniform
+    next();
   }
 
   if (!wave_live || r0 + n >= t.rows) return;
@@ -886,7 +1056,7 @@ __device__ __forceinline__ void store_f32(const Chunk& c, uint64_t orow, uint32_
 // from the cache straight into the operands, no LDS before the merge.  A tile
 // with a masked pair and a value that is not finite reads the values again, row by
 // row, for the pairs that count.
-template <PoolType PT, int DD>
+template <PoolType PT, int DD, bool UNI>
 __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
   constexpr bool I8 = PT == PoolType::I8;
   constexpr int DG = DD / 4, NH = (DD + 63) / 64, NB = 4 * NH;
@@ -901,13 +1071,14 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t last = (t.first + 16 < t.rows ? t.first + 16 : t.rows) - 1;
-  const int64_t pos_lo = t.pos0 + t.first / G, pos_hi = t.pos0 + last / G;
-  int64_t end = pos_hi + 1 < t.len ? pos_hi + 1 : t.len;
-  const int64_t begin = (int64_t)sp * c.keys_per_split;
-  if (end > begin + c.keys_per_split) end = begin + c.keys_per_split;
+  const int pos_lo = t.pos0 + (int)(t.first / G), pos_hi = t.pos0 + (int)(last / G);
+  const int begin = (int)(sp * c.keys_per_split);
+  int end = pos_hi + 1 < t.len ? pos_hi + 1 : t.len;
+  if (end > begin + (int)c.keys_per_split) end = begin + (int)c.keys_per_split;
+  end = __builtin_amdgcn_readfirstlane(end);
   const uint32_t row = t.first + n < t.rows ? t.first + n : t.rows - 1;
   const uint64_t orow = (uint64_t)(t.start + row / G) * H + kvh * G + row % G;
-  const int64_t pos = t.pos0 + row / G;
+  const int pos = t.pos0 + (int)(row / G);
 
   float qb[DG];
 #pragma unroll
@@ -925,19 +1096,13 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
   uint2 kc[2][I8 ? DG / 8 : 1];
   half_t kd[2][I8 ? DG / 8 : 1], vd[2][4][NH];
   uint32_t vc[2][4][NH];
-  uint32_t have = 0, to_s = 0;
-  uint64_t off = kNoRow, cur = 0;  // rows of the tile after the next, and of the next
-  auto find = [&](int64_t t0) { off = row_offset<PT, DD>(c.b, t.seq, kvh, t0 + (lane & 31), end, to_s); };
-  uint32_t cur_s = 0;
+  Rows<PT, DD, 2, UNI> rows(c.b, t.seq, kvh, end, begin + 32 * w, 128);
   auto fetch_k = [&]() {
-    have = (uint32_t)__ballot(off != kNoRow);
-    cur = off != kNoRow ? off : 0;
-    cur_s = off != kNoRow ? to_s : 0;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const uint8_t* kr = c.k + shfl64(cur, 16 * j + n);
+      const uint8_t* kr = rows.row(c.k, j, n);
       if constexpr (I8) {
-        const half_t* sc = reinterpret_cast<const half_t*>(kr + __shfl((int)cur_s, 16 * j + n));
+        const half_t* sc = rows.scale(c.k, j, n);
 #pragma unroll
         for (int p = 0; p < DG / 8; ++p) {
           kc[j][p] = *reinterpret_cast<const uint2*>(kr + DG * g + 8 * p);
@@ -954,15 +1119,13 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int k = 16 * j + 4 * g + i;
-        const uint8_t* vr = c.v + shfl64(cur, k);
-        const uint32_t s = I8 ? (uint32_t)__shfl((int)cur_s, k) : 0u;
+        const uint8_t* vr = rows.row(c.v, j, 4 * g + i);
 #pragma unroll
         for (int h = 0; h < NH; ++h) {
           const int d = 64 * h + 4 * n < DD ? 64 * h + 4 * n : 0;
           if constexpr (I8) {
             vc[j][i][h] = *reinterpret_cast<const uint32_t*>(vr + d);
-            vd[j][i][h] = reinterpret_cast<const half_t*>(vr + s)[d / 32];
+            vd[j][i][h] = rows.scale(c.v, j, 4 * g + i)[d / 32];
           } else {
             vf[j][i][h] = *reinterpret_cast<const float4v*>(vr + 4 * d);
           }
@@ -970,14 +1133,22 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
       }
   };
 
-  int64_t t0 = begin + 32 * w;
+  int t0 = begin + 32 * w;
   if (t0 < end) {
-    find(t0);
+    rows.look(t0);
+    rows.take(t0);
     fetch_k();
     fetch_v();
-    if (t0 + 128 < end) find(t0 + 128);
+    if (t0 + 128 < end) rows.look(t0 + 128);
   }
-  for (; t0 < end; t0 += 128) {
+  auto next = [&]() {
+    if (t0 + 128 >= end) return;
+    rows.take(t0 + 128);
+    fetch_k();
+    if (t0 + 256 < end) rows.look(t0 + 256);
+  };
+  auto tile = [&](uint32_t seen, auto open_c) {
+    constexpr bool OPEN = decltype(open_c)::value;
     float4v sc[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -993,9 +1164,6 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
 #pragma unroll
       for (int s = 0; s < DG; ++s) sc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], qb[s], sc[j], 0, 0, 0);
     }
-    const uint32_t seen = have;
-    const uint64_t rows = cur;
-    const bool open = seen == ~0u && t0 + 31 <= pos_lo;  // uniform
     float4v va[2][4][NH];
     bool bad = false;
 #pragma unroll
@@ -1006,25 +1174,22 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
         for (int h = 0; h < NH; ++h) {
           if constexpr (I8) va[j][i][h] = codes4_f32(vc[j][i][h], (float)vd[j][i][h]);
           else va[j][i][h] = vf[j][i][h];
-          if (!open) {
+          if constexpr (!OPEN) {
             if (!((seen >> (16 * j + 4 * g + i)) & 1)) va[j][i][h] = float4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int e = 0; e < 4; ++e) bad = bad || !__builtin_isfinite(va[j][i][h][e]);
           }
         }
-    const bool alu = !open && __ballot(bad) != 0;
+    const bool alu = !OPEN && __ballot(bad) != 0;
     __builtin_amdgcn_sched_barrier(0);
-    if (t0 + 128 < end) {
-      fetch_k();
-      if (t0 + 256 < end) find(t0 + 256);
-    }
+    if (OPEN) next();
     float top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int k = 16 * j + 4 * g + i;
-        if (!open && (!((seen >> k) & 1) || t0 + k > pos)) sc[j][i] = -INFINITY;
+        if (!OPEN && (!((seen >> k) & 1) || t0 + k > pos)) sc[j][i] = -INFINITY;
         top = fmaxf(top, sc[j][i]);
       }
     top = max4(top) * c.scale_log2;
@@ -1042,7 +1207,7 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][i], c.scale_log2, -m));
-        pv[j][i] = !open && sc[j][i] == -INFINITY ? 0.f : e;
+        pv[j][i] = !OPEN && sc[j][i] == -INFINITY ? 0.f : e;
         sum += pv[j][i];
       }
     l += sum4(sum);
@@ -1062,11 +1227,9 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
           for (int gk = 0; gk < 4; ++gk) {
             const int k = 16 * j + 4 * gk + i;
             const float p = __shfl(pv[j][i], 16 * gk + n);
-            const uint64_t ro = shfl64(rows, k);
-            if (!((seen >> k) & 1)) continue;  // uniform
             const uint32_t slot = (uint32_t)(t0 + k) % c.b.block_size;
-            const uint8_t* page = c.v + ro - (uint64_t)slot * (I8 ? DD : 4 * DD);
-            if (t0 + k > pos) continue;
+            const uint8_t* page = rows.row(c.v, j, 4 * gk + i) - (uint64_t)slot * rows.kRow;
+            if (!((seen >> k) & 1) || t0 + k > pos) continue;
 #pragma unroll
             for (int d = 0; d < NB; ++d)
 #pragma unroll
@@ -1076,9 +1239,19 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
               }
           }
     }
+    if (!OPEN) next();
     // a tile of values and the next one's do not fit the registers together
     __builtin_amdgcn_sched_barrier(0);
     if (t0 + 128 < end) fetch_v();
+  };
+  // The open tiles first, as in the f16 kernel.
+  while (t0 < end && (uint32_t)rows.have() == ~0u && t0 + 31 <= pos_lo) {  // uniform
+    tile(~0u, std::true_type{});
+    t0 += 128;
+  }
+  while (t0 < end) {
+    tile((uint32_t)rows.have(), std::false_type{});
+    t0 += 128;
   }
 
   if (g == 0) {
@@ -1120,7 +1293,7 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
 }
 
 // Many query rows: 64 a workgroup, 16 per wave, 32-key tiles of K and V in LDS.
-template <PoolType PT, int DD>
+template <PoolType PT, int DD, bool UNI>
 __global__ __launch_bounds__(256, 2) void chunk_wide_f32_kernel(Chunk c) {
   constexpr bool I8 = PT == PoolType::I8;
   constexpr int TK = 32, DP = DD + 4, DG = DD / 4, NH = (DD + 63) / 64, NB = 4 * NH;
@@ -1141,17 +1314,17 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_f32_kernel(Chunk c) {
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t last = (t.first + 64 < t.rows ? t.first + 64 : t.rows) - 1;
-  const int64_t pos_lo = t.pos0 + t.first / G, pos_hi = t.pos0 + last / G;
-  int64_t end = pos_hi + 1 < t.len ? pos_hi + 1 : t.len;
-  const int64_t begin = (int64_t)sp * c.keys_per_split;
-  if (end > begin + c.keys_per_split) end = begin + c.keys_per_split;
+  const int pos_lo = t.pos0 + (int)(t.first / G), pos_hi = t.pos0 + (int)(last / G);
+  const int begin = (int)(sp * c.keys_per_split);
+  int end = pos_hi + 1 < t.len ? pos_hi + 1 : t.len;
+  if (end > begin + (int)c.keys_per_split) end = begin + (int)c.keys_per_split;
+  end = __builtin_amdgcn_readfirstlane(end);
   const uint32_t r0 = t.first + 16 * w;
   const bool wave_live = r0 < t.rows;
   const uint32_t row = r0 + n < t.rows ? r0 + n : t.rows - 1;
   const uint64_t orow = (uint64_t)(t.start + row / G) * H + kvh * G + row % G;
-  const int64_t pos = t.pos0 + row / G;
-  const int64_t w_lo = t.pos0 + (wave_live ? r0 : t.rows - 1) / G;
-  const int64_t w_hi = t.pos0 + (r0 + 15 < t.rows ? r0 + 15 : t.rows - 1) / G;
+  const int pos = t.pos0 + (int)(row / G);
+  const int w_hi = __builtin_amdgcn_readfirstlane(t.pos0 + (int)((r0 + 15 < t.rows ? r0 + 15 : t.rows - 1) / G));
   float qb[DG];
 #pragma unroll
   for (int s = 0; s < DG / 4; ++s) {
@@ -1167,31 +1340,31 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_f32_kernel(Chunk c) {
   float4v kf[I8 ? 1 : NU], vf[I8 ? 1 : NU];
   uint2 kc[I8 ? NU : 1], vc[I8 ? NU : 1];
   half_t kd[NU], vd[NU];
-  uint32_t have = 0, to_s = 0;
-  uint64_t off = kNoRow;
-  auto find = [&](int64_t t0) { off = row_offset<PT, DD>(c.b, t.seq, kvh, t0 + (lane & 31), end, to_s); };
+  Rows<PT, DD, 2, UNI> rows(c.b, t.seq, kvh, end, begin, TK);
   auto fetch = [&]() {
-    have = (uint32_t)__ballot(off != kNoRow);
-    const uint64_t o = off != kNoRow ? off : 0;
-    const uint32_t ts = off != kNoRow ? to_s : 0;
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       const int ch = tid + 256 * u < TK * CPR ? tid + 256 * u : TK * CPR - 1;
       const int r = ch / CPR, col = ch % CPR;
-      const uint64_t ro = shfl64(o, r);
-      if constexpr (I8) {
-        const uint32_t s = __shfl((int)ts, r);
-        kc[u] = *reinterpret_cast<const uint2*>(c.k + ro + 8 * col);
-        vc[u] = *reinterpret_cast<const uint2*>(c.v + ro + 8 * col);
-        kd[u] = reinterpret_cast<const half_t*>(c.k + ro + s)[col / 4];
-        vd[u] = reinterpret_cast<const half_t*>(c.v + ro + s)[col / 4];
-      } else {
-        kf[u] = *reinterpret_cast<const float4v*>(c.k + ro + 16 * col);
-        vf[u] = *reinterpret_cast<const float4v*>(c.v + ro + 16 * col);
-      }
+      auto get = [&](int h) {
+        const uint8_t *kr = rows.row(c.k, h, r - 16 * h), *vr = rows.row(c.v, h, r - 16 * h);
+        if constexpr (I8) {
+          kc[u] = *reinterpret_cast<const uint2*>(kr + 8 * col);
+          vc[u] = *reinterpret_cast<const uint2*>(vr + 8 * col);
+          kd[u] = rows.scale(c.k, h, r - 16 * h)[col / 4];
+          vd[u] = rows.scale(c.v, h, r - 16 * h)[col / 4];
+        } else {
+          kf[u] = *reinterpret_cast<const float4v*>(kr + 16 * col);
+          vf[u] = *reinterpret_cast<const float4v*>(vr + 16 * col);
+        }
+      };
+      if constexpr (!UNI) get(r / 16);
+      else if constexpr (16 * CPR % 256 == 0) get(256 * u / (16 * CPR));  // the workgroup's 256 lie in one group of 16 keys
+      else if (r < 16) get(0);
+      else get(1);
     }
   };
-  auto stage = [&](uint32_t seen, bool open, int par) {
+  auto stage = [&](uint32_t seen, bool closed, int par) {
     bool bad = false;
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
@@ -1211,7 +1384,7 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_f32_kernel(Chunk c) {
       }
 #pragma unroll
       for (int e = 0; e < EC; ++e)
-        if (!open) {
+        if (closed) {
           if (!((seen >> r) & 1)) vx[e] = 0.f;
           bad = bad || !__builtin_isfinite(vx[e]);
         }
@@ -1223,7 +1396,7 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_f32_kernel(Chunk c) {
     }
     if (bad) tile_bad[par] = 1;
   };
-  auto tile = [&](int64_t t0, uint32_t seen, int par, auto open_c) {
+  auto tile = [&](int t0, uint32_t seen, int par, auto open_c) {
     constexpr bool OPEN = decltype(open_c)::value;
     float4v sc[2];
 #pragma unroll
@@ -1302,25 +1475,36 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_f32_kernel(Chunk c) {
   };
 
   if (tid == 0) tile_bad[0] = tile_bad[1] = 0;
-  int64_t t0 = begin;
+  int t0 = begin;
   if (t0 < end) {
-    find(t0);
+    rows.look(t0);
+    rows.take(t0);
     fetch();
-    if (t0 + TK < end) find(t0 + TK);
+    if (t0 + TK < end) rows.look(t0 + TK);
+  }
+  auto next = [&]() {
+    if (t0 + TK >= end) return;
+    rows.take(t0 + TK);
+    fetch();
+    if (t0 + 2 * TK < end) rows.look(t0 + 2 * TK);
+  };
+  // The open tiles first, as in the f16 kernel.
+  while (t0 < end && (uint32_t)rows.have() == ~0u && t0 + TK - 1 <= pos_lo) {  // uniform
+    __syncthreads();  // the previous tile's readers are done
+    stage(~0u, false, 0);
+    __syncthreads();
+    next();
+    tile(t0, ~0u, 0, std::true_type{});
+    t0 += TK;
   }
   for (int par = 0; t0 < end; t0 += TK, par ^= 1) {
-    __syncthreads();  // the previous tile's readers are done
-    if (tid == 0) tile_bad[par ^ 1] = 0;
-    const uint32_t seen = have;
-    stage(seen, seen == ~0u && t0 + TK - 1 <= pos_lo, par);
     __syncthreads();
-    if (t0 + TK < end) {
-      fetch();
-      if (t0 + 2 * TK < end) find(t0 + 2 * TK);
-    }
-    if (!wave_live || t0 > w_hi) continue;  // uniform
-    if (seen == ~0u && t0 + TK - 1 <= w_lo) tile(t0, seen, par, std::true_type{});
-    else tile(t0, seen, par, std::false_type{});
+    if (tid == 0) tile_bad[par ^ 1] = 0;
+    const uint32_t seen = (uint32_t)rows.have();
+    stage(seen, true, par);
+    __syncthreads();
+    if (wave_live && t0 <= w_hi) tile(t0, seen, par, std::false_type{});  // uniform
+    next();
   }
   if (wave_live && r0 + n < t.rows) store_f32<DD>(c, orow, sp, ns, g, m, l, ot);
 }
@@ -1331,8 +1515,8 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_f32_kernel(Chunk c) {
 // kernel runs too.
 constexpr uint32_t kNarrowRows = 32;
 
-template <typename T, PoolType PT, int DD>
-hipError_t chunk_mfma(const PagedBatch& b, uint32_t n_heads, const void* q, const void* kp, const void* vp, void* out,
+template <typename T, PoolType PT, int DD, bool UNI>
+hipError_t chunk_mfma_at(const PagedBatch& b, uint32_t n_heads, const void* q, const void* kp, const void* vp, void* out,
                       const nfhip::Workspace& ws, hipStream_t s) {
   Chunk c{};
   c.b = b;
@@ -1357,7 +1541,7 @@ hipError_t chunk_mfma(const PagedBatch& b, uint32_t n_heads, const void* q, cons
   // and partials that fit the workspace.
   const uint64_t most_tiles = wide ? rows / kWideRows + b.n_seqs : rows / (16 * nt) + b.n_seqs;
   const uint64_t units = (wide ? most_tiles : rows / (16 * nt) > b.n_seqs ? rows / (16 * nt) : b.n_seqs) * b.n_kv;
-  const uint32_t target = wide ? 512 : 2048, min_keys = wide ? 512 : 128;
+  const uint32_t target = 512, min_keys = wide ? 512 : 128;
   uint64_t splits = (target + units - 1) / units;
   const uint64_t most = ws.part ? ws.part_floats / ((uint64_t)b.rows * n_heads * (DD + 4)) : 1;
   if (splits > most) splits = most ? most : 1;
@@ -1374,23 +1558,29 @@ hipError_t chunk_mfma(const PagedBatch& b, uint32_t n_heads, const void* q, cons
     c.lo = narrow ? kNarrowRows : 0;
     c.hi = ~0ull;
     const dim3 grid((unsigned)((most_tiles * b.n_kv + 7) / 8 * 8), c.splits);
-    if constexpr (F16) chunk_wide_kernel<PT, DD><<<grid, 256, 0, s>>>(c);
-    else chunk_wide_f32_kernel<PT, DD><<<grid, 256, 0, s>>>(c);
+    if constexpr (F16) chunk_wide_kernel<PT, DD, UNI><<<grid, 256, 0, s>>>(c);
+    else chunk_wide_f32_kernel<PT, DD, UNI><<<grid, 256, 0, s>>>(c);
   }
   if (narrow) {
     c.lo = 0;
     c.hi = wide ? kNarrowRows : ~0ull;
     c.tiles = (uint32_t)(!wide ? most_tiles : b.n_seqs * (F16 ? 1 : kNarrowRows / 16));
     const dim3 grid(c.splits * c.tiles, b.n_kv);
-    if constexpr (!F16) chunk_narrow_f32_kernel<PT, DD><<<grid, 256, 0, s>>>(c);
-    else if (nt == 2) chunk_narrow_kernel<PT, DD, 2><<<grid, 256, 0, s>>>(c);
-    else chunk_narrow_kernel<PT, DD, 1><<<grid, 256, 0, s>>>(c);
+    if constexpr (!F16) chunk_narrow_f32_kernel<PT, DD, UNI><<<grid, 256, 0, s>>>(c);
+    else if (nt == 2) chunk_narrow_kernel<PT, DD, 2, UNI><<<grid, 256, 0, s>>>(c);
+    else chunk_narrow_kernel<PT, DD, 1, UNI><<<grid, 256, 0, s>>>(c);
   }
   if (c.splits > 1) {
-    const uint64_t n = (uint64_t)b.rows * n_heads;
-    chunk_combine_kernel<T, DD><<<dim3((unsigned)((n + 3) / 4)), 256, 0, s>>>(c);
+    chunk_combine_kernel<T, DD><<<dim3(b.rows * n_heads), 256, 0, s>>>(c);
   }
   return hipGetLastError();
+}
+
+template <typename T, PoolType PT, int DD>
+hipError_t chunk_mfma(const PagedBatch& b, uint32_t n_heads, const void* q, const void* kp, const void* vp, void* out,
+                      const nfhip::Workspace& ws, hipStream_t s) {
+  return b.block_size % 16 == 0 ? chunk_mfma_at<T, PT, DD, true>(b, n_heads, q, kp, vp, out, ws, s)
+                                : chunk_mfma_at<T, PT, DD, false>(b, n_heads, q, kp, vp, out, ws, s);
 }
 
 template <typename T, PoolType PT>

@@ -234,8 +234,9 @@ nf_status plan_paged_batch(const nf_tensor_desc* const* dense, uint32_t n_dense,
   if (!fits(batch[1], S + 1, 4)) return fail(why, "row starts hold fewer than K + 1 entries");
   if (!fits(batch[2], S, 4)) return fail(why, "lengths hold fewer than K entries");
   // Positions a sequence may hold: the tables' capacity, or max_seq_len when
-  // it is given and smaller; lengths are int32.
-  uint64_t limit = std::min<uint64_t>((uint64_t)lp.dim * lp.block_size, 0x7FFFFFFFu);
+  // it is given and smaller; lengths are int32, and the kernels step by whole
+  // tiles past the last.
+  uint64_t limit = std::min<uint64_t>((uint64_t)lp.dim * lp.block_size, 0x7FFFF000u);
   if (pc.max_seq) limit = std::min<uint64_t>(limit, pc.max_seq);
   lp.max_seq = (uint32_t)limit;
   const uint64_t block = page_bytes(lp.pool, (uint64_t)lp.block_size * lp.head_dim) * lp.n_kv;
