@@ -384,7 +384,9 @@ template <PoolType PT, int DD, int NT, bool UNI>
 __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
   constexpr bool I8 = PT == PoolType::I8;
   constexpr int KSTEP = DD / 32, DB = DD / 16;
-  constexpr int VP = DD + 8;                         // LDS row (halves)
+  // LDS row (halves): 8 dwords past a multiple of 64 or an odd multiple of 8, so that
+  // the 8 rows that 32 lanes of a transposing read touch lie in different banks
+  constexpr int VP = DD + 16;
   constexpr int VC = I8 ? 16 : 8;                    // elements per 16-byte chunk
   constexpr int CPR = DD / VC, NV = 32 * CPR / 64;   // chunks per row, per lane and tile
   constexpr int NP = KSTEP / 2;                      // I8: 16-code loads per key row
@@ -579,9 +581,14 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
           const float s = sc[u][j][i];
           const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s, c.scale_log2, -mb));
           pv[u][j][i] = !OPEN && s == -INFINITY ? 0.f : e;
-          sum += pv[u][j][i];
-          pb[u][4 * j + i] = (half_t)pv[u][j][i];
         }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const half2v h = __builtin_convertvector(float2s{pv[u][k / 2][2 * (k % 2)], pv[u][k / 2][2 * (k % 2) + 1]}, half2v);
+        pb[u][2 * k] = h[0];
+        pb[u][2 * k + 1] = h[1];
+        sum = __builtin_amdgcn_fdot2(h, half2v{(half_t)1.f, (half_t)1.f}, sum, false);
+      }
       l[u] += sum4(sum);
     }
     __builtin_amdgcn_sched_barrier(0);
@@ -752,13 +759,22 @@ template <PoolType PT, int DD, bool UNI>
 __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
   constexpr bool I8 = PT == PoolType::I8;
   constexpr int KS = DD / 16, DB = DD / 32, KP = DD + 8;
+  // V rows 16 or 48 dwords past a multiple of 64: the 4 rows and 32 dims that 32 lanes
+  // of a transposing read touch then lie in different banks (KP halves: in 4 of them
+  // two share each, X us)
+  constexpr int VP = DD == 96 ? 96 : DD + 32;
   constexpr int VC = I8 ? 16 : 8;
   constexpr int CPR = DD / VC;
   constexpr int NU = (64 * CPR + 255) / 256;
-  __shared__ __attribute__((aligned(16))) half_t ks[64 * KP];
-  __shared__ __attribute__((aligned(16))) half_t vs[64 * KP];
-  __shared__ __attribute__((aligned(16))) float ps[4][32][32];
+  // two buffers for the open tiles; the masked ones use the first, and the second for
+  // the weights of the vector ALU
+  constexpr int BUF = 64 * (KP + VP);
+  static_assert(BUF * sizeof(half_t) >= 4 * 32 * 32 * sizeof(float), "a buffer holds the weights");
+  __shared__ __attribute__((aligned(16))) half_t lds[2 * BUF];
   __shared__ int tile_bad[2];
+  half_t* const ks = lds;
+  half_t* const vs = lds + 64 * KP;
+  float(*const ps)[32][32] = reinterpret_cast<float(*)[32][32]>(lds + BUF);
 
   // Workgroup L runs on XCD L % 8, which has its own L2: each XCD gets the tiles of
   // whole KV heads, late tiles (most keys) first.
@@ -831,7 +847,7 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
       }
     }
   };
-  auto stage = [&](uint64_t seen, auto open_c, int par) {
+  auto stage = [&](uint64_t seen, auto open_c, int par, int buf) {
     constexpr bool OPEN = decltype(open_c)::value;
     bool bad = false;
 #pragma unroll
@@ -855,17 +871,105 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
           if (!((seen >> r) & 1)) vx[e] = half8{};
           bad = bad || any_not_finite(vx[e]);
         }
-        *reinterpret_cast<half8*>(ks + r * KP + VC * col + 8 * e) = kx[e];
-        *reinterpret_cast<half8*>(vs + r * KP + VC * col + 8 * e) = vx[e];
+        *reinterpret_cast<half8*>(ks + buf + r * KP + VC * col + 8 * e) = kx[e];
+        *reinterpret_cast<half8*>(vs + buf + r * VP + VC * col + 8 * e) = vx[e];
       }
     }
     if (!OPEN && bad) tile_bad[par] = 1;
   };
-  const half_t* const vtr = vs + (4 * hf + (lane & 15) / 4) * KP + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  const half_t* const vtr = vs + (4 * hf + (lane & 15) / 4) * VP + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
 
-  auto tile = [&](int t0, uint64_t seen, int par, auto open_c) {
+  // The running maximum for scores whose largest is `top`, and the weights in place of
+  // the scores, rounded to f16 in pairs and summed as rounded.
+  f32x16 sc[2];
+  half8 pb[2][2];
+  auto rescale = [&](float top) {
+    if (__ballot(top > m + kLagLog2) == 0) return;  // uniform
+    const float mn = fmaxf(m, top);
+    const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+    l *= corr;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) ot[d] *= corr;
+    m = mn;
+  };
+  auto weights = [&](auto open_c) {
     constexpr bool OPEN = decltype(open_c)::value;
-    f32x16 sc[2];
+    const float mb = m - kWeightLog2;
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][i + e], c.scale_log2, -mb));
+          sc[j][i + e] = !OPEN && sc[j][i + e] == -INFINITY ? 0.f : x;
+        }
+        const half2v h = __builtin_convertvector(float2s{sc[j][i], sc[j][i + 1]}, half2v);
+        pb[j][i / 8][i % 8] = h[0];
+        pb[j][i / 8][i % 8 + 1] = h[1];
+        sum = __builtin_amdgcn_fdot2(h, half2v{(half_t)1.f, (half_t)1.f}, sum, false);
+      }
+    l += sum2(sum);
+  };
+  auto value_op = [&](int buf, int j, int k, int d) {
+    const uint2 lo = read_tr(vtr + buf + (32 * j + 16 * k) * VP + 32 * d);
+    const uint2 hi = read_tr(vtr + buf + (32 * j + 16 * k + 8) * VP + 32 * d);
+    return __builtin_bit_cast(half8, u32x4{lo.x, lo.y, hi.x, hi.y});
+  };
+
+  // An open tile.  The operands of the next four MFMAs are read from LDS before the
+  // current four are issued, and the first values before the softmax: left to itself
+  // the compiler reads each just before its use.
+  const half_t* const krow = ks + n * KP + 8 * hf;
+  auto open_tile = [&](int buf) {
+    half8 a[2][4];
+    auto keys = [&](int ch) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        a[ch & 1][q] = *reinterpret_cast<const half8*>(krow + buf + 32 * (q & 1) * KP + 16 * (2 * ch + q / 2));
+    };
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[j][i] = 0.f;
+    keys(0);
+#pragma unroll
+    for (int ch = 0; ch < KS / 2; ++ch) {
+      if (ch + 1 < KS / 2) keys(ch + 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        sc[q & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[ch & 1][q], qb[2 * ch + q / 2], sc[q & 1], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    half8 av[2][DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) av[0][d] = value_op(buf, 0, 0, d);
+    __builtin_amdgcn_sched_barrier(0);
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[j][i]);
+    rescale(max2(top) * c.scale_log2);
+    weights(std::true_type{});
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int ch = 0; ch < 4; ++ch) {
+      if (ch < 3)
+#pragma unroll
+        for (int d = 0; d < DB; ++d) av[(ch + 1) & 1][d] = value_op(buf, (ch + 1) / 2, (ch + 1) % 2, d);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+        ot[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av[ch & 1][d], pb[ch / 2][ch % 2], ot[d], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  // A tile with masked pairs or keys without a row.
+  auto masked_tile = [&](int t0, uint64_t seen, int par) {
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -875,7 +979,7 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         if (s % 2 == 0 && j == 0) __builtin_amdgcn_sched_barrier(0);  // bounds the operands that are held at once
-        const half8 a = *reinterpret_cast<const half8*>(ks + (32 * j + n) * KP + 16 * s + 8 * hf);
+        const half8 a = *reinterpret_cast<const half8*>(krow + 32 * j * KP + 16 * s);
         sc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qb[s], sc[j], 0, 0, 0);
       }
     float top = -INFINITY;
@@ -883,48 +987,22 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        if constexpr (!OPEN) {
-          const int k = 32 * j + 8 * (i / 4) + 4 * hf + i % 4;
-          if (!((seen >> k) & 1) || t0 + k > pos) sc[j][i] = -INFINITY;
-        }
+        const int k = 32 * j + 8 * (i / 4) + 4 * hf + i % 4;
+        if (!((seen >> k) & 1) || t0 + k > pos) sc[j][i] = -INFINITY;
         top = fmaxf(top, sc[j][i]);
       }
-    top = max2(top) * c.scale_log2;
-    if (__ballot(top > m + kLagLog2) != 0) {  // uniform
-      const float mn = fmaxf(m, top);
-      const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-      l *= corr;
-#pragma unroll
-      for (int d = 0; d < DB; ++d) ot[d] *= corr;
-      m = mn;
-    }
-    const float mb = m - kWeightLog2;
-    float sum = 0.f;
-    half8 pb[2][2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][i], c.scale_log2, -mb));
-        if constexpr (!OPEN) e = sc[j][i] == -INFINITY ? 0.f : e;
-        sum += e;
-        pb[j][i / 8][i % 8] = (half_t)e;
-        if constexpr (!OPEN) sc[j][i] = e;
-      }
-    l += sum2(sum);
-    if (OPEN || !tile_bad[par]) {
+    rescale(max2(top) * c.scale_log2);
+    weights(std::false_type{});
+    if (!tile_bad[par]) {
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int k = 0; k < 2; ++k) {
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int d = 0; d < DB; ++d) {
-            if (d == 0) __builtin_amdgcn_sched_barrier(0);
-            const uint2 lo = read_tr(vtr + (32 * j + 16 * k) * KP + 32 * d);
-            const uint2 hi = read_tr(vtr + (32 * j + 16 * k + 8) * KP + 32 * d);
-            const half8 av = __builtin_bit_cast(half8, u32x4{lo.x, lo.y, hi.x, hi.y});
-            ot[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, pb[j][k], ot[d], 0, 0, 0);
-          }
+          for (int d = 0; d < DB; ++d)
+            ot[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(value_op(0, j, k, d), pb[j][k], ot[d], 0, 0, 0);
+        }
     } else {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -943,7 +1021,7 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               if (i % 8 == 0) __builtin_amdgcn_sched_barrier(0);
-              ot[d][i] += p * (float)vs[(32 * j + k) * KP + 32 * d + 8 * (i / 4) + 4 * hf + i % 4];
+              ot[d][i] += p * (float)vs[(32 * j + k) * VP + 32 * d + 8 * (i / 4) + 4 * hf + i % 4];
             }
         }
       }
@@ -951,7 +1029,7 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
   };
 
   if (tid == 0) tile_bad[0] = tile_bad[1] = 0;
-  int t0 = begin;
+  int t0 = begin;  // the tile in the registers
   if (t0 < end) {
     rows.look(t0);
     rows.take(t0);
@@ -959,31 +1037,41 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
     if (t0 + 64 < end) rows.look(t0 + 64);
   }
   auto next = [&]() {
-    if (t0 + 64 >= end) return;
-    rows.take(t0 + 64);
+    t0 += 64;
+    if (t0 >= end) return;
+    rows.take(t0);
     fetch();
-    if (t0 + 128 < end) rows.look(t0 + 128);
+    if (t0 + 64 < end) rows.look(t0 + 64);
   };
   // The open tiles come first: those that every row of the workgroup sees whole, up to
-  // the first that has a hole.  Two loops, as one with both bodies does not fit the
-  // registers.
-  while (t0 < end && rows.have() == ~0ull && t0 + 63 <= pos_lo) {  // uniform
-    __syncthreads();  // the previous tile's readers are done
-    stage(~0ull, std::true_type{}, 0);
-    __syncthreads();
+  // the first that has a hole.  While one is computed from its buffer, the next is
+  // staged into the other and the one after that is loaded.  Two loops, as one with
+  // both kinds of tile does not fit the registers.
+  auto open = [&]() { return t0 < end && rows.have() == ~0ull && t0 + 63 <= pos_lo; };  // uniform
+  if (open()) {
+    stage(~0ull, std::true_type{}, 0, 0);
     next();
-    tile(t0, ~0ull, 0, std::true_type{});
-    t0 += 64;
-  }
-  for (int par = 0; t0 < end; t0 += 64, par ^= 1) {
     __syncthreads();
+    for (int buf = 0;; buf = BUF - buf) {
+      const bool more = open();
+      if (more) {
+        stage(~0ull, std::true_type{}, 0, BUF - buf);
+        next();
+      }
+      if (wave_live) open_tile(buf);
+      __syncthreads();
+      if (!more) break;
+    }
+  }
+  for (int par = 0; t0 < end; par ^= 1) {
+    __syncthreads();  // the previous tile's readers are done
     // the other parity's flag was last read before this barrier and is set again
     // only behind the next tile's first barrier
     if (tid == 0) tile_bad[par ^ 1] = 0;
     const uint64_t seen = rows.have();
-    stage(seen, std::false_type{}, par);
+    stage(seen, std::false_type{}, par, 0);
     __syncthreads();
-    if (wave_live && t0 <= w_hi) tile(t0, seen, par, std::false_type{});  // uniform
+    if (wave_live && t0 <= w_hi) masked_tile(t0, seen, par);  // uniform
     next();
   }
 
