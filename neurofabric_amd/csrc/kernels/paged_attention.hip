@@ -187,68 +187,44 @@ __device__ __forceinline__ uint64_t shfl64(uint64_t v, int src) {
   return (uint64_t)(uint32_t)__shfl((int)(uint32_t)v, src) | (uint64_t)(uint32_t)__shfl((int)(uint32_t)(v >> 32), src) << 32;
 }
 
-// Where the rows of a tile of 16 N keys lie.  UNI (block_size a multiple of 16): each
-// 16 keys lie in one block, whose address is the same for the wave and stays in scalar
-// registers, so a lane's address is that and an offset that never changes.  Otherwise
-// lane j looks up key j's row, and the others ask it: 18 exchanges between lanes and
-// the 64-bit additions for each 32-key tile of an I8 cache, where the time is that
-// of instructions (decode of four long sequences 214 us, with UNI 164).
-// look() finds the tile that take() then makes the current one, so that a tile's
-// table entries are read while the one before is computed.  Keys without a row have
-// that of the pool's first key, and no bit in have().
+// Where the rows of a tile of 16 N keys lie.  UNI (block_size a power of two of at least
+// 16): each 16 keys lie in one block, whose address is the same for the wave and stays
+// in scalar registers, so a lane's address is that and an offset that never changes.
+// Otherwise lane j looks up key j's row, and the others ask it: 18 exchanges between
+// lanes and the 64-bit additions for each 32-key tile of an I8 cache, where the time is
+// that of instructions (decode of four long sequences 214 us, with UNI 164).
+// look() reads the table entries of the tile that take() then makes the current one, so
+// that they arrive while the one before is computed; by vector loads, as scalar ones
+// and LDS reads share a counter that can only be waited for as a whole.  Keys without
+// a row have that of the pool's first key, and no bit in have().
 template <PoolType PT, int DD, int N, bool UNI>
 struct Rows {
   static constexpr uint32_t kRow = PT == PoolType::I8 ? DD : PT == PoolType::F16 ? 2 * DD : 4 * DD;
   const PagedBatch& b;
   const uint32_t* table;  // of the sequence
-  uint32_t kvh, page;     // bytes of a page (at most 65536 * 256 * 4)
+  uint32_t page;          // bytes of a page (at most 65536 * 256 * 4)
+  uint64_t block, head;   // bytes of a block, and from its start to the KV head's page
   int end;                // keys below it
-  uint32_t blk, slot, step_blk, step_slot;  // UNI: of the next tile's first key, and a step of tiles
-  uint32_t next_phys[N], next_slot[N];
+  int shift;              // UNI: log2 of block_size
+  uint32_t entry;         // UNI: lane h has the block of the next tile's group h
   uint64_t base[N];
   uint32_t scales[N];
   uint64_t off, next_off;  // else: the lane's key
   uint32_t sc, next_sc;
   uint64_t valid, next_valid;
 
-  __device__ __forceinline__ Rows(const PagedBatch& b_, uint32_t seq, uint32_t kvh_, int end_, int first, int step)
-      : b(b_), table(b_.table + (uint64_t)seq * b_.width), kvh(kvh_),
-        page((uint32_t)nfhip::page_bytes(PT, (uint64_t)b_.block_size * DD)), end(end_) {
-    if constexpr (UNI) {
-      blk = __builtin_amdgcn_readfirstlane((uint32_t)first / b.block_size);
-      slot = (uint32_t)first - blk * b.block_size;
-      step_blk = __builtin_amdgcn_readfirstlane((uint32_t)step / b.block_size);
-      step_slot = (uint32_t)step - step_blk * b.block_size;
-    }
-  }
-  __device__ __forceinline__ uint64_t place(uint32_t phys, uint32_t at) const {
-    return ((uint64_t)phys * b.n_kv + kvh) * page + at * kRow;
-  }
+  __device__ __forceinline__ Rows(const PagedBatch& b_, uint32_t seq, uint32_t kvh, int end_)
+      : b(b_), table(b_.table + (uint64_t)seq * b_.width),
+        page((uint32_t)nfhip::page_bytes(PT, (uint64_t)b_.block_size * DD)), block((uint64_t)b_.n_kv * page),
+        head((uint64_t)kvh * page), end(end_), shift(__builtin_ctz(b_.block_size)) {}
   // From a key's row to its scales.
   __device__ __forceinline__ uint32_t to_scales(uint32_t at) const {
     return PT == PoolType::I8 ? (b.block_size - at) * DD + at * (DD / 16) : 0;
   }
   __device__ __forceinline__ void look(int t0) {
     if constexpr (UNI) {
-      uint32_t k = blk, at = slot;
-      next_valid = 0;
-#pragma unroll
-      for (int h = 0; h < N; ++h) {
-        const int left = end - (t0 + 16 * h);
-        next_phys[h] = left > 0 ? table[k] : ~0u;
-        next_slot[h] = at;
-        at += 16;
-        if (at >= b.block_size) {
-          at = 0;
-          ++k;
-        }
-      }
-      blk += step_blk;
-      slot += step_slot;
-      if (slot >= b.block_size) {
-        slot -= b.block_size;
-        ++blk;
-      }
+      const int p = t0 + 16 * (int)(threadIdx.x & (N - 1));
+      entry = table[(uint32_t)min(p, end - 1) >> shift];  // past the end: the last key's block, whose bits are cleared
     } else {
       const int p = t0 + (int)(threadIdx.x & (16 * N - 1));
       next_off = 0;
@@ -258,7 +234,7 @@ struct Rows {
         const uint32_t k = (uint32_t)p / b.block_size, at = (uint32_t)p - k * b.block_size, phys = table[k];
         ok = phys < b.blocks;
         if (ok) {
-          next_off = place(phys, at);
+          next_off = phys * block + head + at * kRow;
           next_sc = to_scales(at);
         }
       }
@@ -271,12 +247,15 @@ struct Rows {
       valid = 0;
 #pragma unroll
       for (int h = 0; h < N; ++h) {
-        const bool ok = next_phys[h] < b.blocks;
-        base[h] = ok ? place(next_phys[h], next_slot[h]) : 0;
-        scales[h] = ok ? to_scales(next_slot[h]) : 0;
-        const int left = end - (t0 + 16 * h);
-        valid |= (uint64_t)(ok ? (left >= 16 ? 0xFFFFu : (1u << left) - 1) : 0u) << (16 * h);
+        const uint32_t phys = (uint32_t)__builtin_amdgcn_readlane((int)entry, h);
+        const uint32_t at = (uint32_t)(t0 + 16 * h) & (b.block_size - 1);
+        const bool ok = phys < b.blocks;
+        base[h] = ok ? phys * block + head + at * kRow : 0;
+        scales[h] = ok ? to_scales(at) : 0;
+        valid |= (uint64_t)(ok ? 0xFFFFu : 0u) << (16 * h);
       }
+      const int left = end - t0;
+      if (left < 16 * N) valid &= (1ull << left) - 1;
     } else {
       off = next_off;
       sc = next_sc;
@@ -439,7 +418,7 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
   half_t kd[2][KSTEP]; // I8: scales
   u32x4 vraw[NV];
   half_t vd[NV];
-  Rows<PT, DD, 2, UNI> rows(c.b, t.seq, kvh, end, begin + 32 * w, 128);
+  Rows<PT, DD, 2, UNI> rows(c.b, t.seq, kvh, end);
   auto fetch = [&]() {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -814,7 +793,7 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
 
   u32x4 kraw[NU], vraw[NU];
   half_t kd[NU], vd[NU];
-  Rows<PT, DD, 4, UNI> rows(c.b, t.seq, kvh, end, begin, 64);
+  Rows<PT, DD, 4, UNI> rows(c.b, t.seq, kvh, end);
   auto fetch = [&]() {
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
@@ -1184,7 +1163,7 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
   uint2 kc[2][I8 ? DG / 8 : 1];
   half_t kd[2][I8 ? DG / 8 : 1], vd[2][4][NH];
   uint32_t vc[2][4][NH];
-  Rows<PT, DD, 2, UNI> rows(c.b, t.seq, kvh, end, begin + 32 * w, 128);
+  Rows<PT, DD, 2, UNI> rows(c.b, t.seq, kvh, end);
   auto fetch_k = [&]() {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -1428,7 +1407,7 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_f32_kernel(Chunk c) {
   float4v kf[I8 ? 1 : NU], vf[I8 ? 1 : NU];
   uint2 kc[I8 ? NU : 1], vc[I8 ? NU : 1];
   half_t kd[NU], vd[NU];
-  Rows<PT, DD, 2, UNI> rows(c.b, t.seq, kvh, end, begin, TK);
+  Rows<PT, DD, 2, UNI> rows(c.b, t.seq, kvh, end);
   auto fetch = [&]() {
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
@@ -1667,7 +1646,7 @@ hipError_t chunk_mfma_at(const PagedBatch& b, uint32_t n_heads, const void* q, c
 template <typename T, PoolType PT, int DD>
 hipError_t chunk_mfma(const PagedBatch& b, uint32_t n_heads, const void* q, const void* kp, const void* vp, void* out,
                       const nfhip::Workspace& ws, hipStream_t s) {
-  return b.block_size % 16 == 0 ? chunk_mfma_at<T, PT, DD, true>(b, n_heads, q, kp, vp, out, ws, s)
+  return b.block_size >= 16 && (b.block_size & (b.block_size - 1)) == 0 ? chunk_mfma_at<T, PT, DD, true>(b, n_heads, q, kp, vp, out, ws, s)
                                 : chunk_mfma_at<T, PT, DD, false>(b, n_heads, q, kp, vp, out, ws, s);
 }
 
