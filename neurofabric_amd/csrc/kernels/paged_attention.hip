@@ -663,8 +663,47 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
   }
 }
 
-// The splits of every query row whose sequence has more than one.  A workgroup per
-// row: the splits' weights exp2(m - M) are formed once, then each wave sums every
+// The splits of every query row whose sequence has more than one, where they are few:
+// a wave per row.
+constexpr uint32_t kFewSplits = 8;
+template <typename T, int DD>
+__global__ __launch_bounds__(256) void chunk_combine_few_kernel(Chunk c) {
+  constexpr int R = (DD + 63) / 64;
+  const uint32_t o = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  uint32_t seq;
+  int64_t pos;
+  if (o >= c.b.rows * c.n_heads || !find_row_wave(c.b, o / c.n_heads, seq, pos)) return;  // uniform
+  const int len = c.b.lens[seq];
+  const uint32_t ns = splits_of(c, len < (int)c.b.limit ? len : (int)c.b.limit);
+  if (ns == 1) return;
+  const uint64_t first = (uint64_t)o * c.splits;
+  const float2s* ml = reinterpret_cast<const float2s*>(c.ml) + first;
+  float x[kFewSplits][R], M = -INFINITY, L = 0.f, A[R] = {};
+  float2s v[kFewSplits];
+#pragma unroll
+  for (uint32_t s = 0; s < kFewSplits; ++s) {
+    const uint32_t at = s < ns ? s : ns - 1;
+    v[s] = ml[at];
+#pragma unroll
+    for (int r = 0; r < R; ++r) x[s][r] = c.acc[(first + at) * DD + (lane + 64 * r < DD ? lane + 64 * r : DD - 1)];
+  }
+#pragma unroll
+  for (uint32_t s = 0; s < kFewSplits; ++s) M = fmaxf(M, v[s][0]);
+#pragma unroll
+  for (uint32_t s = 0; s < kFewSplits; ++s) {
+    if (s >= ns || v[s][1] == 0.f) continue;  // no key: its row may be anything
+    const float f = v[s][0] == M ? 1.f : __builtin_amdgcn_exp2f(v[s][0] - M);
+    L += f * v[s][1];
+#pragma unroll
+    for (int r = 0; r < R; ++r) A[r] += f * x[s][r];
+  }
+  const float inv = L == 0.f ? 0.f : 1.0f / L;
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (lane + 64 * r < DD) static_cast<T*>(c.out)[(uint64_t)o * DD + lane + 64 * r] = (T)(A[r] * inv);
+}
+
+// The same for many splits.  A workgroup per row: the splits' weights exp2(m - M) are formed once, then each wave sums every
 // fourth split's row (a wave per row, which took them one after the other, needed
 // 54 us for 64 splits of 128 rows of 128).
 constexpr int kSplitsAtOnce = 256;
@@ -723,6 +762,33 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(Chunk c) {
     static_cast<T*>(c.out)[(uint64_t)o * DD + d] = (T)(((part[0][d] + part[1][d]) + (part[2][d] + part[3][d])) * inv);
 }
 
+// Workgroup x of a wide kernel -> KV head and row tile, late tiles (most keys) first.
+// Workgroup x runs on XCD x % 8, and each XCD has its own L2: the tiles of a KV head go
+// to one XCD where heads are a multiple of 8, else in turn to the XCDs that share the
+// head (in halves of the tiles, one XCD had the long sequences: 165 us for three
+// ragged f32 chunks, Y so).
+__device__ __forceinline__ bool wide_tile(const Chunk& c, uint32_t& kvh, uint32_t& idx) {
+  const uint32_t xcd = blockIdx.x % 8, i = blockIdx.x / 8, n_kv = c.b.n_kv;
+  uint32_t tile;
+  if (n_kv % 8 == 0) {
+    kvh = xcd * (n_kv / 8) + i / c.tiles;
+    tile = i % c.tiles;
+  } else if (8 % n_kv == 0) {
+    const uint32_t share = 8 / n_kv;
+    kvh = xcd / share;
+    tile = i * share + xcd % share;
+  } else {
+    kvh = blockIdx.x % n_kv;
+    tile = blockIdx.x / n_kv;
+  }
+  idx = c.tiles - 1 - tile;
+  return tile < c.tiles && kvh < n_kv;
+}
+// Workgroups for it.
+inline uint32_t wide_grid(uint32_t tiles, uint32_t n_kv) {
+  return 8 % n_kv == 0 ? 8 * ((tiles + 8 / n_kv - 1) / (8 / n_kv)) : tiles * n_kv;
+}
+
 // ---- many query rows, f16 --------------------------------------------------------------
 //
 // A workgroup takes 128 query rows of one KV head, 32 per wave (and one split of
@@ -755,13 +821,11 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
   half_t* const vs = lds + 64 * KP;
   float(*const ps)[32][32] = reinterpret_cast<float(*)[32][32]>(lds + BUF);
 
-  // Workgroup L runs on XCD L % 8, which has its own L2: each XCD gets the tiles of
-  // whole KV heads, late tiles (most keys) first.
-  const uint32_t X = gridDim.x, i0 = (blockIdx.x % 8) * (X / 8) + blockIdx.x / 8;
-  if (i0 >= c.tiles * c.b.n_kv) return;
-  const uint32_t kvh = i0 / c.tiles, sp = blockIdx.y;
+  uint32_t kvh, idx;
+  if (!wide_tile(c, kvh, idx)) return;
+  const uint32_t sp = blockIdx.y;
   RowTile t;
-  if (!find_tile(c.b, c.tiles - 1 - i0 % c.tiles, c.group, 128, c.lo, c.hi, t)) return;
+  if (!find_tile(c.b, idx, c.group, 128, c.lo, c.hi, t)) return;
   const uint32_t ns = splits_of(c, t.len);
   if (sp >= ns) return;
   const uint32_t G = c.group, H = c.n_heads;
@@ -1370,11 +1434,11 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_f32_kernel(Chunk c) {
   __shared__ __attribute__((aligned(16))) float vs[TK * DP + 64 * NH - DD];
   __shared__ __attribute__((aligned(16))) float ps[4][TK][16];
   __shared__ int tile_bad[2];
-  const uint32_t X = gridDim.x, i0 = (blockIdx.x % 8) * (X / 8) + blockIdx.x / 8;
-  if (i0 >= c.tiles * c.b.n_kv) return;
-  const uint32_t kvh = i0 / c.tiles, sp = blockIdx.y;
+  uint32_t kvh, idx;
+  if (!wide_tile(c, kvh, idx)) return;
+  const uint32_t sp = blockIdx.y;
   RowTile t;
-  if (!find_tile(c.b, c.tiles - 1 - i0 % c.tiles, c.group, 64, c.lo, c.hi, t)) return;
+  if (!find_tile(c.b, idx, c.group, 64, c.lo, c.hi, t)) return;
   const uint32_t ns = splits_of(c, t.len);
   if (sp >= ns) return;
   const uint32_t G = c.group, H = c.n_heads;
@@ -1608,8 +1672,8 @@ hipError_t chunk_mfma_at(const PagedBatch& b, uint32_t n_heads, const void* q, c
   // and partials that fit the workspace.
   const uint64_t most_tiles = wide ? rows / kWideRows + b.n_seqs : rows / (16 * nt) + b.n_seqs;
   const uint64_t units = (wide ? most_tiles : rows / (16 * nt) > b.n_seqs ? rows / (16 * nt) : b.n_seqs) * b.n_kv;
-  const uint32_t target = 512, min_keys = wide ? 512 : 128;
-  uint64_t splits = (target + units - 1) / units;
+  const uint32_t target = wide ? 1024 : 512, min_keys = wide ? 256 : 128;
+  uint64_t splits = wide && units >= 1024 ? 1 : (target + units - 1) / units;
   const uint64_t most = ws.part ? ws.part_floats / ((uint64_t)b.rows * n_heads * (DD + 4)) : 1;
   if (splits > most) splits = most ? most : 1;
   uint64_t keys = splits > 1 ? (b.limit + splits - 1) / splits : b.limit;
@@ -1624,7 +1688,7 @@ hipError_t chunk_mfma_at(const PagedBatch& b, uint32_t n_heads, const void* q, c
     c.tiles = (uint32_t)most_tiles;
     c.lo = narrow ? kNarrowRows : 0;
     c.hi = ~0ull;
-    const dim3 grid((unsigned)((most_tiles * b.n_kv + 7) / 8 * 8), c.splits);
+    const dim3 grid(wide_grid(c.tiles, b.n_kv), c.splits);
     if constexpr (F16) chunk_wide_kernel<PT, DD, UNI><<<grid, 256, 0, s>>>(c);
     else chunk_wide_f32_kernel<PT, DD, UNI><<<grid, 256, 0, s>>>(c);
   }
@@ -1638,7 +1702,8 @@ hipError_t chunk_mfma_at(const PagedBatch& b, uint32_t n_heads, const void* q, c
     else chunk_narrow_kernel<PT, DD, 1, UNI><<<grid, 256, 0, s>>>(c);
   }
   if (c.splits > 1) {
-    chunk_combine_kernel<T, DD><<<dim3(b.rows * n_heads), 256, 0, s>>>(c);
+    if (c.splits <= kFewSplits) chunk_combine_few_kernel<T, DD><<<dim3((b.rows * n_heads + 3) / 4), 256, 0, s>>>(c);
+    else chunk_combine_kernel<T, DD><<<dim3(b.rows * n_heads), 256, 0, s>>>(c);
   }
   return hipGetLastError();
 }
