@@ -480,12 +480,22 @@ __device__ uint64_t cut_bucket(Shared& sh, Row<T>& r, uint32_t b, uint64_t above
     }
     sh.sub[tid] = 0;
     __syncthreads();
+    uint64_t hi = 0, lo = ~0ull;
 #pragma unroll
     for (int e = 0; e < P; ++e)
       if (left[e]) {
-        atomicMax((unsigned long long*)&sh.most, c[e]);
-        atomicMin((unsigned long long*)&sh.least, c[e]);
+        hi = max(hi, c[e]);
+        lo = min(lo, c[e]);
       }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      hi = max(hi, (uint64_t)__shfl_xor((unsigned long long)hi, o));
+      lo = min(lo, (uint64_t)__shfl_xor((unsigned long long)lo, o));
+    }
+    if (lane == 0) {
+      atomicMax((unsigned long long*)&sh.most, hi);
+      atomicMin((unsigned long long*)&sh.least, lo);
+    }
     __syncthreads();
     const uint64_t most = sh.most, range = most - sh.least;  // not 0: entries differ
     const int shift = max(0, 54 - __builtin_clzll(range));
