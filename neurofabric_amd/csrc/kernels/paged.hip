@@ -71,7 +71,13 @@ __global__ __launch_bounds__(256) void gather_any_kernel(PagedBatch b, const uin
 // kPieces pieces a lane are loaded before the row's place is looked up, so the two
 // latencies overlap.  I8: the 8 (f32) or 4 (f16) lanes of 32 elements find their
 // largest together.
+// SPREAD, for batches too small to fill the chip: a wave takes 64 pieces of K or of V
+// (blockIdx.y: 2 slice + which), which cuts the instructions that one after the other
+// make up such a call (an 80-row I8 append with the attention after it: 39 us, 37
+// spread); at large ones more waves look the same rows up (65536 positions read back:
+// 82 us and 88).
 constexpr int kPieces = 2;
+constexpr uint32_t kSpreadRows = 512;
 
 template <typename T>
 struct Piece {
@@ -98,7 +104,7 @@ __device__ __forceinline__ void put_codes(typename Piece<T>::type x, uint8_t* co
   if (first) *scale = d;
 }
 
-template <typename T, PoolType PT>
+template <typename T, PoolType PT, bool SPREAD>
 __global__ __launch_bounds__(256) void append_kernel(PagedBatch b, const T* __restrict__ kn, const T* __restrict__ vn,
                                                      uint8_t* __restrict__ kp, uint8_t* __restrict__ vp) {
   constexpr uint32_t E = Piece<T>::kElems;
@@ -108,16 +114,22 @@ __global__ __launch_bounds__(256) void append_kernel(PagedBatch b, const T* __re
   const uint32_t per_head = b.dim / E, pieces = b.n_kv * per_head;
   const vec* ks = reinterpret_cast<const vec*>(kn) + (uint64_t)row * pieces;
   const vec* vs = reinterpret_cast<const vec*>(vn) + (uint64_t)row * pieces;
-  vec kx[kPieces], vx[kPieces];
+  constexpr int P = SPREAD ? 1 : kPieces;
+  const uint32_t first = SPREAD ? blockIdx.y / 2 * 64 : 0, last = SPREAD ? min(first + 64, pieces) : pieces;
+  vec kx[P], vx[P];
   auto load = [&](uint32_t u0) {
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
+    for (int i = 0; i < P; ++i) {
       const uint32_t u = u0 + 64 * i + lane < pieces ? u0 + 64 * i + lane : pieces - 1;
-      kx[i] = ks[u];
-      vx[i] = vs[u];
+      if (SPREAD) {
+        kx[i] = (blockIdx.y & 1 ? vs : ks)[u];
+      } else {
+        kx[i] = ks[u];
+        vx[i] = vs[u];
+      }
     }
   };
-  load(0);
+  load(first);
   uint32_t seq;
   int64_t pos;
   if (!find_row_wave(b, row, seq, pos)) return;  // uniform
@@ -125,31 +137,32 @@ __global__ __launch_bounds__(256) void append_kernel(PagedBatch b, const T* __re
   if (phys == ~0u) return;
   const uint32_t slot = (uint32_t)pos % b.block_size;
   const uint64_t page = nfhip::page_bytes(PT, (uint64_t)b.block_size * b.dim), block = (uint64_t)phys * b.n_kv * page;
-  for (uint32_t u0 = 0; u0 < pieces; u0 += 64 * kPieces) {
-    if (u0) load(u0);
+  uint8_t* const p0 = SPREAD && (blockIdx.y & 1) ? vp : kp;
+  for (uint32_t u0 = first; u0 < last; u0 += 64 * P) {
+    if (u0 != first) load(u0);
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
+    for (int i = 0; i < P; ++i) {
       const uint32_t u = u0 + 64 * i + lane;
       const uint32_t head = u / per_head, d = (u - head * per_head) * E;
       const uint64_t at = block + head * page;
       if constexpr (PT != PoolType::I8) {
         if (u >= pieces) break;
         const uint64_t to = at + (uint64_t)(slot * b.dim + d) * sizeof(T);
-        *reinterpret_cast<vec*>(kp + to) = kx[i];
-        *reinterpret_cast<vec*>(vp + to) = vx[i];
+        *reinterpret_cast<vec*>(p0 + to) = kx[i];
+        if (!SPREAD) *reinterpret_cast<vec*>(vp + to) = vx[i];
       } else {
         if (u0 + 64 * i >= pieces) break;  // uniform: groups of 32 elements are never split
         const uint32_t el = slot * b.dim + d;
         const uint64_t sc = at + (uint64_t)b.block_size * b.dim + el / 16;
         if (u >= pieces) continue;
-        put_codes<T>(kx[i], kp + at + el, reinterpret_cast<half_t*>(kp + sc), d % 32 == 0);
-        put_codes<T>(vx[i], vp + at + el, reinterpret_cast<half_t*>(vp + sc), d % 32 == 0);
+        put_codes<T>(kx[i], p0 + at + el, reinterpret_cast<half_t*>(p0 + sc), d % 32 == 0);
+        if (!SPREAD) put_codes<T>(vx[i], vp + at + el, reinterpret_cast<half_t*>(vp + sc), d % 32 == 0);
       }
     }
   }
 }
 
-template <typename T, PoolType PT>
+template <typename T, PoolType PT, bool SPREAD>
 __global__ __launch_bounds__(256) void gather_kernel(PagedBatch b, const uint8_t* __restrict__ kp,
                                                      const uint8_t* __restrict__ vp, T* __restrict__ ko,
                                                      T* __restrict__ vo) {
@@ -165,22 +178,29 @@ __global__ __launch_bounds__(256) void gather_kernel(PagedBatch b, const uint8_t
   const uint32_t per_head = b.dim / E, pieces = b.n_kv * per_head;
   vec* kd = reinterpret_cast<vec*>(ko) + (uint64_t)row * pieces;
   vec* vd = reinterpret_cast<vec*>(vo) + (uint64_t)row * pieces;
+  constexpr int P = SPREAD ? 1 : kPieces, W = SPREAD ? 1 : 2;  // pieces a lane, and K and V of each
+  const uint32_t first = SPREAD ? blockIdx.y / 2 * 64 : 0, last = SPREAD ? min(first + 64, pieces) : pieces;
+  vec* const d0 = SPREAD && (blockIdx.y & 1) ? vd : kd;
+  const uint8_t* const p0 = SPREAD && (blockIdx.y & 1) ? vp : kp;
   if (phys == ~0u) {
-    for (uint32_t u = lane; u < pieces; u += 64) kd[u] = vd[u] = vec{};
+    for (uint32_t u = first + lane; u < last; u += 64) {
+      d0[u] = vec{};
+      if (!SPREAD) vd[u] = vec{};
+    }
     return;
   }
   const uint32_t slot = (uint32_t)pos % b.block_size;
   const uint64_t page = nfhip::page_bytes(PT, (uint64_t)b.block_size * b.dim), block = (uint64_t)phys * b.n_kv * page;
-  for (uint32_t u0 = 0; u0 < pieces; u0 += 64 * kPieces) {
-    vec x[kPieces][2];
+  for (uint32_t u0 = first; u0 < last; u0 += 64 * P) {
+    vec x[P][W];
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
+    for (int i = 0; i < P; ++i) {
       const uint32_t u = u0 + 64 * i + lane < pieces ? u0 + 64 * i + lane : pieces - 1;
       const uint32_t head = u / per_head, el = slot * b.dim + (u - head * per_head) * E;
       const uint64_t at = block + head * page;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint8_t* p = (j ? vp : kp) + at;
+      for (int j = 0; j < W; ++j) {
+        const uint8_t* p = (j ? vp : p0) + at;
         if constexpr (PT != PoolType::I8) {
           x[i][j] = *reinterpret_cast<const vec*>(p + (uint64_t)el * sizeof(T));
         } else {
@@ -197,11 +217,11 @@ __global__ __launch_bounds__(256) void gather_kernel(PagedBatch b, const uint8_t
       }
     }
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
+    for (int i = 0; i < P; ++i) {
       const uint32_t u = u0 + 64 * i + lane;
-      if (u < pieces) {
-        kd[u] = x[i][0];
-        vd[u] = x[i][1];
+      if (u < last) {
+        d0[u] = x[i][0];
+        if (!SPREAD) vd[u] = x[i][W - 1];
       }
     }
   }
@@ -216,10 +236,19 @@ bool pieces_fit(const PagedBatch& b, const void* k, const void* v, const void* k
          (PT != PoolType::I8 || nfhip::page_bytes(PT, (uint64_t)b.block_size * b.dim) % 8 == 0);
 }
 
+// Slices of 64 pieces in a row.
+template <typename T>
+uint32_t slices(const PagedBatch& b) {
+  return (b.n_kv * (b.dim / Piece<T>::kElems) + 63) / 64;
+}
+
 template <typename T, PoolType PT>
 hipError_t append(const PagedBatch& b, const void* kn, const void* vn, void* kp, void* vp, hipStream_t s) {
   if (pieces_fit<T, PT>(b, kn, vn, kp, vp)) {
-    append_kernel<T, PT><<<dim3((b.rows + 3) / 4), 256, 0, s>>>(b, (const T*)kn, (const T*)vn, (uint8_t*)kp, (uint8_t*)vp);
+    const bool spread = b.rows <= kSpreadRows && slices<T>(b) <= 32767;  // the grid's y ends at 65535
+    auto* kernel = spread ? append_kernel<T, PT, true> : append_kernel<T, PT, false>;
+    kernel<<<dim3((b.rows + 3) / 4, spread ? 2 * slices<T>(b) : 1), 256, 0, s>>>(b, (const T*)kn, (const T*)vn,
+                                                                                 (uint8_t*)kp, (uint8_t*)vp);
     return hipGetLastError();
   }
   const uint64_t n = (uint64_t)b.rows * b.n_kv * (PT == PoolType::I8 ? b.dim / 32 : b.dim);
@@ -231,7 +260,10 @@ hipError_t append(const PagedBatch& b, const void* kn, const void* vn, void* kp,
 template <typename T, PoolType PT>
 hipError_t gather(const PagedBatch& b, const void* kp, const void* vp, void* ko, void* vo, hipStream_t s) {
   if (pieces_fit<T, PT>(b, ko, vo, kp, vp)) {
-    gather_kernel<T, PT><<<dim3((b.rows + 3) / 4), 256, 0, s>>>(b, (const uint8_t*)kp, (const uint8_t*)vp, (T*)ko, (T*)vo);
+    const bool spread = b.rows <= kSpreadRows && slices<T>(b) <= 32767;  // the grid's y ends at 65535
+    auto* kernel = spread ? gather_kernel<T, PT, true> : gather_kernel<T, PT, false>;
+    kernel<<<dim3((b.rows + 3) / 4, spread ? 2 * slices<T>(b) : 1), 256, 0, s>>>(b, (const uint8_t*)kp,
+                                                                                 (const uint8_t*)vp, (T*)ko, (T*)vo);
     return hipGetLastError();
   }
   const uint64_t n = (uint64_t)b.rows * b.n_kv * b.dim;
