@@ -263,6 +263,17 @@ struct Rows {
     }
   }
   __device__ __forceinline__ uint64_t have() const { return valid; }
+  // The row of a key of the first two groups that differs between lanes, and its scales.
+  // (Lanes exchange here: no branch around the exchange may leave one out.)
+  __device__ __forceinline__ const uint8_t* row_of(const uint8_t* pool, uint32_t r) const {
+    if constexpr (UNI) return pool + (r < 16 ? base[0] : base[1]) + (r & 15) * kRow;
+    else return pool + shfl64(off, r);
+  }
+  __device__ __forceinline__ const half_t* scale_of(const uint8_t* pool, uint32_t r) const {
+    if constexpr (UNI)
+      return reinterpret_cast<const half_t*>(pool + (r < 16 ? base[0] + scales[0] : base[1] + scales[1]) + (r & 15) * (DD / 16));
+    else return reinterpret_cast<const half_t*>(pool + shfl64(off, r) + (uint32_t)__shfl((int)sc, r));
+  }
   // The row of key 16 h + r, and its scales.
   __device__ __forceinline__ const uint8_t* row(const uint8_t* pool, int h, uint32_t r) const {
     if constexpr (UNI) return pool + base[h] + r * kRow;
@@ -447,8 +458,8 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
         vraw[u] = *reinterpret_cast<const u32x4*>(rows.row(c.v, h, r - 16 * h) + 16 * col);
         if constexpr (I8) vd[u] = rows.scale(c.v, h, r - 16 * h)[col / 2];
       } else {
-        vraw[u] = *reinterpret_cast<const u32x4*>((r < 16 ? rows.row(c.v, 0, r) : rows.row(c.v, 1, r - 16)) + 16 * col);
-        if constexpr (I8) vd[u] = (r < 16 ? rows.scale(c.v, 0, r) : rows.scale(c.v, 1, r - 16))[col / 2];
+        vraw[u] = *reinterpret_cast<const u32x4*>(rows.row_of(c.v, r) + 16 * col);
+        if constexpr (I8) vd[u] = rows.scale_of(c.v, r)[col / 2];
       }
     }
   };

@@ -248,6 +248,71 @@ def test_attention(provider, act, pool, seqs, heads, kv, dim, bs):
     check_attention(provider, rng, batch, act, pool, heads, kv, dim)
 
 
+MORE = [  # block sizes beside powers of two, KV heads beside divisors of 8, many sequences, few and many splits of the keys
+    ([(200, 150), (90, 3)], 10, 5, 128, 48),
+    ([(200, 150), (90, 3)], 6, 3, 64, 80),
+    ([(300, 140)], 6, 6, 128, 128),
+    ([(300, 140)], 16, 16, 64, 16),
+    ([(130, 129), (40, 1)], 6, 3, 96, 8),
+    ([(130, 129), (40, 1), (9, 9)], 8, 2, 96, 64),
+    ([(i % 40 + 1, 1) for i in range(150)], 4, 2, 64, 16),
+    ([(i + 5, i % 5) for i in range(80)] + [(200, 190)], 8, 2, 128, 16),
+    ([(600 + 7 * i, 1) for i in range(20)], 4, 4, 64, 16),
+    ([(1500, 2), (700, 3), (40, 1)], 32, 8, 128, 32),
+    ([(1200, 120)], 2, 2, 128, 16),
+    ([(256, 256)], 1, 1, 64, 16),
+    ([(64, 1), (65, 1), (63, 1), (128, 32), (32, 32)], 1, 1, 128, 16),
+]
+
+
+@pytest.mark.parametrize("act,pool", ACT_POOL)
+@pytest.mark.parametrize("seqs,heads,kv,dim,bs", MORE)
+def test_attention_more(provider, act, pool, seqs, heads, kv, dim, bs):
+    rng = np.random.default_rng(heads * 100 + dim + len(seqs) + bs)
+    batch = ref.Batch(rng, seqs, bs, width=3, behind=1)
+    check_attention(provider, rng, batch, act, pool, heads, kv, dim)
+
+
+@pytest.mark.parametrize("act,pool", ACT_POOL)
+@pytest.mark.parametrize("dim,bs", [(64, 16), (128, 24)])
+def test_rows_of_no_sequence(provider, act, pool, dim, bs):
+    """Starts below zero, past the rows, or decreasing make no sequence; lengths below zero or past the table no keys: the
+    other sequences come out as they are, and no other row is touched."""
+    rng = np.random.default_rng(21)
+    heads, kv = 4, 2
+    good = ref.Batch(rng, [(150, 60), (40, 2), (33, 33)], bs, behind=4)
+    bad = ref.Batch(rng, [(10, 1)] * 7, bs)
+    bad.blocks, bad.width = good.blocks, good.width
+    bad.table = np.full((7, good.width), ref.NONE, np.uint32)
+    bad.table[1], bad.table[3], bad.table[5] = good.table
+    bad.starts = np.array([-5, 0, 60, 60, 62, 62, 95, 1 << 30], np.int32)
+    bad.lens = np.array([100, 150, 3, 40, -7, 33, 1000], np.int32)
+    bad.rows = good.rows
+    pools = [ref.empty_pool(rng, pool, good.blocks, kv, bs, dim) for _ in range(2)]
+    q, was = rows_of(rng, act, good.rows, heads, dim), np.full((good.rows, heads, dim), 3.25, NP[act])
+    x = [rows_of(rng, act, good.rows, kv, dim) for _ in range(2)]
+    with Bufs(provider) as m:
+        kb, out, desc = [m.put(p) for p in pools], m.put(was), m.batch(bad)
+        pc = pc_of(bad, kv, dim, n_heads=heads)
+        provider.dispatch("paged_kv_append", [m.put(r) for r in x] + desc, kb, pc=pc)
+        provider.dispatch("flash_attention_paged_chunk", [m.put(q)] + kb + desc, [out], pc=pc)
+        got = out.read(NP[act], q.size).reshape(q.shape)
+        held = [b.read(np.uint8, p.nbytes) for b, p in zip(kb, pools)]
+        # decreasing starts, far lengths: nothing but ends in time
+        wild = [m.put(bad.table), m.put(np.array([90, 80, 5, 70, 2, 2, 1, 0], np.int32)),
+                m.put(np.array([2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, 7, 9, 2 ** 31 - 1, 0], np.int32))]
+        provider.dispatch("flash_attention_paged_chunk", [m.put(q)] + kb + wild, [m.put(was)], pc=pc)
+        provider.synchronize()
+    ref.append(good, pool, dim, pools, x)
+    for h, p in zip(held, pools):
+        assert np.array_equal(h, p.reshape(-1).view(np.uint8))
+    want, err = ref.attention(good, pool, dim, heads, kv, pools, q, act)
+    mine = np.zeros(good.rows, bool)
+    mine[:95] = True
+    check(got[mine], want[mine], err[mine], (act, pool))
+    assert np.array_equal(got[~mine], was[~mine])
+
+
 @pytest.mark.parametrize("act,dim", [("f32", 40), ("f16", 40), ("f32", 33), ("f16", 1), ("f32", 200)])
 def test_attention_odd_head_dims(provider, act, dim):
     rng = np.random.default_rng(dim)

@@ -84,7 +84,63 @@ def test_sample(provider, n, dtype):
     check(provider, x, u, [h[:3] for h in how], [h[3] for h in how])
 
 
-@pytest.mark.parametrize("n", [5, 3000, 40000])
+@pytest.mark.parametrize("rows,n", [(3, 70000), (8, 131072), (300, 70001)])
+def test_cuts_of_every_size(provider, rows, n):
+    """top_k from one to nearly all with and without the other cuts, rows that are and are not spread over workgroups."""
+    rng = np.random.default_rng(n)
+    x = (rng.standard_normal((rows, n)) * 3).astype(np.float32)
+    ks = [1, 2, 63, 64, 65, 255, 256, 257, 300, 1024, 2047, 2048, 2049, 5000, 40000, n - 1, n, n + 5, 0]
+    ps = [1.0, 0.9, 0.5, 0.999999, 1e-6]
+    how = [(ks[(7 * i + 3) % len(ks)], ps[i % 5], [0.0, 0.0, 1e-7, 0.2][i % 4], [0.6, 1.0, 3.0][i % 3]) for i in range(rows)]
+    check(provider, x, rng.random(rows).astype(np.float32), [(t, p, m) for _, p, m, t in how], [h[0] for h in how])
+
+
+def test_one_more_row_after_another(provider):
+    """The same rows alone, together and again give the same tokens."""
+    rng = np.random.default_rng(2)
+    n = 66000
+    x = (rng.standard_normal((5, n)) * 2).astype(np.float32)
+    u = rng.random(5).astype(np.float32)
+    params = np.array([[1.0, 0.99, 0.0], [0.7, 0.9, 0.0], [1.0, 1.0, 0.0], [1.0, 1.0, 0.1], [0.5, 0.8, 0.0]], np.float32)
+    k = np.array([0, 50, 0, 0, 3000], np.int32)
+    together = [draw(provider, x, u, params, k) for _ in range(3)]
+    for t in together[1:]:
+        assert np.array_equal(t[0], together[0][0]) and np.array_equal(t[1], together[0][1])
+    for r in range(5):
+        t, p = draw(provider, x[r:r + 1], u[r:r + 1], params[r:r + 1], k[r:r + 1])
+        assert t[0] == together[0][0][r] and p[0] == together[0][1][r]
+
+
+def test_captured(provider):
+    """A captured draw follows its buffers at each replay."""
+    from neurofabric_amd import hiprt
+    rng = np.random.default_rng(4)
+    rows, n = 3, 70000
+    bufs = [provider.alloc(abi.NF_DTYPE_F32, rows * n * 4), provider.alloc(abi.NF_DTYPE_F32, rows * 4),
+            provider.alloc(abi.NF_DTYPE_F32, rows * 12), provider.alloc(abi.NF_DTYPE_I32, rows * 4)]
+    outs = [provider.alloc(abi.NF_DTYPE_I32, rows * 4), provider.alloc(abi.NF_DTYPE_F32, rows * 4)]
+    pc = push_constants(seq_len=rows, N=n)
+    tasks = (abi.nf_task_desc * 1)(provider.task("sample_token", bufs, outs, pc=pc))
+    graph = hiprt.Graph(provider.stream(), lambda: provider.run_tasks(tasks))
+    for i in range(4):
+        x = (rng.standard_normal((rows, n)) * 2).astype(np.float32)
+        u = rng.random(rows).astype(np.float32)
+        params = np.array([[1.0, 0.9, 0.0], [0.8, 1.0, 0.01 * i], [0.9, 0.95, 0.0]], np.float32)
+        k = np.array([0, 0, 40 * i], np.int32)
+        for b, a in zip(bufs, (x, u, params, k)):
+            b.write(a)
+        graph.launch()
+        token, prob = outs[0].read(np.int32), outs[1].read(np.float32)
+        for r in range(rows):
+            want, p = reference(x[r], u[r], *params[r], int(k[r]))
+            assert token[r] == want and abs(float(prob[r]) - p) <= 2.0 ** -24 * p + 2.0 ** -39
+        provider.dispatch("sample_token", bufs, outs, pc=pc)
+        assert np.array_equal(outs[0].read(np.int32), token)
+    for b in bufs + outs:
+        b.release()
+
+
+@pytest.mark.parametrize("n", [5, 3000, 40000, 70000])
 def test_ties(provider, n):
     """Few distinct values: the lowest indices stay at every cut."""
     rng = np.random.default_rng(n)
