@@ -38,7 +38,9 @@
  *     seq_len counts every row, M the KV heads (M = 0 in the attention: one per
  *     query head).  Push constants: seq_len, n_heads (attention), head_dim (at
  *     most 256), M, N, K, window_size = block_size (0: 16), max_seq_len = a
- *     bound on LENS (0: N * block_size; longer sequences are cut off there).  A
+ *     bound on LENS (0: N * block_size; longer sequences are cut off there).  At
+ *     most 2^22 rows, 65535 sequences, KV heads and heads, 65536 positions a
+ *     block.  A
  *     tight bound lets the attention launch fewer workgroups.
  *     Pools are [block][M][block_size][head_dim] of the rows' dtype, or I8: the
  *     page of one KV head in a block is then block_size * head_dim int8 codes
@@ -51,10 +53,12 @@
  *     The chunk's own keys have to be in the cache (paged_kv_append before it).
  *     O may be Q's buffer; other overlaps of outputs with operands are not
  *     allowed.  Tables, starts and lengths are read when the op runs, so a
- *     captured op follows their contents at each replay.  A position below 0 or
+ *     captured op follows their contents at each replay; they must not change
+ *     while it runs.  A position below 0 or
  *     past the bound, or in a block that the pools do not hold, has no storage:
  *     append skips it, gather gives zeros for it, attention counts no key; a row
- *     without any key gives zeros.  Rows of no sequence are left as they are.  A
+ *     without any key gives zeros.  Rows of no sequence are left as they are, and
+ *     so are those of a sequence whose rows are not all within seq_len.  A
  *     slot that several rows of one append name ends with any of their values.
  *   sample_token        LOGITS, U, PARAMS, TOP_K -> TOKEN, PROB
  *     LOGITS [seq_len, N] F32 or F16; U f32[seq_len], random numbers of [0, 1);
@@ -66,7 +70,7 @@
  *     least top_p of theirs (>= 1: all; at least one token); of those the ones
  *     with w >= min_p 2^40.  With S the sum of what stays, TOKEN is the first in
  *     index order whose running sum exceeds floor(U S), and PROB = w / S.  T <= 0
- *     takes the first largest logit.  +inf counts as the largest finite value;
+ *     takes the first largest logit; T is taken as at most 1e30.  +inf counts as the largest finite value;
  *     NaN and -inf are never drawn; a row of nothing else gives -1 and 0.  N is
  *     at most 2^22.
  * These ops may use the provider's workspace: replays of graphs that hold them

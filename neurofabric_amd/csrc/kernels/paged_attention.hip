@@ -777,7 +777,7 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(Chunk c) {
 // Workgroup x runs on XCD x % 8, and each XCD has its own L2: the tiles of a KV head go
 // to one XCD where heads are a multiple of 8, else in turn to the XCDs that share the
 // head (in halves of the tiles, one XCD had the long sequences: 165 us for three
-// ragged f32 chunks, Y so).
+// ragged f32 chunks, 133 so).
 __device__ __forceinline__ bool wide_tile(const Chunk& c, uint32_t& kvh, uint32_t& idx) {
   const uint32_t xcd = blockIdx.x % 8, i = blockIdx.x / 8, n_kv = c.b.n_kv;
   uint32_t tile;
@@ -816,8 +816,8 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
   constexpr bool I8 = PT == PoolType::I8;
   constexpr int KS = DD / 16, DB = DD / 32, KP = DD + 8;
   // V rows 16 or 48 dwords past a multiple of 64: the 4 rows and 32 dims that 32 lanes
-  // of a transposing read touch then lie in different banks (KP halves: in 4 of them
-  // two share each, X us)
+  // of a transposing read touch then lie in different banks (in rows of KP, pairs
+  // of them share; 685 and 671 us at the size below)
   constexpr int VP = DD == 96 ? 96 : DD + 32;
   constexpr int VC = I8 ? 16 : 8;
   constexpr int CPR = DD / VC;

@@ -12,7 +12,7 @@
 //   3. of them those with w_i >= min_p 2^40.
 // With S the weights' sum of what stays, the token is the first in index order
 // whose running sum exceeds floor(u S); the probability returned is w_i / S.
-// T <= 0 takes the first largest logit.  A logit of +inf counts as the largest
+// T <= 0 takes the first largest logit; T is taken as at most 1e30.  A logit of +inf counts as the largest
 // finite value; NaN and -inf are never drawn, and a row of nothing else gives
 // token -1 with probability 0.
 #include "../launch.hpp"
@@ -28,6 +28,7 @@ constexpr int kList = 2048;     // candidates that are sorted in LDS
 constexpr int kSmallK = 256;    // top_k up to which the threads' largest logits bound the candidates
 constexpr int kAhead = 4;       // loads a lane has under way before it uses the first
 constexpr double kOne = 1099511627776.0;  // 2^40
+constexpr float kMostT = 1e30f;  // differences of logits past f32 then have no weight
 
 // Unsigned keys in the order of the logits; 0 for a logit that is never drawn.
 // Adding 0 makes -0 the same as +0.
@@ -79,7 +80,8 @@ struct Row {
 
   __device__ __forceinline__ Row(const T* logits, uint32_t row, uint32_t n_, const float* params, const int32_t* top_k)
       : x(logits + (uint64_t)row * n_), n(n_), cut(1), cut_at(n_) {
-    const float temp = params[3 * row], p = params[3 * row + 1], m = params[3 * row + 2];
+    const float t = params[3 * row], p = params[3 * row + 1], m = params[3 * row + 2];
+    const float temp = t > kMostT ? kMostT : t;
     const int32_t kk = top_k[row];
     greedy = !(temp > 0.0f);
     k = p <= 0.0f ? 1u : kk > 0 && (uint32_t)kk < n ? (uint32_t)kk : 0u;  // the shortest prefix is the first token

@@ -215,6 +215,7 @@ nf_status plan_paged_batch(const nf_tensor_desc* const* dense, uint32_t n_dense,
   if (lp.n_kv == 0) return fail(why, "M (KV heads) must be non-zero");
   if (lp.n_kv > 65535 || lp.rows > 65535 || lp.block_size > 65536)
     return fail(why, "more than 65535 KV heads or sequences, or 65536 positions a block");
+  if (lp.seq_len > (1u << 22)) return fail(why, "more than 2^22 rows");
   EType act;
   if (!float_type(dense[0]->dtype, &act)) return fail(why, "rows must be F32 or F16");
   for (uint32_t i = 1; i < n_dense; ++i)

@@ -22,6 +22,7 @@ def reference(x, u, temp, top_p, min_p, k):
     if not len(live):
         return -1, 0.0
     top = x[live].max()
+    temp = min(temp, np.float32(1e30))
     if not temp > 0:
         return int(live[np.argmax(x[live])]), 1.0
     order = live[np.argsort(-x[live], kind="stable")]
@@ -181,6 +182,18 @@ def test_not_finite(provider):
     params = np.tile(np.float32([0.9, 0.9, 0.01]), (12, 1))
     params[8:] = [[np.nan, 0.9, 0.0], [-1, 1, 0], [1, np.nan, np.nan], [np.inf, 1, 2.0]]
     check(provider, x, rng.random(12).astype(np.float32), params, [0, 5, 10, 0, 3, 50, 0, 0, 0, 0, -4, 2000])
+
+
+def test_extreme_temperatures_and_logits(provider):
+    """Differences that overflow f32, temperatures whose products and quotients do."""
+    big = np.finfo(np.float32).max
+    base = np.array([big, -big, 0.0, np.nan, -np.inf, 1.0, big, -1.0, 1e-45, 3e38], np.float32)
+    temps = [np.inf, 3.4e38, 1e30, 1e25, 1.0, 1e-30, 1e-45]
+    x = np.stack([base] * len(temps) + [np.where(np.abs(base) > 2, np.float32(0.5), base)] * len(temps))
+    x[len(temps):, [3, 4]] = np.nan, -np.inf
+    u = np.linspace(0.05, 0.95, len(x)).astype(np.float32)
+    for p, k in ((1.0, 0), (0.7, 0), (1.0, 3), (0.5, 5)):
+        check(provider, x, u, [(t, p, 0.0) for t in temps * 2], [k] * len(x))
 
 
 @pytest.mark.parametrize("dtype", [np.float32, np.float16])

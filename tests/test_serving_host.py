@@ -81,6 +81,7 @@ def test_batch_refusals(lib, call):
     refused(call, lib, pc=args(window_size=65537, **heads), match="65536")
     refused(call, lib, pc=args(seq_len=T + 1, **heads))
     refused(call, lib, pc=args(seq_len=0xFFFFFFFF, **heads))
+    refused(call, lib, pc=args(seq_len=(1 << 22) + 1, **heads), match="rows")
     refused(call, lib, bat=[desc(I32, S * W * 4 - 4)] + batch()[1:], match="tables")
     refused(call, lib, bat=[batch()[0], desc(I32, S * 4), batch()[2]], match="starts")
     refused(call, lib, bat=batch()[:2] + [desc(I32, S * 4 - 4)], match="lengths")
