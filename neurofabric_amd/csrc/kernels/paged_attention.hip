@@ -1311,23 +1311,6 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
 #pragma unroll
       for (int s = 0; s < DG; ++s) sc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], qb[s], sc[j], 0, 0, 0);
     }
-    float4v va[2][4][NH];
-    bool bad = false;
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int h = 0; h < NH; ++h) {
-          if constexpr (I8) va[j][i][h] = codes4_f32(vc[j][i][h], (float)vd[j][i][h]);
-          else va[j][i][h] = vf[j][i][h];
-          if constexpr (!OPEN) {
-            if (!((seen >> (16 * j + 4 * g + i)) & 1)) va[j][i][h] = float4v{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) bad = bad || !__builtin_isfinite(va[j][i][h][e]);
-          }
-        }
-    const bool alu = !OPEN && __ballot(bad) != 0;
     __builtin_amdgcn_sched_barrier(0);
     if (OPEN) next();
     float top = -INFINITY;
@@ -1358,19 +1341,50 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
         sum += pv[j][i];
       }
     l += sum4(sum);
+    // a key's values, zeros without a row
+    auto value = [&](int j, int i, int h) {
+      float4v x;
+      if constexpr (I8) x = codes4_f32(vc[j][i][h], (float)vd[j][i][h]);
+      else x = vf[j][i][h];
+      if (!OPEN && !((seen >> (16 * j + 4 * g + i)) & 1)) x = float4v{0.f, 0.f, 0.f, 0.f};
+      return x;
+    };
+    bool alu = false;
+    if constexpr (!OPEN) {
+      // (again: they do not fit the registers beside the rest of a masked tile)
+      __builtin_amdgcn_sched_barrier(0);
+      fetch_v();
+      bool bad = false;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int h = 0; h < NH; ++h) {
+            const float4v x = value(j, i, h);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) bad = bad || !__builtin_isfinite(x[e]);
+          }
+      alu = __ballot(bad) != 0;
+    }
     if (!alu) {
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int d = 0; d < NB; ++d)
-            ot[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(va[j][i][d / 4][d % 4], pv[j][i], ot[d], 0, 0, 0);
+          for (int h = 0; h < NH; ++h) {
+            const float4v x = value(j, i, h);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              ot[4 * h + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], pv[j][i], ot[4 * h + e], 0, 0, 0);
+          }
     } else {
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
+#pragma unroll 1
           for (int gk = 0; gk < 4; ++gk) {
             const int k = 16 * j + 4 * gk + i;
             const float p = __shfl(pv[j][i], 16 * gk + n);
@@ -1381,6 +1395,7 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
             for (int d = 0; d < NB; ++d)
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
+                if (d % 2 == 0 && r == 0) __builtin_amdgcn_sched_barrier(0);
                 const uint32_t dim = 64 * (d / 4) + 16 * g + 4 * r + d % 4;
                 if (dim < DD) ot[d][r] += p * page_value<PT>(c.b, page, slot, dim);
               }
@@ -1389,7 +1404,7 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
     if (!OPEN) next();
     // a tile of values and the next one's do not fit the registers together
     __builtin_amdgcn_sched_barrier(0);
-    if (t0 + 128 < end) fetch_v();
+    if (OPEN && t0 + 128 < end) fetch_v();
   };
   // The open tiles first, as in the f16 kernel.
   while (t0 < end && (uint32_t)rows.have() == ~0u && t0 + 31 <= pos_lo) {  // uniform
