@@ -1673,9 +1673,19 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_f32_kernel(Chunk c) {
 
 // ---- launch ------------------------------------------------------------------------------
 
-// Query rows of a sequence up to which the narrow kernel takes it where the wide
-// kernel runs too.
-constexpr uint32_t kNarrowRows = 32;
+// Query rows of a sequence, on average, up to which the narrow kernel takes the whole
+// batch.  It reads the cache once per 16 or 32 rows and splits it finely; the wide one
+// once per 128 (f32: 64), and converts I8 tiles for all of them.  Narrow and wide, 8
+// sequences of 4096 positions, 8 KV heads of 128:
+//   f16, 64 rows 52 and 68 us, 96 rows 71 and 65;
+//   I8,  64 rows 36 and 98 us, 96 rows 51 and 87, 128 rows 83 (wide);
+//   f32, 36 rows 144 and 100 us, 64 rows 155 and 111; one of 8192, 32 rows: 28 and 33.
+template <typename T, PoolType PT>
+constexpr uint32_t kNarrowRows = std::is_same<T, float>::value ? 32 : PT == PoolType::I8 ? 96 : 64;
+// Where the wide kernel runs, the sequences that go to the narrow one all the same; more
+// wait for a kernel with too few workgroups (three sequences of up to 96 rows: 42 us, and
+// 54 with the narrow kernel taking those of up to 64).
+constexpr uint32_t kFewRows = 32;
 
 template <typename T, PoolType PT, int DD, bool UNI>
 hipError_t chunk_mfma_at(const PagedBatch& b, uint32_t n_heads, const void* q, const void* kp, const void* vp, void* out,
@@ -1690,21 +1700,29 @@ hipError_t chunk_mfma_at(const PagedBatch& b, uint32_t n_heads, const void* q, c
   c.group = n_heads / b.n_kv;
   c.scale_log2 = 1.4426950408889634f / sqrtf((float)DD);
   const uint64_t rows = (uint64_t)b.rows * c.group;  // query rows per KV head
-  // The wide kernel where sequences have more than kNarrowRows query rows on
-  // average; the narrow one for all of them, or for the short ones among them.
-  // (Lengths are known on the device only: each kernel skips the sequences that
-  // are the other's.)
-  const bool wide = rows > (uint64_t)kNarrowRows * b.n_seqs;
+  // Lengths are known on the device only: each kernel skips the sequences that are the
+  // other's.
+  const bool wide = rows > (uint64_t)kNarrowRows<T, PT> * b.n_seqs;
   const bool narrow = !wide || b.n_seqs > 1;
   constexpr bool F16 = std::is_same<T, half_t>::value;
   constexpr uint32_t kWideRows = F16 ? 128 : 64;  // a wide workgroup's query rows
+  // A narrow workgroup takes 16 rows, or 32 where sequences have more, which then read
+  // the cache once (16 I8 sequences of 20 rows behind up to 4096 positions, with the
+  // append before it: 48 and 37 us; 64 sequences of 4 rows behind up to 8192, f16:
+  // with 16 rows 262 us, with 32 279).
   const uint32_t nt = F16 && (wide || rows > 16ull * b.n_seqs) ? 2 : 1;
-  // Splits of the keys: enough workgroups for the chip, at least kMinKeys keys each,
-  // and partials that fit the workspace.
-  const uint64_t most_tiles = wide ? rows / kWideRows + b.n_seqs : rows / (16 * nt) + b.n_seqs;
-  const uint64_t units = (wide ? most_tiles : rows / (16 * nt) > b.n_seqs ? rows / (16 * nt) : b.n_seqs) * b.n_kv;
-  const uint32_t target = wide ? 1024 : 512, min_keys = wide ? 256 : 128;
-  uint64_t splits = wide && units >= 1024 ? 1 : (target + units - 1) / units;
+  const uint64_t per = wide ? kWideRows : 16 * nt, mean = (rows + b.n_seqs - 1) / b.n_seqs;
+  const uint64_t most_tiles = rows / per + b.n_seqs;
+  // Splits of the keys, with partials that fit the workspace.  Narrow: two workgroups per
+  // CU, not one more (20 sequences of 4096 positions in I8: 41 us; rounded up, a third
+  // of the CUs have a third workgroup, 50).  Wide: four where no sequence is cut short by
+  // the mask or its length, rounded up (three ragged f32 chunks: 117 us, rounded down
+  // 129, with two 129); none where the tiles alone are as many.
+  const uint64_t units = b.n_seqs * ((mean + per - 1) / per) * b.n_kv;
+  uint64_t splits = wide ? (1024 + units - 1) / units : units < 512 ? 512 / units : 1;
+  // fewer keys a split, and reading the partials costs more than they save (one sequence of
+  // 28 rows behind 8192 positions: 18 us, with 128 keys 22)
+  const uint32_t min_keys = wide || nt == 2 ? 256 : 128;
   const uint64_t most = ws.part ? ws.part_floats / ((uint64_t)b.rows * n_heads * (DD + 4)) : 1;
   if (splits > most) splits = most ? most : 1;
   uint64_t keys = splits > 1 ? (b.limit + splits - 1) / splits : b.limit;
@@ -1717,7 +1735,7 @@ hipError_t chunk_mfma_at(const PagedBatch& b, uint32_t n_heads, const void* q, c
   c.acc = ws.part + ((uint64_t)b.rows * n_heads * c.splits * 2 + 3) / 4 * 4;
   if (wide) {
     c.tiles = (uint32_t)most_tiles;
-    c.lo = narrow ? kNarrowRows : 0;
+    c.lo = narrow ? kFewRows : 0;
     c.hi = ~0ull;
     const dim3 grid(wide_grid(c.tiles, b.n_kv), c.splits);
     if constexpr (F16) chunk_wide_kernel<PT, DD, UNI><<<grid, 256, 0, s>>>(c);
@@ -1725,8 +1743,8 @@ hipError_t chunk_mfma_at(const PagedBatch& b, uint32_t n_heads, const void* q, c
   }
   if (narrow) {
     c.lo = 0;
-    c.hi = wide ? kNarrowRows : ~0ull;
-    c.tiles = (uint32_t)(!wide ? most_tiles : b.n_seqs * (F16 ? 1 : kNarrowRows / 16));
+    c.hi = wide ? kFewRows : ~0ull;
+    c.tiles = (uint32_t)(wide ? b.n_seqs * (kFewRows / (16 * nt)) : most_tiles);
     const dim3 grid(c.splits * c.tiles, b.n_kv);
     if constexpr (!F16) chunk_narrow_f32_kernel<PT, DD, UNI><<<grid, 256, 0, s>>>(c);
     else if (nt == 2) chunk_narrow_kernel<PT, DD, 2, UNI><<<grid, 256, 0, s>>>(c);

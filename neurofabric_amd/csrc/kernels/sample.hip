@@ -12,9 +12,9 @@
 //   3. of them those with w_i >= min_p 2^40.
 // With S the weights' sum of what stays, the token is the first in index order
 // whose running sum exceeds floor(u S); the probability returned is w_i / S.
-// T <= 0 takes the first largest logit; T is taken as at most 1e30.  A logit of +inf counts as the largest
-// finite value; NaN and -inf are never drawn, and a row of nothing else gives
-// token -1 with probability 0.
+// T <= 0 takes the first largest logit; T is taken as at most 1e30.  A logit of +inf
+// counts as the largest finite value; NaN and -inf are never drawn, and a row of
+// nothing else gives token -1 with probability 0.
 #include "../launch.hpp"
 #include "common.hpp"
 
@@ -26,7 +26,7 @@ constexpr int kBins = 2048;     // digits of select()
 constexpr int kBuckets = 1024;  // buckets of the histogram of a row's logits
 constexpr int kList = 2048;     // candidates that are sorted in LDS
 constexpr int kSmallK = 256;    // top_k up to which the threads' largest logits bound the candidates
-constexpr int kAhead = 4;       // loads a lane has under way before it uses the first
+constexpr int kAhead = 2;       // loads a lane has under way while it uses as many
 constexpr double kOne = 1099511627776.0;  // 2^40
 constexpr float kMostT = 1e30f;  // differences of logits past f32 then have no weight
 
@@ -122,10 +122,11 @@ struct Row {
 
 // f(logits, first index) for groups of 16 bytes of the elements lo .. hi - 1, by the
 // threads in any order; what is past hi in the last group is NaN, which is never
-// drawn.  Rows start anywhere, and the loads need no alignment.  kAhead loads are under way at a time (a
-// pass is bound by their latency otherwise), moved along by registers: an unrolled
-// loop would be fetched from memory once for every launch, which costs more than it
-// runs (one row of 32000: 35 us, and 23 with the short loop).
+// drawn.  Rows start anywhere, and the loads need no alignment.  kAhead loads are under
+// way while the kAhead before them are used: a pass is bound by their latency
+// otherwise, and a longer body is itself fetched from memory once a launch (with 2, 4
+// and 8, a batch of 64 rows of 128256: 70, 72 and 74 us; one row of 32000: 12.6, 12.9
+// and 13.5).
 template <typename T>
 struct Group {
   static constexpr uint32_t kElems = 16 / sizeof(T);
@@ -186,11 +187,6 @@ __device__ __forceinline__ uint64_t lane64(uint64_t v, int lane) {
          (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane) << 32;
 }
 __device__ __forceinline__ uint64_t wave_sum64(uint64_t v) { return lane64(wave_scan64(v), 63); }
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
-  return v;
-}
 struct Shared {
   uint64_t mass[kBins];       // weights by bucket, or by index; select(): weights or counts by digit
   uint32_t count[kBuckets];   // tokens by bucket
@@ -538,7 +534,8 @@ __device__ uint64_t cut_bucket(Shared& sh, Row<T>& r, uint32_t b, uint64_t above
 
 // The token, from weights by index: sh.mass holds the sums over 2^shift indices each,
 // from index `lo` on.  One wave goes through those of the one that the draw falls in.
-// `t` below 0: drawn here, from the sum of all.
+// `drawn`: t is the draw, less what lies before `lo`, and `whole` the sum of all; else
+// both are formed here.
 template <typename T>
 __device__ void draw_from_bins(Shared& sh, const Row<T>& r, uint32_t lo, uint32_t hi, uint32_t shift, bool drawn, uint64_t t,
                                uint64_t whole, double u, int32_t* token, float* prob) {
@@ -935,10 +932,15 @@ template <typename T>
 hipError_t launch(const T* logits, const float* u, const float* params, const int32_t* top_k, int32_t* token, float* prob,
                   uint32_t rows, uint32_t n, const nfhip::Workspace& ws, hipStream_t s) {
   const uint64_t fits = ws.part ? ws.part_floats * sizeof(float) / sizeof(Part) : 0;
-  // Chunks of a row: enough workgroups for the chip; none where rows alone are, or rows are short.
-  uint32_t chunks = rows >= 256 || n <= 65536 ? 0 : (512 + rows - 1) / rows;
-  chunks = min(chunks, (n + 4095) / 4096);
-  if (chunks <= 1 || fits < (uint64_t)rows * chunks) chunks = 0;
+  // Chunks of a row, for two more launches: four workgroups of 512 per CU, at least four
+  // chunks a row and 4096 logits a chunk.  Rows of 131072 of every kind: 64 rows 72 us
+  // (149 without chunks), 256 rows 142 (180).  Short rows do without, and rows of up to 65536
+  // where they are few: a top_k then ends sooner without chunks (one row of 32000: 13 and
+  // 17 us), which the other kinds make up for only where a batch waits for its slowest row
+  // (by temperature 23 and 18, top_p 29 and 26; 16 rows of every kind 50 and 36).
+  uint64_t chunks64 = n > 65536 || (n > 16384 && rows >= 4) ? (1024 + rows - 1) / rows : 0;
+  if (chunks64) chunks64 = min(min(max(chunks64, (uint64_t)4), (uint64_t)(n + 4095) / 4096), fits / rows);
+  uint32_t chunks = chunks64 > 1 ? (uint32_t)chunks64 : 0;
   const uint32_t step = chunks ? ((n + chunks - 1) / chunks + 7) / 8 * 8 : n;
   if (chunks) chunks = (n + step - 1) / step;
   Part* parts = reinterpret_cast<Part*>(ws.part);
