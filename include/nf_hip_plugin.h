@@ -40,8 +40,9 @@
  *     most 256), M, N, K, window_size = block_size (0: 16), max_seq_len = a
  *     bound on LENS (0: N * block_size; longer sequences are cut off there).  At
  *     most 2^22 rows, 65535 sequences, KV heads and heads, 65536 positions a
- *     block.  A
- *     tight bound lets the attention launch fewer workgroups.
+ *     block.  A tight bound lets the attention launch fewer workgroups.
+ *     An I8 pool is read by the attention as f16 for f16 rows (code * scale
+ *     rounded once, as paged_kv_gather does), exactly for f32 rows.
  *     Pools are [block][M][block_size][head_dim] of the rows' dtype, or I8: the
  *     page of one KV head in a block is then block_size * head_dim int8 codes
  *     followed by block_size * head_dim / 32 fp16 scales (head_dim % 32 == 0).
@@ -70,9 +71,9 @@
  *     least top_p of theirs (>= 1: all; at least one token); of those the ones
  *     with w >= min_p 2^40.  With S the sum of what stays, TOKEN is the first in
  *     index order whose running sum exceeds floor(U S), and PROB = w / S.  T <= 0
- *     takes the first largest logit; T is taken as at most 1e30.  +inf counts as the largest finite value;
- *     NaN and -inf are never drawn; a row of nothing else gives -1 and 0.  N is
- *     at most 2^22.
+ *     takes the first largest logit; T is taken as at most 1e30.  +inf counts as
+ *     the largest finite value; NaN and -inf are never drawn; a row of nothing
+ *     else gives -1 and 0.  N is at most 2^22.
  * These ops may use the provider's workspace: replays of graphs that hold them
  * must not overlap each other or later dispatches (one stream does that).
  */

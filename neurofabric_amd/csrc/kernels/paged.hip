@@ -14,7 +14,8 @@ namespace nfk {
 namespace paged {
 
 // Any head_dim and alignment: a thread per element, or per 32 elements of an
-// I8 pool.  blockIdx.y: 0 = K, 1 = V.
+// I8 pool, each of which looks its row up, which is what bounds it (32768 rows of 8 heads
+// of 100 appended in f16 and read back: 682 us).  blockIdx.y: 0 = K, 1 = V.
 template <typename T, PoolType PT>
 __global__ __launch_bounds__(256) void append_any_kernel(PagedBatch b, const T* __restrict__ kn,
                                                          const T* __restrict__ vn, uint8_t* __restrict__ kp,
@@ -70,12 +71,16 @@ __global__ __launch_bounds__(256) void gather_any_kernel(PagedBatch b, const uin
 // 16-byte pieces of the dense rows (4 f32, 8 f16), a wave per row: K and V of up to
 // kPieces pieces a lane are loaded before the row's place is looked up, so the two
 // latencies overlap.  I8: the 8 (f32) or 4 (f16) lanes of 32 elements find their
-// largest together.
+// largest together.  Bound by HBM: four prompts of up to 2048 rows of 8 heads of 128
+// appended in f16, 55 MB in 9.6 us (the last-level cache holds them between calls), 32768 rows of f32 to
+// I8 in 76 us and back in 46 (512 MB in 119 together, 4.3 TB/s), 65536 of I8 to f16 in 82
+// (411 MB, 5.0 TB/s; a copy of 2 GiB reaches 4.9).  A step's few rows take 3 us each way,
+// the chain start - table - row.
 // SPREAD, for batches too small to fill the chip: a wave takes 64 pieces of K or of V
 // (blockIdx.y: 2 slice + which), which cuts the instructions that one after the other
-// make up such a call (an 80-row I8 append with the attention after it: 39 us, 37
-// spread); at large ones more waves look the same rows up (65536 positions read back:
-// 82 us and 88).
+// make up such a call (appended to I8 and read back: 4 rows 7.8 us, 7.2 spread; 512
+// rows 9.3 and 7.3); at large ones more waves look the same rows up (8192 rows: 30 us
+// and 33; 1024 rows, where either does: 9.6 and 8.7).
 constexpr int kPieces = 2;
 constexpr uint32_t kSpreadRows = 512;
 

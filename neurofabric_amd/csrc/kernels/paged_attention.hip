@@ -18,7 +18,9 @@ constexpr int kTile = 64;
 // Any head_dim, head ratio and alignment.  A workgroup takes one (row, head);
 // its four waves take 64-key tiles in turn: a lane scores one key, then the
 // lanes lie over head_dim for the tile's 64 value rows, and the waves' (m, l,
-// acc) are merged at the end.
+// acc) are merged at the end.  The vector ALU and 4-byte loads bound it: 8
+// sequences of 4096 positions with 32 query and 8 KV heads of 80 take 787 us in
+// f16, where heads of 128 on the MFMA kernel take 23.
 template <typename T, PoolType PT>
 __global__ __launch_bounds__(256) void chunk_any_kernel(PagedBatch b, uint32_t n_heads, float scale,
                                                         const T* __restrict__ q, const uint8_t* __restrict__ kp,
@@ -370,6 +372,10 @@ __device__ __forceinline__ uint2 read_tr(const half_t* p) {
 // that no row sees are stored as zeros, and a tile that has a value that is not
 // finite and a row that does not see some key of it takes the vector ALU, which
 // skips the pairs that are masked.
+// Bound by HBM at f16 (64 sequences of up to 8192 positions, 8 KV heads of 128: 1.35 GB
+// in 262 us, 5.2 TB/s, where a copy of 2 GiB reaches 4.9), by it and the conversion's
+// instructions at I8 (4 of up to 131072: 0.83 GB in 157 us, 5.3 TB/s); with 20 rows
+// a sequence by the conversion (16 of up to 4096: 91 MB in 31 us).
 template <PoolType PT, int DD, int NT, bool UNI>
 __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
   constexpr bool I8 = PT == PoolType::I8;
@@ -714,9 +720,11 @@ __global__ __launch_bounds__(256) void chunk_combine_few_kernel(Chunk c) {
     if (lane + 64 * r < DD) static_cast<T*>(c.out)[(uint64_t)o * DD + lane + 64 * r] = (T)(A[r] * inv);
 }
 
-// The same for many splits.  A workgroup per row: the splits' weights exp2(m - M) are formed once, then each wave sums every
-// fourth split's row (a wave per row, which took them one after the other, needed
-// 54 us for 64 splits of 128 rows of 128).
+// The same for many splits.  A workgroup per row: the splits' weights exp2(m - M) are
+// formed once, then each wave sums every fourth split's row (a wave per row, which took
+// them one after the other, needed 54 us for 64 splits of 128 rows of 128; for few
+// splits this kernel is the slower one: three ragged f32 chunks of up to 389 tokens
+// with 2000 positions 136 us, with a wave per row 117).
 constexpr int kSplitsAtOnce = 256;
 template <typename T, int DD>
 __global__ __launch_bounds__(256) void chunk_combine_kernel(Chunk c) {
@@ -811,6 +819,10 @@ inline uint32_t wide_grid(uint32_t tiles, uint32_t n_kv) {
 // f16, are the B operand of O^T[dim][row] += V^T . P^T as they are.
 // Masking, the lazy rescale and values that are not finite: as above; tiles that
 // every row of the workgroup sees whole skip all of it.
+// Bound by MFMA issue and the softmax between: two sequences of 2048 tokens behind 6144,
+// 32 heads of 128, 481 GFLOP in 613 to 628 us, 770 TFLOP/s, where a matrix product of
+// 8192 in each size reaches 1093 and this kernel without its softmax and staging took
+// 364 us; from I8 953 us, the conversion of every tile for each 128 rows being added.
 template <PoolType PT, int DD, bool UNI>
 __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
   constexpr bool I8 = PT == PoolType::I8;
@@ -1202,7 +1214,8 @@ __device__ __forceinline__ void store_f32(const Chunk& c, uint64_t orow, uint32_
 // Few query rows: 16 a workgroup, its waves take 32-key tiles in turn; K and V go
 // from the cache straight into the operands, no LDS before the merge.  A tile
 // with a masked pair and a value that is not finite reads the values again, row by
-// row, for the pairs that count.
+// row, for the pairs that count.  Bound by HBM (8 sequences of up to 4096 positions,
+// 8 KV heads of 128: 49 us), at short caches by its latency (one of 101: 6.6 us).
 template <PoolType PT, int DD, bool UNI>
 __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
   constexpr bool I8 = PT == PoolType::I8;
@@ -1455,6 +1468,10 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
 }
 
 // Many query rows: 64 a workgroup, 16 per wave, 32-key tiles of K and V in LDS.
+// Bound by the f32 MFMA and what of the grid stands still at the end: two sequences of
+// up to 512 tokens with up to 2048 positions, 32 heads of 128, 299 us; three of up to
+// 389 with 2000, 32 heads of 64, 9.5 GFLOP in 117 us with the combine (13 of them),
+// where a product of 8192 in each size reaches 153 TFLOP/s.
 template <PoolType PT, int DD, bool UNI>
 __global__ __launch_bounds__(256, 2) void chunk_wide_f32_kernel(Chunk c) {
   constexpr bool I8 = PT == PoolType::I8;

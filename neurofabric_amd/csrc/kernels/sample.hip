@@ -25,7 +25,9 @@ constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kBins = 2048;     // digits of select()
 constexpr int kBuckets = 1024;  // buckets of the histogram of a row's logits
 constexpr int kList = 2048;     // candidates that are sorted in LDS
-constexpr int kSmallK = 256;    // top_k up to which the threads' largest logits bound the candidates
+// top_k up to which the threads' largest logits bound the candidates (top_k 40 of one row
+// of 32000: 13 us, by the histogram 26)
+constexpr int kSmallK = 256;
 constexpr int kAhead = 2;       // loads a lane has under way while it uses as many
 constexpr double kOne = 1099511627776.0;  // 2^40
 constexpr float kMostT = 1e30f;  // differences of logits past f32 then have no weight
@@ -595,7 +597,9 @@ __device__ __forceinline__ void add_to_bins(Shared& sh, const Row<T>& r, const t
 
 // The chunks that the two passes over a row's logits are spread over: each leaves
 // its threads' largest logits, then (without a small top_k) its buckets' counts and
-// weights and the sum of its weights that min_p leaves.
+// weights and the sum of its weights that min_p leaves.  Of 64 rows of 128256 in f32 the
+// first pass takes 6.7 us (32.8 MB, 4.9 TB/s), the second, bound by the 64-bit
+// exponentials and the LDS atomics, 18.6, and the row kernel 45 (below).
 constexpr int kChunkThreads = 512;
 struct Part {
   uint64_t sum;
@@ -700,6 +704,10 @@ __global__ __launch_bounds__(kChunkThreads) void sample_histogram_kernel(const T
 }
 
 // A workgroup per row.  Without parts (chunks = 0) it goes over the logits itself.
+// A chain of short steps, each waiting for the one before (one row of 32000 with a
+// top_k of 40: 12.4 us in all); the longest row of a batch is one with top_p alone,
+// whose candidates one CU collects from all of its 0.5 MB (128256 in f32: 12 to 17 of
+// about 45 us, then the cut 8, the chunks' sums 4, the draw 9).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_row_kernel(const T* __restrict__ logits, const float* __restrict__ u,
                                                               const float* __restrict__ params,
