@@ -562,3 +562,22 @@ def test_repeated_calls_give_the_same_bits(provider):
             provider.dispatch("flash_attention_paged_chunk", args, [o], pc=pc_of(batch, 2, 128, n_heads=8))
         first = outs[0].read(np.uint16)
         assert all(np.array_equal(first, o.read(np.uint16)) for o in outs[1:])
+
+
+MIDDLE = [  # around the counts of query rows at which another kernel takes the batch, alone and beside longer and shorter sequences
+    ([(300, 16)], 8, 2, 128, 16),
+    ([(300, 17)], 8, 2, 128, 16),
+    ([(700, 24), (400, 24), (129, 24)], 4, 1, 128, 16),
+    ([(700, 25), (400, 25), (129, 24)], 4, 1, 64, 24),
+    ([(500, 64), (300, 96), (200, 32)], 1, 1, 128, 16),
+    ([(520, 33), (300, 65), (200, 300), (90, 1)], 2, 2, 96, 16),
+    ([(400, 21)] * 20, 3, 1, 64, 32),
+]
+
+
+@pytest.mark.parametrize("act,pool", ACT_POOL)
+@pytest.mark.parametrize("seqs,heads,kv,dim,bs", MIDDLE)
+def test_attention_between_kernels(provider, act, pool, seqs, heads, kv, dim, bs):
+    rng = np.random.default_rng(heads * 100 + dim + len(seqs) + bs)
+    batch = ref.Batch(rng, seqs, bs, width=2, behind=1)
+    check_attention(provider, rng, batch, act, pool, heads, kv, dim)

@@ -205,3 +205,14 @@ def test_frequencies(provider, dtype):
     token, _ = draw(provider, np.tile(x, (rows, 1)), u, np.tile(np.float32([1, 1, 0]), (rows, 1)), np.zeros(rows, np.int32))
     p = np.exp(x.astype(np.float64))
     assert np.abs(np.bincount(token, minlength=n) - rows * p / p.sum()).max() <= 1.0
+
+
+@pytest.mark.parametrize("rows,n", [(3, 65536), (2, 40001), (4, 16384), (4, 16385), (5, 20011), (260, 16400)])
+def test_cuts_of_short_rows(provider, rows, n):
+    """Few and many rows on both sides of the lengths from which rows are spread over workgroups."""
+    rng = np.random.default_rng(n + rows)
+    x = (rng.standard_normal((rows, n)) * 3).astype(np.float32)
+    ks = [0, 40, 300, 3000, 12000, 0, 1, 256]
+    ps = [0.9, 1.0, 0.95, 0.999, 0.5]
+    how = [(ks[(i + n) % len(ks)], ps[i % 5], [0.0, 0.05, 0.0][i % 3], [1.0, 0.7, 4.0, 0.0][i % 4]) for i in range(rows)]
+    check(provider, x, rng.random(rows).astype(np.float32), [(t, p, m) for _, p, m, t in how], [h[0] for h in how])
