@@ -209,6 +209,7 @@ struct Rows {
   int end;                // keys below it
   int shift;              // UNI: log2 of block_size
   uint32_t entry;         // UNI: lane h has the block of the next tile's group h
+  int cur;                // UNI: the current tile's first key
   uint64_t base[N];
   uint32_t scales[N];
   uint64_t off, next_off;  // else: the lane's key
@@ -246,6 +247,7 @@ struct Rows {
   }
   __device__ __forceinline__ void take(int t0) {
     if constexpr (UNI) {
+      cur = t0;
       valid = 0;
 #pragma unroll
       for (int h = 0; h < N; ++h) {
@@ -263,6 +265,15 @@ struct Rows {
       sc = next_sc;
       valid = next_valid;
     }
+  }
+  // base[h], and scales[h] in `to`, for an h that is known when the kernel runs and the same
+  // for the wave; between take() and the next look().
+  __device__ __forceinline__ uint64_t place(int h, uint32_t& to) const {
+    const uint32_t phys = (uint32_t)__builtin_amdgcn_readlane((int)entry, h);
+    const uint32_t at = (uint32_t)(cur + 16 * h) & (b.block_size - 1);
+    const bool ok = phys < b.blocks;
+    to = ok ? to_scales(at) : 0;
+    return ok ? phys * block + head + at * kRow : 0;
   }
   __device__ __forceinline__ uint64_t have() const { return valid; }
   // The row of a key of the first two groups that differs between lanes, and its scales.
@@ -822,7 +833,7 @@ inline uint32_t wide_grid(uint32_t tiles, uint32_t n_kv) {
 // Bound by MFMA issue and the softmax between: two sequences of 2048 tokens behind 6144,
 // 32 heads of 128, 481 GFLOP in 613 to 628 us, 770 TFLOP/s, where a matrix product of
 // 8192 in each size reaches 1093 and this kernel without its softmax and staging took
-// 364 us; from I8 953 us, the conversion of every tile for each 128 rows being added.
+// 364 us.  From I8 607 us: half the bytes to stage, the conversion beside the MFMAs.
 template <PoolType PT, int DD, bool UNI>
 __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
   constexpr bool I8 = PT == PoolType::I8;
@@ -886,30 +897,37 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
     for (int u = 0; u < NU; ++u) {
       const int ch = tid + 256 * u < 64 * CPR ? tid + 256 * u : 64 * CPR - 1;
       const int r = ch / CPR, col = ch % CPR;
-      // a wave's 64 chunks lie in one group of 16 keys, known to be the same for it, or in two
-      const int h = 16 * CPR % 64 == 0 ? __builtin_amdgcn_readfirstlane(r / 16) : r / 16;
-      auto get = [&](int hh) {
-        kraw[u] = *reinterpret_cast<const u32x4*>(rows.row(c.k, hh, r - 16 * hh) + 16 * col);
-        vraw[u] = *reinterpret_cast<const u32x4*>(rows.row(c.v, hh, r - 16 * hh) + 16 * col);
+      if constexpr (!UNI) {
+        kraw[u] = *reinterpret_cast<const u32x4*>(rows.row(c.k, 0, r) + 16 * col);
+        vraw[u] = *reinterpret_cast<const u32x4*>(rows.row(c.v, 0, r) + 16 * col);
         if constexpr (I8) {
-          kd[u] = rows.scale(c.k, hh, r - 16 * hh)[col / 2];
-          vd[u] = rows.scale(c.v, hh, r - 16 * hh)[col / 2];
+          kd[u] = rows.scale(c.k, 0, r)[col / 2];
+          vd[u] = rows.scale(c.v, 0, r)[col / 2];
         }
-      };
-      if constexpr (UNI && 16 * CPR == 256) {
-        get(u);  // F16, 128: the workgroup's 256
-      } else if constexpr (UNI) {
-        const uint64_t ro = h < 2 ? (h ? rows.base[1] : rows.base[0]) : (h == 2 ? rows.base[2] : rows.base[3]);
-        const uint32_t so = h < 2 ? (h ? rows.scales[1] : rows.scales[0]) : (h == 2 ? rows.scales[2] : rows.scales[3]);
-        const uint32_t rr = r - 16 * h;
+      } else {
+        // F16, 128: the workgroup's 256 chunks lie in one group of 16 keys, known here (612 us at
+        // the size above, looked up as the others 640).  Else a wave's 64 lie in one or in
+        // two.  It looks up those alone, by scalar instructions: a choice among the addresses
+        // of all four was made by 64-bit multiplications in the vector ALU (I8, the same
+        // size: 953 us, and 607).
+        const int c0 = 64 * (w + 4 * u), h0 = min(c0, 64 * CPR - 1) / (16 * CPR), h1 = min(c0 + 63, 64 * CPR - 1) / (16 * CPR);
+        uint32_t so = 16 * CPR == 256 ? rows.scales[u] : 0, rr = r - 16 * (16 * CPR == 256 ? u : h0);
+        uint64_t ro = 16 * CPR == 256 ? rows.base[u] : rows.place(h0, so);
+        if constexpr (CPR % 4 != 0) {
+          uint32_t so1;
+          const uint64_t ro1 = rows.place(h1, so1);
+          if (r >= 16 * h1) {
+            rr = r - 16 * h1;
+            ro = ro1;
+            so = so1;
+          }
+        }
         kraw[u] = *reinterpret_cast<const u32x4*>(c.k + ro + rr * rows.kRow + 16 * col);
         vraw[u] = *reinterpret_cast<const u32x4*>(c.v + ro + rr * rows.kRow + 16 * col);
         if constexpr (I8) {
           kd[u] = reinterpret_cast<const half_t*>(c.k + ro + so + rr * (DD / 16))[col / 2];
           vd[u] = reinterpret_cast<const half_t*>(c.v + ro + so + rr * (DD / 16))[col / 2];
         }
-      } else {
-        get(h);
       }
     }
   };
@@ -1478,6 +1496,7 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_f32_kernel(Chunk c) {
   constexpr int TK = 32, DP = DD + 4, DG = DD / 4, NH = (DD + 63) / 64, NB = 4 * NH;
   constexpr int EC = I8 ? 8 : 4;                  // elements per chunk (8 or 16 bytes)
   constexpr int CPR = DD / EC, NU = (TK * CPR + 255) / 256;
+  static_assert(CPR % 4 == 0, "a wave's 64 chunks of a tile lie in one group of 16 keys");
   __shared__ __attribute__((aligned(16))) float ks[TK * DP];
   __shared__ __attribute__((aligned(16))) float vs[TK * DP + 64 * NH - DD];
   __shared__ __attribute__((aligned(16))) float ps[4][TK][16];
@@ -1525,22 +1544,28 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_f32_kernel(Chunk c) {
     for (int u = 0; u < NU; ++u) {
       const int ch = tid + 256 * u < TK * CPR ? tid + 256 * u : TK * CPR - 1;
       const int r = ch / CPR, col = ch % CPR;
-      auto get = [&](int h) {
-        const uint8_t *kr = rows.row(c.k, h, r - 16 * h), *vr = rows.row(c.v, h, r - 16 * h);
+      auto get = [&](const uint8_t* kr, const uint8_t* vr, const half_t* ksc, const half_t* vsc) {
         if constexpr (I8) {
           kc[u] = *reinterpret_cast<const uint2*>(kr + 8 * col);
           vc[u] = *reinterpret_cast<const uint2*>(vr + 8 * col);
-          kd[u] = rows.scale(c.k, h, r - 16 * h)[col / 4];
-          vd[u] = rows.scale(c.v, h, r - 16 * h)[col / 4];
+          kd[u] = ksc[col / 4];
+          vd[u] = vsc[col / 4];
         } else {
           kf[u] = *reinterpret_cast<const float4v*>(kr + 16 * col);
           vf[u] = *reinterpret_cast<const float4v*>(vr + 16 * col);
         }
       };
-      if constexpr (!UNI) get(r / 16);
-      else if constexpr (16 * CPR % 256 == 0) get(256 * u / (16 * CPR));  // the workgroup's 256 lie in one group of 16 keys
-      else if (r < 16) get(0);
-      else get(1);
+      if constexpr (!UNI) {
+        get(rows.row(c.k, 0, r), rows.row(c.v, 0, r), rows.scale(c.k, 0, r), rows.scale(c.v, 0, r));
+      } else {  // a wave's 64 lie in one group of 16 keys
+        const bool whole = 16 * CPR % 256 == 0;  // the workgroup's 256 do
+        const int h = whole ? 256 * u / (16 * CPR) : min(w + 4 * u, TK * CPR / 64 - 1) / (CPR / 4);
+        uint32_t so = whole ? rows.scales[h] : 0;
+        const uint64_t ro = whole ? rows.base[h] : rows.place(h, so);
+        const uint32_t rr = r - 16 * h, sr = so + rr * (DD / 16);
+        get(c.k + ro + rr * rows.kRow, c.v + ro + rr * rows.kRow, reinterpret_cast<const half_t*>(c.k + ro + sr),
+            reinterpret_cast<const half_t*>(c.v + ro + sr));
+      }
     }
   };
   auto stage = [&](uint32_t seen, bool closed, int par) {
@@ -1692,13 +1717,13 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_f32_kernel(Chunk c) {
 
 // Query rows of a sequence, on average, up to which the narrow kernel takes the whole
 // batch.  It reads the cache once per 16 or 32 rows and splits it finely; the wide one
-// once per 128 (f32: 64), and converts I8 tiles for all of them.  Narrow and wide, 8
-// sequences of 4096 positions, 8 KV heads of 128:
-//   f16, 64 rows 52 and 68 us, 96 rows 71 and 65;
-//   I8,  64 rows 36 and 98 us, 96 rows 51 and 87, 128 rows 83 (wide);
+// once per 128 (f32: 64).  Narrow and wide, 8 sequences of 4096 positions, 8 KV heads
+// of 128:
+//   f16, 64 rows 52 and 70 us, 96 rows 70 and 63;
+//   I8,  64 rows 37 and 45 us, 96 rows 51 and 44;
 //   f32, 36 rows 144 and 100 us, 64 rows 155 and 111; one of 8192, 32 rows: 28 and 33.
-template <typename T, PoolType PT>
-constexpr uint32_t kNarrowRows = std::is_same<T, float>::value ? 32 : PT == PoolType::I8 ? 96 : 64;
+template <typename T>
+constexpr uint32_t kNarrowRows = std::is_same<T, float>::value ? 32 : 64;
 // Where the wide kernel runs, the sequences that go to the narrow one all the same; more
 // wait for a kernel with too few workgroups (three sequences of up to 96 rows: 42 us, and
 // 54 with the narrow kernel taking those of up to 64).
@@ -1719,7 +1744,7 @@ hipError_t chunk_mfma_at(const PagedBatch& b, uint32_t n_heads, const void* q, c
   const uint64_t rows = (uint64_t)b.rows * c.group;  // query rows per KV head
   // Lengths are known on the device only: each kernel skips the sequences that are the
   // other's.
-  const bool wide = rows > (uint64_t)kNarrowRows<T, PT> * b.n_seqs;
+  const bool wide = rows > (uint64_t)kNarrowRows<T> * b.n_seqs;
   const bool narrow = !wide || b.n_seqs > 1;
   constexpr bool F16 = std::is_same<T, half_t>::value;
   constexpr uint32_t kWideRows = F16 ? 128 : 64;  // a wide workgroup's query rows
