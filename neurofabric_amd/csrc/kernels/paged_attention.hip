@@ -904,15 +904,18 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
           kd[u] = rows.scale(c.k, 0, r)[col / 2];
           vd[u] = rows.scale(c.v, 0, r)[col / 2];
         }
-      } else {
+      } else if constexpr (16 * CPR == 256) {
         // F16, 128: the workgroup's 256 chunks lie in one group of 16 keys, known here (612 us at
-        // the size above, looked up as the others 640).  Else a wave's 64 lie in one or in
-        // two.  It looks up those alone, by scalar instructions: a choice among the addresses
-        // of all four was made by 64-bit multiplications in the vector ALU (I8, the same
-        // size: 953 us, and 607).
+        // the size above, looked up as the others 640).
+        kraw[u] = *reinterpret_cast<const u32x4*>(rows.row(c.k, u, r - 16 * u) + 16 * col);
+        vraw[u] = *reinterpret_cast<const u32x4*>(rows.row(c.v, u, r - 16 * u) + 16 * col);
+      } else {
+        // A wave's 64 lie in one group, or in two.  It looks up those alone, by scalar
+        // instructions: a choice among the addresses of all four was made by 64-bit
+        // multiplications in the vector ALU (I8, the same size: 953 us, and 607).
         const int c0 = 64 * (w + 4 * u), h0 = min(c0, 64 * CPR - 1) / (16 * CPR), h1 = min(c0 + 63, 64 * CPR - 1) / (16 * CPR);
-        uint32_t so = 16 * CPR == 256 ? rows.scales[u] : 0, rr = r - 16 * (16 * CPR == 256 ? u : h0);
-        uint64_t ro = 16 * CPR == 256 ? rows.base[u] : rows.place(h0, so);
+        uint32_t so, rr = r - 16 * h0;
+        uint64_t ro = rows.place(h0, so);
         if constexpr (CPR % 4 != 0) {
           uint32_t so1;
           const uint64_t ro1 = rows.place(h1, so1);
