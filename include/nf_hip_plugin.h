@@ -58,7 +58,9 @@
  *     while it runs.  A position below 0 or
  *     past the bound, or in a block that the pools do not hold, has no storage:
  *     append skips it, gather gives zeros for it, attention counts no key; a row
- *     without any key gives zeros.  Rows of no sequence are left as they are, and
+ *     without any key gives zeros.  A key whose score is -inf weighs nothing: beside
+ *     other keys it is as if it were not there (its values being finite), and a row
+ *     of such keys alone gives zeros.  Rows of no sequence are left as they are, and
  *     so are those of a sequence whose rows are not all within seq_len.  A
  *     slot that several rows of one append name ends with any of their values.
  *   sample_token        LOGITS, U, PARAMS, TOP_K -> TOKEN, PROB

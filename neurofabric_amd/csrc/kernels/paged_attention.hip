@@ -356,6 +356,11 @@ __device__ __forceinline__ float sum4(float v) {
 // below 2^15.
 constexpr float kWeightLog2 = 7.f, kLagLog2 = 8.f;
 
+// What is taken off the scores in the weights' exponents, for a running maximum `m` and
+// weights times 2^`log2`.  Finite while every score so far is -inf: those weigh
+// exp2(-inf) = 0, where -inf - -inf would be NaN.
+__device__ __forceinline__ float exponent_base(float m, float log2) { return m == -INFINITY ? 0.f : m - log2; }
+
 typedef short short4v __attribute__((ext_vector_type(4)));
 // ds_read_b64_tr_b16: among each 16 lanes, lane i receives element i % 4 of the 8
 // bytes that lane 4e + i / 4 addresses, as its element e.
@@ -579,16 +584,13 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
         for (int d = 0; d < DB; ++d) ot[u][d] *= corr;
         m[u] = mn;
       }
-      const float mb = m[u] - kWeightLog2;
+      const float mb = exponent_base(m[u], kWeightLog2);
       float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float s = sc[u][j][i];
-          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s, c.scale_log2, -mb));
-          pv[u][j][i] = !OPEN && s == -INFINITY ? 0.f : e;
-        }
+        for (int i = 0; i < 4; ++i)
+          pv[u][j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][j][i], c.scale_log2, -mb));
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const half2v h = __builtin_convertvector(float2s{pv[u][k / 2][2 * (k % 2)], pv[u][k / 2][2 * (k % 2) + 1]}, half2v);
@@ -887,7 +889,7 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
   for (int d = 0; d < DB; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) ot[d][i] = 0.f;
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY, l = 0.f, mb = 0.f;  // mb: exponent_base of m
 
   u32x4 kraw[NU], vraw[NU];
   half_t kd[NU], vd[NU];
@@ -978,20 +980,17 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
 #pragma unroll
     for (int d = 0; d < DB; ++d) ot[d] *= corr;
     m = mn;
+    mb = exponent_base(m, kWeightLog2);
   };
-  auto weights = [&](auto open_c) {
-    constexpr bool OPEN = decltype(open_c)::value;
-    const float mb = m - kWeightLog2;
+  auto weights = [&]() {
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int i = 0; i < 16; i += 2) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][i + e], c.scale_log2, -mb));
-          sc[j][i + e] = !OPEN && sc[j][i + e] == -INFINITY ? 0.f : x;
-        }
+        for (int e = 0; e < 2; ++e)
+          sc[j][i + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][i + e], c.scale_log2, -mb));
         const half2v h = __builtin_convertvector(float2s{sc[j][i], sc[j][i + 1]}, half2v);
         pb[j][i / 8][i % 8] = h[0];
         pb[j][i / 8][i % 8 + 1] = h[1];
@@ -1045,7 +1044,7 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[j][i]);
     rescale(max2(top) * c.scale_log2);
-    weights(std::true_type{});
+    weights();
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int ch = 0; ch < 4; ++ch) {
@@ -1084,7 +1083,7 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
         top = fmaxf(top, sc[j][i]);
       }
     rescale(max2(top) * c.scale_log2);
-    weights(std::false_type{});
+    weights();
     if (!tile_bad[par]) {
 #pragma unroll
       for (int j = 0; j < 2; ++j)
@@ -1365,13 +1364,13 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
       for (int d = 0; d < NB; ++d) ot[d] *= corr;
       m = mn;
     }
+    const float mb = exponent_base(m, 0.f);
     float pv[2][4], sum = 0.f;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][i], c.scale_log2, -m));
-        pv[j][i] = !OPEN && sc[j][i] == -INFINITY ? 0.f : e;
+        pv[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][i], c.scale_log2, -mb));
         sum += pv[j][i];
       }
     l += sum4(sum);
@@ -1636,13 +1635,13 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_f32_kernel(Chunk c) {
       for (int d = 0; d < NB; ++d) ot[d] *= corr;
       m = mn;
     }
+    const float mb = exponent_base(m, 0.f);
     float pv[2][4], sum = 0.f;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][i], c.scale_log2, -m));
-        pv[j][i] = !OPEN && sc[j][i] == -INFINITY ? 0.f : e;
+        pv[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][i], c.scale_log2, -mb));
         sum += pv[j][i];
       }
     l += sum4(sum);

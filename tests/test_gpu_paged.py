@@ -581,3 +581,39 @@ def test_attention_between_kernels(provider, act, pool, seqs, heads, kv, dim, bs
     rng = np.random.default_rng(heads * 100 + dim + len(seqs) + bs)
     batch = ref.Batch(rng, seqs, bs, width=2, behind=1)
     check_attention(provider, rng, batch, act, pool, heads, kv, dim)
+
+
+@pytest.mark.parametrize("act,pool", ACT_POOL)
+@pytest.mark.parametrize("dim", [64, 128, 96, 160])
+@pytest.mark.parametrize("rows", [1, 12, 130])
+def test_attention_scores_of_minus_infinity(provider, act, pool, dim, rows):
+    """Keys that score -inf weigh nothing, as if they were not there, wherever they lie: in tiles and splits that hold
+    nothing else, before finite keys and between them; a row with no other key gives zeros.  Elements of K are -inf, or
+    (f32) finite with a product that is not."""
+    rng = np.random.default_rng(dim + rows)
+    heads, kv, bs = 4, 2, 16
+    batch = ref.Batch(rng, [(600, rows), (200, min(rows, 70)), (400, 2), (7, 7)], bs)
+    low = [range(320), range(200), range(64, 128), range(0)]
+    pools = [ref.empty_pool(rng, pool, batch.blocks, kv, bs, dim) for _ in range(2)]
+    q = rows_of(rng, act, batch.rows, heads, dim)
+    q[..., :32] = np.abs(q[..., :32]) + NP[act](2)
+    left = ref.Batch(rng, batch.seqs, bs)  # the same without those keys
+    left.table = batch.table.copy()
+    for s, positions in enumerate(low):
+        for p in positions:
+            b, slot = batch.where(s, p)
+            if pool == "i8":
+                pools[0][b, :, slot * dim:slot * dim + 32] = 0x81  # -127
+                at = bs * dim + slot * dim // 16
+                pools[0][b, :, at:at + 2] = np.full((1, 1), np.inf, np.float16).view(np.uint8)
+            else:
+                pools[0][b, 0, slot, :32] = -np.inf
+                pools[0][b, 1, slot, :32] = -3e38 if pool == "f32" else -np.inf
+            left.table[s, p // bs] = ref.NONE
+    with Bufs(provider) as m:
+        out = m.put(np.zeros_like(q))
+        provider.dispatch("flash_attention_paged_chunk", [m.put(q)] + [m.put(p) for p in pools] + m.batch(batch), [out],
+                          pc=pc_of(batch, kv, dim, n_heads=heads))
+        got = out.read(NP[act], q.size).reshape(q.shape)
+    want, err = ref.attention(left, pool, dim, heads, kv, pools, q, act)
+    check(got, want, err, (act, pool, dim, rows))
