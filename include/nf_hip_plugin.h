@@ -61,8 +61,10 @@
  *     without any key gives zeros.  A key whose score is -inf weighs nothing: beside
  *     other keys it is as if it were not there (its values being finite), and a row
  *     of such keys alone gives zeros.  Rows of no sequence are left as they are, and
- *     so are those of a sequence whose rows are not all within seq_len.  A
- *     slot that several rows of one append name ends with any of their values.
+ *     so are those of a sequence whose rows are not all within seq_len.  The rows
+ *     of one append have to name slots of their own: what a slot holds that two of
+ *     them name is not defined (an I8 slot may get one row's codes and the other's
+ *     scales); no other slot is touched by it.
  *   sample_token        LOGITS, U, PARAMS, TOP_K -> TOKEN, PROB
  *     LOGITS [seq_len, N] F32 or F16; U f32[seq_len], random numbers of [0, 1);
  *     PARAMS f32[seq_len][3] = temperature, top_p, min_p; TOP_K int32[seq_len];

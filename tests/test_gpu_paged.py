@@ -617,3 +617,29 @@ def test_attention_scores_of_minus_infinity(provider, act, pool, dim, rows):
         got = out.read(NP[act], q.size).reshape(q.shape)
     want, err = ref.attention(left, pool, dim, heads, kv, pools, q, act)
     check(got, want, err, (act, pool, dim, rows))
+
+
+@pytest.mark.parametrize("act,pool", ACT_POOL)
+@pytest.mark.parametrize("rows", [1, 9, 300])
+def test_append_of_one_slot_twice(provider, act, pool, rows):
+    """What a slot holds that two rows of one append name is not defined; all other slots are as they would be."""
+    rng = np.random.default_rng(rows)
+    kv, dim, bs = 2, 64, 16
+    batch = ref.Batch(rng, [(rows + 20, rows), (rows + 20, rows), (40, 5)], bs)
+    last = (rows + 19) // bs
+    batch.table[1, last] = batch.table[0, last]  # the last block of both
+    pools = [ref.empty_pool(rng, pool, batch.blocks, kv, bs, dim) for _ in range(2)]
+    x = [rows_of(rng, act, batch.rows, kv, dim) for _ in range(2)]
+    with Bufs(provider) as m:
+        kb = [m.put(p) for p in pools]
+        provider.dispatch("paged_kv_append", [m.put(r) for r in x] + m.batch(batch), kb, pc=pc_of(batch, kv, dim))
+        got = [b.read(np.uint8, p.nbytes).view(p.dtype).reshape(p.shape) for b, p in zip(kb, pools)]
+    ref.append(batch, pool, dim, pools, x)
+    shared = int(batch.table[0, last])
+    first = max(20, bs * last) - bs * last  # the slots of that block that both write
+    for g, p in zip(got, pools):
+        for slot in range(first, (rows + 20) - bs * last):
+            at = np.zeros(dim, np.float32)
+            for a in (g, p):
+                ref.store(a, pool, bs, dim, (shared, slot), np.broadcast_to(at, (kv, dim)))
+        assert np.array_equal(g.view(np.uint8), p.view(np.uint8))
