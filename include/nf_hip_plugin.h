@@ -48,7 +48,8 @@
  *     followed by block_size * head_dim / 32 fp16 scales (head_dim % 32 == 0).
  *     A group of 32 elements x of a row is held as scale = fp16(fp32(max|x| /
  *     127)) and codes x / scale to nearest, ties to even; it stands for code *
- *     scale.  Codes saturate, NaN is held as 0.
+ *     scale.  Codes saturate, NaN is held as 0.  For F16 rows a group without
+ *     infinities has a scale of at most 515.5: code * scale is then finite in f16.
  *     Attention: the row at position p attends to positions 0 .. p with the
  *     scale 1 / sqrt(head_dim); query head h reads KV head h * M / n_heads.
  *     The chunk's own keys have to be in the cache (paged_kv_append before it).

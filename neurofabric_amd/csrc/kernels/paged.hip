@@ -5,7 +5,8 @@
 // I8 pools hold, for 32 consecutive elements x of a row, the scale d =
 // fp16(max|x| / 127) and the codes q = x / d to the nearest integer (ties to
 // even); the cache then stands for q d.  Values beyond 127 of the largest fp16
-// scale saturate, a NaN is held as 0.
+// scale saturate, a NaN is held as 0.  Finite f16 rows take scales of at most 515.5,
+// so that what the cache stands for is finite in f16 too.
 #include <type_traits>
 
 #include "paged.hpp"
@@ -39,7 +40,7 @@ __global__ __launch_bounds__(256) void append_any_kernel(PagedBatch b, const T* 
   } else {
     float amax = 0.0f;
     for (uint32_t i = 0; i < U; ++i) amax = fmaxf(amax, __builtin_fabsf((float)src[i]));
-    const half_t d = scale_of(amax);
+    const half_t d = scale_of<T>(amax);
     const float df = (float)d, inv = df > 0.0f ? 1.0f / df : 0.0f;
     for (uint32_t i = 0; i < U; ++i)
       page[slot * b.dim + d0 + i] = (uint8_t)(df > 0.0f ? code_of_value((float)src[i], df, inv) : 0);
@@ -98,7 +99,7 @@ __device__ __forceinline__ void put_codes(typename Piece<T>::type x, uint8_t* co
   for (int e = 0; e < E; ++e) amax = fmaxf(amax, __builtin_fabsf((float)x[e]));
 #pragma unroll
   for (int o = 1; o < 32 / E; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
-  const half_t d = scale_of(amax);
+  const half_t d = scale_of<T>(amax);
   const float df = (float)d, inv = df > 0.0f ? 1.0f / df : 0.0f;
   uint32_t w[E / 4] = {};
 #pragma unroll

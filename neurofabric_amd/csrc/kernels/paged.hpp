@@ -79,10 +79,14 @@ __device__ __forceinline__ float page_value(const PagedBatch& b, const uint8_t* 
            (float)reinterpret_cast<const half_t*>(page + b.block_size * b.dim)[i / 32];
 }
 
-// The fp16 scale of 32 elements of largest magnitude `amax`: fp16(amax / 127),
-// at most the largest finite fp16.
+// The fp16 scale of 32 elements of type T and largest magnitude `amax`:
+// fp16(amax / 127), at most the largest finite fp16.  Finite f16 elements stay
+// finite where they are read as f16: amax = 65504 would take 516, whose multiple
+// 127 * 516 rounds to infinity, and takes the next scale below.
+template <typename T>
 __device__ __forceinline__ half_t scale_of(float amax) {
   const half_t d = (half_t)(amax / 127.0f);
+  if (sizeof(T) == 2 && amax <= 65504.0f && d > (half_t)515.5f) return (half_t)515.5f;
   return __builtin_isinf((float)d) ? (half_t)65504.0f : d;
 }
 

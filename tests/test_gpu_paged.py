@@ -643,3 +643,39 @@ def test_append_of_one_slot_twice(provider, act, pool, rows):
             for a in (g, p):
                 ref.store(a, pool, bs, dim, (shared, slot), np.broadcast_to(at, (kv, dim)))
         assert np.array_equal(g.view(np.uint8), p.view(np.uint8))
+
+
+@pytest.mark.parametrize("dim", [64, 128, 96, 160])
+@pytest.mark.parametrize("rows", [3, 150])
+def test_largest_f16_values_in_an_i8_cache(provider, dim, rows):
+    """Finite f16 rows stay finite in an I8 cache: read back within half a step of their scale (and the f16 rounding), and
+    attended to, up to the largest value of the type."""
+    rng = np.random.default_rng(dim + rows)
+    heads, kv, bs = 4, 2, 16
+    batch = ref.Batch(rng, [(rows, rows), (5, 5)], bs)
+    x = [(rng.uniform(-6e4, 6e4, (batch.rows, kv, dim))).astype(np.float16) for _ in range(2)]
+    for r in x:
+        r[::2, :, 3::32] = 65504.0
+        r[::2, :, 5::32] = -65504.0
+        r[1::2, :, 7::32] = 65472.0
+        r[0, :, :32] = [65504.0, -65504.0] * 16
+    q = rows_of(rng, "f16", batch.rows, heads, dim, 1e-4)
+    pools = [ref.empty_pool(rng, "i8", batch.blocks, kv, bs, dim) for _ in range(2)]
+    with Bufs(provider) as m:
+        kb, desc = [m.put(p) for p in pools], m.batch(batch)
+        back, out = [m.put(np.zeros_like(r)) for r in x], m.put(np.zeros_like(q))
+        pc = pc_of(batch, kv, dim, n_heads=heads)
+        provider.dispatch("paged_kv_append", [m.put(r) for r in x] + desc, kb, pc=pc)
+        provider.dispatch("paged_kv_gather", kb + desc, back, pc=pc)
+        provider.dispatch("flash_attention_paged_chunk", [m.put(q)] + kb + desc, [out], pc=pc)
+        held = [b.read(np.uint8, p.nbytes).reshape(p.shape) for b, p in zip(kb, pools)]
+        got = [b.read(np.float16, r.size).reshape(r.shape) for b, r in zip(back, x)]
+        o = out.read(np.float16, q.size).reshape(q.shape)
+    for g, r in zip(got, x):
+        top = np.abs(r.astype(np.float64)).reshape(batch.rows, kv, -1, 32).max(-1)
+        # the scale is top / 127 within half a step of fp16; a code is off by half, and its product by half a step
+        step = (top / 127 * (1 + 2.0 ** -11)).repeat(32, -1).reshape(r.shape)
+        check(g, r.astype(np.float64), 0.5 * step + 2.0 ** -11 * 65504, (dim, rows))
+    want, err = ref.attention(batch, "i8", dim, heads, kv, held, q, "f16")
+    assert np.isfinite(want).all()
+    check(o, want, err, (dim, rows))
