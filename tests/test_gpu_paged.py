@@ -679,3 +679,50 @@ def test_largest_f16_values_in_an_i8_cache(provider, dim, rows):
     want, err = ref.attention(batch, "i8", dim, heads, kv, held, q, "f16")
     assert np.isfinite(want).all()
     check(o, want, err, (dim, rows))
+
+
+MANY_ROWS = [  # rows around the count up to which they are spread over more waves, and past it; 16-byte pieces a row (f16, f32)
+    ([(512, 512)], 0, 8, 128, 16),               # 128, 256
+    ([(600, 507), (40, 1)], 5, 8, 128, 16),      # 513 rows in all
+    ([(515, 515), (300, 290), (310, 300)], 2, 3, 96, 8),  # 36, 72
+    ([(700, 650), (450, 450), (9, 3)], 1, 5, 256, 5),     # 160, 320
+    ([(20, 9)] * 130, 3, 2, 32, 16),             # 8, 16; more sequences than a wave has lanes
+]
+
+
+@pytest.mark.parametrize("act,pool", ACT_POOL)
+@pytest.mark.parametrize("seqs,behind,kv,dim,bs", MANY_ROWS)
+def test_append_and_gather_many_rows(provider, act, pool, seqs, behind, kv, dim, bs):
+    """As test_append_and_gather, for prompts: rows of no sequence, and blocks that are missing."""
+    rng = np.random.default_rng(len(seqs) * 1000 + dim + behind)
+    batch = ref.Batch(rng, seqs, bs, behind=behind)
+    batch.table[0, 1] = ref.NONE
+    batch.table[-1, 0] = batch.blocks
+    pools = [ref.empty_pool(rng, pool, batch.blocks, kv, bs, dim, garbage=True) for _ in range(2)]
+    rows = [rows_of(rng, act, batch.rows, kv, dim, s) for s in (1.0, 30.0)]
+    was = [rows_of(rng, act, batch.rows, kv, dim) for _ in range(2)]
+    with Bufs(provider) as m:
+        desc = m.batch(batch)
+        kb = [m.put(p) for p in pools]
+        out = [m.put(w) for w in was]
+        pc = pc_of(batch, kv, dim)
+        provider.dispatch("paged_kv_append", [m.put(r) for r in rows] + desc, kb, pc=pc)
+        provider.dispatch("paged_kv_gather", kb + desc, out, pc=pc)
+        got = [b.read(np.uint8, p.nbytes).reshape(p.view(np.uint8).shape) for b, p in zip(kb, pools)]
+        back = [b.read(NP[act], w.size).reshape(w.shape) for b, w in zip(out, was)]
+    ref.append(batch, pool, dim, pools, rows)
+    for g, p in zip(got, pools):
+        assert np.array_equal(g, p.view(np.uint8))
+    for j in range(2):
+        for r, s, pos in batch.each():
+            w = batch.where(s, pos)
+            was[j][r] = ref.load(pools[j], pool, bs, dim, w).astype(NP[act]) if w else 0.0
+        assert np.array_equal(back[j].view(np.uint8), was[j].view(np.uint8))
+
+
+@pytest.mark.parametrize("act,pool", ACT_POOL)
+def test_attention_more_splits_than_threads(provider, act, pool):
+    """One head of one long sequence: its keys are split over more than 256 workgroups, whose partials one combines."""
+    rng = np.random.default_rng(17)
+    batch = ref.Batch(rng, [(40003, 1)], 16)
+    check_attention(provider, rng, batch, act, pool, 1, 1, 64)
