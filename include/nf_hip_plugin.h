@@ -40,7 +40,8 @@
  *     most 256), M, N, K, window_size = block_size (0: 16), max_seq_len = a
  *     bound on LENS (0: N * block_size; longer sequences are cut off there).  At
  *     most 2^22 rows, 65535 sequences, KV heads and heads, 65536 positions a
- *     block.  A tight bound lets the attention launch fewer workgroups.
+ *     block, 2^32 - 256 elements in a dense operand.  A tight bound lets the
+ *     attention launch fewer workgroups.
  *     An I8 pool is read by the attention as f16 for f16 rows (code * scale
  *     rounded once, as paged_kv_gather does), exactly for f32 rows.
  *     Pools are [block][M][block_size][head_dim] of the rows' dtype, or I8: the
@@ -78,7 +79,7 @@
  *     index order whose running sum exceeds floor(U S), and PROB = w / S.  T <= 0
  *     takes the first largest logit; T is taken as at most 1e30.  +inf counts as
  *     the largest finite value; NaN and -inf are never drawn; a row of nothing
- *     else gives -1 and 0.  N is at most 2^22.
+ *     else gives -1 and 0.  N is at most 2^22, seq_len 65535.
  * These ops may use the provider's workspace: replays of graphs that hold them
  * must not overlap each other or later dispatches (one stream does that).
  */

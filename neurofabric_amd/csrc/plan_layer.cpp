@@ -255,7 +255,8 @@ nf_status plan_paged_rows(bool append, const nf_tensor_desc* const* ins, uint32_
   nf_status st = plan_paged_batch(append ? ins : outs, 2, append ? outs : ins, ins + 2, pc, p, why);
   if (st != NF_OK) return st;
   const uint64_t n = (uint64_t)p->lp.seq_len * p->lp.n_kv * p->lp.head_dim, elt = elt_bytes(p->a);
-  if (n >= kMaxElems) return fail(why, "too many rows");
+  // a thread per element where rows are not whole pieces: a launch holds less than 2^32
+  if (n > kMaxElems - 256) return fail(why, "too many rows");
   const nf_tensor_desc* const* dense = append ? ins : outs;
   if (!fits(dense[0], n, elt) || !fits(dense[1], n, elt))
     return fail(why, "K and V rows hold fewer than seq_len * M * head_dim elements");

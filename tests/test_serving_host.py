@@ -147,3 +147,13 @@ def test_sample(lib):
     refused(sample, lib, prob=desc(F32, 8), match="outputs")
     refused(plan, lib, "sample_token", [desc(F32, 400)] * 3, [desc(I32, 4)] * 2, pc=push_constants(seq_len=1, N=100))
     refused(plan, lib, "sample_token", [desc(F32, 400)] * 4, [desc(I32, 4)], pc=push_constants(seq_len=1, N=100))
+
+
+@pytest.mark.parametrize("call", [append, gather])
+def test_most_elements(lib, call):
+    """A thread per element where rows are not whole pieces: rounded up to workgroups they stay below 2^32."""
+    def rows(t, kv, d):
+        dense, pl = [desc(F16, t * kv * d * 2)] * 2, [pool(F16, kv=kv, d=d)] * 2
+        return dict(rows=dense, pools=pl, pc=args(seq_len=t, M=kv, head_dim=d))
+    assert call(lib, **rows(4095, 4097, 256))["count"] == 2 ** 32 - 256
+    refused(call, lib, **rows(8191, 8193, 64), match="too many rows")  # 2^32 - 64
