@@ -726,3 +726,25 @@ def test_attention_more_splits_than_threads(provider, act, pool):
     rng = np.random.default_rng(17)
     batch = ref.Batch(rng, [(40003, 1)], 16)
     check_attention(provider, rng, batch, act, pool, 1, 1, 64)
+
+
+@pytest.mark.parametrize("kv,dim,bs", [(4, 64, 16), (2, 128, 8), (1, 96, 5)])
+def test_flash_attention_paged_reads_the_cache(provider, kv, dim, bs):
+    """An f32 cache written by paged_kv_append serves flash_attention_paged too: the last token of one sequence."""
+    rng = np.random.default_rng(18)
+    heads, n = 4, 77
+    batch = ref.Batch(rng, [(n, n)], bs)
+    pools = [ref.empty_pool(rng, "f32", batch.blocks, kv, bs, dim) for _ in range(2)]
+    x = [rows_of(rng, "f32", n, kv, dim) for _ in range(2)]
+    q = rows_of(rng, "f32", n, heads, dim)
+    with Bufs(provider) as m:
+        kb, desc = [m.put(p) for p in pools], m.batch(batch)
+        provider.dispatch("paged_kv_append", [m.put(r) for r in x] + desc, kb, pc=pc_of(batch, kv, dim))
+        out = m.put(np.zeros_like(q[-1:]))
+        provider.dispatch("flash_attention_paged", [m.put(q[-1:])] + kb + desc[:1], [out],
+                          pc=push_constants(seq_len=1, n_heads=heads, head_dim=dim, M=kv, N=batch.width, step_idx=n - 1,
+                                            window_size=bs))
+        got = out.read(np.float32, heads * dim).reshape(heads, dim)
+    ref.append(batch, "f32", dim, pools, x)
+    want = ref.attention(batch, "f32", dim, heads, kv, pools, q, "f32")[0][-1]
+    check(got, want, 2e-5 * np.abs(want).max(), (kv, dim, bs))  # what that op's own test holds it to
