@@ -18,9 +18,10 @@ constexpr int kTile = 64;
 // Any head_dim, head ratio and alignment.  A workgroup takes one (row, head);
 // its four waves take 64-key tiles in turn: a lane scores one key, then the
 // lanes lie over head_dim for the tile's 64 value rows, and the waves' (m, l,
-// acc) are merged at the end.  The vector ALU and 4-byte loads bound it: 8
-// sequences of 4096 positions with 32 query and 8 KV heads of 80 take 787 us in
-// f16, where heads of 128 on the MFMA kernel take 23.
+// acc) are merged at the end.  Element loads, which every query head of a KV head
+// makes again, and the vector ALU bound it: single tokens of 8 sequences of 4096
+// positions with 32 query and 8 KV heads of 80 take 650 us in f16, where heads of 128
+// on the MFMA kernel take 31.
 template <typename T, PoolType PT>
 __global__ __launch_bounds__(256) void chunk_any_kernel(PagedBatch b, uint32_t n_heads, float scale,
                                                         const T* __restrict__ q, const uint8_t* __restrict__ kp,
@@ -390,7 +391,7 @@ __device__ __forceinline__ uint2 read_tr(const half_t* p) {
 // skips the pairs that are masked.
 // Bound by HBM at f16 (64 sequences of up to 8192 positions, 8 KV heads of 128: 1.35 GB
 // in 262 us, 5.2 TB/s, where a copy of 2 GiB reaches 4.9), by it and the conversion's
-// instructions at I8 (4 of up to 131072: 0.83 GB in 157 us, 5.3 TB/s); with 20 rows
+// instructions at I8 (4 of up to 131072: 0.83 GB in 158 to 166 us, 5.1 TB/s); with 20 rows
 // a sequence by the conversion (16 of up to 4096: 91 MB in 31 us).
 template <PoolType PT, int DD, int NT, bool UNI>
 __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
@@ -832,10 +833,12 @@ inline uint32_t wide_grid(uint32_t tiles, uint32_t n_kv) {
 // f16, are the B operand of O^T[dim][row] += V^T . P^T as they are.
 // Masking, the lazy rescale and values that are not finite: as above; tiles that
 // every row of the workgroup sees whole skip all of it.
-// Bound by MFMA issue and the softmax between: two sequences of 2048 tokens behind 6144,
-// 32 heads of 128, 481 GFLOP in 613 to 628 us, 770 TFLOP/s, where a matrix product of
-// 8192 in each size reaches 1093 and this kernel without its softmax and staging took
-// 364 us.  From I8 607 us: half the bytes to stage, the conversion beside the MFMAs.
+// No unit bounds it by itself: a wave takes scores, exponentials and P.V one after the
+// other.  Two sequences of 2048 tokens behind 6144, 32 heads of 128, 481 GFLOP in 604 to
+// 638 us (several cards), 750 to 800 TFLOP/s, where a matrix product of 8192 in each size
+// reaches 1093; the MFMA pipes are busy 32 % of the cycles, and without its softmax and
+// staging this kernel took 364 us.  From I8 594 to 631 us: half the bytes to stage, the
+// conversion beside the MFMAs.
 template <PoolType PT, int DD, bool UNI>
 __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
   constexpr bool I8 = PT == PoolType::I8;
@@ -914,7 +917,7 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
       } else {
         // A wave's 64 lie in one group, or in two.  It looks up those alone, by scalar
         // instructions: a choice among the addresses of all four was made by 64-bit
-        // multiplications in the vector ALU (I8, the same size: 953 us, and 607).
+        // multiplications in the vector ALU (I8, the same size: 953 us, and 594 to 631).
         const int c0 = 64 * (w + 4 * u), h0 = min(c0, 64 * CPR - 1) / (16 * CPR), h1 = min(c0 + 63, 64 * CPR - 1) / (16 * CPR);
         uint32_t so, rr = r - 16 * h0;
         uint64_t ro = rows.place(h0, so);
@@ -1488,9 +1491,10 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
 }
 
 // Many query rows: 64 a workgroup, 16 per wave, 32-key tiles of K and V in LDS.
-// Bound by the f32 MFMA and what of the grid stands still at the end: two sequences of
-// up to 512 tokens with up to 2048 positions, 32 heads of 128, 299 us; three of up to
-// 389 with 2000, 32 heads of 64, 9.5 GFLOP in 117 us with the combine (13 of them),
+// Bound by the f32 MFMA, busy 55 % of the cycles, and the waits between: one buffer and two
+// barriers a tile, few row tiles of unlike length, bank conflicts in 7 % of the cycles.
+// Two sequences of 512 tokens with 2048 positions, 32 heads of 128, 293 us; three of up
+// to 389 with 2000, 32 heads of 64, 9.5 GFLOP in 117 us with the combine (13 of them),
 // where a product of 8192 in each size reaches 153 TFLOP/s.
 template <PoolType PT, int DD, bool UNI>
 __global__ __launch_bounds__(256, 2) void chunk_wide_f32_kernel(Chunk c) {
