@@ -325,6 +325,7 @@ def _values(s, pool):
         codes = pages[..., :bs * d].contiguous().view(torch.int8).float()
         scale = pages[..., bs * d:].contiguous().view(torch.float16).float()
         x = (codes.reshape(scale.shape + (32,)) * scale[..., None]).reshape(pages.shape[:-1] + (bs, d))
+        x = x.to(TORCH[case["act"]]).float()  # an 8-bit cache stands for what a gather into the rows' type gives
     return x.transpose(1, 2).reshape(case["seqs"], case["kv"], -1, d)
 
 
@@ -491,7 +492,8 @@ def _exact_head(case, pool, pages, g):
     if case["pool"] != "i8":
         return x.double().reshape(-1, d)
     c = x[:, :bs * d].contiguous().view(torch.int8).double().reshape(-1, d // 32, 32)
-    return (c * x[:, bs * d:].contiguous().view(torch.float16).double().reshape(-1, d // 32, 1)).reshape(-1, d)
+    c = (c * x[:, bs * d:].contiguous().view(torch.float16).double().reshape(-1, d // 32, 1)).reshape(-1, d)
+    return c.to(TORCH[case["act"]]).double()  # by definition: rounded once to the rows' type
 
 
 def _exact_evict(s):
