@@ -28,7 +28,7 @@
  * paged key / value cache, and sampling of the next token.
  *   paged_kv_append     K_new, V_new, TABLES, STARTS, LENS -> K_pool, V_pool
  *   paged_kv_gather     K_pool, V_pool, TABLES, STARTS, LENS -> K, V
- *   flash_attention_paged_chunk   Q, K_pool, V_pool, TABLES, STARTS, LENS -> O
+ *   flash_attention_paged_chunk   Q, K_pool, V_pool, TABLES, STARTS, LENS -> O[, LSE]
  *     The batch is K = n_seqs sequences.  Rows STARTS[s] .. STARTS[s+1]-1
  *     (int32[n_seqs+1], not decreasing) of the dense operands are the last
  *     positions of sequence s, which has LENS[s] (int32[n_seqs]) of them, those
@@ -67,6 +67,48 @@
  *     of one append have to name slots of their own: what a slot holds that two of
  *     them name is not defined (an I8 slot may get one row's codes and the other's
  *     scales); no other slot is touched by it.
+ *     LSE f32[seq_len][n_heads], where it is given: the row's log-sum-exp, ln of the sum of
+ *     exp(score) over its keys, -inf for a row without any; an output of its own, no other
+ *     operand's buffer.
+ *   flash_attention_paged_prefix  Q, K_pool, V_pool, TABLES, STARTS, LENS, GROUPS, PREFIXES -> O[, LSE]
+ *     The same attention where sequences share their first positions, which are read once
+ *     for all of them.  step_idx = n_groups; the sequences GROUPS[g] .. GROUPS[g+1]-1
+ *     (int32[n_groups+1], not decreasing) share their first PREFIXES[g] (int32[n_groups])
+ *     positions: these lie where the table of sequence GROUPS[g] says, and what the others'
+ *     tables name for them is not read.  Sequences before GROUPS[0] and behind the last
+ *     group, and groups with a prefix of 0 or less, share nothing.  A row attends to the
+ *     positions 0 .. p as above, shared or not: a prefix may reach past new rows and past
+ *     a sequence's end.  At most 65535 groups; their contents are read when the op runs.
+ *   paged_kv_weights    Q, K_pool, TABLES, STARTS, LENS, LSE, HELD -> WEIGHTS
+ *     The attention weights that the rows give the cached positions, added up.  HELD and
+ *     WEIGHTS are f32[n_seqs][M][step_idx], an element for each KV head and position, with
+ *     step_idx at least the positions that a sequence may hold.  With LSE the attention's,
+ *       WEIGHTS[s][g][j] = theta HELD[s][g][j] + sum of exp(score of j - LSE[r][h]) over the
+ *     sequence's rows r at positions >= j and the query heads h that read KV head g.  theta
+ *     (0 to 1) lets older weights fade; 0 does not read HELD.  The positions of the rows
+ *     themselves start from 0, and so does one without storage.  A row whose LSE is -inf
+ *     gives nothing, nor does a score of -inf.  Positions past the length (or the bound)
+ *     and sequences without rows are left as they are.  WEIGHTS may be HELD's buffer; other
+ *     overlaps are not allowed.  Operands and limits are those of the attention.
+ *   paged_kv_evict      K_pool, V_pool, WEIGHTS, TABLES, LENS, BUDGET, NEW_TABLES
+ *                       -> K_pool', V_pool', WEIGHTS', NEW_LENS, KEPT
+ *     Of the L positions of a sequence every KV head keeps k = min(keep, L, seq_len), with
+ *     keep and recent = BUDGET[s][0], [1] (int32[n_seqs][2]; below 0: 0): the last r =
+ *     min(recent, k), and of the first L - r the k - r of the largest WEIGHTS (equal ones,
+ *     -0 and 0 among them: the lower position first; NaN and positions without storage are
+ *     below all others).  In order of position they become the positions 0 .. k-1:
+ *     KEPT[s][g][i] (int32[n_seqs][M][seq_len]) is the old position of the new one i,
+ *     WEIGHTS'[s][g][i] its weight, NEW_LENS[s] = k, and its rows go, bit for bit, to block
+ *     NEW_TABLES[s][i / block_size] (uint32[n_seqs][ceil(seq_len / block_size)]), slot
+ *     i % block_size, of K_pool' and V_pool', which may be the pools that are read.  Pools
+ *     F32, F16 or I8, all of one dtype.  A kept position without storage becomes zeros, a
+ *     new one without storage is skipped.  What is behind k is left as it was.  The new
+ *     blocks of two sequences have to differ, and no block that the op reads may be among
+ *     them (a block that several sequences share stays as it is); the other outputs may
+ *     not overlap any operand.  Push constants: M, N, K, head_dim, window_size, max_seq_len,
+ *     step_idx (the length of a row of weights, at least the positions a sequence may hold)
+ *     and seq_len = most positions kept, at most 2^22.  Keys keep what position they were
+ *     rotated for: a server counts positions for that by itself.
  *   sample_token        LOGITS, U, PARAMS, TOP_K -> TOKEN, PROB
  *     LOGITS [seq_len, N] F32 or F16; U f32[seq_len], random numbers of [0, 1);
  *     PARAMS f32[seq_len][3] = temperature, top_p, min_p; TOP_K int32[seq_len];

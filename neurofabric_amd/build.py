@@ -42,6 +42,9 @@ HIP_SOURCES = [
     CSRC / "kernels" / "attention.hip",
     CSRC / "kernels" / "paged.hip",
     CSRC / "kernels" / "paged_attention.hip",
+    CSRC / "kernels" / "paged_prefix.hip",
+    CSRC / "kernels" / "paged_weights.hip",
+    CSRC / "kernels" / "paged_evict.hip",
     CSRC / "kernels" / "sample.hip",
 ]
 CXX_SOURCES = [CSRC / "plan.cpp", CSRC / "plan_layer.cpp", CSRC / "model_ops.cpp"]

@@ -18,6 +18,7 @@ namespace nfk {
 namespace paged {
 
 using nfhip::PagedBatch;
+using nfhip::PagedShared;
 using nfhip::PoolType;
 
 // Sequence and position of row `row`; false when it belongs to none.
@@ -55,6 +56,25 @@ __device__ __forceinline__ bool find_row_wave(const PagedBatch& b, uint32_t row,
   return true;
 }
 
+// The shared positions of a sequence, read through the table of sequence `seq`: none
+// (len 0) for a sequence in no group.  `first` and the prefixes are device data too.
+struct SharedPrefix {
+  uint32_t seq;
+  int64_t len;
+};
+__device__ __forceinline__ SharedPrefix find_prefix(const PagedBatch& b, const PagedShared& sh, uint32_t seq) {
+  uint32_t lo = 0, hi = sh.n_groups;  // first g with first[g + 1] > seq
+  while (lo < hi) {
+    const uint32_t mid = (lo + hi) / 2;
+    if ((int64_t)sh.first[mid + 1] <= (int64_t)seq) lo = mid + 1;
+    else hi = mid;
+  }
+  if (lo >= sh.n_groups) return {seq, 0};
+  const int32_t a = sh.first[lo], n = sh.len[lo];
+  if (a < 0 || (uint32_t)a > seq || n <= 0) return {seq, 0};
+  return {(uint32_t)a, n < (int64_t)b.limit ? n : (int64_t)b.limit};
+}
+
 // Physical block of position `pos` of sequence `seq`, or ~0 without storage.
 __device__ __forceinline__ uint32_t find_block(const PagedBatch& b, uint32_t seq, int64_t pos) {
   if (pos < 0 || pos >= (int64_t)b.limit) return ~0u;
@@ -77,6 +97,14 @@ __device__ __forceinline__ float page_value(const PagedBatch& b, const uint8_t* 
   else
     return (float)(int)reinterpret_cast<const int8_t*>(page)[i] *
            (float)reinterpret_cast<const half_t*>(page + b.block_size * b.dim)[i / 32];
+}
+
+// The same as rows of type T see it: an I8 pool's values are rounded to f16 once for f16
+// rows.
+template <typename T, PoolType PT>
+__device__ __forceinline__ float row_value(const PagedBatch& b, const uint8_t* page, uint32_t slot, uint32_t d) {
+  const float x = page_value<PT>(b, page, slot, d);
+  return PT == PoolType::I8 ? (float)(T)x : x;
 }
 
 // The fp16 scale of 32 elements of type T and largest magnitude `amax`:

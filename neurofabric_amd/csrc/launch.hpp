@@ -158,8 +158,43 @@ hipError_t launch_paged_append(EType t, PoolType pool, const PagedBatch& b, cons
 hipError_t launch_paged_gather(EType t, PoolType pool, const PagedBatch& b, const void* k_pool, const void* v_pool,
                                void* k, void* v, hipStream_t s);
 // Attention of the batch's rows; `ws` holds the partials of keys split over workgroups.
+// lse: [rows, n_heads], or null.
 hipError_t launch_paged_chunk(EType t, PoolType pool, const PagedBatch& b, uint32_t n_heads, const void* q,
-                              const void* k_pool, const void* v_pool, void* out, const Workspace& ws, hipStream_t s);
+                              const void* k_pool, const void* v_pool, void* out, float* lse, const Workspace& ws,
+                              hipStream_t s);
+// The same where the sequences first[g] .. first[g + 1] - 1 share their first len[g]
+// positions, which lie where the table of the first of them says.
+struct PagedShared {
+  const int32_t* first = nullptr;  // [n_groups + 1]
+  const int32_t* len = nullptr;    // [n_groups]
+  uint32_t n_groups = 0;
+};
+hipError_t launch_paged_prefix(EType t, PoolType pool, const PagedBatch& b, const PagedShared& sh, uint32_t n_heads,
+                               const void* q, const void* k_pool, const void* v_pool, void* out, float* lse,
+                               const Workspace& ws, hipStream_t s);
+// weights[s][kv head][position] (rows of `width`) = theta held + the sum of the rows'
+// attention weights; theta 0 does not read `held`.
+hipError_t launch_paged_weights(EType t, PoolType pool, const PagedBatch& b, uint32_t n_heads, const void* q,
+                                const void* k_pool, const float* lse, const float* held, float* weights, uint32_t width,
+                                float theta, hipStream_t s);
+// Eviction: of each sequence and KV head the budget[s][1] last positions and those of the
+// largest weights, budget[s][0] together and at most `top`, in order of position; `kept`
+// [n_seqs, n_kv, top] says which, and their rows go to the blocks of `to` [n_seqs, ceil(top
+// / block_size)] in the second pools, of to_blocks blocks.  b.starts and b.rows are not used.
+struct PagedEvict {
+  const void* k = nullptr;
+  const void* v = nullptr;
+  const float* weights = nullptr;  // [n_seqs, n_kv, width]
+  const int32_t* budget = nullptr; // [n_seqs, 2]
+  const uint32_t* to = nullptr;
+  void* k_to = nullptr;
+  void* v_to = nullptr;
+  float* weights_to = nullptr;
+  int32_t* lens_to = nullptr;
+  int32_t* kept = nullptr;
+  uint32_t width = 0, top = 0, to_blocks = 0;
+};
+hipError_t launch_paged_evict(PoolType pool, const PagedBatch& b, const PagedEvict& e, hipStream_t s);
 
 // ---- sampling (kernels/sample.hip) ---------------------------------------------
 hipError_t launch_sample(EType t, const void* logits, const float* u, const float* params, const int32_t* top_k,

@@ -42,6 +42,9 @@ enum class Path {
   PagedAppend,  // paged_kv_append
   PagedGather,  // paged_kv_gather
   PagedChunk,   // flash_attention_paged_chunk
+  PagedPrefix,  // flash_attention_paged_prefix
+  PagedWeights, // paged_kv_weights
+  PagedEvict,   // paged_kv_evict
   Sample        // sample_token
 };
 
@@ -74,10 +77,13 @@ struct LayerParams {
   uint32_t n_experts = 0, top_k = 0;                     // MoE gating / scatter-gather
   PoolType pool = PoolType::F32;  // serving ops: rows = sequences, dim = block table width,
                                   // max_seq = positions a sequence may hold, count2 = blocks of the pools
+  uint32_t groups = 0, width = 0;  // serving: groups that share a prefix, positions a row of weights holds
+  uint64_t to_blocks = 0;          // paged_kv_evict: blocks of the pools that it writes
   uint64_t count2 = 0;  // attention_prefill: elements of the second output
   float eps = 0.f, theta = 0.f;
   bool decode = false;  // attention with step_idx > 0 (one query token)
   bool append = false;  // attention op that first writes K_new / V_new into the cache
+  bool lse = false;     // chunk / prefix attention with the rows' log-sum-exp as a second output
   bool noop = false;    // nothing to launch (decode at step >= max_seq_len, as the reference)
 };
 

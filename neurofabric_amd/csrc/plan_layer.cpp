@@ -5,7 +5,8 @@
 // (causal_attention, causal_attention_cached, flash_attention_cached,
 // flash_attention_gqa, flash_attention_paged), and the serving ops, which have
 // no counterpart in the reference: paged_kv_append, paged_kv_gather,
-// flash_attention_paged_chunk and sample_token.
+// flash_attention_paged_chunk, flash_attention_paged_prefix, paged_kv_weights,
+// paged_kv_evict and sample_token.
 //
 // Semantics follow the reference's Metal host code (metal_provider.mm:2313-2990,
 // 3034-3079): the f16 variant is picked from the OUTPUT dtype, element counts
@@ -63,6 +64,9 @@ const std::unordered_map<std::string, LayerInfo>& layer_table() {
       {"paged_kv_append", {Path::PagedAppend, EwFn::Add, AttnMode::Paged, true, false, false}},
       {"paged_kv_gather", {Path::PagedGather, EwFn::Add, AttnMode::Paged, true, true, false}},
       {"flash_attention_paged_chunk", {Path::PagedChunk, EwFn::Add, AttnMode::Paged, true, true, false}},
+      {"flash_attention_paged_prefix", {Path::PagedPrefix, EwFn::Add, AttnMode::Paged, true, true, false}},
+      {"paged_kv_weights", {Path::PagedWeights, EwFn::Add, AttnMode::Paged, true, false, false}},
+      {"paged_kv_evict", {Path::PagedEvict, EwFn::Add, AttnMode::Paged, true, false, false}},
       {"sample_token", {Path::Sample, EwFn::Add, AttnMode::Plain, true, false, false}},
   };
   return t;
@@ -268,26 +272,127 @@ nf_status plan_paged_rows(bool append, const nf_tensor_desc* const* ins, uint32_
   return NF_OK;
 }
 
-nf_status plan_paged_chunk(const nf_tensor_desc* const* ins, uint32_t n_in, const nf_tensor_desc* const* outs,
+// The query heads of an attention over a paged cache, and Q.
+nf_status plan_paged_heads(const nf_tensor_desc* q, uint32_t n_heads, Plan* p, std::string* why) {
+  LayerParams& lp = p->lp;
+  lp.n_heads = n_heads;
+  if (lp.n_heads < lp.n_kv) return fail(why, "n_heads must be at least M (KV heads)");
+  if (lp.n_heads > 65535) return fail(why, "more than 65535 heads");
+  const uint64_t n = (uint64_t)lp.seq_len * lp.n_heads * lp.head_dim;
+  if (n >= kMaxElems) return fail(why, "attention problem too large");
+  if (!fits(q, n, elt_bytes(p->a))) return fail(why, "Q holds fewer than seq_len * n_heads * head_dim elements");
+  return NF_OK;
+}
+
+// flash_attention_paged_chunk and, with groups of sequences behind its inputs,
+// flash_attention_paged_prefix.
+nf_status plan_paged_chunk(bool prefix, const nf_tensor_desc* const* ins, uint32_t n_in, const nf_tensor_desc* const* outs,
                            uint32_t n_out, const Pc& pc, Plan* p, std::string* why) {
-  if (n_in < 6 || n_out < 1) return fail(why, "takes 6 inputs and 1 output");
+  if (n_in < (prefix ? 8u : 6u) || n_out < 1) return fail(why, prefix ? "takes 8 inputs and 1 output, or 2" : "takes 6 inputs and 1 output, or 2");
   const nf_tensor_desc* dense[2] = {ins[0], outs[0]};
   Pc c = pc;
   c.M = pc.M ? pc.M : pc.n_heads;
   nf_status st = plan_paged_batch(dense, 2, ins + 1, ins + 3, c, p, why);
   if (st != NF_OK) return st;
   LayerParams& lp = p->lp;
-  lp.n_heads = pc.n_heads;
-  if (lp.n_heads < lp.n_kv) return fail(why, "n_heads must be at least M (KV heads)");
-  if (lp.n_heads > 65535) return fail(why, "more than 65535 heads");
+  st = plan_paged_heads(ins[0], pc.n_heads, p, why);
+  if (st != NF_OK) return st;
   const uint64_t n = (uint64_t)lp.seq_len * lp.n_heads * lp.head_dim, elt = elt_bytes(p->a);
-  if (n >= kMaxElems) return fail(why, "attention problem too large");
-  if (!fits(ins[0], n, elt)) return fail(why, "Q holds fewer than seq_len * n_heads * head_dim elements");
   if (!fits(outs[0], n, elt)) return fail(why, "output holds fewer than seq_len * n_heads * head_dim elements");
   p->count = (uint64_t)lp.seq_len * lp.n_heads;
+  lp.lse = n_out > 1;
+  if (lp.lse) {
+    if (!outs[1]) return fail(why, "null descriptor");
+    if (outs[1]->dtype != NF_DTYPE_F32) return fail(why, "the log-sum-exp must be F32");
+    if (!fits(outs[1], p->count, 4)) return fail(why, "the log-sum-exp holds fewer than seq_len * n_heads elements");
+  }
+  if (prefix) {
+    if (!ins[6] || !ins[7]) return fail(why, "null descriptor");
+    lp.groups = pc.step;
+    if (lp.groups > 65535) return fail(why, "more than 65535 groups");
+    if (!fits(ins[6], (uint64_t)lp.groups + 1, 4)) return fail(why, "groups hold fewer than step_idx + 1 entries");
+    if (!fits(ins[7], lp.groups, 4)) return fail(why, "prefixes hold fewer than step_idx entries");
+  }
   p->act_bytes = n * elt;
-  p->out_bytes = n * elt;
-  p->kernel = std::string("attention_paged_chunk_") + tname(p->a) + "_" + pname(lp.pool);
+  p->out_bytes = n * elt + (n_out > 1 ? 4 * p->count : 0);
+  p->kernel = std::string(prefix ? "attention_paged_prefix_" : "attention_paged_chunk_") + tname(p->a) + "_" + pname(lp.pool);
+  return NF_OK;
+}
+
+// Rows of weights, F32 [K][M][step_idx], one element for each position a sequence may hold.
+nf_status plan_weight_rows(const nf_tensor_desc* const* rows, uint32_t n, Plan* p, std::string* why) {
+  const LayerParams& lp = p->lp;
+  if (lp.width < lp.max_seq) return fail(why, "step_idx (a row of weights) is less than the positions a sequence may hold");
+  for (uint32_t i = 0; i < n; ++i) {
+    if (!rows[i]) return fail(why, "null descriptor");
+    if (rows[i]->dtype != NF_DTYPE_F32) return fail(why, "weights must be F32");
+    if (lp.width && !fits(rows[i], (uint64_t)lp.rows * lp.n_kv, 4ull * lp.width))
+      return fail(why, "weights hold fewer than K * M * step_idx elements");
+  }
+  return NF_OK;
+}
+
+nf_status plan_paged_weights(const nf_tensor_desc* const* ins, uint32_t n_in, const nf_tensor_desc* const* outs,
+                             uint32_t n_out, const Pc& pc, Plan* p, std::string* why) {
+  if (n_in < 7 || n_out < 1) return fail(why, "takes 7 inputs and 1 output");
+  const nf_tensor_desc* pools[2] = {ins[1], ins[1]};
+  Pc c = pc;
+  c.M = pc.M ? pc.M : pc.n_heads;
+  nf_status st = plan_paged_batch(ins, 1, pools, ins + 2, c, p, why);
+  if (st != NF_OK) return st;
+  LayerParams& lp = p->lp;
+  st = plan_paged_heads(ins[0], pc.n_heads, p, why);
+  if (st != NF_OK) return st;
+  p->count = (uint64_t)lp.seq_len * lp.n_heads;
+  if (!ins[5]) return fail(why, "null descriptor");
+  if (ins[5]->dtype != NF_DTYPE_F32) return fail(why, "the log-sum-exp must be F32");
+  if (!fits(ins[5], p->count, 4)) return fail(why, "the log-sum-exp holds fewer than seq_len * n_heads elements");
+  if (!(pc.theta >= 0.f && pc.theta <= 1.f)) return fail(why, "theta must be in 0 .. 1");
+  lp.theta = pc.theta;
+  lp.width = pc.step;
+  const nf_tensor_desc* rows[2] = {ins[6], outs[0]};
+  st = plan_weight_rows(rows, 2, p, why);
+  if (st != NF_OK) return st;
+  p->act_bytes = p->count * (lp.head_dim * elt_bytes(p->a) + 4);
+  p->out_bytes = 4ull * lp.rows * lp.n_kv * lp.width;
+  p->kernel = std::string("paged_weights_") + tname(p->a) + "_" + pname(lp.pool);
+  return NF_OK;
+}
+
+nf_status plan_paged_evict(const nf_tensor_desc* const* ins, uint32_t n_in, const nf_tensor_desc* const* outs,
+                           uint32_t n_out, const Pc& pc, Plan* p, std::string* why) {
+  if (n_in < 7 || n_out < 5) return fail(why, "takes 7 inputs and 5 outputs");
+  for (uint32_t i = 0; i < 7; ++i)
+    if (!ins[i] || (i < 5 && !outs[i])) return fail(why, "null descriptor");
+  // There are no dense rows: those of the pools' dtype stand for them.
+  nf_tensor_desc row = *ins[0];
+  if (row.dtype == NF_DTYPE_I8) row.dtype = NF_DTYPE_F16;
+  const nf_tensor_desc* dense[1] = {&row};
+  const nf_tensor_desc* batch[3] = {ins[3], nullptr, ins[4]};
+  nf_tensor_desc starts = *ins[4];  // nor row starts
+  starts.size_bytes = ~0ull;
+  batch[1] = &starts;
+  nf_status st = plan_paged_batch(dense, 1, ins, batch, pc, p, why);
+  if (st != NF_OK) return st;
+  LayerParams& lp = p->lp;
+  lp.width = pc.step;
+  const uint64_t S = lp.rows;
+  if (outs[0]->dtype != ins[0]->dtype || outs[1]->dtype != ins[0]->dtype)
+    return fail(why, "the pools that are read and written must have one dtype");
+  const nf_tensor_desc* rows[2] = {ins[2], outs[2]};
+  st = plan_weight_rows(rows, 2, p, why);
+  if (st != NF_OK) return st;
+  if (!fits(ins[5], 2 * S, 4)) return fail(why, "budgets hold fewer than K * 2 entries");
+  const uint64_t pages = ((uint64_t)lp.seq_len + lp.block_size - 1) / lp.block_size;
+  if (!fits(ins[6], S * pages, 4)) return fail(why, "new block tables hold fewer than K * ceil(seq_len / block_size) entries");
+  if (!fits(outs[3], S, 4)) return fail(why, "new lengths hold fewer than K entries");
+  if (!fits(outs[4], S * lp.n_kv, 4ull * lp.seq_len)) return fail(why, "kept positions hold fewer than K * M * seq_len entries");
+  const uint64_t block = page_bytes(lp.pool, (uint64_t)lp.block_size * lp.head_dim) * lp.n_kv;
+  lp.to_blocks = std::min<uint64_t>(std::min(outs[0]->size_bytes, outs[1]->size_bytes) / block, 0xFFFFFFFFu);
+  p->count = S * lp.n_kv * lp.seq_len;
+  p->act_bytes = 4ull * S * lp.n_kv * lp.width;
+  p->out_bytes = p->count * 8;
+  p->kernel = std::string("paged_evict_") + pname(lp.pool);
   return NF_OK;
 }
 
@@ -516,8 +621,19 @@ nf_status make_layer_plan(const char* op_name, const nf_tensor_desc* const* ins,
       if (st != NF_OK) return st;
       break;
     }
-    case Path::PagedChunk: {
-      nf_status st = plan_paged_chunk(ins, n_in, outs, n_out, pc, &p, why);
+    case Path::PagedChunk:
+    case Path::PagedPrefix: {
+      nf_status st = plan_paged_chunk(info.path == Path::PagedPrefix, ins, n_in, outs, n_out, pc, &p, why);
+      if (st != NF_OK) return st;
+      break;
+    }
+    case Path::PagedWeights: {
+      nf_status st = plan_paged_weights(ins, n_in, outs, n_out, pc, &p, why);
+      if (st != NF_OK) return st;
+      break;
+    }
+    case Path::PagedEvict: {
+      nf_status st = plan_paged_evict(ins, n_in, outs, n_out, pc, &p, why);
       if (st != NF_OK) return st;
       break;
     }

@@ -644,7 +644,37 @@ hipError_t run_plan(const Plan& pl, Buffer* const* in, Buffer* const* out, int g
                                  out[1]->dev, s);
     case Path::PagedChunk:
       return launch_paged_chunk(pl.a, pl.lp.pool, paged_batch(pl, in + 3), pl.lp.n_heads, in[0]->dev, in[1]->dev,
-                                in[2]->dev, out[0]->dev, ws, s);
+                                in[2]->dev, out[0]->dev, pl.lp.lse ? static_cast<float*>(out[1]->dev) : nullptr, ws, s);
+    case Path::PagedPrefix: {
+      PagedShared sh;
+      sh.first = static_cast<const int32_t*>(in[6]->dev);
+      sh.len = static_cast<const int32_t*>(in[7]->dev);
+      sh.n_groups = pl.lp.groups;
+      return launch_paged_prefix(pl.a, pl.lp.pool, paged_batch(pl, in + 3), sh, pl.lp.n_heads, in[0]->dev, in[1]->dev,
+                                 in[2]->dev, out[0]->dev, pl.lp.lse ? static_cast<float*>(out[1]->dev) : nullptr, ws, s);
+    }
+    case Path::PagedWeights:
+      return launch_paged_weights(pl.a, pl.lp.pool, paged_batch(pl, in + 2), pl.lp.n_heads, in[0]->dev, in[1]->dev,
+                                  static_cast<const float*>(in[5]->dev), static_cast<const float*>(in[6]->dev),
+                                  static_cast<float*>(out[0]->dev), pl.lp.width, pl.lp.theta, s);
+    case Path::PagedEvict: {
+      Buffer* const batch[3] = {in[3], in[4], in[4]};  // row starts are not used
+      PagedEvict e;
+      e.k = in[0]->dev;
+      e.v = in[1]->dev;
+      e.weights = static_cast<const float*>(in[2]->dev);
+      e.budget = static_cast<const int32_t*>(in[5]->dev);
+      e.to = static_cast<const uint32_t*>(in[6]->dev);
+      e.k_to = out[0]->dev;
+      e.v_to = out[1]->dev;
+      e.weights_to = static_cast<float*>(out[2]->dev);
+      e.lens_to = static_cast<int32_t*>(out[3]->dev);
+      e.kept = static_cast<int32_t*>(out[4]->dev);
+      e.width = pl.lp.width;
+      e.top = pl.lp.seq_len;
+      e.to_blocks = (uint32_t)pl.lp.to_blocks;
+      return launch_paged_evict(pl.lp.pool, paged_batch(pl, batch), e, s);
+    }
     case Path::Sample:
       return launch_sample(pl.a, in[0]->dev, static_cast<const float*>(in[1]->dev),
                            static_cast<const float*>(in[2]->dev), static_cast<const int32_t*>(in[3]->dev),
