@@ -42,6 +42,7 @@ HIP_SOURCES = [
     CSRC / "kernels" / "attention.hip",
     CSRC / "kernels" / "paged.hip",
     CSRC / "kernels" / "paged_attention.hip",
+    CSRC / "kernels" / "paged_lse.hip",
     CSRC / "kernels" / "paged_prefix.hip",
     CSRC / "kernels" / "paged_weights.hip",
     CSRC / "kernels" / "paged_evict.hip",

@@ -131,7 +131,16 @@ struct RowTile {
   uint32_t start;             // the sequence's first token
   int pos0;                   // position of that token
   int len;                    // positions of the sequence, at most `limit`
+  // kShared:
+  uint32_t pre;               // sequence whose table the shared positions are read through
+  int shared;                 // shared positions
+  uint32_t last;              // a group's rows: one past its last sequence; else 0
+  uint32_t slot, splits;      // of the rows' partials this part's first one; splits of its keys
 };
+
+// What a kernel serves: flash_attention_paged_chunk, the same with the rows'
+// log-sum-exp, or flash_attention_paged_prefix (with it where it is wanted).
+enum Form { kChunk, kLse, kShared };
 
 __device__ __forceinline__ bool find_tile(const PagedBatch& b, uint32_t idx, uint32_t G, uint32_t per, uint64_t lo,
                                           uint64_t hi, RowTile& t) {
@@ -187,11 +196,159 @@ struct Chunk {
   uint32_t tiles;  // grid size: row tiles per KV head
   uint64_t lo, hi; // query rows of the sequences that this launch takes
   float scale_log2;  // scale * log2(e): softmax in base 2
+  // kLse, kShared:
+  float* lse;    // output, or null
+  float* lsum;   // partials, f16: sum of the weights as they were before they were rounded
+  PagedShared sh;  // kShared
+  bool apart;      // the groups' shared keys are parts of their own
 };
 
 // Splits that a sequence of `len` positions takes.
 __device__ __forceinline__ uint32_t splits_of(const Chunk& c, int len) {
   return len <= 0 ? 1u : ((uint32_t)len + c.keys_per_split - 1) / c.keys_per_split;
+}
+
+// The keys of a sequence with shared positions, as the tiles count them.  A tile lies on
+// one side of the border `shared`, and starts at a multiple of 16: the shared keys count
+// 0 .. shared - 1, the own ones follow at the next multiple of 64, from the last multiple
+// of 16 that is not past the border (the keys between are masked).  Apart: no shared keys.
+struct Border {
+  int split, shift;  // count from which keys are own, and what is taken off it for the position
+  int end;           // counts below it
+};
+__device__ __forceinline__ Border find_border(bool apart, int shared, int end) {
+  if (end <= shared) return {0x7FFFFFFF, 0, apart || end < 0 ? 0 : end};
+  const int split = apart ? 0 : (shared + 63) & ~63, shift = split - (shared & ~15);
+  return {split, shift, end + shift};
+}
+// Splits of the partials of a row: those of its group's part, then those of its own.
+struct Slots {
+  uint32_t group, own;
+};
+__device__ __forceinline__ Slots find_slots(const Chunk& c, int shared, int len) {
+  const uint32_t group = c.apart && shared > 0 ? splits_of(c, shared) : 0;
+  const int n = find_border(c.apart, shared, len).end;
+  return {group, n <= 0 && group ? 0 : splits_of(c, n)};
+}
+
+// kShared: tile `idx` of KV head and batch in the order of the parts: first the groups'
+// shared keys (where they are apart), then the sequences; of a part, all tiles of a split
+// after each other, so that they share its keys in the caches.  `from` and `done` hold the
+// place that a call with a smaller idx came to.
+__device__ __forceinline__ bool find_part(const Chunk& c, uint32_t idx, uint32_t per, RowTile& t, uint32_t& sp,
+                                          uint32_t& from, uint32_t& done) {
+  const PagedBatch& b = c.b;
+  const int lane = threadIdx.x & 63;
+  const uint32_t groups = c.apart ? c.sh.n_groups : 0, parts = groups + b.n_seqs;
+  for (; from < parts; from += 64) {
+    const uint32_t e = from + lane;
+    uint32_t n = 0, start = 0, seq = 0, pre = 0, last = 0, slot = 0, splits = 0;
+    int32_t len = 0, pos0 = 0, shared = 0;
+    if (e < groups) {
+      const int32_t a = c.sh.first[e], z = c.sh.first[e + 1], p = c.sh.len[e];
+      if (a >= 0 && z > a && (uint32_t)a < b.n_seqs && p > 0) {
+        last = (uint32_t)z < b.n_seqs ? (uint32_t)z : b.n_seqs;
+        seq = pre = (uint32_t)a;
+        shared = len = p < (int64_t)b.limit ? p : (int)b.limit;
+        const int64_t r0 = b.starts[a] > 0 ? b.starts[a] : 0, r1 = b.starts[last];
+        const int64_t r2 = r1 < (int64_t)b.rows ? r1 : (int64_t)b.rows;
+        start = (uint32_t)r0;
+        n = r2 > r0 ? (uint32_t)(r2 - r0) : 0;
+        splits = splits_of(c, shared);
+      }
+    } else if (e < parts) {
+      seq = e - groups;
+      const int64_t a = b.starts[seq], z = b.starts[seq + 1];
+      const int32_t l = b.lens[seq];
+      if (a >= 0 && z > a && z <= (int64_t)b.rows) {
+        n = (uint32_t)(z - a);
+        start = (uint32_t)a;
+        pos0 = (int)((uint32_t)l - n);
+        len = l < (int64_t)b.limit ? l : (int)b.limit;
+        const SharedPrefix p = find_prefix(b, c.sh, seq);
+        pre = p.seq;
+        shared = (int)p.len;
+        const Slots s = find_slots(c, shared, len);
+        slot = s.group;
+        splits = s.own;
+      }
+    }
+    const uint64_t rows = (uint64_t)n * c.group;
+    const uint32_t tiles = rows > c.lo && rows <= c.hi ? (uint32_t)((rows + per - 1) / per) : 0;
+    const uint32_t mine = tiles * splits;
+    uint32_t up = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t v = __shfl_up(up, o);
+      if (lane >= o) up += v;
+    }
+    const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)up, 63);
+    if (idx - done < total) {
+      const uint32_t i = idx - done;
+      const int at = __builtin_ctzll(__ballot(up > i));
+      auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, at); };
+      const uint32_t k = i - of(up - mine), nt = of(tiles);
+      sp = k / nt;
+      t.first = (k - sp * nt) * per;
+      t.seq = of(seq);
+      t.rows = of((uint32_t)rows);
+      t.start = of(start);
+      t.pos0 = (int)of((uint32_t)pos0);
+      t.len = (int)of((uint32_t)len);
+      t.pre = of(pre);
+      t.shared = (int)of((uint32_t)shared);
+      t.last = of(last);
+      t.slot = of(slot);
+      t.splits = of(splits);
+      return true;
+    }
+    done += total;
+  }
+  return false;
+}
+
+// Whether every row of a group sees all of the shared keys.
+__device__ __forceinline__ bool see_all(const PagedBatch& b, const RowTile& t) {
+  bool all = true;
+  for (uint32_t s0 = t.seq; s0 < t.last; s0 += 64) {
+    const uint32_t s = s0 + (threadIdx.x & 63);
+    if (s < t.last && b.starts[s + 1] > b.starts[s])
+      all = all && (int64_t)b.lens[s] - ((int64_t)b.starts[s + 1] - (int64_t)b.starts[s]) + 1 >= (int64_t)t.shared;
+  }
+  return __ballot(!all) == 0;
+}
+constexpr int kEverywhere = 0x3FFFFFFF;  // the position of a row that sees all keys
+
+// Position of a query row's token: of a group's rows, that in whatever sequence it is.
+template <Form FORM>
+__device__ __forceinline__ int row_pos(const PagedBatch& b, const RowTile& t, uint32_t token, bool all) {
+  if (FORM != kShared || t.last == 0) return t.pos0 + (int)token;
+  if (all) return kEverywhere;
+  uint32_t seq;
+  int64_t pos;
+  return find_row(b, t.start + token, seq, pos) ? pos < kEverywhere ? (int)pos : kEverywhere : -1;
+}
+
+// The keys of a tile of rows, from its first row's token to its last's.
+struct Keys {
+  Border at;
+  int lo;  // every row sees the positions up to it
+  int hi;  // none sees one past it
+};
+template <Form FORM>
+__device__ __forceinline__ Keys find_keys(const Chunk& c, const RowTile& t, uint32_t first_token, uint32_t last_token, bool all) {
+  const int lo = t.pos0 + (int)first_token, hi = t.pos0 + (int)last_token;
+  const int end = hi + 1 < t.len ? hi + 1 : t.len;
+  if constexpr (FORM == kShared) {
+    if (t.last) return {{0x7FFFFFFF, 0, t.shared}, all ? kEverywhere : -1, kEverywhere};
+    return {find_border(c.apart, t.shared, end), lo, hi};
+  }
+  return {{0, 0, end}, lo, hi};
+}
+
+// ln of a sum of weights 2^(x - m + log2), times the sum that m stands for.
+__device__ __forceinline__ float lse_of(float m, float l, float log2) {
+  return l == 0.f ? -INFINITY : (m + (__builtin_amdgcn_logf(l) - log2)) * 0.6931471805599453f;
 }
 
 __device__ __forceinline__ uint64_t shfl64(uint64_t v, int src) {
@@ -208,7 +365,8 @@ __device__ __forceinline__ uint64_t shfl64(uint64_t v, int src) {
 // that they arrive while the one before is computed; by vector loads, as scalar ones
 // and LDS reads share a counter that can only be waited for as a whole.  Keys without
 // a row have that of the pool's first key, and no bit in have().
-template <PoolType PT, int DD, int N, bool UNI>
+// SHARE: keys are counted as Border says; at() is the position of a tile's first key.
+template <PoolType PT, int DD, int N, bool UNI, bool SHARE>
 struct Rows {
   static constexpr uint32_t kRow = PT == PoolType::I8 ? DD : PT == PoolType::F16 ? 2 * DD : 4 * DD;
   const PagedBatch& b;
@@ -225,50 +383,74 @@ struct Rows {
   uint32_t sc, next_sc;
   uint64_t valid, next_valid;
 
-  __device__ __forceinline__ Rows(const PagedBatch& b_, uint32_t seq, uint32_t kvh, int end_)
-      : b(b_), table(b_.table + (uint64_t)seq * b_.width),
+  const uint32_t* common;  // SHARE: the table of the shared keys
+  Border border;
+  int shared;
+
+  __device__ __forceinline__ Rows(const PagedBatch& b_, const RowTile& t, uint32_t kvh, int end_, const Border& at_)
+      : b(b_), table(b_.table + (uint64_t)t.seq * b_.width),
         page((uint32_t)nfhip::page_bytes(PT, (uint64_t)b_.block_size * DD)), block((uint64_t)b_.n_kv * page),
-        head((uint64_t)kvh * page), end(end_), shift(__builtin_ctz(b_.block_size)) {}
+        head((uint64_t)kvh * page), end(end_), shift(__builtin_ctz(b_.block_size)) {
+    if constexpr (SHARE) {
+      common = b_.table + (uint64_t)t.pre * b_.width;
+      border = at_;
+      shared = t.shared;
+    }
+  }
+  __device__ __forceinline__ bool own(int t0) const { return !SHARE || t0 >= border.split; }
+  __device__ __forceinline__ int at(int t0) const { return SHARE && own(t0) ? t0 - border.shift : t0; }
+  // The table of a tile's keys, and the position below which they lie.
+  __device__ __forceinline__ const uint32_t* table_of(int t0) const { return own(t0) ? table : common; }
+  __device__ __forceinline__ int end_of(int t0) const {
+    return !SHARE ? end : own(t0) ? end - border.shift : shared < end ? shared : end;
+  }
+  // The keys of a tile that are not before the border, as bits.
+  __device__ __forceinline__ uint64_t behind(int t0) const {
+    if (!SHARE || !own(t0)) return ~0ull;
+    const int before = shared - at(t0);  // at most 15
+    return before <= 0 ? ~0ull : ~0ull << before;
+  }
   // From a key's row to its scales.
   __device__ __forceinline__ uint32_t to_scales(uint32_t at) const {
     return PT == PoolType::I8 ? (b.block_size - at) * DD + at * (DD / 16) : 0;
   }
   __device__ __forceinline__ void look(int t0) {
     if constexpr (UNI) {
-      const int p = t0 + 16 * (int)(threadIdx.x & (N - 1));
-      entry = table[(uint32_t)min(p, end - 1) >> shift];  // past the end: the last key's block, whose bits are cleared
+      const int p = at(t0) + 16 * (int)(threadIdx.x & (N - 1));
+      entry = table_of(t0)[(uint32_t)min(p, end_of(t0) - 1) >> shift];  // past the end: the last key's block, whose bits are cleared
     } else {
-      const int p = t0 + (int)(threadIdx.x & (16 * N - 1));
+      const int p = at(t0) + (int)(threadIdx.x & (16 * N - 1));
       next_off = 0;
       next_sc = 0;
       bool ok = false;
-      if (p < end) {
-        const uint32_t k = (uint32_t)p / b.block_size, at = (uint32_t)p - k * b.block_size, phys = table[k];
+      if (p < end_of(t0)) {
+        const uint32_t k = (uint32_t)p / b.block_size, at = (uint32_t)p - k * b.block_size, phys = table_of(t0)[k];
         ok = phys < b.blocks;
         if (ok) {
           next_off = phys * block + head + at * kRow;
           next_sc = to_scales(at);
         }
       }
-      next_valid = __ballot(ok);
+      next_valid = __ballot(ok) & behind(t0);
       if constexpr (N < 4) next_valid &= (1ull << (16 * N)) - 1;
     }
   }
   __device__ __forceinline__ void take(int t0) {
     if constexpr (UNI) {
-      cur = t0;
+      cur = at(t0);
       valid = 0;
 #pragma unroll
       for (int h = 0; h < N; ++h) {
         const uint32_t phys = (uint32_t)__builtin_amdgcn_readlane((int)entry, h);
-        const uint32_t at = (uint32_t)(t0 + 16 * h) & (b.block_size - 1);
+        const uint32_t at = (uint32_t)(cur + 16 * h) & (b.block_size - 1);
         const bool ok = phys < b.blocks;
         base[h] = ok ? phys * block + head + at * kRow : 0;
         scales[h] = ok ? to_scales(at) : 0;
         valid |= (uint64_t)(ok ? 0xFFFFu : 0u) << (16 * h);
       }
-      const int left = end - t0;
-      if (left < 16 * N) valid &= (1ull << left) - 1;
+      const int left = end_of(t0) - cur;
+      if (left < 16 * N) valid &= SHARE && left <= 0 ? 0 : (1ull << left) - 1;
+      valid &= behind(t0);
     } else {
       off = next_off;
       sc = next_sc;
@@ -401,8 +583,10 @@ __device__ __forceinline__ uint2 read_tr(const half_t* p) {
 // in 262 us, 5.2 TB/s, where a copy of 2 GiB reaches 4.9), by it and the conversion's
 // instructions at I8 (4 of up to 131072: 0.83 GB in 158 to 166 us, 5.1 TB/s); with 20 rows
 // a sequence by the conversion (16 of up to 4096: 91 MB in 31 us).
-template <PoolType PT, int DD, int NT, bool UNI>
-__global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
+// kLse, kShared: the log-sum-exp takes the weights as they were before they are rounded.
+template <PoolType PT, int DD, int NT, bool UNI, Form FORM>
+__device__ __forceinline__ void narrow_tile(const Chunk& c, const RowTile& t, uint32_t sp, uint32_t ns, uint32_t kvh) {
+  constexpr bool SHARE = FORM == kShared, LSE = FORM != kChunk;
   constexpr bool I8 = PT == PoolType::I8;
   constexpr int KSTEP = DD / 32, DB = DD / 16;
   // LDS row (halves): 8 dwords past a multiple of 64 or an odd multiple of 8, so that
@@ -413,22 +597,17 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
   constexpr int NP = KSTEP / 2;                      // I8: 16-code loads per key row
   __shared__ __attribute__((aligned(16))) half_t vs[4][32 * VP];
   __shared__ __attribute__((aligned(16))) float ps[4][32][16];
-  __shared__ float wm[4][16 * NT], wl[4][16 * NT];
+  __shared__ float wm[4][16 * NT], wl[4][16 * NT], wx[LSE ? 4 : 1][16 * NT];
   static_assert(sizeof(float) * 16 * DD <= sizeof(half_t) * 32 * VP, "a wave's rows merge in its part of vs");
 
-  const uint32_t sp = blockIdx.x % c.splits, kvh = blockIdx.y;
-  RowTile t;
-  if (!find_tile(c.b, blockIdx.x / c.splits, c.group, 16 * NT, c.lo, c.hi, t)) return;
-  const uint32_t ns = splits_of(c, t.len);
-  if (sp >= ns) return;
   const uint32_t G = c.group, H = c.n_heads;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t live = t.rows - t.first < 16u * NT ? t.rows - t.first : 16u * NT;
-  // positions of the tile's rows, first to last
-  const int pos_lo = t.pos0 + (int)(t.first / G), pos_hi = t.pos0 + (int)((t.first + live - 1) / G);
-  const int begin = (int)(sp * c.keys_per_split);
-  int end = pos_hi + 1 < t.len ? pos_hi + 1 : t.len;  // keys below it
+  const bool all = SHARE && t.last && see_all(c.b, t);
+  const Keys keys = find_keys<FORM>(c, t, t.first / G, (t.first + live - 1) / G, all);
+  const int pos_lo = keys.lo, begin = (int)(sp * c.keys_per_split);
+  int end = keys.at.end;  // keys below it
   if (end > begin + (int)c.keys_per_split) end = begin + (int)c.keys_per_split;
   end = __builtin_amdgcn_readfirstlane(end);
 
@@ -437,7 +616,7 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
 #pragma unroll
   for (int u = 0; u < NT; ++u) {
     const uint32_t r = t.first + 16 * u + n < t.rows ? t.first + 16 * u + n : t.rows - 1;
-    pos[u] = t.pos0 + (int)(r / G);
+    pos[u] = row_pos<FORM>(c.b, t, r / G, all);
     const half_t* qr = static_cast<const half_t*>(c.q) + ((uint64_t)(t.start + r / G) * H + kvh * G + r % G) * DD;
 #pragma unroll
     for (int s = 0; s < KSTEP; ++s) {
@@ -446,11 +625,11 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
     }
   }
   float4v ot[NT][DB];
-  float m[NT], l[NT];
+  float m[NT], l[NT], lx[NT];
 #pragma unroll
   for (int u = 0; u < NT; ++u) {
     m[u] = -INFINITY;
-    l[u] = 0.f;
+    l[u] = lx[u] = 0.f;
 #pragma unroll
     for (int d = 0; d < DB; ++d) ot[u][d] = float4v{0.f, 0.f, 0.f, 0.f};
   }
@@ -460,7 +639,7 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
   half_t kd[2][KSTEP]; // I8: scales
   u32x4 vraw[NV];
   half_t vd[NV];
-  Rows<PT, DD, 2, UNI> rows(c.b, t.seq, kvh, end);
+  Rows<PT, DD, 2, UNI, SHARE> rows(c.b, t, kvh, end, keys.at);
   auto fetch = [&]() {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -581,7 +760,7 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int k = 16 * j + 4 * g + i;
-          if (!OPEN && (!((seen >> k) & 1) || t0 + k > pos[u])) sc[u][j][i] = -INFINITY;
+          if (!OPEN && (!((seen >> k) & 1) || rows.at(t0) + k > pos[u])) sc[u][j][i] = -INFINITY;
           top = fmaxf(top, sc[u][j][i]);
         }
       top = max4(top) * c.scale_log2;
@@ -589,6 +768,7 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
         const float mn = fmaxf(m[u], top);
         const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[u] - mn);
         l[u] *= corr;
+        lx[u] *= corr;
 #pragma unroll
         for (int d = 0; d < DB; ++d) ot[u][d] *= corr;
         m[u] = mn;
@@ -608,6 +788,9 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
         sum = __builtin_amdgcn_fdot2(h, half2v{(half_t)1.f, (half_t)1.f}, sum, false);
       }
       l[u] += sum4(sum);
+      if constexpr (LSE)
+        lx[u] += sum4(((pv[u][0][0] + pv[u][0][1]) + (pv[u][0][2] + pv[u][0][3])) +
+                      ((pv[u][1][0] + pv[u][1][1]) + (pv[u][1][2] + pv[u][1][3])));
     }
     __builtin_amdgcn_sched_barrier(0);
     if (!alu) {
@@ -630,7 +813,7 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll 1
         for (int k = 0; k < 32; ++k) {
-          if (!((seen >> k) & 1) || t0 + k > pos[u]) continue;
+          if (!((seen >> k) & 1) || rows.at(t0) + k > pos[u]) continue;
           const float p = ps[w][k][n];
 #pragma unroll
           for (int d = 0; d < DB; ++d) {
@@ -649,7 +832,7 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
   };
   // The open tiles come first: those that every row sees whole, up to the first that
   // has a hole.  Two loops, as one with both bodies does not fit the registers.
-  while (t0 < end && (uint32_t)rows.have() == ~0u && t0 + 31 <= pos_lo) {  // uniform
+  while (t0 < end && (uint32_t)rows.have() == ~0u && rows.at(t0) + 31 <= pos_lo) {  // uniform
     tile(~0u, std::true_type{});
     t0 += 128;
   }
@@ -664,6 +847,7 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
     if (g == 0) {
       wm[w][16 * u + n] = m[u];
       wl[w][16 * u + n] = l[u];
+      if constexpr (LSE) wx[w][16 * u + n] = lx[u];
     }
 #pragma unroll
   for (int u = 0; u < NT; ++u) {
@@ -676,7 +860,7 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
       const int r = idx / (DD / 4), d = idx % (DD / 4) * 4;
       const uint32_t row = t.first + 16 * u + r;
       if (row >= t.rows) break;
-      float M = -INFINITY, L = 0.f;
+      float M = -INFINITY, L = 0.f, X = 0.f;
 #pragma unroll
       for (int v = 0; v < 4; ++v) M = fmaxf(M, wm[v][16 * u + r]);
       float4v A = {0.f, 0.f, 0.f, 0.f};
@@ -685,6 +869,7 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
         const float mv = wm[v][16 * u + r];
         const float f = mv == M ? 1.f : __builtin_amdgcn_exp2f(mv - M);
         L += f * wl[v][16 * u + r];
+        if constexpr (LSE) X += f * wx[v][16 * u + r];
         A += f * *reinterpret_cast<const float4v*>(reinterpret_cast<const float*>(vs[v]) + r * DD + d);
       }
       const uint64_t o = (uint64_t)(t.start + row / G) * H + kvh * G + row % G;
@@ -693,36 +878,86 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
         half2v a = {(half_t)(A[0] * inv), (half_t)(A[1] * inv)}, bb = {(half_t)(A[2] * inv), (half_t)(A[3] * inv)};
         *reinterpret_cast<uint2*>(static_cast<half_t*>(c.out) + o * DD + d) =
             uint2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, bb)};
+        if (LSE && c.lse && d == 0) c.lse[o] = lse_of(M, X, kWeightLog2);
       } else {
-        const uint64_t p = o * c.splits + sp;
+        const uint64_t p = o * c.splits + (SHARE ? t.slot : 0) + sp;
         if (d == 0) *reinterpret_cast<float2s*>(c.ml + 2 * p) = float2s{M, L};
+        if (LSE && d == 0) c.lsum[p] = X;
         *reinterpret_cast<float4v*>(c.acc + p * DD + d) = A;
       }
     }
   }
 }
 
+template <PoolType PT, int DD, int NT, bool UNI, Form FORM>
+__global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
+  const uint32_t sp = blockIdx.x % c.splits, kvh = blockIdx.y;
+  RowTile t;
+  if (!find_tile(c.b, blockIdx.x / c.splits, c.group, 16 * NT, c.lo, c.hi, t)) return;
+  const uint32_t ns = splits_of(c, t.len);
+  if (sp < ns) narrow_tile<PT, DD, NT, UNI, FORM>(c, t, sp, ns, kvh);
+}
+
+// kShared: as many workgroups as run at once take the tiles of all parts in turn, as
+// only the device knows how many there are.  `ns` of a part: 1 says that no other has
+// partials of its rows.
+template <typename F>
+__device__ __forceinline__ void each_part(const Chunk& c, uint32_t per, F f) {
+  uint32_t from = 0, done = 0;
+  for (uint32_t id = blockIdx.x;; id += gridDim.x) {
+    RowTile t;
+    uint32_t sp;
+    if (!find_part(c, id / c.b.n_kv, per, t, sp, from, done)) return;
+    f(t, sp, t.last == 0 && t.slot == 0 ? t.splits : t.splits + 1, id % c.b.n_kv);
+    __syncthreads();  // the next tile's LDS
+  }
+}
+template <PoolType PT, int DD, int NT, bool UNI>
+__global__ __launch_bounds__(256, 2) void shared_narrow_kernel(Chunk c) {
+  each_part(c, 16 * NT, [&](const RowTile& t, uint32_t sp, uint32_t ns, uint32_t kvh) {
+    narrow_tile<PT, DD, NT, UNI, kShared>(c, t, sp, ns, kvh);
+  });
+}
+
 // The splits of every query row whose sequence has more than one, where they are few:
 // a wave per row.
 constexpr uint32_t kFewSplits = 8;
-template <typename T, int DD>
+//
+// Splits of a row's partials, 1 where its tile has written the output itself.
+template <Form FORM>
+__device__ __forceinline__ uint32_t row_splits(const Chunk& c, uint32_t seq) {
+  const int l = c.b.lens[seq], len = l < (int)c.b.limit ? l : (int)c.b.limit;
+  if constexpr (FORM == kShared) {
+    const Slots s = find_slots(c, (int)find_prefix(c.b, c.sh, seq).len, len);
+    return s.group + s.own;
+  }
+  return splits_of(c, len);
+}
+// Whether they are to be combined.
+template <Form FORM>
+__device__ __forceinline__ bool row_direct(const Chunk& c, uint32_t seq, uint32_t ns) {
+  return ns == 1 && (FORM != kShared || !c.apart || find_prefix(c.b, c.sh, seq).len == 0);
+}
+template <typename T, int DD, Form FORM>
 __global__ __launch_bounds__(256) void chunk_combine_few_kernel(Chunk c) {
+  constexpr bool HALF = std::is_same<T, half_t>::value, LSE = FORM != kChunk;
   constexpr int R = (DD + 63) / 64;
   const uint32_t o = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   uint32_t seq;
   int64_t pos;
   if (o >= c.b.rows * c.n_heads || !find_row_wave(c.b, o / c.n_heads, seq, pos)) return;  // uniform
-  const int len = c.b.lens[seq];
-  const uint32_t ns = splits_of(c, len < (int)c.b.limit ? len : (int)c.b.limit);
-  if (ns == 1) return;
+  const uint32_t ns = row_splits<FORM>(c, seq);
+  if (row_direct<FORM>(c, seq, ns)) return;
   const uint64_t first = (uint64_t)o * c.splits;
   const float2s* ml = reinterpret_cast<const float2s*>(c.ml) + first;
-  float x[kFewSplits][R], M = -INFINITY, L = 0.f, A[R] = {};
+  float x[kFewSplits][R], M = -INFINITY, L = 0.f, X = 0.f, A[R] = {};
   float2s v[kFewSplits];
+  float vx[kFewSplits];
 #pragma unroll
   for (uint32_t s = 0; s < kFewSplits; ++s) {
     const uint32_t at = s < ns ? s : ns - 1;
     v[s] = ml[at];
+    if (LSE) vx[s] = HALF ? c.lsum[first + at] : v[s][1];
 #pragma unroll
     for (int r = 0; r < R; ++r) x[s][r] = c.acc[(first + at) * DD + (lane + 64 * r < DD ? lane + 64 * r : DD - 1)];
   }
@@ -733,9 +968,11 @@ __global__ __launch_bounds__(256) void chunk_combine_few_kernel(Chunk c) {
     if (s >= ns || v[s][1] == 0.f) continue;  // no key: its row may be anything
     const float f = v[s][0] == M ? 1.f : __builtin_amdgcn_exp2f(v[s][0] - M);
     L += f * v[s][1];
+    if (LSE) X += f * vx[s];
 #pragma unroll
     for (int r = 0; r < R; ++r) A[r] += f * x[s][r];
   }
+  if (LSE && c.lse && lane == 0) c.lse[o] = lse_of(M, X, HALF ? kWeightLog2 : 0.f);
   const float inv = L == 0.f ? 0.f : 1.0f / L;
 #pragma unroll
   for (int r = 0; r < R; ++r)
@@ -748,22 +985,22 @@ __global__ __launch_bounds__(256) void chunk_combine_few_kernel(Chunk c) {
 // splits this kernel is the slower one: three ragged f32 chunks of up to 389 tokens
 // with 2000 positions 136 us, with a wave per row 117).
 constexpr int kSplitsAtOnce = 256;
-template <typename T, int DD>
+template <typename T, int DD, Form FORM>
 __global__ __launch_bounds__(256) void chunk_combine_kernel(Chunk c) {
+  constexpr bool HALF = std::is_same<T, half_t>::value, LSE = FORM != kChunk;
   constexpr int R = (DD + 63) / 64;
   __shared__ float weight[kSplitsAtOnce];
   __shared__ float part[4][64 * R];
-  __shared__ float wave_m[4], wave_l[4];
+  __shared__ float wave_m[4], wave_l[4], wave_x[4];
   const uint32_t o = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   uint32_t seq;
   int64_t pos;
   if (!find_row_wave(c.b, o / c.n_heads, seq, pos)) return;  // uniform
-  const int l = c.b.lens[seq];
-  const uint32_t ns = splits_of(c, l < (int)c.b.limit ? l : (int)c.b.limit);
-  if (ns == 1) return;
+  const uint32_t ns = row_splits<FORM>(c, seq);
+  if (row_direct<FORM>(c, seq, ns)) return;
   const uint64_t first = (uint64_t)o * c.splits;
   const float2s* ml = reinterpret_cast<const float2s*>(c.ml) + first;
-  float M = -INFINITY, L = 0.f;
+  float M = -INFINITY, L = 0.f, X = 0.f;
   for (uint32_t s = tid; s < ns; s += 256) M = fmaxf(M, ml[s][0]);
 #pragma unroll
   for (int k = 32; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor(M, k));
@@ -778,6 +1015,7 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(Chunk c) {
       const float f = v[0] == M ? 1.f : __builtin_amdgcn_exp2f(v[0] - M);
       weight[tid] = v[1] == 0.f ? 0.f : f;  // no key: its row may be anything
       L += v[1] == 0.f ? 0.f : f * v[1];
+      if (LSE) X += v[1] == 0.f ? 0.f : f * (HALF ? c.lsum[first + s0 + tid] : v[1]);
     }
     __syncthreads();
     const uint32_t n = ns - s0 < (uint32_t)kSplitsAtOnce ? ns - s0 : kSplitsAtOnce;
@@ -794,10 +1032,16 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(Chunk c) {
   }
   L = wave_sum(L);
   if (lane == 0) wave_l[wave] = L;
+  if (LSE) {
+    X = wave_sum(X);
+    if (lane == 0) wave_x[wave] = X;
+  }
 #pragma unroll
   for (int r = 0; r < R; ++r) part[wave][lane + 64 * r] = A[r];
   __syncthreads();
   L = (wave_l[0] + wave_l[1]) + (wave_l[2] + wave_l[3]);
+  if (LSE && c.lse && tid == 0)
+    c.lse[o] = lse_of(M, (wave_x[0] + wave_x[1]) + (wave_x[2] + wave_x[3]), HALF ? kWeightLog2 : 0.f);
   const float inv = L == 0.f ? 0.f : 1.0f / L;
   for (uint32_t d = tid; d < DD; d += 256)
     static_cast<T*>(c.out)[(uint64_t)o * DD + d] = (T)(((part[0][d] + part[1][d]) + (part[2][d] + part[3][d])) * inv);
@@ -847,8 +1091,9 @@ inline uint32_t wide_grid(uint32_t tiles, uint32_t n_kv) {
 // reaches 1093; the MFMA pipes are busy 32 % of the cycles, and without its softmax and
 // staging this kernel took 364 us.  From I8 594 to 631 us: half the bytes to stage, the
 // conversion beside the MFMAs.
-template <PoolType PT, int DD, bool UNI>
-__global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
+template <PoolType PT, int DD, bool UNI, Form FORM>
+__device__ __forceinline__ void wide_rows(const Chunk& c, const RowTile& t, uint32_t sp, uint32_t ns, uint32_t kvh) {
+  constexpr bool SHARE = FORM == kShared, LSE = FORM != kChunk;
   constexpr bool I8 = PT == PoolType::I8;
   constexpr int KS = DD / 16, DB = DD / 32, KP = DD + 8;
   // V rows 16 or 48 dwords past a multiple of 64: the 4 rows and 32 dims that 32 lanes
@@ -868,20 +1113,14 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
   half_t* const vs = lds + 64 * KP;
   float(*const ps)[32][32] = reinterpret_cast<float(*)[32][32]>(lds + BUF);
 
-  uint32_t kvh, idx;
-  if (!wide_tile(c, kvh, idx)) return;
-  const uint32_t sp = blockIdx.y;
-  RowTile t;
-  if (!find_tile(c.b, idx, c.group, 128, c.lo, c.hi, t)) return;
-  const uint32_t ns = splits_of(c, t.len);
-  if (sp >= ns) return;
   const uint32_t G = c.group, H = c.n_heads;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, hf = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t last = (t.first + 128 < t.rows ? t.first + 128 : t.rows) - 1;
-  const int pos_lo = t.pos0 + (int)(t.first / G), pos_hi = t.pos0 + (int)(last / G);
-  const int begin = (int)(sp * c.keys_per_split);
-  int end = pos_hi + 1 < t.len ? pos_hi + 1 : t.len;
+  const bool all = SHARE && t.last && see_all(c.b, t);
+  const Keys keys = find_keys<FORM>(c, t, t.first / G, last / G, all);
+  const int pos_lo = keys.lo, begin = (int)(sp * c.keys_per_split);
+  int end = keys.at.end;
   if (end > begin + (int)c.keys_per_split) end = begin + (int)c.keys_per_split;
   end = __builtin_amdgcn_readfirstlane(end);
 
@@ -889,8 +1128,9 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
   const bool wave_live = r0 < t.rows;
   const uint32_t row = r0 + n < t.rows ? r0 + n : t.rows - 1;
   const uint64_t orow = (uint64_t)(t.start + row / G) * H + kvh * G + row % G;
-  const int pos = t.pos0 + (int)(row / G);
-  const int w_hi = __builtin_amdgcn_readfirstlane(t.pos0 + (int)((r0 + 31 < t.rows ? r0 + 31 : t.rows - 1) / G));
+  const int pos = row_pos<FORM>(c.b, t, row / G, all);
+  const int w_hi = SHARE && t.last ? kEverywhere
+                                   : __builtin_amdgcn_readfirstlane(t.pos0 + (int)((r0 + 31 < t.rows ? r0 + 31 : t.rows - 1) / G));
   half8 qb[KS];
 #pragma unroll
   for (int s = 0; s < KS; ++s)
@@ -901,10 +1141,11 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) ot[d][i] = 0.f;
   float m = -INFINITY, l = 0.f, mb = 0.f;  // mb: exponent_base of m
+  float lx = 0.f;  // LSE: the sum of the weights as they were before they are rounded
 
   u32x4 kraw[NU], vraw[NU];
   half_t kd[NU], vd[NU];
-  Rows<PT, DD, 4, UNI> rows(c.b, t.seq, kvh, end);
+  Rows<PT, DD, 4, UNI, SHARE> rows(c.b, t, kvh, end, keys.at);
   auto fetch = [&]() {
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
@@ -988,13 +1229,14 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
     const float mn = fmaxf(m, top);
     const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
     l *= corr;
+    lx *= corr;
 #pragma unroll
     for (int d = 0; d < DB; ++d) ot[d] *= corr;
     m = mn;
     mb = exponent_base(m, kWeightLog2);
   };
   auto weights = [&]() {
-    float sum = 0.f;
+    float sum = 0.f, whole = 0.f;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -1006,8 +1248,10 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
         pb[j][i / 8][i % 8] = h[0];
         pb[j][i / 8][i % 8 + 1] = h[1];
         sum = __builtin_amdgcn_fdot2(h, half2v{(half_t)1.f, (half_t)1.f}, sum, false);
+        if constexpr (LSE) whole += sc[j][i] + sc[j][i + 1];
       }
     l += sum2(sum);
+    if constexpr (LSE) lx += sum2(whole);
   };
   auto value_op = [&](int buf, int j, int k, int d) {
     const uint2 lo = read_tr(vtr + buf + (32 * j + 16 * k) * VP + 32 * d);
@@ -1090,7 +1334,7 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int k = 32 * j + 8 * (i / 4) + 4 * hf + i % 4;
-        if (!((seen >> k) & 1) || t0 + k > pos) sc[j][i] = -INFINITY;
+        if (!((seen >> k) & 1) || rows.at(t0) + k > pos) sc[j][i] = -INFINITY;
         top = fmaxf(top, sc[j][i]);
       }
     rescale(max2(top) * c.scale_log2);
@@ -1116,7 +1360,7 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll 1
         for (int k = 0; k < 32; ++k) {
-          if (!((seen >> (32 * j + k)) & 1) || t0 + 32 * j + k > pos) continue;
+          if (!((seen >> (32 * j + k)) & 1) || rows.at(t0) + 32 * j + k > pos) continue;
           const float p = ps[w][k][n];
 #pragma unroll
           for (int d = 0; d < DB; ++d)
@@ -1149,7 +1393,7 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
   // the first that has a hole.  While one is computed from its buffer, the next is
   // staged into the other and the one after that is loaded.  Two loops, as one with
   // both kinds of tile does not fit the registers.
-  auto open = [&]() { return t0 < end && rows.have() == ~0ull && t0 + 63 <= pos_lo; };  // uniform
+  auto open = [&]() { return t0 < end && rows.have() == ~0ull && rows.at(t0) + 63 <= pos_lo; };  // uniform
   if (open()) {
     stage(~0ull, std::true_type{}, 0, 0);
     next();
@@ -1173,7 +1417,7 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
     const uint64_t seen = rows.have();
     stage(seen, std::false_type{}, par, 0);
     __syncthreads();
-    if (wave_live && t0 <= w_hi) masked_tile(t0, seen, par);  // uniform
+    if (wave_live && rows.at(t0) <= w_hi) masked_tile(t0, seen, par);  // uniform
     next();
   }
 
@@ -1190,9 +1434,11 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
         *reinterpret_cast<uint2*>(o + 32 * d + 8 * q + 4 * hf) =
             uint2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
       }
+    if (LSE && c.lse && hf == 0) c.lse[orow] = lse_of(m, lx, kWeightLog2);
   } else {
-    const uint64_t p = orow * c.splits + sp;
+    const uint64_t p = orow * c.splits + (SHARE ? t.slot : 0) + sp;
     if (hf == 0) *reinterpret_cast<float2s*>(c.ml + 2 * p) = float2s{m, l};
+    if (LSE && hf == 0) c.lsum[p] = lx;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -1200,6 +1446,23 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
         *reinterpret_cast<float4v*>(c.acc + p * DD + 32 * d + 8 * q + 4 * hf) =
             float4v{ot[d][4 * q], ot[d][4 * q + 1], ot[d][4 * q + 2], ot[d][4 * q + 3]};
   }
+}
+
+template <PoolType PT, int DD, bool UNI, Form FORM>
+__global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
+  uint32_t kvh, idx;
+  if (!wide_tile(c, kvh, idx)) return;
+  const uint32_t sp = blockIdx.y;
+  RowTile t;
+  if (!find_tile(c.b, idx, c.group, 128, c.lo, c.hi, t)) return;
+  const uint32_t ns = splits_of(c, t.len);
+  if (sp < ns) wide_rows<PT, DD, UNI, FORM>(c, t, sp, ns, kvh);
+}
+template <PoolType PT, int DD, bool UNI>
+__global__ __launch_bounds__(256, 2) void shared_wide_kernel(Chunk c) {
+  each_part(c, 128, [&](const RowTile& t, uint32_t sp, uint32_t ns, uint32_t kvh) {
+    wide_rows<PT, DD, UNI, kShared>(c, t, sp, ns, kvh);
+  });
 }
 
 // ---- f32 rows -----------------------------------------------------------------------
@@ -1227,11 +1490,12 @@ __device__ __forceinline__ float4v codes4_f32(uint32_t w, float d) {
 }
 
 // One row's output or partial, from the layout above.
-template <int DD>
+template <int DD, Form FORM>
 __device__ __forceinline__ void store_f32(const Chunk& c, uint64_t orow, uint32_t sp, uint32_t ns, int g, float m, float l,
                                           const float4v* ot) {
   float* dst = ns == 1 ? static_cast<float*>(c.out) + orow * DD : c.acc + (orow * c.splits + sp) * DD;
   const float f = ns > 1 ? 1.0f : l == 0.f ? 0.f : 1.0f / l;
+  if (FORM != kChunk && ns == 1 && c.lse && g == 0) c.lse[orow] = lse_of(m, l, 0.f);
   if (ns > 1 && g == 0) *reinterpret_cast<float2s*>(c.ml + 2 * (orow * c.splits + sp)) = float2s{m, l};
 #pragma unroll
   for (int h = 0; h < (DD + 63) / 64; ++h)
@@ -1247,29 +1511,26 @@ __device__ __forceinline__ void store_f32(const Chunk& c, uint64_t orow, uint32_
 // with a masked pair and a value that is not finite reads the values again, row by
 // row, for the pairs that count.  Bound by HBM (8 sequences of up to 4096 positions,
 // 8 KV heads of 128: 49 us), at short caches by its latency (one of 101: 6.6 us).
-template <PoolType PT, int DD, bool UNI>
-__global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
+template <PoolType PT, int DD, bool UNI, Form FORM>
+__device__ __forceinline__ void narrow_f32_tile(const Chunk& c, const RowTile& t, uint32_t sp, uint32_t ns, uint32_t kvh) {
+  constexpr bool SHARE = FORM == kShared;
   constexpr bool I8 = PT == PoolType::I8;
   constexpr int DG = DD / 4, NH = (DD + 63) / 64, NB = 4 * NH;
   __shared__ __attribute__((aligned(16))) float merge[4][16 * 64 * NH];
   __shared__ float wm[4][16], wl[4][16];
-  const uint32_t sp = blockIdx.x % c.splits, kvh = blockIdx.y;
-  RowTile t;
-  if (!find_tile(c.b, blockIdx.x / c.splits, c.group, 16, c.lo, c.hi, t)) return;
-  const uint32_t ns = splits_of(c, t.len);
-  if (sp >= ns) return;
   const uint32_t G = c.group, H = c.n_heads;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t last = (t.first + 16 < t.rows ? t.first + 16 : t.rows) - 1;
-  const int pos_lo = t.pos0 + (int)(t.first / G), pos_hi = t.pos0 + (int)(last / G);
-  const int begin = (int)(sp * c.keys_per_split);
-  int end = pos_hi + 1 < t.len ? pos_hi + 1 : t.len;
+  const bool all = SHARE && t.last && see_all(c.b, t);
+  const Keys keys = find_keys<FORM>(c, t, t.first / G, last / G, all);
+  const int pos_lo = keys.lo, begin = (int)(sp * c.keys_per_split);
+  int end = keys.at.end;
   if (end > begin + (int)c.keys_per_split) end = begin + (int)c.keys_per_split;
   end = __builtin_amdgcn_readfirstlane(end);
   const uint32_t row = t.first + n < t.rows ? t.first + n : t.rows - 1;
   const uint64_t orow = (uint64_t)(t.start + row / G) * H + kvh * G + row % G;
-  const int pos = t.pos0 + (int)(row / G);
+  const int pos = row_pos<FORM>(c.b, t, row / G, all);
 
   float qb[DG];
 #pragma unroll
@@ -1287,7 +1548,7 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
   uint2 kc[2][I8 ? DG / 8 : 1];
   half_t kd[2][I8 ? DG / 8 : 1], vd[2][4][NH];
   uint32_t vc[2][4][NH];
-  Rows<PT, DD, 2, UNI> rows(c.b, t.seq, kvh, end);
+  Rows<PT, DD, 2, UNI, SHARE> rows(c.b, t, kvh, end, keys.at);
   auto fetch_k = [&]() {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -1363,7 +1624,7 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int k = 16 * j + 4 * g + i;
-        if (!OPEN && (!((seen >> k) & 1) || t0 + k > pos)) sc[j][i] = -INFINITY;
+        if (!OPEN && (!((seen >> k) & 1) || rows.at(t0) + k > pos)) sc[j][i] = -INFINITY;
         top = fmaxf(top, sc[j][i]);
       }
     top = max4(top) * c.scale_log2;
@@ -1432,9 +1693,9 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
           for (int gk = 0; gk < 4; ++gk) {
             const int k = 16 * j + 4 * gk + i;
             const float p = __shfl(pv[j][i], 16 * gk + n);
-            const uint32_t slot = (uint32_t)(t0 + k) % c.b.block_size;
+            const uint32_t slot = (uint32_t)(rows.at(t0) + k) % c.b.block_size;
             const uint8_t* page = rows.row(c.v, j, 4 * gk + i) - (uint64_t)slot * rows.kRow;
-            if (!((seen >> k) & 1) || t0 + k > pos) continue;
+            if (!((seen >> k) & 1) || rows.at(t0) + k > pos) continue;
 #pragma unroll
             for (int d = 0; d < NB; ++d)
 #pragma unroll
@@ -1451,7 +1712,7 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
     if (OPEN && t0 + 128 < end) fetch_v();
   };
   // The open tiles first, as in the f16 kernel.
-  while (t0 < end && (uint32_t)rows.have() == ~0u && t0 + 31 <= pos_lo) {  // uniform
+  while (t0 < end && (uint32_t)rows.have() == ~0u && rows.at(t0) + 31 <= pos_lo) {  // uniform
     tile(~0u, std::true_type{});
     t0 += 128;
   }
@@ -1490,12 +1751,28 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
     if (ns == 1) {
       const float inv = L == 0.f ? 0.f : 1.0f / L;
       *reinterpret_cast<float4v*>(static_cast<float*>(c.out) + o * DD + d) = A * inv;
+      if (FORM != kChunk && c.lse && d == 0) c.lse[o] = lse_of(M, L, 0.f);
     } else {
-      const uint64_t p = o * c.splits + sp;
+      const uint64_t p = o * c.splits + (SHARE ? t.slot : 0) + sp;
       if (d == 0) *reinterpret_cast<float2s*>(c.ml + 2 * p) = float2s{M, L};
       *reinterpret_cast<float4v*>(c.acc + p * DD + d) = A;
     }
   }
+}
+
+template <PoolType PT, int DD, bool UNI, Form FORM>
+__global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
+  const uint32_t sp = blockIdx.x % c.splits, kvh = blockIdx.y;
+  RowTile t;
+  if (!find_tile(c.b, blockIdx.x / c.splits, c.group, 16, c.lo, c.hi, t)) return;
+  const uint32_t ns = splits_of(c, t.len);
+  if (sp < ns) narrow_f32_tile<PT, DD, UNI, FORM>(c, t, sp, ns, kvh);
+}
+template <PoolType PT, int DD, bool UNI>
+__global__ __launch_bounds__(256, 2) void shared_narrow_f32_kernel(Chunk c) {
+  each_part(c, 16, [&](const RowTile& t, uint32_t sp, uint32_t ns, uint32_t kvh) {
+    narrow_f32_tile<PT, DD, UNI, kShared>(c, t, sp, ns, kvh);
+  });
 }
 
 // Many query rows: 64 a workgroup, 16 per wave, 32-key tiles of K and V in LDS.
@@ -1504,8 +1781,9 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
 // Two sequences of 512 tokens with 2048 positions, 32 heads of 128, 293 us; three of up
 // to 389 with 2000, 32 heads of 64, 9.5 GFLOP in 117 us with the combine (13 of them),
 // where a product of 8192 in each size reaches 153 TFLOP/s.
-template <PoolType PT, int DD, bool UNI>
-__global__ __launch_bounds__(256, 2) void chunk_wide_f32_kernel(Chunk c) {
+template <PoolType PT, int DD, bool UNI, Form FORM>
+__device__ __forceinline__ void wide_f32_rows(const Chunk& c, const RowTile& t, uint32_t sp, uint32_t ns, uint32_t kvh) {
+  constexpr bool SHARE = FORM == kShared;
   constexpr bool I8 = PT == PoolType::I8;
   constexpr int TK = 32, DP = DD + 4, DG = DD / 4, NH = (DD + 63) / 64, NB = 4 * NH;
   constexpr int EC = I8 ? 8 : 4;                  // elements per chunk (8 or 16 bytes)
@@ -1515,28 +1793,23 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_f32_kernel(Chunk c) {
   __shared__ __attribute__((aligned(16))) float vs[TK * DP + 64 * NH - DD];
   __shared__ __attribute__((aligned(16))) float ps[4][TK][16];
   __shared__ int tile_bad[2];
-  uint32_t kvh, idx;
-  if (!wide_tile(c, kvh, idx)) return;
-  const uint32_t sp = blockIdx.y;
-  RowTile t;
-  if (!find_tile(c.b, idx, c.group, 64, c.lo, c.hi, t)) return;
-  const uint32_t ns = splits_of(c, t.len);
-  if (sp >= ns) return;
   const uint32_t G = c.group, H = c.n_heads;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t last = (t.first + 64 < t.rows ? t.first + 64 : t.rows) - 1;
-  const int pos_lo = t.pos0 + (int)(t.first / G), pos_hi = t.pos0 + (int)(last / G);
-  const int begin = (int)(sp * c.keys_per_split);
-  int end = pos_hi + 1 < t.len ? pos_hi + 1 : t.len;
+  const bool all = SHARE && t.last && see_all(c.b, t);
+  const Keys keys = find_keys<FORM>(c, t, t.first / G, last / G, all);
+  const int pos_lo = keys.lo, begin = (int)(sp * c.keys_per_split);
+  int end = keys.at.end;
   if (end > begin + (int)c.keys_per_split) end = begin + (int)c.keys_per_split;
   end = __builtin_amdgcn_readfirstlane(end);
   const uint32_t r0 = t.first + 16 * w;
   const bool wave_live = r0 < t.rows;
   const uint32_t row = r0 + n < t.rows ? r0 + n : t.rows - 1;
   const uint64_t orow = (uint64_t)(t.start + row / G) * H + kvh * G + row % G;
-  const int pos = t.pos0 + (int)(row / G);
-  const int w_hi = __builtin_amdgcn_readfirstlane(t.pos0 + (int)((r0 + 15 < t.rows ? r0 + 15 : t.rows - 1) / G));
+  const int pos = row_pos<FORM>(c.b, t, row / G, all);
+  const int w_hi = SHARE && t.last ? kEverywhere
+                                   : __builtin_amdgcn_readfirstlane(t.pos0 + (int)((r0 + 15 < t.rows ? r0 + 15 : t.rows - 1) / G));
   float qb[DG];
 #pragma unroll
   for (int s = 0; s < DG / 4; ++s) {
@@ -1552,7 +1825,7 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_f32_kernel(Chunk c) {
   float4v kf[I8 ? 1 : NU], vf[I8 ? 1 : NU];
   uint2 kc[I8 ? NU : 1], vc[I8 ? NU : 1];
   half_t kd[NU], vd[NU];
-  Rows<PT, DD, 2, UNI> rows(c.b, t.seq, kvh, end);
+  Rows<PT, DD, 2, UNI, SHARE> rows(c.b, t, kvh, end, keys.at);
   auto fetch = [&]() {
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
@@ -1634,7 +1907,7 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_f32_kernel(Chunk c) {
       for (int i = 0; i < 4; ++i) {
         if constexpr (!OPEN) {
           const int k = 16 * j + 4 * g + i;
-          if (!((seen >> k) & 1) || t0 + k > pos) sc[j][i] = -INFINITY;
+          if (!((seen >> k) & 1) || rows.at(t0) + k > pos) sc[j][i] = -INFINITY;
         }
         top = fmaxf(top, sc[j][i]);
       }
@@ -1677,7 +1950,7 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_f32_kernel(Chunk c) {
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
       for (int k = 0; k < TK; ++k) {
-        if (!((seen >> k) & 1) || t0 + k > pos) continue;
+        if (!((seen >> k) & 1) || rows.at(t0) + k > pos) continue;
         const float p = ps[w][k][n];
 #pragma unroll
         for (int d = 0; d < NB; ++d)
@@ -1707,7 +1980,7 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_f32_kernel(Chunk c) {
     if (t0 + 2 * TK < end) rows.look(t0 + 2 * TK);
   };
   // The open tiles first, as in the f16 kernel.
-  while (t0 < end && (uint32_t)rows.have() == ~0u && t0 + TK - 1 <= pos_lo) {  // uniform
+  while (t0 < end && (uint32_t)rows.have() == ~0u && rows.at(t0) + TK - 1 <= pos_lo) {  // uniform
     __syncthreads();  // the previous tile's readers are done
     stage(~0u, false, 0);
     __syncthreads();
@@ -1721,11 +1994,175 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_f32_kernel(Chunk c) {
     const uint32_t seen = (uint32_t)rows.have();
     stage(seen, true, par);
     __syncthreads();
-    if (wave_live && t0 <= w_hi) tile(t0, seen, par, std::false_type{});  // uniform
+    if (wave_live && rows.at(t0) <= w_hi) tile(t0, seen, par, std::false_type{});  // uniform
     next();
   }
-  if (wave_live && r0 + n < t.rows) store_f32<DD>(c, orow, sp, ns, g, m, l, ot);
+  if (wave_live && r0 + n < t.rows) store_f32<DD, FORM>(c, orow, (SHARE ? t.slot : 0) + sp, ns, g, m, l, ot);
 }
+
+template <PoolType PT, int DD, bool UNI, Form FORM>
+__global__ __launch_bounds__(256, 2) void chunk_wide_f32_kernel(Chunk c) {
+  uint32_t kvh, idx;
+  if (!wide_tile(c, kvh, idx)) return;
+  const uint32_t sp = blockIdx.y;
+  RowTile t;
+  if (!find_tile(c.b, idx, c.group, 64, c.lo, c.hi, t)) return;
+  const uint32_t ns = splits_of(c, t.len);
+  if (sp < ns) wide_f32_rows<PT, DD, UNI, FORM>(c, t, sp, ns, kvh);
+}
+template <PoolType PT, int DD, bool UNI>
+__global__ __launch_bounds__(256, 2) void shared_wide_f32_kernel(Chunk c) {
+  each_part(c, 64, [&](const RowTile& t, uint32_t sp, uint32_t ns, uint32_t kvh) {
+    wide_f32_rows<PT, DD, UNI, kShared>(c, t, sp, ns, kvh);
+  });
+}
+
+// ---- launch ------------------------------------------------------------------------------
+
+// Query rows of a sequence, on average, up to which the narrow kernel takes the whole
+// batch.  It reads the cache once per 16 or 32 rows and splits it finely; the wide one
+// once per 128 (f32: 64).  Narrow and wide, 8 sequences of 4096 positions, 8 KV heads
+// of 128:
+//   f16, 64 rows 52 and 70 us, 96 rows 70 and 63;
+//   I8,  64 rows 37 and 45 us, 96 rows 51 and 44;
+//   f32, 36 rows 144 and 100 us, 64 rows 155 and 111; one of 8192, 32 rows: 28 and 33.
+template <typename T>
+constexpr uint32_t kNarrowRows = std::is_same<T, float>::value ? 32 : 64;
+// Where the wide kernel runs, the sequences that go to the narrow one all the same; more
+// wait for a kernel with too few workgroups (three sequences of up to 96 rows: 42 us, and
+// 54 with the narrow kernel taking those of up to 64).
+constexpr uint32_t kFewRows = 32;
+
+// Partials take this many floats for each split of a query row: its maximum, its sums and
+// the output row, and what aligns them.
+constexpr uint32_t kPartFloats = 4;
+inline void place_parts(Chunk& c, const nfhip::Workspace& ws, uint32_t dim) {
+  const uint64_t n = (uint64_t)c.b.rows * c.n_heads * c.splits;
+  c.ml = ws.part;
+  c.acc = ws.part + (n * 2 + 3) / 4 * 4;
+  c.lsum = c.acc + n * dim;
+}
+
+struct Operands {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  float* lse;
+};
+inline Chunk chunk_of(const PagedBatch& b, uint32_t n_heads, const Operands& o) {
+  Chunk c{};
+  c.b = b;
+  c.q = o.q;
+  c.k = static_cast<const uint8_t*>(o.k);
+  c.v = static_cast<const uint8_t*>(o.v);
+  c.out = o.out;
+  c.lse = o.lse;
+  c.n_heads = n_heads;
+  c.group = n_heads / b.n_kv;
+  c.scale_log2 = 1.4426950408889634f / sqrtf((float)b.dim);
+  return c;
+}
+
+template <typename T, PoolType PT, int DD, bool UNI, Form FORM>
+hipError_t chunk_mfma_at(const PagedBatch& b, uint32_t n_heads, const Operands& o, const nfhip::Workspace& ws, hipStream_t s) {
+  Chunk c = chunk_of(b, n_heads, o);
+  const uint64_t rows = (uint64_t)b.rows * c.group;  // query rows per KV head
+  // Lengths are known on the device only: each kernel skips the sequences that are the
+  // other's.
+  const bool wide = rows > (uint64_t)kNarrowRows<T> * b.n_seqs;
+  const bool narrow = !wide || b.n_seqs > 1;
+  constexpr bool F16 = std::is_same<T, half_t>::value;
+  constexpr uint32_t kWideRows = F16 ? 128 : 64;  // a wide workgroup's query rows
+  // A narrow workgroup takes 16 rows, or 32 where sequences have more, which then read
+  // the cache once (16 I8 sequences of 20 rows behind up to 4096 positions, with the
+  // append before it: 48 and 37 us; 64 sequences of 4 rows behind up to 8192, f16:
+  // with 16 rows 262 us, with 32 279).
+  const uint32_t nt = F16 && (wide || rows > 16ull * b.n_seqs) ? 2 : 1;
+  const uint64_t per = wide ? kWideRows : 16 * nt, mean = (rows + b.n_seqs - 1) / b.n_seqs;
+  const uint64_t most_tiles = rows / per + b.n_seqs;
+  // Splits of the keys, with partials that fit the workspace.  Narrow: two workgroups per
+  // CU, not one more (20 sequences of 4096 positions in I8: 41 us; rounded up, a third
+  // of the CUs have a third workgroup, 50).  Wide: four where no sequence is cut short by
+  // the mask or its length, rounded up (three ragged f32 chunks: 117 us, rounded down
+  // 129, with two 129); none where the tiles alone are as many.
+  const uint64_t units = b.n_seqs * ((mean + per - 1) / per) * b.n_kv;
+  uint64_t splits = wide ? (1024 + units - 1) / units : units < 512 ? 512 / units : 1;
+  // fewer keys a split, and reading the partials costs more than they save (one sequence of
+  // 28 rows behind 8192 positions: 18 us, with 128 keys 22)
+  const uint32_t min_keys = wide || nt == 2 ? 256 : 128;
+  const uint64_t most = ws.part ? ws.part_floats / ((uint64_t)b.rows * n_heads * (DD + kPartFloats)) : 1;
+  if (splits > most) splits = most ? most : 1;
+  uint64_t keys = splits > 1 ? (b.limit + splits - 1) / splits : b.limit;
+  keys = keys < min_keys ? min_keys : keys;
+  keys = (keys + 127) / 128 * 128;
+  c.keys_per_split = (uint32_t)keys;
+  c.splits = (uint32_t)((b.limit + keys - 1) / keys);
+  if (c.splits == 0) c.splits = 1;
+  place_parts(c, ws, DD);
+  if (wide) {
+    c.tiles = (uint32_t)most_tiles;
+    c.lo = narrow ? kFewRows : 0;
+    c.hi = ~0ull;
+    const dim3 grid(wide_grid(c.tiles, b.n_kv), c.splits);
+    if constexpr (F16) chunk_wide_kernel<PT, DD, UNI, FORM><<<grid, 256, 0, s>>>(c);
+    else chunk_wide_f32_kernel<PT, DD, UNI, FORM><<<grid, 256, 0, s>>>(c);
+  }
+  if (narrow) {
+    c.lo = 0;
+    c.hi = wide ? kFewRows : ~0ull;
+    c.tiles = (uint32_t)(wide ? b.n_seqs * (kFewRows / (16 * nt)) : most_tiles);
+    const dim3 grid(c.splits * c.tiles, b.n_kv);
+    if constexpr (!F16) chunk_narrow_f32_kernel<PT, DD, UNI, FORM><<<grid, 256, 0, s>>>(c);
+    else if (nt == 2) chunk_narrow_kernel<PT, DD, 2, UNI, FORM><<<grid, 256, 0, s>>>(c);
+    else chunk_narrow_kernel<PT, DD, 1, UNI, FORM><<<grid, 256, 0, s>>>(c);
+  }
+  if (c.splits > 1) {
+    if (c.splits <= kFewSplits) chunk_combine_few_kernel<T, DD, FORM><<<dim3((b.rows * n_heads + 3) / 4), 256, 0, s>>>(c);
+    else chunk_combine_kernel<T, DD, FORM><<<dim3(b.rows * n_heads), 256, 0, s>>>(c);
+  }
+  return hipGetLastError();
+}
+
+// Blocks of a power of two of at least 16 positions.
+inline bool uniform_blocks(const PagedBatch& b) { return b.block_size >= 16 && (b.block_size & (b.block_size - 1)) == 0; }
+
+// 16-byte rows, and whole groups of query heads: what the MFMA kernels take.  An I8 page of
+// block_size head_dim 17/16 bytes has to be whole chunks.
+template <PoolType PT>
+bool pieces_fit(const PagedBatch& b, uint32_t n_heads, const Operands& o) {
+  const uintptr_t all = reinterpret_cast<uintptr_t>(o.q) | reinterpret_cast<uintptr_t>(o.k) |
+                        reinterpret_cast<uintptr_t>(o.v) | reinterpret_cast<uintptr_t>(o.out);
+  return all % 16 == 0 && n_heads % b.n_kv == 0 && b.blocks > 0 && b.limit > 0 &&
+         (PT != PoolType::I8 || b.block_size * b.dim % 256 == 0) && (b.dim == 128 || b.dim == 96 || b.dim == 64);
+}
+
+template <typename T, PoolType PT, Form FORM>
+hipError_t chunk(const PagedBatch& b, uint32_t n_heads, const Operands& o, const nfhip::Workspace& ws, hipStream_t s) {
+  if (pieces_fit<PT>(b, n_heads, o)) {
+    const bool uni = uniform_blocks(b);
+    if (b.dim == 128) return (uni ? chunk_mfma_at<T, PT, 128, true, FORM> : chunk_mfma_at<T, PT, 128, false, FORM>)(b, n_heads, o, ws, s);
+    if (b.dim == 96) return (uni ? chunk_mfma_at<T, PT, 96, true, FORM> : chunk_mfma_at<T, PT, 96, false, FORM>)(b, n_heads, o, ws, s);
+    return (uni ? chunk_mfma_at<T, PT, 64, true, FORM> : chunk_mfma_at<T, PT, 64, false, FORM>)(b, n_heads, o, ws, s);
+  }
+  const float scale = 1.0f / sqrtf((float)b.dim);
+  chunk_any_kernel<T, PT, false><<<dim3(b.rows, n_heads), 256, 0, s>>>(b, PagedShared{}, n_heads, scale, (const T*)o.q,
+                                                                       (const uint8_t*)o.k, (const uint8_t*)o.v, (T*)o.out, o.lse);
+  return hipGetLastError();
+}
+
+// The chunk attention of one form, for all types.
+template <Form FORM>
+hipError_t chunk_all(nfhip::EType t, PoolType pool, const PagedBatch& b, uint32_t n_heads, const Operands& o,
+                     const nfhip::Workspace& ws, hipStream_t s) {
+  if (t == nfhip::EType::F16)
+    return pool == PoolType::I8 ? chunk<half_t, PoolType::I8, FORM>(b, n_heads, o, ws, s)
+                                : chunk<half_t, PoolType::F16, FORM>(b, n_heads, o, ws, s);
+  return pool == PoolType::I8 ? chunk<float, PoolType::I8, FORM>(b, n_heads, o, ws, s)
+                              : chunk<float, PoolType::F32, FORM>(b, n_heads, o, ws, s);
+}
+hipError_t chunk_lse(nfhip::EType t, PoolType pool, const PagedBatch& b, uint32_t n_heads, const Operands& o,
+                     const nfhip::Workspace& ws, hipStream_t s);  // paged_lse.hip
 
 }  // namespace paged
 }  // namespace nfk

@@ -349,7 +349,8 @@ def test_lse_and_weights(provider, act, pool, seqs, heads, kv, dim, bs):
 @pytest.mark.parametrize("act,pool", ACT_POOL)
 @pytest.mark.parametrize("dim", [128, 64, 96])
 def test_weights_add_up_to_the_rows(provider, act, pool, dim):
-    """With theta 0 a sequence's weights add up to its rows times the heads of a KV head."""
+    """With theta 0 a sequence's weights add up to its rows times the heads of a KV head; the output with a log-sum-exp is
+    the one without."""
     rng = np.random.default_rng(41)
     heads, kv = 8, 2
     batch = ref.Batch(rng, [(300, 1), (150, 40), (90, 90), (33, 5)], 16)
@@ -357,6 +358,14 @@ def test_weights_add_up_to_the_rows(provider, act, pool, dim):
     got = run_weights(provider, rng, batch, act, pool, heads, kv, dim, z, q, pools, theta=0.0)
     for s, (n, r) in enumerate(batch.seqs):
         assert np.allclose(got[s, :, :n].astype(np.float64).sum(1), r * heads / kv, rtol=2e-5)
+    outs = []
+    with Bufs(provider) as m:
+        ins = [m.put(q)] + [m.put(p) for p in pools] + m.batch(batch)
+        for second in ([], [m.put(z)]):
+            o = m.put(np.zeros_like(q))
+            provider.dispatch("flash_attention_paged_chunk", ins, [o] + second, pc=pc_of(batch, kv, dim, n_heads=heads))
+            outs.append(o.read(np.uint8, q.nbytes))
+    assert np.array_equal(*outs)
 
 
 @pytest.mark.parametrize("act,pool", ACT_POOL)
