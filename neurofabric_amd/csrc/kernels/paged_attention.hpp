@@ -16,6 +16,10 @@
 namespace nfk {
 namespace paged {
 
+// Keys are split for two workgroups a CU.  Where a third fits, some CUs get it and others
+// none: four long I8 sequences 216 us, kept to two 158.
+#define NF_TWO_PER_CU __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(2, 2)))
+
 constexpr int kMaxDim = 256;
 constexpr int kTile = 64;
 
@@ -890,7 +894,7 @@ __device__ __forceinline__ void narrow_tile(const Chunk& c, const RowTile& t, ui
 }
 
 template <PoolType PT, int DD, int NT, bool UNI, Form FORM>
-__global__ __launch_bounds__(256, 2) void chunk_narrow_kernel(Chunk c) {
+__global__ NF_TWO_PER_CU void chunk_narrow_kernel(Chunk c) {
   const uint32_t sp = blockIdx.x % c.splits, kvh = blockIdx.y;
   RowTile t;
   if (!find_tile(c.b, blockIdx.x / c.splits, c.group, 16 * NT, c.lo, c.hi, t)) return;
@@ -913,7 +917,7 @@ __device__ __forceinline__ void each_part(const Chunk& c, uint32_t per, F f) {
   }
 }
 template <PoolType PT, int DD, int NT, bool UNI>
-__global__ __launch_bounds__(256, 2) void shared_narrow_kernel(Chunk c) {
+__global__ NF_TWO_PER_CU void shared_narrow_kernel(Chunk c) {
   each_part(c, 16 * NT, [&](const RowTile& t, uint32_t sp, uint32_t ns, uint32_t kvh) {
     narrow_tile<PT, DD, NT, UNI, kShared>(c, t, sp, ns, kvh);
   });
@@ -1459,7 +1463,7 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
   if (sp < ns) wide_rows<PT, DD, UNI, FORM>(c, t, sp, ns, kvh);
 }
 template <PoolType PT, int DD, bool UNI>
-__global__ __launch_bounds__(256, 2) void shared_wide_kernel(Chunk c) {
+__global__ NF_TWO_PER_CU void shared_wide_kernel(Chunk c) {
   each_part(c, 128, [&](const RowTile& t, uint32_t sp, uint32_t ns, uint32_t kvh) {
     wide_rows<PT, DD, UNI, kShared>(c, t, sp, ns, kvh);
   });
@@ -1769,7 +1773,7 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
   if (sp < ns) narrow_f32_tile<PT, DD, UNI, FORM>(c, t, sp, ns, kvh);
 }
 template <PoolType PT, int DD, bool UNI>
-__global__ __launch_bounds__(256, 2) void shared_narrow_f32_kernel(Chunk c) {
+__global__ NF_TWO_PER_CU void shared_narrow_f32_kernel(Chunk c) {
   each_part(c, 16, [&](const RowTile& t, uint32_t sp, uint32_t ns, uint32_t kvh) {
     narrow_f32_tile<PT, DD, UNI, kShared>(c, t, sp, ns, kvh);
   });
@@ -2011,7 +2015,7 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_f32_kernel(Chunk c) {
   if (sp < ns) wide_f32_rows<PT, DD, UNI, FORM>(c, t, sp, ns, kvh);
 }
 template <PoolType PT, int DD, bool UNI>
-__global__ __launch_bounds__(256, 2) void shared_wide_f32_kernel(Chunk c) {
+__global__ NF_TWO_PER_CU void shared_wide_f32_kernel(Chunk c) {
   each_part(c, 64, [&](const RowTile& t, uint32_t sp, uint32_t ns, uint32_t kvh) {
     wide_f32_rows<PT, DD, UNI, kShared>(c, t, sp, ns, kvh);
   });
