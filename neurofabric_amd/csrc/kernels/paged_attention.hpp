@@ -140,6 +140,7 @@ struct RowTile {
   int shared;                 // shared positions
   uint32_t last;              // a group's rows: one past its last sequence; else 0
   uint32_t slot, splits;      // of the rows' partials this part's first one; splits of its keys
+  uint32_t keys;              // keys of a split
 };
 
 // What a kernel serves: flash_attention_paged_chunk, the same with the rows'
@@ -203,8 +204,11 @@ struct Chunk {
   // kLse, kShared:
   float* lse;    // output, or null
   float* lsum;   // partials, f16: sum of the weights as they were before they were rounded
-  PagedShared sh;  // kShared
-  bool apart;      // the groups' shared keys are parts of their own
+  // kShared (keys_per_split: the least):
+  PagedShared sh;
+  bool apart;       // the groups' shared keys are parts of their own
+  uint32_t target;  // splits of a KV head's keys that are aimed at
+  uint32_t* keys;   // where the attention leaves the keys of a split for the combination
 };
 
 // Splits that a sequence of `len` positions takes.
@@ -225,61 +229,84 @@ __device__ __forceinline__ Border find_border(bool apart, int shared, int end) {
   const int split = apart ? 0 : (shared + 63) & ~63, shift = split - (shared & ~15);
   return {split, shift, end + shift};
 }
-// Splits of the partials of a row: those of its group's part, then those of its own.
+// Splits of the partials of a row, of `keys` keys each: those of its group's part, then
+// those of its own.
 struct Slots {
   uint32_t group, own;
 };
-__device__ __forceinline__ Slots find_slots(const Chunk& c, int shared, int len) {
-  const uint32_t group = c.apart && shared > 0 ? splits_of(c, shared) : 0;
-  const int n = find_border(c.apart, shared, len).end;
-  return {group, n <= 0 && group ? 0 : splits_of(c, n)};
+__device__ __forceinline__ uint32_t cut(int n, uint32_t keys) { return n <= 0 ? 1u : ((uint32_t)n + keys - 1) / keys; }
+__device__ __forceinline__ Slots find_slots(bool apart, uint32_t keys, int shared, int len) {
+  const uint32_t group = apart && shared > 0 ? cut(shared, keys) : 0;
+  const int n = find_border(apart, shared, len).end;
+  return {group, n <= 0 && group ? 0 : cut(n, keys)};
 }
 
-// kShared: tile `idx` of KV head and batch in the order of the parts: first the groups'
-// shared keys (where they are apart), then the sequences; of a part, all tiles of a split
-// after each other, so that they share its keys in the caches.  `from` and `done` hold the
-// place that a call with a smaller idx came to.
-__device__ __forceinline__ bool find_part(const Chunk& c, uint32_t idx, uint32_t per, RowTile& t, uint32_t& sp,
-                                          uint32_t& from, uint32_t& done) {
+// kShared: the batch as parts, first the groups' shared keys (where they are apart), then
+// the sequences.  Part e: its rows, and the keys that its tiles count.
+struct Part {
+  uint32_t n, start, seq, pre, last;
+  int len, pos0, shared, keys;
+};
+__device__ __forceinline__ Part find_part(const Chunk& c, uint32_t e) {
   const PagedBatch& b = c.b;
+  const uint32_t groups = c.apart ? c.sh.n_groups : 0;
+  Part p{};
+  if (e < groups) {
+    const int32_t a = c.sh.first[e], z = c.sh.first[e + 1], len = c.sh.len[e];
+    if (a < 0 || z <= a || (uint32_t)a >= b.n_seqs || len <= 0) return p;
+    p.last = (uint32_t)z < b.n_seqs ? (uint32_t)z : b.n_seqs;
+    p.seq = p.pre = (uint32_t)a;
+    p.shared = p.len = p.keys = len < (int64_t)b.limit ? len : (int)b.limit;
+    const int64_t r0 = b.starts[a] > 0 ? b.starts[a] : 0, r1 = b.starts[p.last];
+    const int64_t r2 = r1 < (int64_t)b.rows ? r1 : (int64_t)b.rows;
+    p.start = (uint32_t)r0;
+    p.n = r2 > r0 ? (uint32_t)(r2 - r0) : 0;
+  } else if (e < groups + b.n_seqs) {
+    p.seq = e - groups;
+    const int64_t a = b.starts[p.seq], z = b.starts[p.seq + 1];
+    const int32_t l = b.lens[p.seq];
+    if (a < 0 || z <= a || z > (int64_t)b.rows) return p;
+    p.n = (uint32_t)(z - a);
+    p.start = (uint32_t)a;
+    p.pos0 = (int)((uint32_t)l - p.n);
+    p.len = l < (int64_t)b.limit ? l : (int)b.limit;
+    const SharedPrefix pre = find_prefix(b, c.sh, p.seq);
+    p.pre = pre.seq;
+    p.shared = (int)pre.len;
+    p.keys = find_border(c.apart, p.shared, p.len).end;
+  }
+  return p;
+}
+
+// Tile and split `idx` of a KV head.  The keys of a split are chosen here, as only the
+// device knows the lengths: the tiles' keys over `target`, at least keys_per_split.  All
+// tiles of a part's split come after each other, so that they share its keys in the
+// caches.  Tiles of up to `few` rows take `narrow` of them, others `wide`.
+template <uint32_t FEW, uint32_t NARROW, uint32_t WIDE>
+__device__ __forceinline__ bool find_shared_tile(const Chunk& c, uint32_t idx, RowTile& t, uint32_t& sp) {
   const int lane = threadIdx.x & 63;
-  const uint32_t groups = c.apart ? c.sh.n_groups : 0, parts = groups + b.n_seqs;
-  for (; from < parts; from += 64) {
-    const uint32_t e = from + lane;
-    uint32_t n = 0, start = 0, seq = 0, pre = 0, last = 0, slot = 0, splits = 0;
-    int32_t len = 0, pos0 = 0, shared = 0;
-    if (e < groups) {
-      const int32_t a = c.sh.first[e], z = c.sh.first[e + 1], p = c.sh.len[e];
-      if (a >= 0 && z > a && (uint32_t)a < b.n_seqs && p > 0) {
-        last = (uint32_t)z < b.n_seqs ? (uint32_t)z : b.n_seqs;
-        seq = pre = (uint32_t)a;
-        shared = len = p < (int64_t)b.limit ? p : (int)b.limit;
-        const int64_t r0 = b.starts[a] > 0 ? b.starts[a] : 0, r1 = b.starts[last];
-        const int64_t r2 = r1 < (int64_t)b.rows ? r1 : (int64_t)b.rows;
-        start = (uint32_t)r0;
-        n = r2 > r0 ? (uint32_t)(r2 - r0) : 0;
-        splits = splits_of(c, shared);
-      }
-    } else if (e < parts) {
-      seq = e - groups;
-      const int64_t a = b.starts[seq], z = b.starts[seq + 1];
-      const int32_t l = b.lens[seq];
-      if (a >= 0 && z > a && z <= (int64_t)b.rows) {
-        n = (uint32_t)(z - a);
-        start = (uint32_t)a;
-        pos0 = (int)((uint32_t)l - n);
-        len = l < (int64_t)b.limit ? l : (int)b.limit;
-        const SharedPrefix p = find_prefix(b, c.sh, seq);
-        pre = p.seq;
-        shared = (int)p.len;
-        const Slots s = find_slots(c, shared, len);
-        slot = s.group;
-        splits = s.own;
-      }
-    }
-    const uint64_t rows = (uint64_t)n * c.group;
-    const uint32_t tiles = rows > c.lo && rows <= c.hi ? (uint32_t)((rows + per - 1) / per) : 0;
-    const uint32_t mine = tiles * splits;
+  const uint32_t parts = (c.apart ? c.sh.n_groups : 0) + c.b.n_seqs;
+  auto tiles_of = [&](const Part& p) {
+    const uint64_t rows = (uint64_t)p.n * c.group;
+    return (uint32_t)(rows <= FEW ? (rows + NARROW - 1) / NARROW : (rows + WIDE - 1) / WIDE);
+  };
+  Part p;
+  float work = 0.f;  // (a sum of whole numbers in one order: the same in every workgroup)
+  for (uint32_t e0 = 0; e0 < parts; e0 += 64) {
+    p = find_part(c, e0 + lane);
+    work += p.keys > 0 ? (float)p.keys * (float)tiles_of(p) : 0.f;
+  }
+  work = wave_sum(work) / (float)c.target;
+  uint32_t keys = work < 1e9f ? ((uint32_t)work + 128) / 128 * 128 : 1u << 30;
+  keys = (uint32_t)__builtin_amdgcn_readfirstlane((int)(keys > c.keys_per_split ? keys : c.keys_per_split));
+  t.keys = keys;
+  uint32_t done = 0;
+  for (uint32_t e0 = 0; e0 < parts; e0 += 64) {
+    if (parts > 64) p = find_part(c, e0 + lane);
+    const uint32_t tiles = tiles_of(p);
+    Slots s = {0, p.last ? cut(p.shared, keys) : 0};
+    if (p.last == 0) s = find_slots(c.apart, keys, p.shared, p.len);
+    const uint32_t mine = tiles * s.own;
     uint32_t up = mine;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -291,19 +318,19 @@ __device__ __forceinline__ bool find_part(const Chunk& c, uint32_t idx, uint32_t
       const uint32_t i = idx - done;
       const int at = __builtin_ctzll(__ballot(up > i));
       auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, at); };
-      const uint32_t k = i - of(up - mine), nt = of(tiles);
+      const uint32_t k = i - of(up - mine), nt = of(tiles), rows = of(p.n) * c.group;
       sp = k / nt;
-      t.first = (k - sp * nt) * per;
-      t.seq = of(seq);
-      t.rows = of((uint32_t)rows);
-      t.start = of(start);
-      t.pos0 = (int)of((uint32_t)pos0);
-      t.len = (int)of((uint32_t)len);
-      t.pre = of(pre);
-      t.shared = (int)of((uint32_t)shared);
-      t.last = of(last);
-      t.slot = of(slot);
-      t.splits = of(splits);
+      t.first = (k - sp * nt) * (rows <= FEW ? NARROW : WIDE);
+      t.seq = of(p.seq);
+      t.rows = rows;
+      t.start = of(p.start);
+      t.pos0 = (int)of((uint32_t)p.pos0);
+      t.len = (int)of((uint32_t)p.len);
+      t.pre = of(p.pre);
+      t.shared = (int)of((uint32_t)p.shared);
+      t.last = of(p.last);
+      t.slot = of(s.group);
+      t.splits = of(s.own);
       return true;
     }
     done += total;
@@ -588,8 +615,15 @@ __device__ __forceinline__ uint2 read_tr(const half_t* p) {
 // instructions at I8 (4 of up to 131072: 0.83 GB in 158 to 166 us, 5.1 TB/s); with 20 rows
 // a sequence by the conversion (16 of up to 4096: 91 MB in 31 us).
 // kLse, kShared: the log-sum-exp takes the weights as they were before they are rounded.
+template <int DD, int NT, bool LSE>
+struct NarrowLds {
+  __attribute__((aligned(16))) half_t vs[4][32 * (DD + 16)];
+  __attribute__((aligned(16))) float ps[4][32][16];
+  float wm[4][16 * NT], wl[4][16 * NT], wx[LSE ? 4 : 1][16 * NT];
+};
 template <PoolType PT, int DD, int NT, bool UNI, Form FORM>
-__device__ __forceinline__ void narrow_tile(const Chunk& c, const RowTile& t, uint32_t sp, uint32_t ns, uint32_t kvh) {
+__device__ __forceinline__ void narrow_tile(const Chunk& c, const RowTile& t, uint32_t sp, uint32_t ns, uint32_t kvh,
+                                            NarrowLds<DD, NT, FORM != kChunk>& lds) {
   constexpr bool SHARE = FORM == kShared, LSE = FORM != kChunk;
   constexpr bool I8 = PT == PoolType::I8;
   constexpr int KSTEP = DD / 32, DB = DD / 16;
@@ -599,9 +633,11 @@ __device__ __forceinline__ void narrow_tile(const Chunk& c, const RowTile& t, ui
   constexpr int VC = I8 ? 16 : 8;                    // elements per 16-byte chunk
   constexpr int CPR = DD / VC, NV = 32 * CPR / 64;   // chunks per row, per lane and tile
   constexpr int NP = KSTEP / 2;                      // I8: 16-code loads per key row
-  __shared__ __attribute__((aligned(16))) half_t vs[4][32 * VP];
-  __shared__ __attribute__((aligned(16))) float ps[4][32][16];
-  __shared__ float wm[4][16 * NT], wl[4][16 * NT], wx[LSE ? 4 : 1][16 * NT];
+  auto& vs = lds.vs;
+  auto& ps = lds.ps;
+  auto& wm = lds.wm;
+  auto& wl = lds.wl;
+  auto& wx = lds.wx;
   static_assert(sizeof(float) * 16 * DD <= sizeof(half_t) * 32 * VP, "a wave's rows merge in its part of vs");
 
   const uint32_t G = c.group, H = c.n_heads;
@@ -610,9 +646,10 @@ __device__ __forceinline__ void narrow_tile(const Chunk& c, const RowTile& t, ui
   const uint32_t live = t.rows - t.first < 16u * NT ? t.rows - t.first : 16u * NT;
   const bool all = SHARE && t.last && see_all(c.b, t);
   const Keys keys = find_keys<FORM>(c, t, t.first / G, (t.first + live - 1) / G, all);
-  const int pos_lo = keys.lo, begin = (int)(sp * c.keys_per_split);
+  const uint32_t cut_keys = SHARE ? t.keys : c.keys_per_split;
+  const int pos_lo = keys.lo, begin = (int)(sp * cut_keys);
   int end = keys.at.end;  // keys below it
-  if (end > begin + (int)c.keys_per_split) end = begin + (int)c.keys_per_split;
+  if (end > begin + (int)cut_keys) end = begin + (int)cut_keys;
   end = __builtin_amdgcn_readfirstlane(end);
 
   half8 qb[NT][KSTEP];
@@ -899,28 +936,8 @@ __global__ NF_TWO_PER_CU void chunk_narrow_kernel(Chunk c) {
   RowTile t;
   if (!find_tile(c.b, blockIdx.x / c.splits, c.group, 16 * NT, c.lo, c.hi, t)) return;
   const uint32_t ns = splits_of(c, t.len);
-  if (sp < ns) narrow_tile<PT, DD, NT, UNI, FORM>(c, t, sp, ns, kvh);
-}
-
-// kShared: as many workgroups as run at once take the tiles of all parts in turn, as
-// only the device knows how many there are.  `ns` of a part: 1 says that no other has
-// partials of its rows.
-template <typename F>
-__device__ __forceinline__ void each_part(const Chunk& c, uint32_t per, F f) {
-  uint32_t from = 0, done = 0;
-  for (uint32_t id = blockIdx.x;; id += gridDim.x) {
-    RowTile t;
-    uint32_t sp;
-    if (!find_part(c, id / c.b.n_kv, per, t, sp, from, done)) return;
-    f(t, sp, t.last == 0 && t.slot == 0 ? t.splits : t.splits + 1, id % c.b.n_kv);
-    __syncthreads();  // the next tile's LDS
-  }
-}
-template <PoolType PT, int DD, int NT, bool UNI>
-__global__ NF_TWO_PER_CU void shared_narrow_kernel(Chunk c) {
-  each_part(c, 16 * NT, [&](const RowTile& t, uint32_t sp, uint32_t ns, uint32_t kvh) {
-    narrow_tile<PT, DD, NT, UNI, kShared>(c, t, sp, ns, kvh);
-  });
+  __shared__ NarrowLds<DD, NT, FORM != kChunk> lds;
+  if (sp < ns) narrow_tile<PT, DD, NT, UNI, FORM>(c, t, sp, ns, kvh, lds);
 }
 
 // The splits of every query row whose sequence has more than one, where they are few:
@@ -932,7 +949,7 @@ template <Form FORM>
 __device__ __forceinline__ uint32_t row_splits(const Chunk& c, uint32_t seq) {
   const int l = c.b.lens[seq], len = l < (int)c.b.limit ? l : (int)c.b.limit;
   if constexpr (FORM == kShared) {
-    const Slots s = find_slots(c, (int)find_prefix(c.b, c.sh, seq).len, len);
+    const Slots s = find_slots(c.apart, *c.keys, (int)find_prefix(c.b, c.sh, seq).len, len);
     return s.group + s.own;
   }
   return splits_of(c, len);
@@ -1095,24 +1112,28 @@ inline uint32_t wide_grid(uint32_t tiles, uint32_t n_kv) {
 // reaches 1093; the MFMA pipes are busy 32 % of the cycles, and without its softmax and
 // staging this kernel took 364 us.  From I8 594 to 631 us: half the bytes to stage, the
 // conversion beside the MFMAs.
+// V rows 16 or 48 dwords past a multiple of 64: the 4 rows and 32 dims that 32 lanes
+// of a transposing read touch then lie in different banks (in rows of DD + 8, pairs
+// of them share; 685 and 671 us at the size above).  Two buffers for the open tiles; the
+// masked ones use the first, and the second for the weights of the vector ALU.
+template <int DD>
+struct WideLds {
+  static constexpr int KP = DD + 8, VP = DD == 96 ? 96 : DD + 32, BUF = 64 * (KP + VP);
+  __attribute__((aligned(16))) half_t lds[2 * BUF];
+  int tile_bad[2];
+};
 template <PoolType PT, int DD, bool UNI, Form FORM>
-__device__ __forceinline__ void wide_rows(const Chunk& c, const RowTile& t, uint32_t sp, uint32_t ns, uint32_t kvh) {
+__device__ __forceinline__ void wide_rows(const Chunk& c, const RowTile& t, uint32_t sp, uint32_t ns, uint32_t kvh,
+                                          WideLds<DD>& mem) {
   constexpr bool SHARE = FORM == kShared, LSE = FORM != kChunk;
   constexpr bool I8 = PT == PoolType::I8;
-  constexpr int KS = DD / 16, DB = DD / 32, KP = DD + 8;
-  // V rows 16 or 48 dwords past a multiple of 64: the 4 rows and 32 dims that 32 lanes
-  // of a transposing read touch then lie in different banks (in rows of KP, pairs
-  // of them share; 685 and 671 us at the size below)
-  constexpr int VP = DD == 96 ? 96 : DD + 32;
+  constexpr int KS = DD / 16, DB = DD / 32, KP = WideLds<DD>::KP, VP = WideLds<DD>::VP, BUF = WideLds<DD>::BUF;
   constexpr int VC = I8 ? 16 : 8;
   constexpr int CPR = DD / VC;
   constexpr int NU = (64 * CPR + 255) / 256;
-  // two buffers for the open tiles; the masked ones use the first, and the second for
-  // the weights of the vector ALU
-  constexpr int BUF = 64 * (KP + VP);
   static_assert(BUF * sizeof(half_t) >= 4 * 32 * 32 * sizeof(float), "a buffer holds the weights");
-  __shared__ __attribute__((aligned(16))) half_t lds[2 * BUF];
-  __shared__ int tile_bad[2];
+  half_t* const lds = mem.lds;
+  auto& tile_bad = mem.tile_bad;
   half_t* const ks = lds;
   half_t* const vs = lds + 64 * KP;
   float(*const ps)[32][32] = reinterpret_cast<float(*)[32][32]>(lds + BUF);
@@ -1123,9 +1144,10 @@ __device__ __forceinline__ void wide_rows(const Chunk& c, const RowTile& t, uint
   const uint32_t last = (t.first + 128 < t.rows ? t.first + 128 : t.rows) - 1;
   const bool all = SHARE && t.last && see_all(c.b, t);
   const Keys keys = find_keys<FORM>(c, t, t.first / G, last / G, all);
-  const int pos_lo = keys.lo, begin = (int)(sp * c.keys_per_split);
+  const uint32_t cut_keys = SHARE ? t.keys : c.keys_per_split;
+  const int pos_lo = keys.lo, begin = (int)(sp * cut_keys);
   int end = keys.at.end;
-  if (end > begin + (int)c.keys_per_split) end = begin + (int)c.keys_per_split;
+  if (end > begin + (int)cut_keys) end = begin + (int)cut_keys;
   end = __builtin_amdgcn_readfirstlane(end);
 
   const uint32_t r0 = t.first + 32 * w;
@@ -1460,13 +1482,26 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
   RowTile t;
   if (!find_tile(c.b, idx, c.group, 128, c.lo, c.hi, t)) return;
   const uint32_t ns = splits_of(c, t.len);
-  if (sp < ns) wide_rows<PT, DD, UNI, FORM>(c, t, sp, ns, kvh);
+  __shared__ WideLds<DD> lds;
+  if (sp < ns) wide_rows<PT, DD, UNI, FORM>(c, t, sp, ns, kvh, lds);
 }
-template <PoolType PT, int DD, bool UNI>
-__global__ NF_TWO_PER_CU void shared_wide_kernel(Chunk c) {
-  each_part(c, 128, [&](const RowTile& t, uint32_t sp, uint32_t ns, uint32_t kvh) {
-    wide_rows<PT, DD, UNI, kShared>(c, t, sp, ns, kvh);
-  });
+
+// kShared: narrow and wide tiles in one launch, whose workgroups find out which theirs is.
+// `ns` of a part: 1 says that no other has partials of its rows.
+template <PoolType PT, int DD, int NT, bool UNI>
+__global__ NF_TWO_PER_CU void shared_kernel(Chunk c) {
+  __shared__ union {
+    NarrowLds<DD, NT, true> narrow;
+    WideLds<DD> wide;
+  } lds;
+  RowTile t;
+  uint32_t sp;
+  const uint32_t kvh = blockIdx.x, idx = blockIdx.z * gridDim.y + blockIdx.y;
+  if (!find_shared_tile<64, 16 * NT, 128>(c, idx, t, sp)) return;
+  if (idx == 0 && kvh == 0 && threadIdx.x == 0) *c.keys = t.keys;
+  const uint32_t ns = t.last == 0 && t.slot == 0 ? t.splits : t.splits + 1;
+  if (t.rows <= 64) narrow_tile<PT, DD, NT, UNI, kShared>(c, t, sp, ns, kvh, lds.narrow);
+  else wide_rows<PT, DD, UNI, kShared>(c, t, sp, ns, kvh, lds.wide);
 }
 
 // ---- f32 rows -----------------------------------------------------------------------
@@ -1515,22 +1550,30 @@ __device__ __forceinline__ void store_f32(const Chunk& c, uint64_t orow, uint32_
 // with a masked pair and a value that is not finite reads the values again, row by
 // row, for the pairs that count.  Bound by HBM (8 sequences of up to 4096 positions,
 // 8 KV heads of 128: 49 us), at short caches by its latency (one of 101: 6.6 us).
+template <int DD>
+struct NarrowLdsF32 {
+  __attribute__((aligned(16))) float merge[4][16 * 64 * ((DD + 63) / 64)];
+  float wm[4][16], wl[4][16];
+};
 template <PoolType PT, int DD, bool UNI, Form FORM>
-__device__ __forceinline__ void narrow_f32_tile(const Chunk& c, const RowTile& t, uint32_t sp, uint32_t ns, uint32_t kvh) {
+__device__ __forceinline__ void narrow_f32_tile(const Chunk& c, const RowTile& t, uint32_t sp, uint32_t ns, uint32_t kvh,
+                                                NarrowLdsF32<DD>& lds) {
   constexpr bool SHARE = FORM == kShared;
   constexpr bool I8 = PT == PoolType::I8;
   constexpr int DG = DD / 4, NH = (DD + 63) / 64, NB = 4 * NH;
-  __shared__ __attribute__((aligned(16))) float merge[4][16 * 64 * NH];
-  __shared__ float wm[4][16], wl[4][16];
+  auto& merge = lds.merge;
+  auto& wm = lds.wm;
+  auto& wl = lds.wl;
   const uint32_t G = c.group, H = c.n_heads;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t last = (t.first + 16 < t.rows ? t.first + 16 : t.rows) - 1;
   const bool all = SHARE && t.last && see_all(c.b, t);
   const Keys keys = find_keys<FORM>(c, t, t.first / G, last / G, all);
-  const int pos_lo = keys.lo, begin = (int)(sp * c.keys_per_split);
+  const uint32_t cut_keys = SHARE ? t.keys : c.keys_per_split;
+  const int pos_lo = keys.lo, begin = (int)(sp * cut_keys);
   int end = keys.at.end;
-  if (end > begin + (int)c.keys_per_split) end = begin + (int)c.keys_per_split;
+  if (end > begin + (int)cut_keys) end = begin + (int)cut_keys;
   end = __builtin_amdgcn_readfirstlane(end);
   const uint32_t row = t.first + n < t.rows ? t.first + n : t.rows - 1;
   const uint64_t orow = (uint64_t)(t.start + row / G) * H + kvh * G + row % G;
@@ -1770,13 +1813,8 @@ __global__ __launch_bounds__(256, 2) void chunk_narrow_f32_kernel(Chunk c) {
   RowTile t;
   if (!find_tile(c.b, blockIdx.x / c.splits, c.group, 16, c.lo, c.hi, t)) return;
   const uint32_t ns = splits_of(c, t.len);
-  if (sp < ns) narrow_f32_tile<PT, DD, UNI, FORM>(c, t, sp, ns, kvh);
-}
-template <PoolType PT, int DD, bool UNI>
-__global__ NF_TWO_PER_CU void shared_narrow_f32_kernel(Chunk c) {
-  each_part(c, 16, [&](const RowTile& t, uint32_t sp, uint32_t ns, uint32_t kvh) {
-    narrow_f32_tile<PT, DD, UNI, kShared>(c, t, sp, ns, kvh);
-  });
+  __shared__ NarrowLdsF32<DD> lds;
+  if (sp < ns) narrow_f32_tile<PT, DD, UNI, FORM>(c, t, sp, ns, kvh, lds);
 }
 
 // Many query rows: 64 a workgroup, 16 per wave, 32-key tiles of K and V in LDS.
@@ -1785,27 +1823,37 @@ __global__ NF_TWO_PER_CU void shared_narrow_f32_kernel(Chunk c) {
 // Two sequences of 512 tokens with 2048 positions, 32 heads of 128, 293 us; three of up
 // to 389 with 2000, 32 heads of 64, 9.5 GFLOP in 117 us with the combine (13 of them),
 // where a product of 8192 in each size reaches 153 TFLOP/s.
+template <int DD>
+struct WideLdsF32 {
+  __attribute__((aligned(16))) float ks[32 * (DD + 4)];
+  __attribute__((aligned(16))) float vs[32 * (DD + 4) + 64 * ((DD + 63) / 64) - DD];
+  __attribute__((aligned(16))) float ps[4][32][16];
+  int tile_bad[2];
+};
 template <PoolType PT, int DD, bool UNI, Form FORM>
-__device__ __forceinline__ void wide_f32_rows(const Chunk& c, const RowTile& t, uint32_t sp, uint32_t ns, uint32_t kvh) {
+__device__ __forceinline__ void wide_f32_rows(const Chunk& c, const RowTile& t, uint32_t sp, uint32_t ns, uint32_t kvh,
+                                              WideLdsF32<DD>& lds) {
   constexpr bool SHARE = FORM == kShared;
   constexpr bool I8 = PT == PoolType::I8;
   constexpr int TK = 32, DP = DD + 4, DG = DD / 4, NH = (DD + 63) / 64, NB = 4 * NH;
   constexpr int EC = I8 ? 8 : 4;                  // elements per chunk (8 or 16 bytes)
   constexpr int CPR = DD / EC, NU = (TK * CPR + 255) / 256;
   static_assert(CPR % 4 == 0, "a wave's 64 chunks of a tile lie in one group of 16 keys");
-  __shared__ __attribute__((aligned(16))) float ks[TK * DP];
-  __shared__ __attribute__((aligned(16))) float vs[TK * DP + 64 * NH - DD];
-  __shared__ __attribute__((aligned(16))) float ps[4][TK][16];
-  __shared__ int tile_bad[2];
+  static_assert(TK == 32, "as in WideLdsF32");
+  auto& ks = lds.ks;
+  auto& vs = lds.vs;
+  auto& ps = lds.ps;
+  auto& tile_bad = lds.tile_bad;
   const uint32_t G = c.group, H = c.n_heads;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t last = (t.first + 64 < t.rows ? t.first + 64 : t.rows) - 1;
   const bool all = SHARE && t.last && see_all(c.b, t);
   const Keys keys = find_keys<FORM>(c, t, t.first / G, last / G, all);
-  const int pos_lo = keys.lo, begin = (int)(sp * c.keys_per_split);
+  const uint32_t cut_keys = SHARE ? t.keys : c.keys_per_split;
+  const int pos_lo = keys.lo, begin = (int)(sp * cut_keys);
   int end = keys.at.end;
-  if (end > begin + (int)c.keys_per_split) end = begin + (int)c.keys_per_split;
+  if (end > begin + (int)cut_keys) end = begin + (int)cut_keys;
   end = __builtin_amdgcn_readfirstlane(end);
   const uint32_t r0 = t.first + 16 * w;
   const bool wave_live = r0 < t.rows;
@@ -2012,13 +2060,23 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_f32_kernel(Chunk c) {
   RowTile t;
   if (!find_tile(c.b, idx, c.group, 64, c.lo, c.hi, t)) return;
   const uint32_t ns = splits_of(c, t.len);
-  if (sp < ns) wide_f32_rows<PT, DD, UNI, FORM>(c, t, sp, ns, kvh);
+  __shared__ WideLdsF32<DD> lds;
+  if (sp < ns) wide_f32_rows<PT, DD, UNI, FORM>(c, t, sp, ns, kvh, lds);
 }
 template <PoolType PT, int DD, bool UNI>
-__global__ NF_TWO_PER_CU void shared_wide_f32_kernel(Chunk c) {
-  each_part(c, 64, [&](const RowTile& t, uint32_t sp, uint32_t ns, uint32_t kvh) {
-    wide_f32_rows<PT, DD, UNI, kShared>(c, t, sp, ns, kvh);
-  });
+__global__ NF_TWO_PER_CU void shared_f32_kernel(Chunk c) {
+  __shared__ union {
+    NarrowLdsF32<DD> narrow;
+    WideLdsF32<DD> wide;
+  } lds;
+  RowTile t;
+  uint32_t sp;
+  const uint32_t kvh = blockIdx.x, idx = blockIdx.z * gridDim.y + blockIdx.y;
+  if (!find_shared_tile<32, 16, 64>(c, idx, t, sp)) return;
+  if (idx == 0 && kvh == 0 && threadIdx.x == 0) *c.keys = t.keys;
+  const uint32_t ns = t.last == 0 && t.slot == 0 ? t.splits : t.splits + 1;
+  if (t.rows <= 32) narrow_f32_tile<PT, DD, UNI, kShared>(c, t, sp, ns, kvh, lds.narrow);
+  else wide_f32_rows<PT, DD, UNI, kShared>(c, t, sp, ns, kvh, lds.wide);
 }
 
 // ---- launch ------------------------------------------------------------------------------

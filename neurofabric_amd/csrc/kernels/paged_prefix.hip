@@ -15,51 +15,45 @@ namespace paged {
 
 // Query rows of a sequence, on average, up to which the shared keys are apart.
 constexpr uint32_t kApartRows = 64;
-// Workgroups of a launch: two on each CU.
+// Workgroups that run at once, two on each CU, and the fewest keys that one takes.
 constexpr uint32_t kResident = 512;
+constexpr uint32_t kMinKeys = 256;
 
 template <typename T, PoolType PT, int DD, bool UNI>
 hipError_t prefix_at(const PagedBatch& b, const PagedShared& sh, uint32_t n_heads, const Operands& o,
                      const nfhip::Workspace& ws, hipStream_t s) {
   constexpr bool F16 = std::is_same<T, half_t>::value;
-  constexpr uint32_t kWideRows = F16 ? 128 : 64;
+  constexpr uint32_t kWideRows = F16 ? 128 : 64, kFew = F16 ? 64 : 32;
   Chunk c = chunk_of(b, n_heads, o);
   c.sh = sh;
   const uint64_t rows = (uint64_t)b.rows * c.group, mean = (rows + b.n_seqs - 1) / b.n_seqs;
-  const uint64_t most = ws.part ? ws.part_floats / ((uint64_t)b.rows * n_heads * (DD + kPartFloats)) : 1;
+  const uint64_t floats = ws.part ? ws.part_floats - 4 : 0;
+  const uint64_t most = floats / ((uint64_t)b.rows * n_heads * (DD + kPartFloats));
   c.apart = sh.n_groups > 0 && sh.n_groups < b.n_seqs && mean <= kApartRows && most >= 4;
   const uint32_t nt = F16 && mean > 16 ? 2 : 1;
-  const bool wide = rows > kNarrowRows<T>;
-  const uint64_t per = (c.apart ? wide : mean > kNarrowRows<T>) ? kWideRows : 16 * nt;
-  // Tiles that share the keys between them; a row has partials of two parts at most.
-  const uint64_t tiles = (c.apart ? (rows + per - 1) / per : b.n_seqs * ((mean + per - 1) / per)) * b.n_kv;
-  uint64_t splits = tiles < kResident ? kResident / tiles : 1;
-  const uint64_t limit = (uint64_t)b.limit + 80, parts = c.apart ? 2 : 0;  // (as Border counts)
-  if (splits > most - parts && most >= parts + 1) splits = most - parts;
-  if (!c.apart && most < 2) splits = 1;
-  uint64_t keys = (limit + splits - 1) / splits;
-  if (keys < 256) keys = 256;
+  // The fewest keys of a split for which the partials fit (`limit` as Border counts); a row
+  // has them of two parts at most.
+  const uint64_t limit = (uint64_t)b.limit + 80, parts = c.apart ? 2 : 0;
+  uint64_t keys = most >= 2 ? (limit + most - parts - 1) / (most - parts) : limit;
+  if (keys < kMinKeys) keys = kMinKeys;
   keys = (keys + 127) / 128 * 128;
   c.keys_per_split = (uint32_t)keys;
   c.splits = (uint32_t)((limit + keys - 1) / keys + parts);
+  c.target = (kResident + b.n_kv - 1) / b.n_kv;
+  c.keys = reinterpret_cast<uint32_t*>(ws.part + floats);
   place_parts(c, ws, DD);
-  auto grid = [&](uint64_t at) {  // workgroups for tiles of `at` rows
-    const uint64_t n = ((c.apart ? 2 : 1) * (rows / at + b.n_seqs) + sh.n_groups) * c.splits * b.n_kv;
-    return dim3((unsigned)(n < kResident ? n : kResident));
+  // At most so many tiles and splits of a KV head: a part's last tile and split may be short.
+  auto tiles = [&](uint64_t n) {  // of n parts that have all rows between them
+    if (n > b.rows) n = b.rows;
+    const uint64_t few = rows < kFew * n ? rows : kFew * n;
+    return rows / kWideRows + few / (16 * nt) + n;
   };
-  if (wide) {
-    c.lo = kNarrowRows<T>;
-    c.hi = ~0ull;
-    if constexpr (F16) shared_wide_kernel<PT, DD, UNI><<<grid(kWideRows), 256, 0, s>>>(c);
-    else shared_wide_f32_kernel<PT, DD, UNI><<<grid(kWideRows), 256, 0, s>>>(c);
-  }
-  if (!wide || b.n_seqs > 1) {
-    c.lo = 0;
-    c.hi = kNarrowRows<T>;
-    if constexpr (!F16) shared_narrow_f32_kernel<PT, DD, UNI><<<grid(16), 256, 0, s>>>(c);
-    else if (nt == 2) shared_narrow_kernel<PT, DD, 2, UNI><<<grid(32), 256, 0, s>>>(c);
-    else shared_narrow_kernel<PT, DD, 1, UNI><<<grid(16), 256, 0, s>>>(c);
-  }
+  const uint64_t items = tiles(b.n_seqs) + (c.apart ? tiles(sh.n_groups) : 0) + c.target + 1;
+  const uint64_t y = items < 32768 ? items : 32768;
+  const dim3 grid(b.n_kv, (unsigned)y, (unsigned)((items + y - 1) / y));
+  if constexpr (!F16) shared_f32_kernel<PT, DD, UNI><<<grid, 256, 0, s>>>(c);
+  else if (nt == 2) shared_kernel<PT, DD, 2, UNI><<<grid, 256, 0, s>>>(c);
+  else shared_kernel<PT, DD, 1, UNI><<<grid, 256, 0, s>>>(c);
   if (c.splits > 1) {
     if (c.splits <= kFewSplits) chunk_combine_few_kernel<T, DD, kShared><<<dim3((b.rows * n_heads + 3) / 4), 256, 0, s>>>(c);
     else chunk_combine_kernel<T, DD, kShared><<<dim3(b.rows * n_heads), 256, 0, s>>>(c);
