@@ -141,6 +141,7 @@ struct RowTile {
   uint32_t last;              // a group's rows: one past its last sequence; else 0
   uint32_t slot, splits;      // of the rows' partials this part's first one; splits of its keys
   uint32_t keys;              // keys of a split
+  bool all;                   // every row of the group sees all shared positions
 };
 
 // What a kernel serves: flash_attention_paged_chunk, the same with the rows'
@@ -208,7 +209,9 @@ struct Chunk {
   PagedShared sh;
   bool apart;       // the groups' shared keys are parts of their own
   uint32_t target;  // splits of a KV head's keys that are aimed at
-  uint32_t* keys;   // where the attention leaves the keys of a split for the combination
+  uint32_t* keys;   // the keys of a split, for the combination
+  const uint2* items;       // large batches: (part, tile and split) of each workgroup, in turn,
+  const struct Part* parts; // and the parts; else null
 };
 
 // Splits that a sequence of `len` positions takes.
@@ -242,71 +245,148 @@ __device__ __forceinline__ Slots find_slots(bool apart, uint32_t keys, int share
 }
 
 // kShared: the batch as parts, first the groups' shared keys (where they are apart), then
-// the sequences.  Part e: its rows, and the keys that its tiles count.
+// the sequences.
 struct Part {
-  uint32_t n, start, seq, pre, last;
-  int len, pos0, shared, keys;
+  uint32_t n, start;        // rows
+  uint32_t seq, pre, last;  // as in RowTile
+  int len, pos0, shared;
+  int keys;                 // that its tiles count
+  uint32_t group, splits;   // splits of its keys, and of its group's
+  uint32_t all;
 };
-__device__ __forceinline__ Part find_part(const Chunk& c, uint32_t e) {
-  const PagedBatch& b = c.b;
-  const uint32_t groups = c.apart ? c.sh.n_groups : 0;
-  Part p{};
-  if (e < groups) {
-    const int32_t a = c.sh.first[e], z = c.sh.first[e + 1], len = c.sh.len[e];
-    if (a < 0 || z <= a || (uint32_t)a >= b.n_seqs || len <= 0) return p;
-    p.last = (uint32_t)z < b.n_seqs ? (uint32_t)z : b.n_seqs;
-    p.seq = p.pre = (uint32_t)a;
-    p.shared = p.len = p.keys = len < (int64_t)b.limit ? len : (int)b.limit;
-    const int64_t r0 = b.starts[a] > 0 ? b.starts[a] : 0, r1 = b.starts[p.last];
-    const int64_t r2 = r1 < (int64_t)b.rows ? r1 : (int64_t)b.rows;
-    p.start = (uint32_t)r0;
-    p.n = r2 > r0 ? (uint32_t)(r2 - r0) : 0;
-  } else if (e < groups + b.n_seqs) {
-    p.seq = e - groups;
-    const int64_t a = b.starts[p.seq], z = b.starts[p.seq + 1];
-    const int32_t l = b.lens[p.seq];
-    if (a < 0 || z <= a || z > (int64_t)b.rows) return p;
-    p.n = (uint32_t)(z - a);
-    p.start = (uint32_t)a;
-    p.pos0 = (int)((uint32_t)l - p.n);
-    p.len = l < (int64_t)b.limit ? l : (int)b.limit;
-    const SharedPrefix pre = find_prefix(b, c.sh, p.seq);
-    p.pre = pre.seq;
-    p.shared = (int)pre.len;
-    p.keys = find_border(c.apart, p.shared, p.len).end;
-  }
-  return p;
-}
-
-// Tile and split `idx` of a KV head.  The keys of a split are chosen here, as only the
-// device knows the lengths: the tiles' keys over `target`, at least keys_per_split.  All
-// tiles of a part's split come after each other, so that they share its keys in the
-// caches.  Tiles of up to `few` rows take `narrow` of them, others `wide`.
+// Rows of up to kFew query rows are cut into tiles of 16 NT, others of kWide.
 template <uint32_t FEW, uint32_t NARROW, uint32_t WIDE>
-__device__ __forceinline__ bool find_shared_tile(const Chunk& c, uint32_t idx, RowTile& t, uint32_t& sp) {
-  const int lane = threadIdx.x & 63;
-  const uint32_t parts = (c.apart ? c.sh.n_groups : 0) + c.b.n_seqs;
-  auto tiles_of = [&](const Part& p) {
+struct Cut {
+  static __device__ __forceinline__ uint32_t tiles(const Chunk& c, const Part& p) {
     const uint64_t rows = (uint64_t)p.n * c.group;
     return (uint32_t)(rows <= FEW ? (rows + NARROW - 1) / NARROW : (rows + WIDE - 1) / WIDE);
-  };
-  Part p;
-  float work = 0.f;  // (a sum of whole numbers in one order: the same in every workgroup)
-  for (uint32_t e0 = 0; e0 < parts; e0 += 64) {
-    p = find_part(c, e0 + lane);
-    work += p.keys > 0 ? (float)p.keys * (float)tiles_of(p) : 0.f;
   }
-  work = wave_sum(work) / (float)c.target;
-  uint32_t keys = work < 1e9f ? ((uint32_t)work + 128) / 128 * 128 : 1u << 30;
-  keys = (uint32_t)__builtin_amdgcn_readfirstlane((int)(keys > c.keys_per_split ? keys : c.keys_per_split));
-  t.keys = keys;
+  // Tile and split k of a part.  All tiles of a split come after each other, so that they
+  // share its keys in the caches.
+  static __device__ __forceinline__ void tile(const Chunk& c, const Part& p, uint32_t nt, uint32_t k, RowTile& t, uint32_t& sp) {
+    sp = k / nt;
+    t.rows = p.n * c.group;
+    t.first = (k - sp * nt) * (t.rows <= FEW ? NARROW : WIDE);
+    t.seq = p.seq;
+    t.start = p.start;
+    t.pos0 = p.pos0;
+    t.len = p.len;
+    t.pre = p.pre;
+    t.shared = p.shared;
+    t.last = p.last;
+    t.slot = p.group;
+    t.splits = p.splits;
+    t.all = p.all != 0;
+  }
+};
+// A sequence's part, but for its splits.
+__device__ __forceinline__ Part sequence_part(const Chunk& c, uint32_t seq, int64_t a, int64_t z, int32_t l, const SharedPrefix& pre) {
+  Part p{};
+  if (a < 0 || z <= a || z > (int64_t)c.b.rows) return p;
+  p.n = (uint32_t)(z - a);
+  p.start = (uint32_t)a;
+  p.seq = seq;
+  p.pos0 = (int)((uint32_t)l - p.n);
+  p.len = l < (int64_t)c.b.limit ? l : (int)c.b.limit;
+  p.pre = pre.seq;
+  p.shared = (int)pre.len;
+  p.keys = find_border(c.apart, p.shared, p.len).end;
+  return p;
+}
+// A group's: r0, r1 the first row of its first sequence and of the one behind its last.
+__device__ __forceinline__ Part group_part(const Chunk& c, int32_t a, uint32_t last, int32_t len, int64_t r0, int64_t r1) {
+  Part p{};
+  if (r0 < 0) r0 = 0;
+  if (r1 > (int64_t)c.b.rows) r1 = c.b.rows;
+  if (r1 <= r0) return p;
+  p.n = (uint32_t)(r1 - r0);
+  p.start = (uint32_t)r0;
+  p.seq = p.pre = (uint32_t)a;
+  p.last = last;
+  p.shared = p.len = p.keys = len < (int64_t)c.b.limit ? len : (int)c.b.limit;
+  return p;
+}
+__device__ __forceinline__ bool good_group(const PagedBatch& b, int32_t a, int32_t z, int32_t len) {
+  return a >= 0 && z > a && (uint32_t)a < b.n_seqs && len > 0;
+}
+__device__ __forceinline__ void cut_part(const Chunk& c, uint32_t keys, Part& p) {
+  p.group = 0;
+  p.splits = cut(p.shared, keys);
+  if (p.last) return;
+  const Slots s = find_slots(c.apart, keys, p.shared, p.len);
+  p.group = s.group;
+  p.splits = s.own;
+}
+// The keys of a split: all tiles' keys over `target`, at least keys_per_split; only the
+// device knows the lengths.  `work` is the same in all workgroups, being summed in one order.
+__device__ __forceinline__ uint32_t keys_of(const Chunk& c, float work) {
+  work /= (float)c.target;
+  const uint32_t keys = work < 1e9f ? ((uint32_t)work + 128) / 128 * 128 : 1u << 30;
+  return keys > c.keys_per_split ? keys : c.keys_per_split;
+}
+
+// Tile and split `idx` of a KV head, for up to 128 parts and 64 groups: a lane looks at two
+// parts, all loads in one round, which is the time that this takes (a search per sequence,
+// 64 at a time: 4 us of 22 for 64 sequences behind 64 positions).
+constexpr uint32_t kFewParts = 128, kFewGroups = 64;
+template <typename CUT>
+__device__ __forceinline__ bool find_few(const Chunk& c, uint32_t idx, RowTile& t, uint32_t& sp) {
+  const PagedBatch& b = c.b;
+  const int lane = threadIdx.x & 63;
+  const uint32_t groups = c.apart ? c.sh.n_groups : 0;
+  int32_t ga = 0, gz = 0, gl = 0;  // lane g: group g
+  if ((uint32_t)lane < c.sh.n_groups) {
+    ga = c.sh.first[lane];
+    gz = c.sh.first[lane + 1];
+    gl = c.sh.len[lane];
+  }
+  // Sequences are at parts groups .. groups + n_seqs - 1.
+  int32_t a[2], z[2], l[2];
+  uint32_t seq[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t e = 64 * i + lane;
+    seq[i] = e - groups;
+    a[i] = z[i] = l[i] = 0;
+    if (e >= groups && seq[i] < b.n_seqs) {
+      a[i] = b.starts[seq[i]];
+      z[i] = b.starts[seq[i] + 1];
+      l[i] = b.lens[seq[i]];
+    }
+  }
+  // The group of each sequence, as find_prefix() has it: the first whose end is past it.
+  SharedPrefix pre[2] = {{seq[0], 0}, {seq[1], 0}};
+  bool found[2] = {false, false};
+  for (uint32_t g = 0; g < c.sh.n_groups; ++g) {  // uniform
+    const int32_t fa = __builtin_amdgcn_readlane(ga, (int)g), fz = __builtin_amdgcn_readlane(gz, (int)g);
+    const int32_t n = __builtin_amdgcn_readlane(gl, (int)g);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (!found[i] && (int64_t)fz > (int64_t)seq[i]) {
+        found[i] = true;
+        if (fa >= 0 && (uint32_t)fa <= seq[i] && n > 0) pre[i] = {(uint32_t)fa, n < (int64_t)b.limit ? n : (int64_t)b.limit};
+      }
+  }
+  Part p[2];
+  float work = 0.f;
+  // A group's rows, from the lanes of its sequences.
+  const uint32_t last = (uint32_t)gz < b.n_seqs ? (uint32_t)gz : b.n_seqs;
+  const bool good = (uint32_t)lane < groups && good_group(b, ga, gz, gl);
+  const uint32_t e0 = good ? groups + (uint32_t)ga : 0, e1 = good ? groups + last - 1 : 0;
+  const int32_t x0 = __shfl(a[0], (int)(e0 & 63)), x1 = __shfl(a[1], (int)(e0 & 63));
+  const int32_t y0 = __shfl(z[0], (int)(e1 & 63)), y1 = __shfl(z[1], (int)(e1 & 63));
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    p[i] = sequence_part(c, seq[i], a[i], z[i], l[i], pre[i]);
+    if (i == 0 && good) p[i] = group_part(c, ga, last, gl, e0 < 64 ? x0 : x1, e1 < 64 ? y0 : y1);
+    work += p[i].keys > 0 ? (float)p[i].keys * (float)CUT::tiles(c, p[i]) : 0.f;
+  }
+  t.keys = (uint32_t)__builtin_amdgcn_readfirstlane((int)keys_of(c, wave_sum(work)));
   uint32_t done = 0;
-  for (uint32_t e0 = 0; e0 < parts; e0 += 64) {
-    if (parts > 64) p = find_part(c, e0 + lane);
-    const uint32_t tiles = tiles_of(p);
-    Slots s = {0, p.last ? cut(p.shared, keys) : 0};
-    if (p.last == 0) s = find_slots(c.apart, keys, p.shared, p.len);
-    const uint32_t mine = tiles * s.own;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    cut_part(c, t.keys, p[i]);
+    const uint32_t tiles = CUT::tiles(c, p[i]), mine = tiles * p[i].splits;
     uint32_t up = mine;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -315,22 +395,28 @@ __device__ __forceinline__ bool find_shared_tile(const Chunk& c, uint32_t idx, R
     }
     const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)up, 63);
     if (idx - done < total) {
-      const uint32_t i = idx - done;
-      const int at = __builtin_ctzll(__ballot(up > i));
+      const uint32_t k = idx - done;
+      const int at = __builtin_ctzll(__ballot(up > k));
       auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, at); };
-      const uint32_t k = i - of(up - mine), nt = of(tiles), rows = of(p.n) * c.group;
-      sp = k / nt;
-      t.first = (k - sp * nt) * (rows <= FEW ? NARROW : WIDE);
-      t.seq = of(p.seq);
-      t.rows = rows;
-      t.start = of(p.start);
-      t.pos0 = (int)of((uint32_t)p.pos0);
-      t.len = (int)of((uint32_t)p.len);
-      t.pre = of(p.pre);
-      t.shared = (int)of((uint32_t)p.shared);
-      t.last = of(p.last);
-      t.slot = of(s.group);
-      t.splits = of(s.own);
+      Part q;
+      q.n = of(p[i].n);
+      q.start = of(p[i].start);
+      q.seq = of(p[i].seq);
+      q.pre = of(p[i].pre);
+      q.last = of(p[i].last);
+      q.len = (int)of((uint32_t)p[i].len);
+      q.pos0 = (int)of((uint32_t)p[i].pos0);
+      q.shared = (int)of((uint32_t)p[i].shared);
+      q.group = of(p[i].group);
+      q.splits = of(p[i].splits);
+      bool all = true;
+      if (q.last)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          if (p[j].last == 0 && p[j].n > 0 && p[j].seq >= q.seq && p[j].seq < q.last)
+            all = all && (int64_t)p[j].pos0 + 1 >= (int64_t)q.shared;
+      q.all = __ballot(!all) == 0;
+      CUT::tile(c, q, of(tiles), k - of(up - mine), t, sp);
       return true;
     }
     done += total;
@@ -338,16 +424,100 @@ __device__ __forceinline__ bool find_shared_tile(const Chunk& c, uint32_t idx, R
   return false;
 }
 
-// Whether every row of a group sees all of the shared keys.
-__device__ __forceinline__ bool see_all(const PagedBatch& b, const RowTile& t) {
-  bool all = true;
-  for (uint32_t s0 = t.seq; s0 < t.last; s0 += 64) {
-    const uint32_t s = s0 + (threadIdx.x & 63);
-    if (s < t.last && b.starts[s + 1] > b.starts[s])
-      all = all && (int64_t)b.lens[s] - ((int64_t)b.starts[s + 1] - (int64_t)b.starts[s]) + 1 >= (int64_t)t.shared;
-  }
-  return __ballot(!all) == 0;
+// The same from what plan_kernel left.
+template <typename CUT>
+__device__ __forceinline__ bool find_planned(const Chunk& c, uint32_t idx, RowTile& t, uint32_t& sp) {
+  if (idx >= c.keys[1]) return false;
+  const uint2 it = c.items[idx];
+  const Part p = c.parts[__builtin_amdgcn_readfirstlane((int)it.x)];
+  t.keys = c.keys[0];
+  CUT::tile(c, p, CUT::tiles(c, p), (uint32_t)__builtin_amdgcn_readfirstlane((int)it.y), t, sp);
+  return true;
 }
+
+// Large batches: one workgroup writes the parts, and the part and the tile and split of
+// each workgroup of the attention to come.  keys[0]: keys of a split, keys[1]: workgroups
+// of a KV head, at most `room`.
+template <typename CUT>
+__global__ __launch_bounds__(1024) void plan_kernel(Chunk c, Part* parts, uint2* items, uint32_t room) {
+  __shared__ float sums[16];
+  __shared__ uint32_t counts[16];
+  const PagedBatch& b = c.b;
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const uint32_t groups = c.apart ? c.sh.n_groups : 0, n = groups + b.n_seqs;
+  float work = 0.f;
+  for (uint32_t e = tid; e < n; e += 1024) {
+    Part p{};
+    if (e < groups) {
+      const int32_t a = c.sh.first[e], z = c.sh.first[e + 1], len = c.sh.len[e];
+      if (good_group(b, a, z, len)) {
+        const uint32_t last = (uint32_t)z < b.n_seqs ? (uint32_t)z : b.n_seqs;
+        p = group_part(c, a, last, len, b.starts[a], b.starts[last]);
+        p.all = 1;  // unless a sequence finds otherwise
+      }
+    } else {
+      const uint32_t seq = e - groups;
+      p = sequence_part(c, seq, b.starts[seq], b.starts[seq + 1], b.lens[seq], find_prefix(b, c.sh, seq));
+    }
+    parts[e] = p;
+    work += p.keys > 0 ? (float)p.keys * (float)CUT::tiles(c, p) : 0.f;
+  }
+  work = wave_sum(work);
+  if (lane == 0) sums[wave] = work;
+  __syncthreads();  // and the parts
+  work = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) work += sums[i];
+  const uint32_t keys = keys_of(c, work);
+  // A sequence that does not see all of its group's positions says so.
+  if (groups)
+    for (uint32_t e = groups + tid; e < n; e += 1024) {
+      const Part& p = parts[e];
+      if (p.n == 0 || p.shared == 0 || (int64_t)p.pos0 + 1 >= (int64_t)p.shared) continue;
+      uint32_t lo = 0, hi = groups;  // its group, as in find_prefix()
+      while (lo < hi) {
+        const uint32_t mid = (lo + hi) / 2;
+        if ((int64_t)c.sh.first[mid + 1] <= (int64_t)p.seq) lo = mid + 1;
+        else hi = mid;
+      }
+      if (lo < groups) parts[lo].all = 0;
+    }
+  __syncthreads();
+  uint32_t done = 0;
+  for (uint32_t e0 = 0; e0 < n; e0 += 1024) {
+    const uint32_t e = e0 + tid;
+    uint32_t mine = 0;
+    if (e < n) {
+      Part p = parts[e];
+      cut_part(c, keys, p);
+      parts[e].group = p.group;
+      parts[e].splits = p.splits;
+      mine = CUT::tiles(c, p) * p.splits;
+    }
+    uint32_t up = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t v = __shfl_up(up, o);
+      if ((int)lane >= o) up += v;
+    }
+    __syncthreads();
+    if (lane == 63) counts[wave] = up;
+    __syncthreads();
+    uint32_t at = done + up - mine;
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i) {
+      if (i < wave) at += counts[i];
+      done += counts[i];
+    }
+    for (uint32_t k = 0; k < mine; ++k)
+      if (at + k < room) items[at + k] = uint2{e, k};
+  }
+  if (tid == 0) {
+    c.keys[0] = keys;
+    c.keys[1] = done < room ? done : room;
+  }
+}
+
 constexpr int kEverywhere = 0x3FFFFFFF;  // the position of a row that sees all keys
 
 // Position of a query row's token: of a group's rows, that in whatever sequence it is.
@@ -644,7 +814,7 @@ __device__ __forceinline__ void narrow_tile(const Chunk& c, const RowTile& t, ui
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t live = t.rows - t.first < 16u * NT ? t.rows - t.first : 16u * NT;
-  const bool all = SHARE && t.last && see_all(c.b, t);
+  const bool all = SHARE && t.last && t.all;
   const Keys keys = find_keys<FORM>(c, t, t.first / G, (t.first + live - 1) / G, all);
   const uint32_t cut_keys = SHARE ? t.keys : c.keys_per_split;
   const int pos_lo = keys.lo, begin = (int)(sp * cut_keys);
@@ -1142,7 +1312,7 @@ __device__ __forceinline__ void wide_rows(const Chunk& c, const RowTile& t, uint
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, hf = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t last = (t.first + 128 < t.rows ? t.first + 128 : t.rows) - 1;
-  const bool all = SHARE && t.last && see_all(c.b, t);
+  const bool all = SHARE && t.last && t.all;
   const Keys keys = find_keys<FORM>(c, t, t.first / G, last / G, all);
   const uint32_t cut_keys = SHARE ? t.keys : c.keys_per_split;
   const int pos_lo = keys.lo, begin = (int)(sp * cut_keys);
@@ -1497,8 +1667,13 @@ __global__ NF_TWO_PER_CU void shared_kernel(Chunk c) {
   RowTile t;
   uint32_t sp;
   const uint32_t kvh = blockIdx.x, idx = blockIdx.z * gridDim.y + blockIdx.y;
-  if (!find_shared_tile<64, 16 * NT, 128>(c, idx, t, sp)) return;
-  if (idx == 0 && kvh == 0 && threadIdx.x == 0) *c.keys = t.keys;
+  using C = Cut<64, 16 * NT, 128>;
+  if (c.items) {
+    if (!find_planned<C>(c, idx, t, sp)) return;
+  } else {
+    if (!find_few<C>(c, idx, t, sp)) return;
+    if (idx == 0 && kvh == 0 && threadIdx.x == 0) c.keys[0] = t.keys;
+  }
   const uint32_t ns = t.last == 0 && t.slot == 0 ? t.splits : t.splits + 1;
   if (t.rows <= 64) narrow_tile<PT, DD, NT, UNI, kShared>(c, t, sp, ns, kvh, lds.narrow);
   else wide_rows<PT, DD, UNI, kShared>(c, t, sp, ns, kvh, lds.wide);
@@ -1568,7 +1743,7 @@ __device__ __forceinline__ void narrow_f32_tile(const Chunk& c, const RowTile& t
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t last = (t.first + 16 < t.rows ? t.first + 16 : t.rows) - 1;
-  const bool all = SHARE && t.last && see_all(c.b, t);
+  const bool all = SHARE && t.last && t.all;
   const Keys keys = find_keys<FORM>(c, t, t.first / G, last / G, all);
   const uint32_t cut_keys = SHARE ? t.keys : c.keys_per_split;
   const int pos_lo = keys.lo, begin = (int)(sp * cut_keys);
@@ -1848,7 +2023,7 @@ __device__ __forceinline__ void wide_f32_rows(const Chunk& c, const RowTile& t, 
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t last = (t.first + 64 < t.rows ? t.first + 64 : t.rows) - 1;
-  const bool all = SHARE && t.last && see_all(c.b, t);
+  const bool all = SHARE && t.last && t.all;
   const Keys keys = find_keys<FORM>(c, t, t.first / G, last / G, all);
   const uint32_t cut_keys = SHARE ? t.keys : c.keys_per_split;
   const int pos_lo = keys.lo, begin = (int)(sp * cut_keys);
@@ -2072,8 +2247,13 @@ __global__ NF_TWO_PER_CU void shared_f32_kernel(Chunk c) {
   RowTile t;
   uint32_t sp;
   const uint32_t kvh = blockIdx.x, idx = blockIdx.z * gridDim.y + blockIdx.y;
-  if (!find_shared_tile<32, 16, 64>(c, idx, t, sp)) return;
-  if (idx == 0 && kvh == 0 && threadIdx.x == 0) *c.keys = t.keys;
+  using C = Cut<32, 16, 64>;
+  if (c.items) {
+    if (!find_planned<C>(c, idx, t, sp)) return;
+  } else {
+    if (!find_few<C>(c, idx, t, sp)) return;
+    if (idx == 0 && kvh == 0 && threadIdx.x == 0) c.keys[0] = t.keys;
+  }
   const uint32_t ns = t.last == 0 && t.slot == 0 ? t.splits : t.splits + 1;
   if (t.rows <= 32) narrow_f32_tile<PT, DD, UNI, kShared>(c, t, sp, ns, kvh, lds.narrow);
   else wide_f32_rows<PT, DD, UNI, kShared>(c, t, sp, ns, kvh, lds.wide);

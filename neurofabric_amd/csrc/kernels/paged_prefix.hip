@@ -27,10 +27,26 @@ hipError_t prefix_at(const PagedBatch& b, const PagedShared& sh, uint32_t n_head
   Chunk c = chunk_of(b, n_heads, o);
   c.sh = sh;
   const uint64_t rows = (uint64_t)b.rows * c.group, mean = (rows + b.n_seqs - 1) / b.n_seqs;
-  const uint64_t floats = ws.part ? ws.part_floats - 4 : 0;
-  const uint64_t most = floats / ((uint64_t)b.rows * n_heads * (DD + kPartFloats));
-  c.apart = sh.n_groups > 0 && sh.n_groups < b.n_seqs && mean <= kApartRows && most >= 4;
   const uint32_t nt = F16 && mean > 16 ? 2 : 1;
+  c.target = (kResident + b.n_kv - 1) / b.n_kv;
+  // At most so many tiles and splits of a KV head: a part's last tile and split may be short.
+  auto tiles = [&](uint64_t n) {  // of n parts that have all rows between them
+    if (n > b.rows) n = b.rows;
+    const uint64_t few = rows < kFew * n ? rows : kFew * n;
+    return rows / kWideRows + few / (16 * nt) + n;
+  };
+  auto items_of = [&](bool apart) { return tiles(b.n_seqs) + (apart ? tiles(sh.n_groups) : 0) + c.target + 1; };
+  // The workspace's end: two numbers, and the plan of a large batch.
+  auto plan_floats = [&](bool apart) {
+    const uint64_t n = b.n_seqs + (apart ? sh.n_groups : 0);
+    return n <= kFewParts && sh.n_groups <= kFewGroups ? 4 : 4 + n * (sizeof(Part) / 4) + items_of(apart) * 2;
+  };
+  auto splits_in = [&](uint64_t used) {  // of all rows' keys
+    return ws.part_floats > used ? (ws.part_floats - used) / ((uint64_t)b.rows * n_heads * (DD + kPartFloats)) : 0;
+  };
+  c.apart = sh.n_groups > 0 && sh.n_groups < b.n_seqs && mean <= kApartRows && splits_in(plan_floats(true)) >= 4;
+  const uint64_t used = plan_floats(c.apart), most = splits_in(used), items = items_of(c.apart);
+  if (!ws.part || ws.part_floats < used) return hipErrorOutOfMemory;
   // The fewest keys of a split for which the partials fit (`limit` as Border counts); a row
   // has them of two parts at most.
   const uint64_t limit = (uint64_t)b.limit + 80, parts = c.apart ? 2 : 0;
@@ -39,16 +55,16 @@ hipError_t prefix_at(const PagedBatch& b, const PagedShared& sh, uint32_t n_head
   keys = (keys + 127) / 128 * 128;
   c.keys_per_split = (uint32_t)keys;
   c.splits = (uint32_t)((limit + keys - 1) / keys + parts);
-  c.target = (kResident + b.n_kv - 1) / b.n_kv;
-  c.keys = reinterpret_cast<uint32_t*>(ws.part + floats);
   place_parts(c, ws, DD);
-  // At most so many tiles and splits of a KV head: a part's last tile and split may be short.
-  auto tiles = [&](uint64_t n) {  // of n parts that have all rows between them
-    if (n > b.rows) n = b.rows;
-    const uint64_t few = rows < kFew * n ? rows : kFew * n;
-    return rows / kWideRows + few / (16 * nt) + n;
-  };
-  const uint64_t items = tiles(b.n_seqs) + (c.apart ? tiles(sh.n_groups) : 0) + c.target + 1;
+  c.keys = reinterpret_cast<uint32_t*>(ws.part + (ws.part_floats - used) / 4 * 4);
+  if (used > 4) {
+    Part* const plan = reinterpret_cast<Part*>(c.keys + 4);
+    uint2* const list = reinterpret_cast<uint2*>(plan + b.n_seqs + (c.apart ? sh.n_groups : 0));
+    if (nt == 2) plan_kernel<Cut<kFew, 32, kWideRows>><<<1, 1024, 0, s>>>(c, plan, list, (uint32_t)items);
+    else plan_kernel<Cut<kFew, 16, kWideRows>><<<1, 1024, 0, s>>>(c, plan, list, (uint32_t)items);
+    c.parts = plan;
+    c.items = list;
+  }
   const uint64_t y = items < 32768 ? items : 32768;
   const dim3 grid(b.n_kv, (unsigned)y, (unsigned)((items + y - 1) / y));
   if constexpr (!F16) shared_f32_kernel<PT, DD, UNI><<<grid, 256, 0, s>>>(c);

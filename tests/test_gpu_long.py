@@ -84,6 +84,12 @@ PREFIX = [  # sequences (positions, rows), groups (first, one past the last, sha
     ([(600, 40)] + [(530 + i, 1) for i in range(30)], [(0, 31, 512)], 8, 2, 128, 16),
     ([(130, 1)] * 40, [(0, 40, 128)], 4, 4, 64, 64),
     ([(150, 1)] * 12, [(0, 12, 144)], 64, 8, 128, 48),
+    # more sequences, or groups, than a workgroup looks through by itself
+    ([(140 + i % 9, 1 + i % 2) for i in range(150)], [(0, 70, 96), (70, 149, 130)], 4, 2, 64, 16),
+    ([(60 + i % 7, 1) for i in range(160)], [(2 * i, 2 * i + 2, 16 + i % 33) for i in range(80)], 4, 1, 64, 16),
+    ([(60 + i % 7, i % 3) for i in range(100)], [(i, i + 1, i % 40) for i in range(99)], 4, 2, 64, 8),
+    ([(90, 70 if i % 40 == 3 else 1) for i in range(127)], [(0, 127, 17)], 2, 1, 128, 16),
+    ([(90, 70 if i % 40 == 3 else 1) for i in range(128)], [(0, 128, 48)], 2, 1, 96, 16),
 ]
 
 
