@@ -209,7 +209,7 @@ struct Chunk {
   PagedShared sh;
   bool apart;       // the groups' shared keys are parts of their own
   uint32_t target;  // splits of a KV head's keys that are aimed at
-  uint32_t* keys;   // the keys of a split, for the combination
+  uint32_t* keys;   // the keys of a split of a group's part and of an own one, for the combination
   const uint2* items;       // large batches: (part, tile and split) of each workgroup, in turn,
   const struct Part* parts; // and the parts; else null
 };
@@ -232,16 +232,16 @@ __device__ __forceinline__ Border find_border(bool apart, int shared, int end) {
   const int split = apart ? 0 : (shared + 63) & ~63, shift = split - (shared & ~15);
   return {split, shift, end + shift};
 }
-// Splits of the partials of a row, of `keys` keys each: those of its group's part, then
-// those of its own.
+// Splits of the partials of a row: those of its group's part, of keys.x keys each, then
+// those of its own, of keys.y.
 struct Slots {
   uint32_t group, own;
 };
 __device__ __forceinline__ uint32_t cut(int n, uint32_t keys) { return n <= 0 ? 1u : ((uint32_t)n + keys - 1) / keys; }
-__device__ __forceinline__ Slots find_slots(bool apart, uint32_t keys, int shared, int len) {
-  const uint32_t group = apart && shared > 0 ? cut(shared, keys) : 0;
+__device__ __forceinline__ Slots find_slots(bool apart, uint2 keys, int shared, int len) {
+  const uint32_t group = apart && shared > 0 ? cut(shared, keys.x) : 0;
   const int n = find_border(apart, shared, len).end;
-  return {group, n <= 0 && group ? 0 : cut(n, keys)};
+  return {group, n <= 0 && group ? 0 : cut(n, keys.y)};
 }
 
 // kShared: the batch as parts, first the groups' shared keys (where they are apart), then
@@ -263,7 +263,13 @@ struct Cut {
   }
   // Tile and split k of a part.  All tiles of a split come after each other, so that they
   // share its keys in the caches.
-  static __device__ __forceinline__ void tile(const Chunk& c, const Part& p, uint32_t nt, uint32_t k, RowTile& t, uint32_t& sp) {
+  // The time of a tile's key, that of a narrow one's being 2/5 of a wide one's.
+  static __device__ __forceinline__ float cost(const Chunk& c, const Part& p) {
+    return (uint64_t)p.n * c.group <= FEW ? 0.4f : 1.f;
+  }
+  static __device__ __forceinline__ void tile(const Chunk& c, const Part& p, uint32_t nt, uint32_t k, uint2 keys, RowTile& t,
+                                              uint32_t& sp) {
+    t.keys = p.last ? keys.x : keys.y;
     sp = k / nt;
     t.rows = p.n * c.group;
     t.first = (k - sp * nt) * (t.rows <= FEW ? NARROW : WIDE);
@@ -309,20 +315,57 @@ __device__ __forceinline__ Part group_part(const Chunk& c, int32_t a, uint32_t l
 __device__ __forceinline__ bool good_group(const PagedBatch& b, int32_t a, int32_t z, int32_t len) {
   return a >= 0 && z > a && (uint32_t)a < b.n_seqs && len > 0;
 }
-__device__ __forceinline__ void cut_part(const Chunk& c, uint32_t keys, Part& p) {
+__device__ __forceinline__ void cut_part(const Chunk& c, uint2 keys, Part& p) {
   p.group = 0;
-  p.splits = cut(p.shared, keys);
+  p.splits = cut(p.shared, keys.x);
   if (p.last) return;
   const Slots s = find_slots(c.apart, keys, p.shared, p.len);
   p.group = s.group;
   p.splits = s.own;
 }
-// The keys of a split: all tiles' keys over `target`, at least keys_per_split; only the
-// device knows the lengths.  `work` is the same in all workgroups, being summed in one order.
-__device__ __forceinline__ uint32_t keys_of(const Chunk& c, float work) {
-  work /= (float)c.target;
-  const uint32_t keys = work < 1e9f ? ((uint32_t)work + 128) / 128 * 128 : 1u << 30;
-  return keys > c.keys_per_split ? keys : c.keys_per_split;
+
+// What the parts' tiles have to do, in keys of a wide tile.
+struct Work {
+  float shared = 0.f, own = 0.f;                // tiles times keys
+  float shared_cost = 0.f, own_cost = 0.f;      // and their time
+  float tiles = 0.f;                            // own tiles
+  template <typename CUT>
+  __device__ __forceinline__ void add(const Chunk& c, const Part& p) {
+    if (p.keys <= 0 || p.n == 0) return;
+    const float n = (float)CUT::tiles(c, p), w = n * (float)p.keys, cost = w * CUT::cost(c, p);
+    if (p.last) {
+      shared += w;
+      shared_cost += cost;
+    } else {
+      own += w;
+      own_cost += cost;
+      tiles += n;
+    }
+  }
+};
+// The keys of a split; only the device knows the lengths.  With S workgroups at once, which
+// `target` is for a KV head, split k keys take F + k in time, F = 200 (finding the tile, its
+// first keys, its partials: 9 us, 64 keys 2.4), so W shared keys take W / k workgroups that
+// long, which leaves the others the time (S - W / k)(F + k).  k is such that the own parts,
+// B = own keys + F for each tile, and a fifth more, as they do not fill it evenly, just fit:
+//   S k^2 + (S F - W - B) k - W F = 0.
+// Own keys are cut where their tile would take longer than that, into no more pieces than
+// there are workgroups left.  (32 sequences with own parts of up to 1024 positions behind
+// 32768 in I8: all keys cut alike 54.8 us, without the fifth 52.7, so {I8}.)
+__device__ __forceinline__ uint2 keys_of(const Chunk& c, const Work& w) {
+  const float S = (float)c.target, F = 200.f;
+  float shared = 0.f, own = w.own / S;
+  if (w.shared > 0.f) {
+    const float W = w.shared_cost, B = 1.2f * (w.own_cost + F * w.tiles), b = S * F - W - B;
+    const float k = (__builtin_sqrtf(b * b + 4.f * S * W * F) - b) / (2.f * S);
+    shared = k * (w.shared / W);
+    own = w.own_cost > 0.f ? fmaxf(k * (w.own / w.own_cost), w.own / (fmaxf(S - W / k, 0.f) + 8.f)) : 0.f;
+  }
+  auto whole = [&](float k) {
+    const uint32_t n = k < 1e9f ? ((uint32_t)k + 64) / 64 * 64 : 1u << 30;
+    return n > c.keys_per_split ? n : c.keys_per_split;
+  };
+  return {whole(shared), whole(own)};
 }
 
 // Tile and split `idx` of a KV head, for up to 128 parts and 64 groups: a lane looks at two
@@ -330,7 +373,7 @@ __device__ __forceinline__ uint32_t keys_of(const Chunk& c, float work) {
 // 64 at a time: 4 us of 22 for 64 sequences behind 64 positions).
 constexpr uint32_t kFewParts = 128, kFewGroups = 64;
 template <typename CUT>
-__device__ __forceinline__ bool find_few(const Chunk& c, uint32_t idx, RowTile& t, uint32_t& sp) {
+__device__ __forceinline__ bool find_few(const Chunk& c, uint32_t idx, RowTile& t, uint32_t& sp, uint2& keys) {
   const PagedBatch& b = c.b;
   const int lane = threadIdx.x & 63;
   const uint32_t groups = c.apart ? c.sh.n_groups : 0;
@@ -368,7 +411,7 @@ __device__ __forceinline__ bool find_few(const Chunk& c, uint32_t idx, RowTile& 
       }
   }
   Part p[2];
-  float work = 0.f;
+  Work work;
   // A group's rows, from the lanes of its sequences.
   const uint32_t last = (uint32_t)gz < b.n_seqs ? (uint32_t)gz : b.n_seqs;
   const bool good = (uint32_t)lane < groups && good_group(b, ga, gz, gl);
@@ -379,13 +422,20 @@ __device__ __forceinline__ bool find_few(const Chunk& c, uint32_t idx, RowTile& 
   for (int i = 0; i < 2; ++i) {
     p[i] = sequence_part(c, seq[i], a[i], z[i], l[i], pre[i]);
     if (i == 0 && good) p[i] = group_part(c, ga, last, gl, e0 < 64 ? x0 : x1, e1 < 64 ? y0 : y1);
-    work += p[i].keys > 0 ? (float)p[i].keys * (float)CUT::tiles(c, p[i]) : 0.f;
+    work.add<CUT>(c, p[i]);
   }
-  t.keys = (uint32_t)__builtin_amdgcn_readfirstlane((int)keys_of(c, wave_sum(work)));
+  work.shared = wave_sum(work.shared);
+  work.own = wave_sum(work.own);
+  work.shared_cost = wave_sum(work.shared_cost);
+  work.own_cost = wave_sum(work.own_cost);
+  work.tiles = wave_sum(work.tiles);
+  keys = keys_of(c, work);
+  keys.x = (uint32_t)__builtin_amdgcn_readfirstlane((int)keys.x);
+  keys.y = (uint32_t)__builtin_amdgcn_readfirstlane((int)keys.y);
   uint32_t done = 0;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    cut_part(c, t.keys, p[i]);
+    cut_part(c, keys, p[i]);
     const uint32_t tiles = CUT::tiles(c, p[i]), mine = tiles * p[i].splits;
     uint32_t up = mine;
 #pragma unroll
@@ -416,7 +466,7 @@ __device__ __forceinline__ bool find_few(const Chunk& c, uint32_t idx, RowTile& 
           if (p[j].last == 0 && p[j].n > 0 && p[j].seq >= q.seq && p[j].seq < q.last)
             all = all && (int64_t)p[j].pos0 + 1 >= (int64_t)q.shared;
       q.all = __ballot(!all) == 0;
-      CUT::tile(c, q, of(tiles), k - of(up - mine), t, sp);
+      CUT::tile(c, q, of(tiles), k - of(up - mine), keys, t, sp);
       return true;
     }
     done += total;
@@ -427,25 +477,23 @@ __device__ __forceinline__ bool find_few(const Chunk& c, uint32_t idx, RowTile& 
 // The same from what plan_kernel left.
 template <typename CUT>
 __device__ __forceinline__ bool find_planned(const Chunk& c, uint32_t idx, RowTile& t, uint32_t& sp) {
-  if (idx >= c.keys[1]) return false;
+  if (idx >= c.keys[2]) return false;
   const uint2 it = c.items[idx];
   const Part p = c.parts[__builtin_amdgcn_readfirstlane((int)it.x)];
-  t.keys = c.keys[0];
-  CUT::tile(c, p, CUT::tiles(c, p), (uint32_t)__builtin_amdgcn_readfirstlane((int)it.y), t, sp);
+  CUT::tile(c, p, CUT::tiles(c, p), (uint32_t)__builtin_amdgcn_readfirstlane((int)it.y), uint2{c.keys[0], c.keys[1]}, t, sp);
   return true;
 }
 
 // Large batches: one workgroup writes the parts, and the part and the tile and split of
-// each workgroup of the attention to come.  keys[0]: keys of a split, keys[1]: workgroups
-// of a KV head, at most `room`.
+// each workgroup of the attention to come; keys[2]: workgroups of a KV head, at most `room`.
 template <typename CUT>
 __global__ __launch_bounds__(1024) void plan_kernel(Chunk c, Part* parts, uint2* items, uint32_t room) {
-  __shared__ float sums[16];
+  __shared__ float sums[5][16];
   __shared__ uint32_t counts[16];
   const PagedBatch& b = c.b;
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t groups = c.apart ? c.sh.n_groups : 0, n = groups + b.n_seqs;
-  float work = 0.f;
+  Work work;
   for (uint32_t e = tid; e < n; e += 1024) {
     Part p{};
     if (e < groups) {
@@ -460,15 +508,22 @@ __global__ __launch_bounds__(1024) void plan_kernel(Chunk c, Part* parts, uint2*
       p = sequence_part(c, seq, b.starts[seq], b.starts[seq + 1], b.lens[seq], find_prefix(b, c.sh, seq));
     }
     parts[e] = p;
-    work += p.keys > 0 ? (float)p.keys * (float)CUT::tiles(c, p) : 0.f;
+    work.add<CUT>(c, p);
   }
-  work = wave_sum(work);
-  if (lane == 0) sums[wave] = work;
-  __syncthreads();  // and the parts
-  work = 0.f;
+  float* const of[5] = {&work.shared, &work.own, &work.shared_cost, &work.own_cost, &work.tiles};
 #pragma unroll
-  for (int i = 0; i < 16; ++i) work += sums[i];
-  const uint32_t keys = keys_of(c, work);
+  for (int j = 0; j < 5; ++j) {
+    const float x = wave_sum(*of[j]);
+    if (lane == 0) sums[j][wave] = x;
+  }
+  __syncthreads();  // and the parts
+#pragma unroll
+  for (int j = 0; j < 5; ++j) {
+    *of[j] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) *of[j] += sums[j][i];
+  }
+  const uint2 keys = keys_of(c, work);
   // A sequence that does not see all of its group's positions says so.
   if (groups)
     for (uint32_t e = groups + tid; e < n; e += 1024) {
@@ -513,8 +568,9 @@ __global__ __launch_bounds__(1024) void plan_kernel(Chunk c, Part* parts, uint2*
       if (at + k < room) items[at + k] = uint2{e, k};
   }
   if (tid == 0) {
-    c.keys[0] = keys;
-    c.keys[1] = done < room ? done : room;
+    c.keys[0] = keys.x;
+    c.keys[1] = keys.y;
+    c.keys[2] = done < room ? done : room;
   }
 }
 
@@ -1119,7 +1175,7 @@ template <Form FORM>
 __device__ __forceinline__ uint32_t row_splits(const Chunk& c, uint32_t seq) {
   const int l = c.b.lens[seq], len = l < (int)c.b.limit ? l : (int)c.b.limit;
   if constexpr (FORM == kShared) {
-    const Slots s = find_slots(c.apart, *c.keys, (int)find_prefix(c.b, c.sh, seq).len, len);
+    const Slots s = find_slots(c.apart, uint2{c.keys[0], c.keys[1]}, (int)find_prefix(c.b, c.sh, seq).len, len);
     return s.group + s.own;
   }
   return splits_of(c, len);
@@ -1671,8 +1727,12 @@ __global__ NF_TWO_PER_CU void shared_kernel(Chunk c) {
   if (c.items) {
     if (!find_planned<C>(c, idx, t, sp)) return;
   } else {
-    if (!find_few<C>(c, idx, t, sp)) return;
-    if (idx == 0 && kvh == 0 && threadIdx.x == 0) c.keys[0] = t.keys;
+    uint2 keys;
+    if (!find_few<C>(c, idx, t, sp, keys)) return;
+    if (idx == 0 && kvh == 0 && threadIdx.x == 0) {
+      c.keys[0] = keys.x;
+      c.keys[1] = keys.y;
+    }
   }
   const uint32_t ns = t.last == 0 && t.slot == 0 ? t.splits : t.splits + 1;
   if (t.rows <= 64) narrow_tile<PT, DD, NT, UNI, kShared>(c, t, sp, ns, kvh, lds.narrow);
@@ -2251,8 +2311,12 @@ __global__ NF_TWO_PER_CU void shared_f32_kernel(Chunk c) {
   if (c.items) {
     if (!find_planned<C>(c, idx, t, sp)) return;
   } else {
-    if (!find_few<C>(c, idx, t, sp)) return;
-    if (idx == 0 && kvh == 0 && threadIdx.x == 0) c.keys[0] = t.keys;
+    uint2 keys;
+    if (!find_few<C>(c, idx, t, sp, keys)) return;
+    if (idx == 0 && kvh == 0 && threadIdx.x == 0) {
+      c.keys[0] = keys.x;
+      c.keys[1] = keys.y;
+    }
   }
   const uint32_t ns = t.last == 0 && t.slot == 0 ? t.splits : t.splits + 1;
   if (t.rows <= 32) narrow_f32_tile<PT, DD, UNI, kShared>(c, t, sp, ns, kvh, lds.narrow);

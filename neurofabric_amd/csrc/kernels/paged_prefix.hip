@@ -30,13 +30,14 @@ hipError_t prefix_at(const PagedBatch& b, const PagedShared& sh, uint32_t n_head
   const uint32_t nt = F16 && mean > 16 ? 2 : 1;
   c.target = (kResident + b.n_kv - 1) / b.n_kv;
   // At most so many tiles and splits of a KV head: a part's last tile and split may be short.
-  auto tiles = [&](uint64_t n) {  // of n parts that have all rows between them
+  auto tiles = [&](uint64_t n) {  // of n parts that have all rows between them, `group` at least each
     if (n > b.rows) n = b.rows;
-    const uint64_t few = rows < kFew * n ? rows : kFew * n;
-    return rows / kWideRows + few / (16 * nt) + n;
+    const uint64_t few = rows < kFew * n ? rows : kFew * n, most = rows / kWideRows + few / (16 * nt) + n;
+    const uint64_t more = n + (rows - n * c.group) / (16 * nt);
+    return c.group <= 16 * nt && more < most ? more : most;
   };
-  auto items_of = [&](bool apart) { return tiles(b.n_seqs) + (apart ? tiles(sh.n_groups) : 0) + c.target + 1; };
-  // The workspace's end: two numbers, and the plan of a large batch.
+  auto items_of = [&](bool apart) { return tiles(b.n_seqs) + (apart ? tiles(sh.n_groups) : 0) + c.target + 16; };
+  // The workspace's end: a few numbers, and the plan of a large batch.
   auto plan_floats = [&](bool apart) {
     const uint64_t n = b.n_seqs + (apart ? sh.n_groups : 0);
     return n <= kFewParts && sh.n_groups <= kFewGroups ? 4 : 4 + n * (sizeof(Part) / 4) + items_of(apart) * 2;
