@@ -6,9 +6,7 @@
 // themselves start from 0.  Positions past the length, and sequences without rows,
 // are left as they are.  An 8-bit cache is read as f16 for f16 rows, as the
 // attention reads it.
-#include <type_traits>
-
-#include "paged.hpp"
+#include "paged_attention.hpp"
 
 namespace nfk {
 namespace paged {
@@ -22,6 +20,8 @@ struct Weigh {
   float* out;
   uint32_t n_heads, width;
   float theta, scale;
+  uint32_t keys;    // of a workgroup
+  uint64_t lo, hi;  // query rows of a KV head of the sequences that a launch takes
 };
 
 // The sequence's first row, rows and positions; false without rows or positions.
@@ -93,9 +93,457 @@ __global__ __launch_bounds__(256) void weights_any_kernel(Weigh w) {
   }
 }
 
+// ---- on MFMA ---------------------------------------------------------------------------
+//
+// S[row][key] = Q . K^T with the keys as the columns: a lane has one key (of a tile) and
+// some of the rows, so a position's weights are added up in its registers, and over the 4
+// (or 2) lanes of a column at the end.  Keys are the B operand as the cache holds them, a
+// lane's 16 bytes; exp(x - lse) is one v_exp_f32 of base 2.  No sum leaves the workgroup,
+// and its order is fixed.
+
+// What is taken off a row's score in base 2; a row that counts for nothing has infinity.
+__device__ __forceinline__ float base_of(float lse) { return lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f; }
+
+// The sequence of a workgroup, its keys and query rows; false for none.
+struct Task {
+  Span t;
+  RowTile tile;
+  uint32_t group, live;
+  int begin, end;
+};
+__device__ __forceinline__ bool find_task(const Weigh& w, uint32_t chunk, uint32_t seq, Task& k) {
+  if (!find_span(w.b, seq, k.t)) return false;
+  k.group = w.n_heads / w.b.n_kv;
+  const uint64_t rows = (uint64_t)k.t.rows * k.group;
+  const int64_t begin = (int64_t)chunk * w.keys;
+  if (rows <= w.lo || rows > w.hi || begin >= (int64_t)k.t.len) return false;
+  k.live = (uint32_t)rows;
+  k.begin = (int)begin;
+  k.end = begin + (int64_t)w.keys < (int64_t)k.t.len ? (int)(begin + w.keys) : k.t.len;
+  k.tile.seq = seq;
+  return true;
+}
+__device__ __forceinline__ uint64_t q_row(const Weigh& w, const Task& k, uint32_t r, uint32_t kvh) {
+  return (uint64_t)(k.t.start + r / k.group) * w.n_heads + kvh * k.group + r % k.group;
+}
+// A position's element: its old weight, faded, and the sum of the new ones.
+__device__ __forceinline__ float held_of(const Weigh& w, uint64_t row0, const Task& k, int p) {
+  return w.theta != 0.f && p < k.end && (int64_t)p < k.t.pos0 ? w.theta * w.held[row0 + p] : 0.f;
+}
+
+// Keys of one 16-key group as B operands, f16 (16x16x32) or f32 (16x16x4, whose order of
+// dims is free: step s of lane group g is dim DD/4 g + s).
+template <typename T, PoolType PT, int DD>
+struct Keys16;
+template <PoolType PT, int DD>
+struct Keys16<half_t, PT, DD> {
+  static constexpr bool I8 = PT == PoolType::I8;
+  static constexpr int KS = DD / 32;
+  u32x4 raw[I8 ? 1 : KS];
+  uint2 codes[I8 ? KS : 1];
+  half_t scale[I8 ? KS : 1];
+  template <typename R>
+  __device__ __forceinline__ void fetch(const R& rows, const uint8_t* pool, int j, int n, int g) {
+    const uint8_t* kr = rows.row(pool, j, n);
+    if constexpr (I8) {
+      const half_t* sc = rows.scale(pool, j, n);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        codes[s] = *reinterpret_cast<const uint2*>(kr + 32 * s + 8 * g);
+        scale[s] = sc[s];
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) raw[s] = *reinterpret_cast<const u32x4*>(kr + 64 * s + 16 * g);
+    }
+  }
+  __device__ __forceinline__ half8 get(int s) const {
+    if constexpr (I8) return dequant8(codes[s], scale[s]);
+    else return __builtin_bit_cast(half8, raw[s]);
+  }
+};
+template <PoolType PT, int DD>
+struct Keys16<float, PT, DD> {
+  static constexpr bool I8 = PT == PoolType::I8;
+  static constexpr int DG = DD / 4;
+  float4v raw[I8 ? 1 : DG / 4];
+  uint2 codes[I8 ? DG / 8 : 1];
+  half_t scale[I8 ? DG / 8 : 1];
+  template <typename R>
+  __device__ __forceinline__ void fetch(const R& rows, const uint8_t* pool, int j, int n, int g) {
+    const uint8_t* kr = rows.row(pool, j, n);
+    if constexpr (I8) {
+      const half_t* sc = rows.scale(pool, j, n);
+#pragma unroll
+      for (int p = 0; p < DG / 8; ++p) {
+        codes[p] = *reinterpret_cast<const uint2*>(kr + DG * g + 8 * p);
+        scale[p] = sc[(DG * g + 8 * p) / 32];
+      }
+    } else {
+#pragma unroll
+      for (int p = 0; p < DG / 4; ++p) raw[p] = *reinterpret_cast<const float4v*>(kr + 4 * (DG * g + 4 * p));
+    }
+  }
+  __device__ __forceinline__ void all(float* x) const {
+    if constexpr (I8) {
+#pragma unroll
+      for (int p = 0; p < DG / 8; ++p) codes8_f32(codes[p], (float)scale[p], x + 8 * p);
+    } else {
+#pragma unroll
+      for (int p = 0; p < DG; ++p) x[p] = raw[p / 4][p % 4];
+    }
+  }
+};
+// 16 query rows as the A operand.
+template <typename T, int DD>
+struct Query16;
+template <int DD>
+struct Query16<half_t, DD> {
+  half8 x[DD / 32];
+  __device__ __forceinline__ void fetch(const void* q, uint64_t row, int g) {
+#pragma unroll
+    for (int s = 0; s < DD / 32; ++s) x[s] = *reinterpret_cast<const half8*>(static_cast<const half_t*>(q) + row * DD + 32 * s + 8 * g);
+  }
+  template <PoolType PT>
+  __device__ __forceinline__ float4v dot(const Keys16<half_t, PT, DD>& k) const {
+    float4v c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < DD / 32; ++s) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[s], k.get(s), c, 0, 0, 0);
+    return c;
+  }
+};
+template <int DD>
+struct Query16<float, DD> {
+  float4v x[DD / 16];
+  __device__ __forceinline__ void fetch(const void* q, uint64_t row, int g) {
+#pragma unroll
+    for (int s = 0; s < DD / 16; ++s)
+      x[s] = *reinterpret_cast<const float4v*>(static_cast<const float*>(q) + row * DD + DD / 4 * g + 4 * s);
+  }
+  template <PoolType PT>
+  __device__ __forceinline__ float4v dot(const Keys16<float, PT, DD>& k) const {
+    float b[DD / 4];
+    k.all(b);
+    float4v c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < DD / 4; ++s) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[s / 4][s % 4], b[s], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// Single tokens and short chunks, up to 16 NT query rows, which stay in registers while
+// the waves take 32-key tiles in turn, the next one's loads in flight.
+template <typename T, PoolType PT, int DD, int NT, bool UNI>
+__global__ __launch_bounds__(256) void weights_few_kernel(Weigh w) {
+  Task k;
+  const uint32_t kvh = blockIdx.y;
+  if (!find_task(w, blockIdx.x, blockIdx.z, k)) return;
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const float scale_log2 = w.scale * 1.4426950408889634f;
+  const uint64_t row0 = ((uint64_t)k.tile.seq * w.b.n_kv + kvh) * w.width;
+  Rows<PT, DD, 2, UNI, false> rows(w.b, k.tile, kvh, k.end, Border{});
+  int t0 = k.begin + 32 * wave;
+  if (t0 >= k.end) return;
+  rows.look(t0);
+  Query16<T, DD> qa[NT];
+  float base[NT][4];
+  int pos[NT][4];
+#pragma unroll
+  for (int u = 0; u < NT; ++u) {
+    qa[u].fetch(w.q, q_row(w, k, min(16u * u + n, k.live - 1), kvh), g);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t r = 16 * u + 4 * g + i, at = min(r, k.live - 1);
+      pos[u][i] = (int)k.t.pos0 + (int)(at / k.group);
+      base[u][i] = r < k.live ? base_of(w.lse[q_row(w, k, at, kvh)]) : INFINITY;
+    }
+  }
+  Keys16<T, PT, DD> keys[2];
+  auto fetch = [&]() {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) keys[j].fetch(rows, w.k, j, n, g);
+  };
+  rows.take(t0);
+  fetch();
+  if (t0 + 128 < k.end) rows.look(t0 + 128);
+  for (;;) {
+    const uint32_t seen = (uint32_t)rows.have();
+    const int p = t0 + 16 * (g & 1) + n;
+    const float held = held_of(w, row0, k, p);
+    float4v sc[NT][2];
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) sc[u][j] = qa[u].dot(keys[j]);
+    const int next = t0 + 128;
+    if (next < k.end) {  // uniform
+      rows.take(next);
+      fetch();
+      if (next + 128 < k.end) rows.look(next + 128);
+    }
+    float x[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      x[j] = 0.f;
+#pragma unroll
+      for (int u = 0; u < NT; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][j][i], scale_log2, -base[u][i]));
+          x[j] += t0 + 16 * j + n <= pos[u][i] ? e : 0.f;
+        }
+      x[j] = sum4((seen >> (16 * j + n)) & 1 ? x[j] : 0.f);
+    }
+    if (g < 2 && p < k.end) w.out[row0 + p] = held + (g ? x[1] : x[0]);
+    if (next >= k.end) break;
+    t0 = next;
+  }
+}
+
+// Many query rows, f16: 64 keys a wave stay in registers as B operands, 32-row tiles of the
+// queries go through LDS for all four waves, two buffers, on v_mfma_f32_32x32x16_f16.
+// Per tile and wave 16 MFMAs beside 32 exponentials a lane.
+template <PoolType PT, int DD, bool UNI>
+__global__ __launch_bounds__(256, 2) void weights_many_kernel(Weigh w) {
+  constexpr int KS = DD / 16, QP = DD + 8, CPR = DD / 8, NU = (32 * CPR + 255) / 256;
+  __shared__ __attribute__((aligned(16))) half_t qs[2][32 * QP];
+  __shared__ __attribute__((aligned(16))) float base[2][32];
+  __shared__ __attribute__((aligned(16))) int place[2][32];
+  Task k;
+  const uint32_t kvh = blockIdx.y;
+  if (!find_task(w, blockIdx.x, blockIdx.z, k)) return;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, hf = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const float scale_log2 = w.scale * 1.4426950408889634f;
+  const uint64_t row0 = ((uint64_t)k.tile.seq * w.b.n_kv + kvh) * w.width;
+  const int t0 = k.begin + 64 * wave;  // (a workgroup's keys: 256)
+  // the wave's keys
+  Rows<PT, DD, 4, UNI, false> rows(w.b, k.tile, kvh, k.end, Border{});
+  half8 kb[2][KS];
+  uint64_t seen = 0;
+  if (t0 < k.end) {  // uniform
+    rows.look(t0);
+    rows.take(t0);
+    seen = rows.have();
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      // lanes exchange for the rows' places, so both groups of 16 are asked for by all
+      const uint8_t* r0 = rows.row(w.k, 2 * j, n & 15);
+      const uint8_t* r1 = rows.row(w.k, 2 * j + 1, n & 15);
+      const uint8_t* kr = n < 16 ? r0 : r1;
+      if constexpr (PT == PoolType::I8) {
+        const half_t* s0 = rows.scale(w.k, 2 * j, n & 15);
+        const half_t* s1 = rows.scale(w.k, 2 * j + 1, n & 15);
+        const half_t* sc = n < 16 ? s0 : s1;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) kb[j][s] = dequant8(*reinterpret_cast<const uint2*>(kr + 16 * s + 8 * hf), sc[s / 2]);
+      } else {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) kb[j][s] = *reinterpret_cast<const half8*>(kr + 32 * s + 16 * hf);
+      }
+    }
+  }
+  const float held0 = held_of(w, row0, k, t0 + lane);
+
+  // The first tile with a row that sees a key of the workgroup.
+  const int64_t skip = (int64_t)k.begin - k.t.pos0;
+  uint32_t r0 = skip <= 0 ? 0 : (uint32_t)skip * k.group / 32 * 32;
+  u32x4 raw[NU];
+  float b0 = 0.f;
+  int p0 = 0;
+  auto fetch = [&](uint32_t r) {
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int ch = tid + 256 * u < 32 * CPR ? tid + 256 * u : 32 * CPR - 1;
+      const uint32_t at = min(r + ch / CPR, k.live - 1);
+      raw[u] = *reinterpret_cast<const u32x4*>(static_cast<const half_t*>(w.q) + q_row(w, k, at, kvh) * DD + 8 * (ch % CPR));
+    }
+    if (tid < 32) {
+      const uint32_t at = min(r + tid, k.live - 1);
+      b0 = r + tid < k.live ? base_of(w.lse[q_row(w, k, at, kvh)]) : INFINITY;
+      p0 = (int)k.t.pos0 + (int)(at / k.group);
+    }
+  };
+  auto stage = [&](int buf) {
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int ch = tid + 256 * u;
+      if (32 * CPR % 256 == 0 || ch < 32 * CPR) *reinterpret_cast<u32x4*>(&qs[buf][ch / CPR * QP + 8 * (ch % CPR)]) = raw[u];
+    }
+    if (tid < 32) {
+      base[buf][tid] = b0;
+      place[buf][tid] = p0;
+    }
+  };
+  float x[2] = {0.f, 0.f};
+  if (r0 < k.live) {  // uniform
+    fetch(r0);
+    stage(0);
+    __syncthreads();
+    for (int buf = 0;; buf ^= 1) {
+      const bool more = r0 + 32 < k.live;
+      if (more) fetch(r0 + 32);
+      if (t0 < k.end) {  // uniform
+        f32x16 sc[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[j][i] = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const half8 a = *reinterpret_cast<const half8*>(&qs[buf][n * QP + 16 * s + 8 * hf]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) sc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, kb[j][s], sc[j], 0, 0, 0);
+        }
+        const bool open = (int64_t)k.t.pos0 + r0 / k.group >= (int64_t)t0 + 63;  // all rows see all keys
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float4v bs = *reinterpret_cast<const float4v*>(&base[buf][8 * q + 4 * hf]);
+          if (open) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) x[j] += __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][4 * q + i], scale_log2, -bs[i]));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int pos = place[buf][8 * q + 4 * hf + i];
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][4 * q + i], scale_log2, -bs[i]));
+                x[j] += t0 + 32 * j + n <= pos ? e : 0.f;
+              }
+            }
+          }
+        }
+      }
+      if (!more) break;
+      stage(buf ^ 1);  // its readers passed the last barrier
+      __syncthreads();
+      r0 += 32;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) x[j] = sum2((seen >> (32 * j + n)) & 1 ? x[j] : 0.f);
+  if (t0 + lane < k.end) w.out[row0 + t0 + lane] = held0 + (hf ? x[1] : x[0]);
+}
+
+// Many query rows, f32: 32 keys a wave stay in registers, 16-row tiles of the queries come
+// straight from the caches, the next one in flight; the f32 MFMA's time hides them.
+template <PoolType PT, int DD, bool UNI>
+__global__ __launch_bounds__(256, 2) void weights_many_f32_kernel(Weigh w) {
+  constexpr int DG = DD / 4;
+  Task k;
+  const uint32_t kvh = blockIdx.y;
+  if (!find_task(w, blockIdx.x, blockIdx.z, k)) return;
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const float scale_log2 = w.scale * 1.4426950408889634f;
+  const uint64_t row0 = ((uint64_t)k.tile.seq * w.b.n_kv + kvh) * w.width;
+  const int t0 = k.begin + 32 * wave;  // (a workgroup's keys: 128)
+  if (t0 >= k.end) return;
+  Rows<PT, DD, 2, UNI, false> rows(w.b, k.tile, kvh, k.end, Border{});
+  rows.look(t0);
+  rows.take(t0);
+  const uint32_t seen = (uint32_t)rows.have();
+  float kb[2][DG];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    Keys16<float, PT, DD> keys;
+    keys.fetch(rows, w.k, j, n, g);
+    keys.all(kb[j]);
+  }
+  const int p = t0 + 16 * (g & 1) + n;
+  const float held = held_of(w, row0, k, p);
+  const int64_t skip = (int64_t)t0 - k.t.pos0;
+  uint32_t r0 = skip <= 0 ? 0 : (uint32_t)skip * k.group / 16 * 16;
+  Query16<float, DD> qa;
+  float base[4];
+  auto fetch = [&](uint32_t r) {
+    qa.fetch(w.q, q_row(w, k, min(r + n, k.live - 1), kvh), g);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t at = r + 4 * g + i;
+      base[i] = at < k.live ? base_of(w.lse[q_row(w, k, at, kvh)]) : INFINITY;
+    }
+  };
+  float x[2] = {0.f, 0.f};
+  if (r0 < k.live) fetch(r0);
+  for (; r0 < k.live; r0 += 16) {
+    float4v sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int s = 0; s < DG; ++s)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) sc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(qa.x[s / 4][s % 4], kb[j][s], sc[j], 0, 0, 0);
+    const float4v bs = {base[0], base[1], base[2], base[3]};
+    if (r0 + 16 < k.live) fetch(r0 + 16);
+    const int64_t first = k.t.pos0 + r0 / k.group;
+    if (first >= (int64_t)t0 + 31) {  // uniform: all rows see all keys
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[j] += __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][i], scale_log2, -bs[i]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t pos = k.t.pos0 + (r0 + 4 * g + i) / k.group;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][i], scale_log2, -bs[i]));
+          x[j] += (int64_t)t0 + 16 * j + n <= pos ? e : 0.f;
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) x[j] = sum4((seen >> (16 * j + n)) & 1 ? x[j] : 0.f);
+  if (g < 2 && p < k.end) w.out[row0 + p] = held + (g ? x[1] : x[0]);
+}
+
+// ---- launch ------------------------------------------------------------------------------
+
+template <typename T, PoolType PT, int DD, bool UNI>
+hipError_t weights_mfma(Weigh& w, hipStream_t s) {
+  constexpr bool F16 = std::is_same<T, half_t>::value;
+  constexpr uint32_t kManyKeys = F16 ? 256 : 128;
+  const PagedBatch& b = w.b;
+  const uint64_t rows = (uint64_t)b.rows * (w.n_heads / b.n_kv), pairs = (uint64_t)b.n_kv * b.n_seqs;
+  // Rows of a sequence are known on the device only: each kernel leaves the sequences that
+  // are the other's.
+  const uint32_t few_rows = rows > 16ull * b.n_seqs ? 32 : 16;
+  const bool many = rows > few_rows, few = b.n_seqs > 1 || !many;
+  if (many) {
+    w.lo = few_rows;
+    w.hi = ~0ull;
+    w.keys = kManyKeys;
+    const dim3 grid((unsigned)((b.limit + (uint64_t)kManyKeys - 1) / kManyKeys), b.n_kv, b.n_seqs);
+    if constexpr (F16) weights_many_kernel<PT, DD, UNI><<<grid, 256, 0, s>>>(w);
+    else weights_many_f32_kernel<PT, DD, UNI><<<grid, 256, 0, s>>>(w);
+  }
+  if (few) {
+    // keys of a workgroup: some 4096 workgroups where no sequence is shorter than the bound
+    uint64_t keys = ((uint64_t)b.limit * pairs / 4096 + 127) / 128 * 128;
+    keys = keys < 128 ? 128 : keys > 2048 ? 2048 : keys;
+    w.lo = 0;
+    w.hi = few_rows;
+    w.keys = (uint32_t)keys;
+    const dim3 grid((unsigned)((b.limit + keys - 1) / keys), b.n_kv, b.n_seqs);
+    if (few_rows == 32) weights_few_kernel<T, PT, DD, 2, UNI><<<grid, 256, 0, s>>>(w);
+    else weights_few_kernel<T, PT, DD, 1, UNI><<<grid, 256, 0, s>>>(w);
+  }
+  return hipGetLastError();
+}
+
 template <typename T, PoolType PT>
 hipError_t weights(Weigh& w, hipStream_t s) {
   const PagedBatch& b = w.b;
+  if (pieces_fit<PT>(b, w.n_heads, Operands{w.q, w.k, nullptr, nullptr, nullptr})) {
+    const bool uni = uniform_blocks(b);
+    if (b.dim == 128) return (uni ? weights_mfma<T, PT, 128, true> : weights_mfma<T, PT, 128, false>)(w, s);
+    if (b.dim == 96) return (uni ? weights_mfma<T, PT, 96, true> : weights_mfma<T, PT, 96, false>)(w, s);
+    return (uni ? weights_mfma<T, PT, 64, true> : weights_mfma<T, PT, 64, false>)(w, s);
+  }
   const uint64_t tiles = ((uint64_t)b.limit + 63) / 64, most = (65536 + (uint64_t)b.n_kv * b.n_seqs - 1) / ((uint64_t)b.n_kv * b.n_seqs);
   const dim3 grid((unsigned)(tiles < most ? tiles : most), b.n_kv, b.n_seqs);
   weights_any_kernel<T, PT><<<grid, 256, 0, s>>>(w);
@@ -112,7 +560,7 @@ hipError_t launch_paged_weights(EType t, PoolType pool, const PagedBatch& b, uin
                                 float theta, hipStream_t s) {
   using namespace nfk;
   if (b.rows == 0 || b.n_seqs == 0 || b.limit == 0) return hipSuccess;
-  paged::Weigh w{b, q, static_cast<const uint8_t*>(k_pool), lse, held, weights, n_heads, width, theta, 1.0f / sqrtf((float)b.dim)};
+  paged::Weigh w{b, q, static_cast<const uint8_t*>(k_pool), lse, held, weights, n_heads, width, theta, 1.0f / sqrtf((float)b.dim), 0, 0, 0};
   if (t == EType::F16)
     return pool == PoolType::I8 ? paged::weights<half_t, PoolType::I8>(w, s) : paged::weights<half_t, PoolType::F16>(w, s);
   return pool == PoolType::I8 ? paged::weights<float, PoolType::I8>(w, s) : paged::weights<float, PoolType::F32>(w, s);
