@@ -123,6 +123,24 @@ __device__ __forceinline__ bool find_task(const Weigh& w, uint32_t chunk, uint32
   k.tile.seq = seq;
   return true;
 }
+// Sequence number `at` among those with more than `lo` query rows; n_seqs for none.
+__device__ __forceinline__ uint32_t find_many(const Weigh& w, uint32_t at) {
+  const PagedBatch& b = w.b;
+  const uint32_t group = w.n_heads / b.n_kv;
+  for (uint32_t s0 = 0; s0 < b.n_seqs; s0 += 64) {
+    const uint32_t s = s0 + (threadIdx.x & 63);
+    Span t;
+    const uint64_t mine = __ballot(s < b.n_seqs && find_span(b, s, t) && (uint64_t)t.rows * group > w.lo);
+    const uint32_t n = (uint32_t)__popcll(mine);
+    if (at < n) {
+      uint64_t left = mine;
+      for (; at > 0; --at) left &= left - 1;
+      return s0 + (uint32_t)__builtin_ctzll(left);
+    }
+    at -= n;
+  }
+  return b.n_seqs;
+}
 __device__ __forceinline__ uint64_t q_row(const Weigh& w, const Task& k, uint32_t r, uint32_t kvh) {
   return (uint64_t)(k.t.start + r / k.group) * w.n_heads + kvh * k.group + r % k.group;
 }
@@ -138,19 +156,28 @@ struct Keys16;
 template <PoolType PT, int DD>
 struct Keys16<half_t, PT, DD> {
   static constexpr bool I8 = PT == PoolType::I8;
-  static constexpr int KS = DD / 32;
-  u32x4 raw[I8 ? 1 : KS];
-  uint2 codes[I8 ? KS : 1];
+  static constexpr int KS = DD / 32, NP = KS / 2;
+  // I8: 16 codes are a lane's operands of two steps, the order of dims being free
+  u32x4 raw[I8 ? (NP > 0 ? NP : 1) : KS];
+  uint2 odd;  // I8, odd KS: the last 32 dims
   half_t scale[I8 ? KS : 1];
+  // The dim of a lane's first element in step s.
+  static __device__ __forceinline__ int dim(int s, int g) {
+    return !I8 || s >= 2 * NP ? 32 * s + 8 * g : 64 * (s / 2) + 16 * g + 8 * (s % 2);
+  }
   template <typename R>
   __device__ __forceinline__ void fetch(const R& rows, const uint8_t* pool, int j, int n, int g) {
     const uint8_t* kr = rows.row(pool, j, n);
     if constexpr (I8) {
       const half_t* sc = rows.scale(pool, j, n);
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        codes[s] = *reinterpret_cast<const uint2*>(kr + 32 * s + 8 * g);
-        scale[s] = sc[s];
+      for (int p = 0; p < NP; ++p) {
+        raw[p] = *reinterpret_cast<const u32x4*>(kr + 64 * p + 16 * g);
+        scale[2 * p] = sc[2 * p + (g >> 1)];
+      }
+      if constexpr (KS % 2) {
+        odd = *reinterpret_cast<const uint2*>(kr + 64 * NP + 8 * g);
+        scale[KS - 1] = sc[KS - 1];
       }
     } else {
 #pragma unroll
@@ -158,8 +185,9 @@ struct Keys16<half_t, PT, DD> {
     }
   }
   __device__ __forceinline__ half8 get(int s) const {
-    if constexpr (I8) return dequant8(codes[s], scale[s]);
-    else return __builtin_bit_cast(half8, raw[s]);
+    if constexpr (!I8) return __builtin_bit_cast(half8, raw[s]);
+    else if (s >= 2 * NP) return dequant8(odd, scale[KS - 1]);
+    else return dequant8(s % 2 ? uint2{raw[s / 2][2], raw[s / 2][3]} : uint2{raw[s / 2][0], raw[s / 2][1]}, scale[s / 2 * 2]);
   }
 };
 template <PoolType PT, int DD>
@@ -195,16 +223,16 @@ struct Keys16<float, PT, DD> {
   }
 };
 // 16 query rows as the A operand.
-template <typename T, int DD>
+template <typename T, PoolType PT, int DD>
 struct Query16;
-template <int DD>
-struct Query16<half_t, DD> {
+template <PoolType PT, int DD>
+struct Query16<half_t, PT, DD> {
   half8 x[DD / 32];
   __device__ __forceinline__ void fetch(const void* q, uint64_t row, int g) {
 #pragma unroll
-    for (int s = 0; s < DD / 32; ++s) x[s] = *reinterpret_cast<const half8*>(static_cast<const half_t*>(q) + row * DD + 32 * s + 8 * g);
+    for (int s = 0; s < DD / 32; ++s)
+      x[s] = *reinterpret_cast<const half8*>(static_cast<const half_t*>(q) + row * DD + Keys16<half_t, PT, DD>::dim(s, g));
   }
-  template <PoolType PT>
   __device__ __forceinline__ float4v dot(const Keys16<half_t, PT, DD>& k) const {
     float4v c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -212,15 +240,14 @@ struct Query16<half_t, DD> {
     return c;
   }
 };
-template <int DD>
-struct Query16<float, DD> {
+template <PoolType PT, int DD>
+struct Query16<float, PT, DD> {
   float4v x[DD / 16];
   __device__ __forceinline__ void fetch(const void* q, uint64_t row, int g) {
 #pragma unroll
     for (int s = 0; s < DD / 16; ++s)
       x[s] = *reinterpret_cast<const float4v*>(static_cast<const float*>(q) + row * DD + DD / 4 * g + 4 * s);
   }
-  template <PoolType PT>
   __device__ __forceinline__ float4v dot(const Keys16<float, PT, DD>& k) const {
     float b[DD / 4];
     k.all(b);
@@ -246,7 +273,7 @@ __global__ __launch_bounds__(256) void weights_few_kernel(Weigh w) {
   int t0 = k.begin + 32 * wave;
   if (t0 >= k.end) return;
   rows.look(t0);
-  Query16<T, DD> qa[NT];
+  Query16<T, PT, DD> qa[NT];
   float base[NT][4];
   int pos[NT][4];
 #pragma unroll
@@ -302,17 +329,18 @@ __global__ __launch_bounds__(256) void weights_few_kernel(Weigh w) {
 }
 
 // Many query rows, f16: 64 keys a wave stay in registers as B operands, 32-row tiles of the
-// queries go through LDS for all four waves, two buffers, on v_mfma_f32_32x32x16_f16.
-// Per tile and wave 16 MFMAs beside 32 exponentials a lane.
+// queries go through LDS for all four waves on v_mfma_f32_32x32x16_f16.  Per tile and wave
+// there are DD / 8 MFMAs and 32 exponentials a lane, about as long: those of the tile before
+// are issued between the MFMAs of the next one.
 template <PoolType PT, int DD, bool UNI>
 __global__ __launch_bounds__(256, 2) void weights_many_kernel(Weigh w) {
   constexpr int KS = DD / 16, QP = DD + 8, CPR = DD / 8, NU = (32 * CPR + 255) / 256;
-  __shared__ __attribute__((aligned(16))) half_t qs[2][32 * QP];
-  __shared__ __attribute__((aligned(16))) float base[2][32];
-  __shared__ __attribute__((aligned(16))) int place[2][32];
+  __shared__ __attribute__((aligned(16))) half_t qs[3][32 * QP];
+  __shared__ __attribute__((aligned(16))) float base[3][32];
+  __shared__ __attribute__((aligned(16))) int place[3][32];
   Task k;
-  const uint32_t kvh = blockIdx.y;
-  if (!find_task(w, blockIdx.x, blockIdx.z, k)) return;
+  const uint32_t kvh = blockIdx.y, seq = find_many(w, blockIdx.z);
+  if (seq >= w.b.n_seqs || !find_task(w, blockIdx.x, seq, k)) return;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, hf = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const float scale_log2 = w.scale * 1.4426950408889634f;
@@ -377,51 +405,103 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Weigh w) {
     }
   };
   float x[2] = {0.f, 0.f};
+  // The scores of the tile in buffer `buf` into `next`, and the weights of those of `last`,
+  // whose tile (first row `r`, bases in buffer `old`) every row of which sees all keys (OPEN).
+  auto step = [&](int buf, f32x16* next, int old, const f32x16* last, uint32_t r, auto open_c) {
+    constexpr bool OPEN = decltype(open_c)::value;
+    half8 a[3];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) a[s] = *reinterpret_cast<const half8*>(&qs[buf][n * QP + 16 * s + 8 * hf]);
+    float4v bs[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) bs[q] = *reinterpret_cast<const float4v*>(&base[old][8 * q + 4 * hf]);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) next[j][i] = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      if (s + 2 < KS) a[(s + 2) % 3] = *reinterpret_cast<const half8*>(&qs[buf][n * QP + 16 * (s + 2) + 8 * hf]);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        next[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[s % 3], kb[j][s], next[j], 0, 0, 0);
+        constexpr int EACH = 16 / KS;  // KS = 8, 6, 4: 2, 2 (and 4 more at the end), 4
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+          const int i = EACH * s + e;
+          float v = __builtin_amdgcn_exp2f(__builtin_fmaf(last[j][i], scale_log2, -bs[i / 4][i % 4]));
+          if constexpr (!OPEN) v = t0 + 32 * j + n <= place[old][8 * (i / 4) + 4 * hf + i % 4] ? v : 0.f;
+          x[j] += v;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 16 / KS * KS; i < 16; ++i) {
+        float v = __builtin_amdgcn_exp2f(__builtin_fmaf(last[j][i], scale_log2, -bs[i / 4][i % 4]));
+        if constexpr (!OPEN) v = t0 + 32 * j + n <= place[old][8 * (i / 4) + 4 * hf + i % 4] ? v : 0.f;
+        x[j] += v;
+      }
+    (void)r;
+  };
   if (r0 < k.live) {  // uniform
+    // A first tile whose rows count for nothing stands before the first.
     fetch(r0);
     stage(0);
+    if (tid < 32) {
+      base[2][tid] = INFINITY;
+      place[2][tid] = 0x7FFFFFFF;
+    }
+    if (r0 + 32 < k.live) fetch(r0 + 32);
     __syncthreads();
-    for (int buf = 0;; buf ^= 1) {
-      const bool more = r0 + 32 < k.live;
-      if (more) fetch(r0 + 32);
-      if (t0 < k.end) {  // uniform
-        f32x16 sc[2];
+    f32x16 sc[2][2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sc[j][i] = 0.f;
+      for (int i = 0; i < 16; ++i) sc[1][j][i] = 0.f;
+    int buf = 0, old = 2;
+    uint32_t r = r0;  // the tile in buf
+    bool open = true; // the one in old: all rows see all keys
+    // Two tiles a round, so that the scores' registers are known.
+    for (;;) {
+      bool done = false;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          const half8 a = *reinterpret_cast<const half8*>(&qs[buf][n * QP + 16 * s + 8 * hf]);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) sc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, kb[j][s], sc[j], 0, 0, 0);
+      for (int h = 0; h < 2; ++h) {
+        if (done) break;
+        const int nb = 3 - buf - old;
+        const bool more = r + 32 < k.live;
+        if (more) {
+          stage(nb);  // its readers passed the last barrier
+          if (r + 64 < k.live) fetch(r + 64);
         }
-        const bool open = (int64_t)k.t.pos0 + r0 / k.group >= (int64_t)t0 + 63;  // all rows see all keys
+        if (t0 < k.end) {  // uniform
+          if (open) step(buf, sc[h], old, sc[h ^ 1], r, std::true_type{});
+          else step(buf, sc[h], old, sc[h ^ 1], r, std::false_type{});
+        }
+        open = (int64_t)k.t.pos0 + r / k.group >= (int64_t)t0 + 63;
+        old = buf;
+        buf = nb;
+        r += 32;
+        __syncthreads();
+        if (!more) {
+          // the last tile's weights
+          if (t0 < k.end) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float4v bs = *reinterpret_cast<const float4v*>(&base[buf][8 * q + 4 * hf]);
-          if (open) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) x[j] += __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][4 * q + i], scale_log2, -bs[i]));
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int pos = place[buf][8 * q + 4 * hf + i];
+            for (int i = 0; i < 16; ++i) {
+              const int at = 8 * (i / 4) + 4 * hf + i % 4;
 #pragma unroll
               for (int j = 0; j < 2; ++j) {
-                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][4 * q + i], scale_log2, -bs[i]));
-                x[j] += t0 + 32 * j + n <= pos ? e : 0.f;
+                const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[h][j][i], scale_log2, -base[old][at]));
+                x[j] += t0 + 32 * j + n <= place[old][at] ? v : 0.f;
               }
             }
           }
+          done = true;
         }
       }
-      if (!more) break;
-      stage(buf ^ 1);  // its readers passed the last barrier
-      __syncthreads();
-      r0 += 32;
+      if (done) break;
     }
   }
 #pragma unroll
@@ -435,8 +515,8 @@ template <PoolType PT, int DD, bool UNI>
 __global__ __launch_bounds__(256, 2) void weights_many_f32_kernel(Weigh w) {
   constexpr int DG = DD / 4;
   Task k;
-  const uint32_t kvh = blockIdx.y;
-  if (!find_task(w, blockIdx.x, blockIdx.z, k)) return;
+  const uint32_t kvh = blockIdx.y, seq = find_many(w, blockIdx.z);
+  if (seq >= w.b.n_seqs || !find_task(w, blockIdx.x, seq, k)) return;
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const float scale_log2 = w.scale * 1.4426950408889634f;
@@ -458,7 +538,7 @@ __global__ __launch_bounds__(256, 2) void weights_many_f32_kernel(Weigh w) {
   const float held = held_of(w, row0, k, p);
   const int64_t skip = (int64_t)t0 - k.t.pos0;
   uint32_t r0 = skip <= 0 ? 0 : (uint32_t)skip * k.group / 16 * 16;
-  Query16<float, DD> qa;
+  Query16<float, PT, DD> qa;
   float base[4];
   auto fetch = [&](uint32_t r) {
     qa.fetch(w.q, q_row(w, k, min(r + n, k.live - 1), kvh), g);
@@ -517,7 +597,9 @@ hipError_t weights_mfma(Weigh& w, hipStream_t s) {
     w.lo = few_rows;
     w.hi = ~0ull;
     w.keys = kManyKeys;
-    const dim3 grid((unsigned)((b.limit + (uint64_t)kManyKeys - 1) / kManyKeys), b.n_kv, b.n_seqs);
+    const uint64_t most = rows / (few_rows + 1);  // such sequences
+    const dim3 grid((unsigned)((b.limit + (uint64_t)kManyKeys - 1) / kManyKeys), b.n_kv,
+                    (unsigned)(most < b.n_seqs ? most : b.n_seqs));
     if constexpr (F16) weights_many_kernel<PT, DD, UNI><<<grid, 256, 0, s>>>(w);
     else weights_many_f32_kernel<PT, DD, UNI><<<grid, 256, 0, s>>>(w);
   }
