@@ -380,17 +380,38 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Weigh w) {
   u32x4 raw[NU];
   float b0 = 0.f;
   int p0 = 0;
-  auto fetch = [&](uint32_t r) {
+  // Token and head of a row, 32 rows further with each tile.
+  struct Row {
+    uint32_t token, head;
+  };
+  const uint32_t tokens = 32 / k.group, heads = 32 % k.group;
+  auto row_at = [&](uint32_t r) { return Row{r / k.group, r % k.group}; };
+  auto go_on = [&](Row& r) {
+    r.token += tokens;
+    r.head += heads;
+    if (r.head >= k.group) {
+      r.head -= k.group;
+      ++r.token;
+    }
+  };
+  auto place_of = [&](const Row& r) {  // past the last token: the last row
+    const bool in = r.token < k.t.rows;
+    return (uint64_t)(k.t.start + (in ? r.token : k.t.rows - 1)) * w.n_heads + kvh * k.group + (in ? r.head : k.group - 1);
+  };
+  Row at[NU], mine = row_at(r0 + (tid & 31)), first = row_at(r0);
+#pragma unroll
+  for (int u = 0; u < NU; ++u) at[u] = row_at(r0 + (tid + 256 * u < 32 * CPR ? tid + 256 * u : 32 * CPR - 1) / CPR);
+  auto fetch = [&]() {  // the next tile
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       const int ch = tid + 256 * u < 32 * CPR ? tid + 256 * u : 32 * CPR - 1;
-      const uint32_t at = min(r + ch / CPR, k.live - 1);
-      raw[u] = *reinterpret_cast<const u32x4*>(static_cast<const half_t*>(w.q) + q_row(w, k, at, kvh) * DD + 8 * (ch % CPR));
+      raw[u] = *reinterpret_cast<const u32x4*>(static_cast<const half_t*>(w.q) + place_of(at[u]) * DD + 8 * (ch % CPR));
+      go_on(at[u]);
     }
     if (tid < 32) {
-      const uint32_t at = min(r + tid, k.live - 1);
-      b0 = r + tid < k.live ? base_of(w.lse[q_row(w, k, at, kvh)]) : INFINITY;
-      p0 = (int)k.t.pos0 + (int)(at / k.group);
+      b0 = mine.token < k.t.rows ? base_of(w.lse[place_of(mine)]) : INFINITY;
+      p0 = (int)k.t.pos0 + (int)mine.token;
+      go_on(mine);
     }
   };
   auto stage = [&](int buf) {
@@ -406,8 +427,8 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Weigh w) {
   };
   float x[2] = {0.f, 0.f};
   // The scores of the tile in buffer `buf` into `next`, and the weights of those of `last`,
-  // whose tile (first row `r`, bases in buffer `old`) every row of which sees all keys (OPEN).
-  auto step = [&](int buf, f32x16* next, int old, const f32x16* last, uint32_t r, auto open_c) {
+  // whose tile (bases in buffer `old`) has no row that does not see all keys (OPEN).
+  auto step = [&](int buf, f32x16* next, int old, const f32x16* last, auto open_c) {
     constexpr bool OPEN = decltype(open_c)::value;
     half8 a[3];
 #pragma unroll
@@ -444,17 +465,16 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Weigh w) {
         if constexpr (!OPEN) v = t0 + 32 * j + n <= place[old][8 * (i / 4) + 4 * hf + i % 4] ? v : 0.f;
         x[j] += v;
       }
-    (void)r;
   };
   if (r0 < k.live) {  // uniform
     // A first tile whose rows count for nothing stands before the first.
-    fetch(r0);
+    fetch();
     stage(0);
     if (tid < 32) {
       base[2][tid] = INFINITY;
       place[2][tid] = 0x7FFFFFFF;
     }
-    if (r0 + 32 < k.live) fetch(r0 + 32);
+    if (r0 + 32 < k.live) fetch();
     __syncthreads();
     f32x16 sc[2][2];
 #pragma unroll
@@ -474,13 +494,14 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Weigh w) {
         const bool more = r + 32 < k.live;
         if (more) {
           stage(nb);  // its readers passed the last barrier
-          if (r + 64 < k.live) fetch(r + 64);
+          if (r + 64 < k.live) fetch();
         }
         if (t0 < k.end) {  // uniform
-          if (open) step(buf, sc[h], old, sc[h ^ 1], r, std::true_type{});
-          else step(buf, sc[h], old, sc[h ^ 1], r, std::false_type{});
+          if (open) step(buf, sc[h], old, sc[h ^ 1], std::true_type{});
+          else step(buf, sc[h], old, sc[h ^ 1], std::false_type{});
         }
-        open = (int64_t)k.t.pos0 + r / k.group >= (int64_t)t0 + 63;
+        open = (int64_t)k.t.pos0 + first.token >= (int64_t)t0 + 63;
+        go_on(first);
         old = buf;
         buf = nb;
         r += 32;
@@ -604,8 +625,10 @@ hipError_t weights_mfma(Weigh& w, hipStream_t s) {
     else weights_many_f32_kernel<PT, DD, UNI><<<grid, 256, 0, s>>>(w);
   }
   if (few) {
-    // keys of a workgroup: some 4096 workgroups where no sequence is shorter than the bound
-    uint64_t keys = ((uint64_t)b.limit * pairs / 4096 + 127) / 128 * 128;
+    // Keys of a workgroup, some 8192 workgroups where no sequence is shorter than the bound:
+    // 64 sequences of up to 8192 positions, f16, by 256, 512 and 1024 keys 170, 160, 165 us;
+    // 16 of up to 32768, I8, 107, 103, 113.
+    uint64_t keys = ((uint64_t)b.limit * pairs / 8192 + 127) / 128 * 128;
     keys = keys < 128 ? 128 : keys > 2048 ? 2048 : keys;
     w.lo = 0;
     w.hi = few_rows;
