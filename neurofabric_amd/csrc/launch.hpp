@@ -194,7 +194,7 @@ struct PagedEvict {
   int32_t* kept = nullptr;
   uint32_t width = 0, top = 0, to_blocks = 0;
 };
-hipError_t launch_paged_evict(PoolType pool, const PagedBatch& b, const PagedEvict& e, hipStream_t s);
+hipError_t launch_paged_evict(PoolType pool, const PagedBatch& b, const PagedEvict& e, const Workspace& ws, hipStream_t s);
 
 // ---- sampling (kernels/sample.hip) ---------------------------------------------
 hipError_t launch_sample(EType t, const void* logits, const float* u, const float* params, const int32_t* top_k,

@@ -673,7 +673,7 @@ hipError_t run_plan(const Plan& pl, Buffer* const* in, Buffer* const* out, int g
       e.width = pl.lp.width;
       e.top = pl.lp.seq_len;
       e.to_blocks = (uint32_t)pl.lp.to_blocks;
-      return launch_paged_evict(pl.lp.pool, paged_batch(pl, batch), e, s);
+      return launch_paged_evict(pl.lp.pool, paged_batch(pl, batch), e, ws, s);
     }
     case Path::Sample:
       return launch_sample(pl.a, in[0]->dev, static_cast<const float*>(in[1]->dev),

@@ -447,6 +447,8 @@ EVICT = [  # lengths, (keep, recent) of each, most kept, KV heads, head_dim, blo
     ([50, 60], [(0, 0), (-3, 5)], 10, 2, 32, 5),
     ([90, 70], [(200, 300), (40, -1)], 60, 2, 64, 7),     # more than there are, more than `most`
     ([20000, 40000], [(5000, 500), (9000, 1)], 9000, 1, 32, 16),
+    ([16500, 3, 0, 8192, 4097], [(2000, 30), (5, 1), (4, 4), (8192, 0), (4096, 4096)], 8192, 2, 32, 16),
+    ([9000 - 60 * i for i in range(130)], [(90, 7)] * 130, 90, 2, 32, 16),
 ]
 
 
@@ -505,6 +507,10 @@ def test_evict_order_of_weights(provider):
         held = kinds[rng.integers(0, len(kinds), (2, 2, 1504))]
         held[1] = 0.125 if keep != 80 else np.nan
         run_evict(provider, rng, "f16", [n, n], [(keep, recent)] * 2, keep, 2, 64, 16, held=held, width=1504)
+    for keep, recent in ((4000, 300), (17000, 0), (30, 0)):  # a row of several workgroups
+        held = kinds[rng.integers(0, len(kinds), (2, 1, 18003))]
+        held[1] = 0.125 if keep != 30 else np.nan
+        run_evict(provider, rng, "f16", [17003, 17999], [(keep, recent)] * 2, keep, 1, 32, 16, held=held, width=18003)
 
 
 def test_evict_without_storage(provider):
