@@ -22,6 +22,10 @@ struct Weigh {
   float theta, scale;
   uint32_t keys;    // of a workgroup
   uint64_t lo, hi;  // query rows of a KV head of the sequences that a launch takes
+  // Many rows: cuts of a sequence's rows, and where each leaves its sums, [cut][sequence
+  // among those][KV head][limit], if there is more than one.
+  uint32_t cuts, many;
+  float* part;
 };
 
 // The sequence's first row, rows and positions; false without rows or positions.
@@ -98,8 +102,9 @@ __global__ __launch_bounds__(256) void weights_any_kernel(Weigh w) {
 // S[row][key] = Q . K^T with the keys as the columns: a lane has one key (of a tile) and
 // some of the rows, so a position's weights are added up in its registers, and over the 4
 // (or 2) lanes of a column at the end.  Keys are the B operand as the cache holds them, a
-// lane's 16 bytes; exp(x - lse) is one v_exp_f32 of base 2.  No sum leaves the workgroup,
-// and its order is fixed.
+// lane's 16 bytes; exp(x - lse) is one v_exp_f32 of base 2.  Where a sequence has many rows
+// and few keys, its rows are cut as well, and the cuts' sums joined by another kernel.  The
+// order of every sum is fixed.
 
 // What is taken off a row's score in base 2; a row that counts for nothing has infinity.
 __device__ __forceinline__ float base_of(float lse) { return lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f; }
@@ -328,6 +333,36 @@ __global__ __launch_bounds__(256) void weights_few_kernel(Weigh w) {
   }
 }
 
+// Tiles of `per` rows from the row `r0` on: those of cut `cut`.
+struct Rows2 {
+  uint32_t from, to;
+};
+__device__ __forceinline__ Rows2 cut_rows(const Weigh& w, const Task& k, uint32_t r0, uint32_t per, uint32_t cut) {
+  if (r0 >= k.live) return {0, 0};
+  const uint64_t n = (k.live - r0 + per - 1) / per;
+  const uint64_t end = r0 + n * (cut + 1) / w.cuts * per;
+  return {r0 + (uint32_t)(n * cut / w.cuts) * per, end < k.live ? (uint32_t)end : k.live};
+}
+// A position's sum: the element, or a cut's part of it.
+__device__ __forceinline__ void put_sum(const Weigh& w, uint32_t cut, uint32_t kvh, uint64_t row0, int p, float held, float x) {
+  if (w.cuts == 1) w.out[row0 + p] = held + x;
+  else w.part[(((uint64_t)cut * w.many + blockIdx.z) * w.b.n_kv + kvh) * w.b.limit + p] = x;
+}
+// The cuts' sums, in order, and what was held.
+__global__ __launch_bounds__(256) void weights_join_kernel(Weigh w) {
+  Task k;
+  const uint32_t kvh = blockIdx.y, seq = find_many(w, blockIdx.z);
+  if (seq >= w.b.n_seqs || !find_task(w, blockIdx.x, seq, k)) return;
+  const int p = k.begin + (int)threadIdx.x;
+  if (p >= k.end) return;
+  const uint64_t row0 = ((uint64_t)seq * w.b.n_kv + kvh) * w.width;
+  const float held = held_of(w, row0, k, p);
+  const float* part = w.part + ((uint64_t)blockIdx.z * w.b.n_kv + kvh) * w.b.limit + p;
+  float x = 0.f;
+  for (uint32_t c = 0; c < w.cuts; ++c) x += part[(uint64_t)c * w.many * w.b.n_kv * w.b.limit];
+  w.out[row0 + p] = held + x;
+}
+
 // Many query rows, f16: 64 keys a wave stay in registers as B operands, 32-row tiles of the
 // queries go through LDS for all four waves on v_mfma_f32_32x32x16_f16.  Per tile and wave
 // there are DD / 8 MFMAs and 32 exponentials a lane, about as long: those of the tile before
@@ -339,8 +374,8 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Weigh w) {
   __shared__ __attribute__((aligned(16))) float base[3][32];
   __shared__ __attribute__((aligned(16))) int place[3][32];
   Task k;
-  const uint32_t kvh = blockIdx.y, seq = find_many(w, blockIdx.z);
-  if (seq >= w.b.n_seqs || !find_task(w, blockIdx.x, seq, k)) return;
+  const uint32_t kvh = blockIdx.y, seq = find_many(w, blockIdx.z), cut = blockIdx.x % w.cuts;
+  if (seq >= w.b.n_seqs || !find_task(w, blockIdx.x / w.cuts, seq, k)) return;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, hf = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const float scale_log2 = w.scale * 1.4426950408889634f;
@@ -376,7 +411,8 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Weigh w) {
 
   // The first tile with a row that sees a key of the workgroup.
   const int64_t skip = (int64_t)k.begin - k.t.pos0;
-  uint32_t r0 = skip <= 0 ? 0 : (uint32_t)skip * k.group / 32 * 32;
+  const Rows2 mine_rows = cut_rows(w, k, skip <= 0 ? 0 : (uint32_t)skip * k.group / 32 * 32, 32, cut);
+  const uint32_t r0 = mine_rows.from, r_end = mine_rows.to;
   u32x4 raw[NU];
   float b0 = 0.f;
   int p0 = 0;
@@ -466,7 +502,7 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Weigh w) {
         x[j] += v;
       }
   };
-  if (r0 < k.live) {  // uniform
+  if (r0 < r_end) {  // uniform
     // A first tile whose rows count for nothing stands before the first.
     fetch();
     stage(0);
@@ -474,7 +510,7 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Weigh w) {
       base[2][tid] = INFINITY;
       place[2][tid] = 0x7FFFFFFF;
     }
-    if (r0 + 32 < k.live) fetch();
+    if (r0 + 32 < r_end) fetch();
     __syncthreads();
     f32x16 sc[2][2];
 #pragma unroll
@@ -491,10 +527,10 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Weigh w) {
       for (int h = 0; h < 2; ++h) {
         if (done) break;
         const int nb = 3 - buf - old;
-        const bool more = r + 32 < k.live;
+        const bool more = r + 32 < r_end;
         if (more) {
           stage(nb);  // its readers passed the last barrier
-          if (r + 64 < k.live) fetch();
+          if (r + 64 < r_end) fetch();
         }
         if (t0 < k.end) {  // uniform
           if (open) step(buf, sc[h], old, sc[h ^ 1], std::true_type{});
@@ -527,7 +563,7 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Weigh w) {
   }
 #pragma unroll
   for (int j = 0; j < 2; ++j) x[j] = sum2((seen >> (32 * j + n)) & 1 ? x[j] : 0.f);
-  if (t0 + lane < k.end) w.out[row0 + t0 + lane] = held0 + (hf ? x[1] : x[0]);
+  if (t0 + lane < k.end) put_sum(w, cut, kvh, row0, t0 + lane, held0, hf ? x[1] : x[0]);
 }
 
 // Many query rows, f32: 32 keys a wave stay in registers, 16-row tiles of the queries come
@@ -536,8 +572,8 @@ template <PoolType PT, int DD, bool UNI>
 __global__ __launch_bounds__(256, 2) void weights_many_f32_kernel(Weigh w) {
   constexpr int DG = DD / 4;
   Task k;
-  const uint32_t kvh = blockIdx.y, seq = find_many(w, blockIdx.z);
-  if (seq >= w.b.n_seqs || !find_task(w, blockIdx.x, seq, k)) return;
+  const uint32_t kvh = blockIdx.y, seq = find_many(w, blockIdx.z), cut = blockIdx.x % w.cuts;
+  if (seq >= w.b.n_seqs || !find_task(w, blockIdx.x / w.cuts, seq, k)) return;
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const float scale_log2 = w.scale * 1.4426950408889634f;
@@ -558,7 +594,9 @@ __global__ __launch_bounds__(256, 2) void weights_many_f32_kernel(Weigh w) {
   const int p = t0 + 16 * (g & 1) + n;
   const float held = held_of(w, row0, k, p);
   const int64_t skip = (int64_t)t0 - k.t.pos0;
-  uint32_t r0 = skip <= 0 ? 0 : (uint32_t)skip * k.group / 16 * 16;
+  const Rows2 mine_rows = cut_rows(w, k, skip <= 0 ? 0 : (uint32_t)skip * k.group / 16 * 16, 16, cut);
+  uint32_t r0 = mine_rows.from;
+  const uint32_t r_end = mine_rows.to;
   Query16<float, PT, DD> qa;
   float base[4];
   auto fetch = [&](uint32_t r) {
@@ -570,15 +608,15 @@ __global__ __launch_bounds__(256, 2) void weights_many_f32_kernel(Weigh w) {
     }
   };
   float x[2] = {0.f, 0.f};
-  if (r0 < k.live) fetch(r0);
-  for (; r0 < k.live; r0 += 16) {
+  if (r0 < r_end) fetch(r0);
+  for (; r0 < r_end; r0 += 16) {
     float4v sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
     for (int s = 0; s < DG; ++s)
 #pragma unroll
       for (int j = 0; j < 2; ++j) sc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(qa.x[s / 4][s % 4], kb[j][s], sc[j], 0, 0, 0);
     const float4v bs = {base[0], base[1], base[2], base[3]};
-    if (r0 + 16 < k.live) fetch(r0 + 16);
+    if (r0 + 16 < r_end) fetch(r0 + 16);
     const int64_t first = k.t.pos0 + r0 / k.group;
     if (first >= (int64_t)t0 + 31) {  // uniform: all rows see all keys
 #pragma unroll
@@ -599,13 +637,13 @@ __global__ __launch_bounds__(256, 2) void weights_many_f32_kernel(Weigh w) {
   }
 #pragma unroll
   for (int j = 0; j < 2; ++j) x[j] = sum4((seen >> (16 * j + n)) & 1 ? x[j] : 0.f);
-  if (g < 2 && p < k.end) w.out[row0 + p] = held + (g ? x[1] : x[0]);
+  if (g < 2 && p < k.end) put_sum(w, cut, kvh, row0, p, held, g ? x[1] : x[0]);
 }
 
 // ---- launch ------------------------------------------------------------------------------
 
 template <typename T, PoolType PT, int DD, bool UNI>
-hipError_t weights_mfma(Weigh& w, hipStream_t s) {
+hipError_t weights_mfma(Weigh& w, const nfhip::Workspace& ws, hipStream_t s) {
   constexpr bool F16 = std::is_same<T, half_t>::value;
   constexpr uint32_t kManyKeys = F16 ? 256 : 128;
   const PagedBatch& b = w.b;
@@ -619,10 +657,24 @@ hipError_t weights_mfma(Weigh& w, hipStream_t s) {
     w.hi = ~0ull;
     w.keys = kManyKeys;
     const uint64_t most = rows / (few_rows + 1);  // such sequences
-    const dim3 grid((unsigned)((b.limit + (uint64_t)kManyKeys - 1) / kManyKeys), b.n_kv,
-                    (unsigned)(most < b.n_seqs ? most : b.n_seqs));
+    w.many = (uint32_t)(most < b.n_seqs ? most : b.n_seqs);
+    const uint64_t chunks = (b.limit + (uint64_t)kManyKeys - 1) / kManyKeys, wgs = chunks * b.n_kv * w.many;
+    // Cuts of the rows for two workgroups a CU, of four tiles at least, as far as their sums
+    // fit the workspace (494 tokens of 4 heads over 4833 positions, one KV head, f32: 296 us
+    // without).
+    const uint64_t tile_rows = F16 ? 128 : 64, mean = rows / w.many, floats = (uint64_t)w.many * b.n_kv * b.limit;
+    uint64_t cuts = wgs < 512 ? 512 / wgs : 1;
+    if (cuts > mean / tile_rows) cuts = mean / tile_rows;
+    if (!ws.part || cuts * floats > ws.part_floats) cuts = ws.part ? ws.part_floats / floats : 1;
+    w.cuts = (uint32_t)(cuts < 1 ? 1 : cuts);
+    w.part = ws.part;
+    const dim3 grid((unsigned)(chunks * w.cuts), b.n_kv, w.many);
     if constexpr (F16) weights_many_kernel<PT, DD, UNI><<<grid, 256, 0, s>>>(w);
     else weights_many_f32_kernel<PT, DD, UNI><<<grid, 256, 0, s>>>(w);
+    if (w.cuts > 1) {
+      w.keys = 256;
+      weights_join_kernel<<<dim3((unsigned)((b.limit + 255ull) / 256), b.n_kv, w.many), 256, 0, s>>>(w);
+    }
   }
   if (few) {
     // Keys of a workgroup, some 8192 workgroups where no sequence is shorter than the bound:
@@ -641,13 +693,13 @@ hipError_t weights_mfma(Weigh& w, hipStream_t s) {
 }
 
 template <typename T, PoolType PT>
-hipError_t weights(Weigh& w, hipStream_t s) {
+hipError_t weights(Weigh& w, const nfhip::Workspace& ws, hipStream_t s) {
   const PagedBatch& b = w.b;
   if (pieces_fit<PT>(b, w.n_heads, Operands{w.q, w.k, nullptr, nullptr, nullptr})) {
     const bool uni = uniform_blocks(b);
-    if (b.dim == 128) return (uni ? weights_mfma<T, PT, 128, true> : weights_mfma<T, PT, 128, false>)(w, s);
-    if (b.dim == 96) return (uni ? weights_mfma<T, PT, 96, true> : weights_mfma<T, PT, 96, false>)(w, s);
-    return (uni ? weights_mfma<T, PT, 64, true> : weights_mfma<T, PT, 64, false>)(w, s);
+    if (b.dim == 128) return (uni ? weights_mfma<T, PT, 128, true> : weights_mfma<T, PT, 128, false>)(w, ws, s);
+    if (b.dim == 96) return (uni ? weights_mfma<T, PT, 96, true> : weights_mfma<T, PT, 96, false>)(w, ws, s);
+    return (uni ? weights_mfma<T, PT, 64, true> : weights_mfma<T, PT, 64, false>)(w, ws, s);
   }
   const uint64_t tiles = ((uint64_t)b.limit + 63) / 64, most = (65536 + (uint64_t)b.n_kv * b.n_seqs - 1) / ((uint64_t)b.n_kv * b.n_seqs);
   const dim3 grid((unsigned)(tiles < most ? tiles : most), b.n_kv, b.n_seqs);
@@ -662,13 +714,13 @@ namespace nfhip {
 
 hipError_t launch_paged_weights(EType t, PoolType pool, const PagedBatch& b, uint32_t n_heads, const void* q,
                                 const void* k_pool, const float* lse, const float* held, float* weights, uint32_t width,
-                                float theta, hipStream_t s) {
+                                float theta, const Workspace& ws, hipStream_t s) {
   using namespace nfk;
   if (b.rows == 0 || b.n_seqs == 0 || b.limit == 0) return hipSuccess;
-  paged::Weigh w{b, q, static_cast<const uint8_t*>(k_pool), lse, held, weights, n_heads, width, theta, 1.0f / sqrtf((float)b.dim), 0, 0, 0};
+  paged::Weigh w{b, q, static_cast<const uint8_t*>(k_pool), lse, held, weights, n_heads, width, theta, 1.0f / sqrtf((float)b.dim), 0, 0, 0, 1, 0, nullptr};
   if (t == EType::F16)
-    return pool == PoolType::I8 ? paged::weights<half_t, PoolType::I8>(w, s) : paged::weights<half_t, PoolType::F16>(w, s);
-  return pool == PoolType::I8 ? paged::weights<float, PoolType::I8>(w, s) : paged::weights<float, PoolType::F32>(w, s);
+    return pool == PoolType::I8 ? paged::weights<half_t, PoolType::I8>(w, ws, s) : paged::weights<half_t, PoolType::F16>(w, ws, s);
+  return pool == PoolType::I8 ? paged::weights<float, PoolType::I8>(w, ws, s) : paged::weights<float, PoolType::F32>(w, ws, s);
 }
 
 }  // namespace nfhip

@@ -176,7 +176,7 @@ hipError_t launch_paged_prefix(EType t, PoolType pool, const PagedBatch& b, cons
 // attention weights; theta 0 does not read `held`.
 hipError_t launch_paged_weights(EType t, PoolType pool, const PagedBatch& b, uint32_t n_heads, const void* q,
                                 const void* k_pool, const float* lse, const float* held, float* weights, uint32_t width,
-                                float theta, hipStream_t s);
+                                float theta, const Workspace& ws, hipStream_t s);
 // Eviction: of each sequence and KV head the budget[s][1] last positions and those of the
 // largest weights, budget[s][0] together and at most `top`, in order of position; `kept`
 // [n_seqs, n_kv, top] says which, and their rows go to the blocks of `to` [n_seqs, ceil(top

@@ -656,7 +656,7 @@ hipError_t run_plan(const Plan& pl, Buffer* const* in, Buffer* const* out, int g
     case Path::PagedWeights:
       return launch_paged_weights(pl.a, pl.lp.pool, paged_batch(pl, in + 2), pl.lp.n_heads, in[0]->dev, in[1]->dev,
                                   static_cast<const float*>(in[5]->dev), static_cast<const float*>(in[6]->dev),
-                                  static_cast<float*>(out[0]->dev), pl.lp.width, pl.lp.theta, s);
+                                  static_cast<float*>(out[0]->dev), pl.lp.width, pl.lp.theta, ws, s);
     case Path::PagedEvict: {
       Buffer* const batch[3] = {in[3], in[4], in[4]};  // row starts are not used
       PagedEvict e;

@@ -315,6 +315,8 @@ CHUNK = [  # sequences (positions, rows), heads, KV heads, head_dim, block size
     ([(64, 1), (65, 1), (63, 1), (128, 32), (32, 32)], 1, 1, 128, 16),
     ([(300, 140)], 16, 16, 64, 16),
     ([(130, 129), (40, 1), (9, 9)], 8, 2, 96, 64),
+    ([(600, 500), (90, 2), (300, 260)], 8, 1, 64, 16),   # rows cut as well
+    ([(1100, 900)], 4, 1, 96, 8),
 ]
 
 
