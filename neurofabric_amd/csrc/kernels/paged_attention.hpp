@@ -142,6 +142,7 @@ struct RowTile {
   uint32_t slot, splits;      // of the rows' partials this part's first one; splits of its keys
   uint32_t keys;              // keys of a split
   bool all;                   // every row of the group sees all shared positions
+  bool wide;                  // of a part of many rows; `rows` is then the tile's end
 };
 
 // What a kernel serves: flash_attention_paged_chunk, the same with the rows'
@@ -254,7 +255,9 @@ struct Part {
   uint32_t group, splits;   // splits of its keys, and of its group's
   uint32_t all;
 };
-// Rows of up to kFew query rows are cut into tiles of 16 NT, others of kWide.
+// Parts of up to FEW query rows are cut into tiles of NARROW, others into as few of up to WIDE
+// as there have to be, of like heights: a workgroup of two full tiles is not beside one of
+// two nearly empty ones (four groups of 160 rows, 128 and 32 of them a tile: 52 us).
 template <uint32_t FEW, uint32_t NARROW, uint32_t WIDE>
 struct Cut {
   static __device__ __forceinline__ uint32_t tiles(const Chunk& c, const Part& p) {
@@ -271,8 +274,11 @@ struct Cut {
                                               uint32_t& sp) {
     t.keys = p.last ? keys.x : keys.y;
     sp = k / nt;
-    t.rows = p.n * c.group;
-    t.first = (k - sp * nt) * (t.rows <= FEW ? NARROW : WIDE);
+    const uint32_t rows = p.n * c.group, wave = WIDE / 4;
+    t.wide = rows > FEW;
+    const uint32_t per = t.wide ? ((rows + nt - 1) / nt + wave - 1) / wave * wave : NARROW;
+    t.first = (k - sp * nt) * per;
+    t.rows = t.wide && t.first + per < rows ? t.first + per : rows;
     t.seq = p.seq;
     t.start = p.start;
     t.pos0 = p.pos0;
@@ -1735,7 +1741,7 @@ __global__ NF_TWO_PER_CU void shared_kernel(Chunk c) {
     }
   }
   const uint32_t ns = t.last == 0 && t.slot == 0 ? t.splits : t.splits + 1;
-  if (t.rows <= 64) narrow_tile<PT, DD, NT, UNI, kShared>(c, t, sp, ns, kvh, lds.narrow);
+  if (!t.wide) narrow_tile<PT, DD, NT, UNI, kShared>(c, t, sp, ns, kvh, lds.narrow);
   else wide_rows<PT, DD, UNI, kShared>(c, t, sp, ns, kvh, lds.wide);
 }
 
@@ -2319,7 +2325,7 @@ __global__ NF_TWO_PER_CU void shared_f32_kernel(Chunk c) {
     }
   }
   const uint32_t ns = t.last == 0 && t.slot == 0 ? t.splits : t.splits + 1;
-  if (t.rows <= 32) narrow_f32_tile<PT, DD, UNI, kShared>(c, t, sp, ns, kvh, lds.narrow);
+  if (!t.wide) narrow_f32_tile<PT, DD, UNI, kShared>(c, t, sp, ns, kvh, lds.narrow);
   else wide_f32_rows<PT, DD, UNI, kShared>(c, t, sp, ns, kvh, lds.wide);
 }
 
