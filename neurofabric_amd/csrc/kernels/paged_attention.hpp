@@ -270,6 +270,11 @@ struct Cut {
   static __device__ __forceinline__ float cost(const Chunk& c, const Part& p) {
     return (uint64_t)p.n * c.group <= FEW ? 0.4f : 1.f;
   }
+  // And what a tile takes besides: finding it, its first keys, its partials; two tiles of 16
+  // rows merge one after the other.
+  static __device__ __forceinline__ float fixed(const Chunk& c, const Part& p) {
+    return (uint64_t)p.n * c.group <= FEW && NARROW == 32 ? 500.f : 200.f;
+  }
   static __device__ __forceinline__ void tile(const Chunk& c, const Part& p, uint32_t nt, uint32_t k, uint2 keys, RowTile& t,
                                               uint32_t& sp) {
     t.keys = p.last ? keys.x : keys.y;
@@ -334,7 +339,7 @@ __device__ __forceinline__ void cut_part(const Chunk& c, uint2 keys, Part& p) {
 struct Work {
   float shared = 0.f, own = 0.f;                // tiles times keys
   float shared_cost = 0.f, own_cost = 0.f;      // and their time
-  float tiles = 0.f;                            // own tiles
+  float fixed = 0.f;                            // what own tiles take besides
   template <typename CUT>
   __device__ __forceinline__ void add(const Chunk& c, const Part& p) {
     if (p.keys <= 0 || p.n == 0) return;
@@ -345,7 +350,7 @@ struct Work {
     } else {
       own += w;
       own_cost += cost;
-      tiles += n;
+      fixed += n * CUT::fixed(c, p);
     }
   }
 };
@@ -353,7 +358,8 @@ struct Work {
 // `target` is for a KV head, split k keys take F + k in time, F = 200 (finding the tile, its
 // first keys, its partials: 9 us, 64 keys 2.4), so W shared keys take W / k workgroups that
 // long, which leaves the others the time (S - W / k)(F + k).  k is such that the own parts,
-// B = own keys + F for each tile, and a fifth more, as they do not fill it evenly, just fit:
+// B = own keys and what each tile takes besides, and a fifth more, as they do not fill it
+// evenly, just fit:
 //   S k^2 + (S F - W - B) k - W F = 0.
 // Own keys are cut where their tile would take longer than that, into no more pieces than
 // there are workgroups left.  (32 sequences with own parts of up to 1024 positions behind
@@ -362,7 +368,7 @@ __device__ __forceinline__ uint2 keys_of(const Chunk& c, const Work& w) {
   const float S = (float)c.target, F = 200.f;
   float shared = 0.f, own = w.own / S;
   if (w.shared > 0.f) {
-    const float W = w.shared_cost, B = 1.2f * (w.own_cost + F * w.tiles), b = S * F - W - B;
+    const float W = w.shared_cost, B = 1.2f * (w.own_cost + w.fixed), b = S * F - W - B;
     const float k = (__builtin_sqrtf(b * b + 4.f * S * W * F) - b) / (2.f * S);
     shared = k * (w.shared / W);
     own = w.own_cost > 0.f ? fmaxf(k * (w.own / w.own_cost), w.own / (fmaxf(S - W / k, 0.f) + 8.f)) : 0.f;
@@ -434,7 +440,7 @@ __device__ __forceinline__ bool find_few(const Chunk& c, uint32_t idx, RowTile& 
   work.own = wave_sum(work.own);
   work.shared_cost = wave_sum(work.shared_cost);
   work.own_cost = wave_sum(work.own_cost);
-  work.tiles = wave_sum(work.tiles);
+  work.fixed = wave_sum(work.fixed);
   keys = keys_of(c, work);
   keys.x = (uint32_t)__builtin_amdgcn_readfirstlane((int)keys.x);
   keys.y = (uint32_t)__builtin_amdgcn_readfirstlane((int)keys.y);
@@ -516,7 +522,7 @@ __global__ __launch_bounds__(1024) void plan_kernel(Chunk c, Part* parts, uint2*
     parts[e] = p;
     work.add<CUT>(c, p);
   }
-  float* const of[5] = {&work.shared, &work.own, &work.shared_cost, &work.own_cost, &work.tiles};
+  float* const of[5] = {&work.shared, &work.own, &work.shared_cost, &work.own_cost, &work.fixed};
 #pragma unroll
   for (int j = 0; j < 5; ++j) {
     const float x = wave_sum(*of[j]);
@@ -1298,6 +1304,62 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(Chunk c) {
   const float inv = L == 0.f ? 0.f : 1.0f / L;
   for (uint32_t d = tid; d < DD; d += 256)
     static_cast<T*>(c.out)[(uint64_t)o * DD + d] = (T)(((part[0][d] + part[1][d]) + (part[2][d] + part[3][d])) * inv);
+}
+
+// kShared, many rows: a wave per row for any number of splits, whose weights its lanes
+// form; the rows of eight splits are in flight (five tokens of 32 sequences behind four
+// prompts, 5120 rows of some 8 partials: a workgroup per row 13 us).
+constexpr uint32_t kManyRows = 1024;
+template <typename T, int DD>
+__global__ __launch_bounds__(256) void shared_combine_kernel(Chunk c) {
+  constexpr bool HALF = std::is_same<T, half_t>::value;
+  constexpr int R = (DD + 63) / 64, AHEAD = 8;
+  const uint32_t o = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  uint32_t seq;
+  int64_t pos;
+  if (o >= c.b.rows * c.n_heads || !find_row_wave(c.b, o / c.n_heads, seq, pos)) return;  // uniform
+  const uint32_t ns = row_splits<kShared>(c, seq);
+  if (row_direct<kShared>(c, seq, ns)) return;
+  const uint64_t first = (uint64_t)o * c.splits;
+  const float2s* ml = reinterpret_cast<const float2s*>(c.ml) + first;
+  float M = -INFINITY, L = 0.f, X = 0.f, A[R] = {};
+  for (uint32_t s = lane; s < ns; s += 64) M = fmaxf(M, ml[s][0]);
+#pragma unroll
+  for (int k = 32; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor(M, k));
+  for (uint32_t s0 = 0; s0 < ns; s0 += 64) {
+    const uint32_t n = ns - s0 < 64 ? ns - s0 : 64;
+    float f = 0.f;
+    if (lane < n) {
+      const float2s v = ml[s0 + lane];
+      if (v[1] != 0.f) {  // else no key: its row may be anything
+        f = v[0] == M ? 1.f : __builtin_amdgcn_exp2f(v[0] - M);
+        L += f * v[1];
+        X += f * (HALF ? c.lsum[first + s0 + lane] : v[1]);
+      }
+    }
+    for (uint32_t s = 0; s < n; s += AHEAD) {
+      float x[AHEAD][R];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          x[i][r] = c.acc[(first + s0 + (s + i < n ? s + i : n - 1)) * DD + (lane + 64 * r < DD ? lane + 64 * r : DD - 1)];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const float fi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), (int)((s + i) & 63)));
+        if (s + i < n && fi != 0.f)  // uniform
+#pragma unroll
+          for (int r = 0; r < R; ++r) A[r] += fi * x[i][r];
+      }
+    }
+  }
+  L = wave_sum(L);
+  X = wave_sum(X);
+  if (c.lse && lane == 0) c.lse[o] = lse_of(M, X, HALF ? kWeightLog2 : 0.f);
+  const float inv = L == 0.f ? 0.f : 1.0f / L;
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (lane + 64 * r < DD) static_cast<T*>(c.out)[(uint64_t)o * DD + lane + 64 * r] = (T)(A[r] * inv);
 }
 
 // Workgroup x of a wide kernel -> KV head and row tile, late tiles (most keys) first.

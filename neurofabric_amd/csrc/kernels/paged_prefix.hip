@@ -72,8 +72,10 @@ hipError_t prefix_at(const PagedBatch& b, const PagedShared& sh, uint32_t n_head
   else if (nt == 2) shared_kernel<PT, DD, 2, UNI><<<grid, 256, 0, s>>>(c);
   else shared_kernel<PT, DD, 1, UNI><<<grid, 256, 0, s>>>(c);
   if (c.splits > 1) {
-    if (c.splits <= kFewSplits) chunk_combine_few_kernel<T, DD, kShared><<<dim3((b.rows * n_heads + 3) / 4), 256, 0, s>>>(c);
-    else chunk_combine_kernel<T, DD, kShared><<<dim3(b.rows * n_heads), 256, 0, s>>>(c);
+    const uint32_t outs = b.rows * n_heads;
+    if (c.splits <= kFewSplits) chunk_combine_few_kernel<T, DD, kShared><<<dim3((outs + 3) / 4), 256, 0, s>>>(c);
+    else if (outs >= kManyRows) shared_combine_kernel<T, DD><<<dim3((outs + 3) / 4), 256, 0, s>>>(c);
+    else chunk_combine_kernel<T, DD, kShared><<<dim3(outs), 256, 0, s>>>(c);
   }
   return hipGetLastError();
 }
