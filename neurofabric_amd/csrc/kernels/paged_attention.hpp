@@ -141,6 +141,7 @@ struct RowTile {
   uint32_t last;              // a group's rows: one past its last sequence; else 0
   uint32_t slot, splits;      // of the rows' partials this part's first one; splits of its keys
   uint32_t keys;              // keys of a split
+  uint32_t base, stride;      // partials: query row (token, head) of the first, splits of each
   bool all;                   // every row of the group sees all shared positions
   bool wide;                  // of a part of many rows; `rows` is then the tile's end
 };
@@ -210,7 +211,9 @@ struct Chunk {
   PagedShared sh;
   bool apart;       // the groups' shared keys are parts of their own
   uint32_t target;  // splits of a KV head's keys that are aimed at
-  uint32_t* keys;   // the keys of a split of a group's part and of an own one, for the combination
+  bool last_round;  // few parts, and partials of all rows do not fit: only the last sequences' keys may be cut
+  uint64_t room;    // splits of query rows that do fit
+  uint32_t* keys;   // Cuts, for the combination
   const uint2* items;       // large batches: (part, tile and split) of each workgroup, in turn,
   const struct Part* parts; // and the parts; else null
 };
@@ -233,16 +236,38 @@ __device__ __forceinline__ Border find_border(bool apart, int shared, int end) {
   const int split = apart ? 0 : (shared + 63) & ~63, shift = split - (shared & ~15);
   return {split, shift, end + shift};
 }
-// Splits of the partials of a row: those of its group's part, of keys.x keys each, then
-// those of its own, of keys.y.
+// How keys are cut: a group's part into splits of `shared` keys, an own one of `own`; with
+// last_round those of the sequences from `seq` on into `pieces`, whose rows begin at
+// (token, head) `row`, the others not at all.
+struct Cuts {
+  uint32_t shared, own, seq, pieces, row;
+};
+// (A sequence behind `seq` whose rows begin before its, as descending STARTS make one, has
+// no partials.)
+__device__ __forceinline__ uint32_t own_keys(const Chunk& c, const Cuts& k, uint32_t seq, uint32_t start, int n) {
+  if (!c.last_round) return k.own;
+  return seq < k.seq || start * c.n_heads < k.row || n <= 0 ? 1u << 30 : ((uint32_t)n / k.pieces + 64) / 64 * 64;
+}
+__device__ __forceinline__ Cuts load_cuts(const Chunk& c) { return {c.keys[0], c.keys[1], c.keys[2], c.keys[3], c.keys[4]}; }
+__device__ __forceinline__ void store_cuts(const Chunk& c, const Cuts& k) {
+  c.keys[0] = k.shared;
+  c.keys[1] = k.own;
+  c.keys[2] = k.seq;
+  c.keys[3] = k.pieces;
+  c.keys[4] = k.row;
+}
+// The first query row that has partials, and the splits of each.
+__device__ __forceinline__ uint32_t first_row(const Chunk& c) { return c.last_round ? c.keys[4] : 0; }
+__device__ __forceinline__ uint32_t stride_of(const Chunk& c) { return c.last_round ? c.keys[3] : c.splits; }
+// Splits of the partials of a row: those of its group's part, then those of its own.
 struct Slots {
   uint32_t group, own;
 };
 __device__ __forceinline__ uint32_t cut(int n, uint32_t keys) { return n <= 0 ? 1u : ((uint32_t)n + keys - 1) / keys; }
-__device__ __forceinline__ Slots find_slots(bool apart, uint2 keys, int shared, int len) {
-  const uint32_t group = apart && shared > 0 ? cut(shared, keys.x) : 0;
-  const int n = find_border(apart, shared, len).end;
-  return {group, n <= 0 && group ? 0 : cut(n, keys.y)};
+__device__ __forceinline__ Slots find_slots(const Chunk& c, const Cuts& k, uint32_t seq, uint32_t start, int shared, int len) {
+  const uint32_t group = c.apart && shared > 0 ? cut(shared, k.shared) : 0;
+  const int n = find_border(c.apart, shared, len).end;
+  return {group, n <= 0 && group ? 0 : cut(n, own_keys(c, k, seq, start, n))};
 }
 
 // kShared: the batch as parts, first the groups' shared keys (where they are apart), then
@@ -275,9 +300,11 @@ struct Cut {
   static __device__ __forceinline__ float fixed(const Chunk& c, const Part& p) {
     return (uint64_t)p.n * c.group <= FEW && NARROW == 32 ? 500.f : 200.f;
   }
-  static __device__ __forceinline__ void tile(const Chunk& c, const Part& p, uint32_t nt, uint32_t k, uint2 keys, RowTile& t,
+  static __device__ __forceinline__ void tile(const Chunk& c, const Part& p, uint32_t nt, uint32_t k, const Cuts& keys, RowTile& t,
                                               uint32_t& sp) {
-    t.keys = p.last ? keys.x : keys.y;
+    t.keys = p.last ? keys.shared : own_keys(c, keys, p.seq, p.start, p.keys);
+    t.base = c.last_round ? keys.row : 0;
+    t.stride = c.last_round ? keys.pieces : c.splits;
     sp = k / nt;
     const uint32_t rows = p.n * c.group, wave = WIDE / 4;
     t.wide = rows > FEW;
@@ -326,11 +353,11 @@ __device__ __forceinline__ Part group_part(const Chunk& c, int32_t a, uint32_t l
 __device__ __forceinline__ bool good_group(const PagedBatch& b, int32_t a, int32_t z, int32_t len) {
   return a >= 0 && z > a && (uint32_t)a < b.n_seqs && len > 0;
 }
-__device__ __forceinline__ void cut_part(const Chunk& c, uint2 keys, Part& p) {
+__device__ __forceinline__ void cut_part(const Chunk& c, const Cuts& keys, Part& p) {
   p.group = 0;
-  p.splits = cut(p.shared, keys.x);
+  p.splits = cut(p.shared, keys.shared);
   if (p.last) return;
-  const Slots s = find_slots(c.apart, keys, p.shared, p.len);
+  const Slots s = find_slots(c, keys, p.seq, p.start, p.shared, p.len);
   p.group = s.group;
   p.splits = s.own;
 }
@@ -364,7 +391,7 @@ struct Work {
 // Own keys are cut where their tile would take longer than that, into no more pieces than
 // there are workgroups left.  (32 sequences with own parts of up to 1024 positions behind
 // 32768 in I8: all keys cut alike 54.8 us, without the fifth 52.7, so {I8}.)
-__device__ __forceinline__ uint2 keys_of(const Chunk& c, const Work& w) {
+__device__ __forceinline__ Cuts keys_of(const Chunk& c, const Work& w) {
   const float S = (float)c.target, F = 200.f;
   float shared = 0.f, own = w.own / S;
   if (w.shared > 0.f) {
@@ -377,7 +404,24 @@ __device__ __forceinline__ uint2 keys_of(const Chunk& c, const Work& w) {
     const uint32_t n = k < 1e9f ? ((uint32_t)k + 64) / 64 * 64 : 1u << 30;
     return n > c.keys_per_split ? n : c.keys_per_split;
   };
-  return {whole(shared), whole(own)};
+  return {whole(shared), whole(own), 0xFFFFFFFFu, 1, 0};
+}
+// With last_round: T tiles of a KV head are q rounds of the S workgroups at once and r more,
+// which would take a round of their own.  The last sequences with r tiles between them are
+// cut into as many pieces as still fit that round, which then takes 1 / pieces of one (16
+// questions of up to 200 tokens behind 8192, 88 tiles, S 64: uncut 700 us, so 608).
+constexpr uint32_t kMostPieces = 4;
+__device__ __forceinline__ uint32_t more_tiles(const Chunk& c, uint32_t tiles) {
+  return tiles > c.target ? tiles % c.target : 0;
+}
+__device__ __forceinline__ void cut_last(const Chunk& c, Cuts& k, uint32_t seq, uint32_t tiles, uint32_t token) {
+  uint32_t n = tiles ? c.target / tiles : 1;
+  if (n > kMostPieces) n = kMostPieces;
+  while (n > 1 && (uint64_t)(c.b.rows - token) * c.n_heads * n > c.room) --n;
+  if (n <= 1) return;
+  k.seq = seq;
+  k.pieces = n;
+  k.row = token * c.n_heads;
 }
 
 // Tile and split `idx` of a KV head, for up to 128 parts and 64 groups: a lane looks at two
@@ -385,7 +429,7 @@ __device__ __forceinline__ uint2 keys_of(const Chunk& c, const Work& w) {
 // 64 at a time: 4 us of 22 for 64 sequences behind 64 positions).
 constexpr uint32_t kFewParts = 128, kFewGroups = 64;
 template <typename CUT>
-__device__ __forceinline__ bool find_few(const Chunk& c, uint32_t idx, RowTile& t, uint32_t& sp, uint2& keys) {
+__device__ __forceinline__ bool find_few(const Chunk& c, uint32_t idx, RowTile& t, uint32_t& sp, Cuts& keys) {
   const PagedBatch& b = c.b;
   const int lane = threadIdx.x & 63;
   const uint32_t groups = c.apart ? c.sh.n_groups : 0;
@@ -442,8 +486,33 @@ __device__ __forceinline__ bool find_few(const Chunk& c, uint32_t idx, RowTile& 
   work.own_cost = wave_sum(work.own_cost);
   work.fixed = wave_sum(work.fixed);
   keys = keys_of(c, work);
-  keys.x = (uint32_t)__builtin_amdgcn_readfirstlane((int)keys.x);
-  keys.y = (uint32_t)__builtin_amdgcn_readfirstlane((int)keys.y);
+  keys.shared = (uint32_t)__builtin_amdgcn_readfirstlane((int)keys.shared);
+  keys.own = (uint32_t)__builtin_amdgcn_readfirstlane((int)keys.own);
+  if (c.last_round) {  // (all parts are sequences)
+    uint32_t up[2], total = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      up[i] = CUT::tiles(c, p[i]);
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t v = __shfl_up(up[i], o);
+        if (lane >= o) up[i] += v;
+      }
+      up[i] += total;
+      total = (uint32_t)__builtin_amdgcn_readlane((int)up[i], 63);
+    }
+    const uint32_t more = more_tiles(c, total);
+    auto from = [&](const Part& q, uint32_t before) {  // the last sequence that has `more` tiles from it on
+      const uint32_t rest = total - before + CUT::tiles(c, q);
+      const uint64_t has = __ballot(q.n > 0 && rest >= more);
+      if (has == 0) return false;
+      const int at = 63 - __builtin_clzll(has);
+      auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, at); };
+      cut_last(c, keys, of(q.seq), of(rest), of(q.start));
+      return true;
+    };
+    if (more && !from(p[1], up[1])) from(p[0], up[0]);
+  }
   uint32_t done = 0;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -471,6 +540,7 @@ __device__ __forceinline__ bool find_few(const Chunk& c, uint32_t idx, RowTile& 
       q.shared = (int)of((uint32_t)p[i].shared);
       q.group = of(p[i].group);
       q.splits = of(p[i].splits);
+      q.keys = (int)of((uint32_t)p[i].keys);
       bool all = true;
       if (q.last)
 #pragma unroll
@@ -489,15 +559,15 @@ __device__ __forceinline__ bool find_few(const Chunk& c, uint32_t idx, RowTile& 
 // The same from what plan_kernel left.
 template <typename CUT>
 __device__ __forceinline__ bool find_planned(const Chunk& c, uint32_t idx, RowTile& t, uint32_t& sp) {
-  if (idx >= c.keys[2]) return false;
+  if (idx >= c.keys[5]) return false;
   const uint2 it = c.items[idx];
   const Part p = c.parts[__builtin_amdgcn_readfirstlane((int)it.x)];
-  CUT::tile(c, p, CUT::tiles(c, p), (uint32_t)__builtin_amdgcn_readfirstlane((int)it.y), uint2{c.keys[0], c.keys[1]}, t, sp);
+  CUT::tile(c, p, CUT::tiles(c, p), (uint32_t)__builtin_amdgcn_readfirstlane((int)it.y), load_cuts(c), t, sp);
   return true;
 }
 
 // Large batches: one workgroup writes the parts, and the part and the tile and split of
-// each workgroup of the attention to come; keys[2]: workgroups of a KV head, at most `room`.
+// each workgroup of the attention to come; keys[5]: workgroups of a KV head, at most `room`.
 template <typename CUT>
 __global__ __launch_bounds__(1024) void plan_kernel(Chunk c, Part* parts, uint2* items, uint32_t room) {
   __shared__ float sums[5][16];
@@ -535,7 +605,7 @@ __global__ __launch_bounds__(1024) void plan_kernel(Chunk c, Part* parts, uint2*
 #pragma unroll
     for (int i = 0; i < 16; ++i) *of[j] += sums[j][i];
   }
-  const uint2 keys = keys_of(c, work);
+  const Cuts keys = keys_of(c, work);
   // A sequence that does not see all of its group's positions says so.
   if (groups)
     for (uint32_t e = groups + tid; e < n; e += 1024) {
@@ -580,9 +650,8 @@ __global__ __launch_bounds__(1024) void plan_kernel(Chunk c, Part* parts, uint2*
       if (at + k < room) items[at + k] = uint2{e, k};
   }
   if (tid == 0) {
-    c.keys[0] = keys.x;
-    c.keys[1] = keys.y;
-    c.keys[2] = done < room ? done : room;
+    store_cuts(c, keys);
+    c.keys[5] = done < room ? done : room;
   }
 }
 
@@ -613,6 +682,13 @@ __device__ __forceinline__ Keys find_keys(const Chunk& c, const RowTile& t, uint
     return {find_border(c.apart, t.shared, end), lo, hi};
   }
   return {{0, 0, end}, lo, hi};
+}
+
+// A query row's partial of split `sp` of a tile's part.
+template <bool SHARE>
+__device__ __forceinline__ uint64_t part_of(const Chunk& c, const RowTile& t, uint64_t orow, uint32_t sp) {
+  if constexpr (SHARE) return (orow - t.base) * t.stride + t.slot + sp;
+  else return orow * c.splits + sp;
 }
 
 // ln of a sum of weights 2^(x - m + log2), times the sum that m stands for.
@@ -1159,7 +1235,7 @@ __device__ __forceinline__ void narrow_tile(const Chunk& c, const RowTile& t, ui
             uint2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, bb)};
         if (LSE && c.lse && d == 0) c.lse[o] = lse_of(M, X, kWeightLog2);
       } else {
-        const uint64_t p = o * c.splits + (SHARE ? t.slot : 0) + sp;
+        const uint64_t p = part_of<SHARE>(c, t, o, sp);
         if (d == 0) *reinterpret_cast<float2s*>(c.ml + 2 * p) = float2s{M, L};
         if (LSE && d == 0) c.lsum[p] = X;
         *reinterpret_cast<float4v*>(c.acc + p * DD + d) = A;
@@ -1187,7 +1263,7 @@ template <Form FORM>
 __device__ __forceinline__ uint32_t row_splits(const Chunk& c, uint32_t seq) {
   const int l = c.b.lens[seq], len = l < (int)c.b.limit ? l : (int)c.b.limit;
   if constexpr (FORM == kShared) {
-    const Slots s = find_slots(c.apart, uint2{c.keys[0], c.keys[1]}, (int)find_prefix(c.b, c.sh, seq).len, len);
+    const Slots s = find_slots(c, load_cuts(c), seq, (uint32_t)c.b.starts[seq], (int)find_prefix(c.b, c.sh, seq).len, len);
     return s.group + s.own;
   }
   return splits_of(c, len);
@@ -1306,51 +1382,45 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(Chunk c) {
     static_cast<T*>(c.out)[(uint64_t)o * DD + d] = (T)(((part[0][d] + part[1][d]) + (part[2][d] + part[3][d])) * inv);
 }
 
-// kShared, many rows: a wave per row for any number of splits, whose weights its lanes
-// form; the rows of eight splits are in flight (five tokens of 32 sequences behind four
-// prompts, 5120 rows of some 8 partials: a workgroup per row 13 us).
-constexpr uint32_t kManyRows = 1024;
+// kShared, many rows: a wave per row, whose lanes form its splits' weights; the rows of
+// eight splits are in flight.  (Five tokens of 32 sequences behind four prompts, 5120 rows
+// of some 8 partials: a workgroup per row 13 us, so 6.6; 1024 rows of 44: 8.0 and 8.6.)
+// So many rows have at most 60 splits: more do not fit the workspace.
+constexpr uint32_t kManyRows = 2048;
 template <typename T, int DD>
 __global__ __launch_bounds__(256) void shared_combine_kernel(Chunk c) {
   constexpr bool HALF = std::is_same<T, half_t>::value;
   constexpr int R = (DD + 63) / 64, AHEAD = 8;
-  const uint32_t o = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const uint32_t lane = threadIdx.x & 63, row0 = first_row(c), o = row0 + blockIdx.x * 4 + (threadIdx.x >> 6);
   uint32_t seq;
   int64_t pos;
   if (o >= c.b.rows * c.n_heads || !find_row_wave(c.b, o / c.n_heads, seq, pos)) return;  // uniform
   const uint32_t ns = row_splits<kShared>(c, seq);
   if (row_direct<kShared>(c, seq, ns)) return;
-  const uint64_t first = (uint64_t)o * c.splits;
+  const uint64_t first = (uint64_t)(o - row0) * stride_of(c);
   const float2s* ml = reinterpret_cast<const float2s*>(c.ml) + first;
-  float M = -INFINITY, L = 0.f, X = 0.f, A[R] = {};
-  for (uint32_t s = lane; s < ns; s += 64) M = fmaxf(M, ml[s][0]);
+  const float2s v = lane < ns ? ml[lane] : float2s{-INFINITY, 0.f};
+  float M = v[0], L = 0.f, X = 0.f, A[R] = {}, f = 0.f;
 #pragma unroll
   for (int k = 32; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor(M, k));
-  for (uint32_t s0 = 0; s0 < ns; s0 += 64) {
-    const uint32_t n = ns - s0 < 64 ? ns - s0 : 64;
-    float f = 0.f;
-    if (lane < n) {
-      const float2s v = ml[s0 + lane];
-      if (v[1] != 0.f) {  // else no key: its row may be anything
-        f = v[0] == M ? 1.f : __builtin_amdgcn_exp2f(v[0] - M);
-        L += f * v[1];
-        X += f * (HALF ? c.lsum[first + s0 + lane] : v[1]);
-      }
-    }
-    for (uint32_t s = 0; s < n; s += AHEAD) {
-      float x[AHEAD][R];
+  if (v[1] != 0.f) {  // else no key: its row may be anything
+    f = v[0] == M ? 1.f : __builtin_amdgcn_exp2f(v[0] - M);
+    L = f * v[1];
+    X = f * (HALF ? c.lsum[first + lane] : v[1]);
+  }
+  for (uint32_t s = 0; s < ns; s += AHEAD) {
+    float x[AHEAD][R];
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i)
+    for (int i = 0; i < AHEAD; ++i)
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-          x[i][r] = c.acc[(first + s0 + (s + i < n ? s + i : n - 1)) * DD + (lane + 64 * r < DD ? lane + 64 * r : DD - 1)];
+      for (int r = 0; r < R; ++r)
+        x[i][r] = c.acc[(first + (s + i < ns ? s + i : ns - 1)) * DD + (lane + 64 * r < DD ? lane + 64 * r : DD - 1)];
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) {
-        const float fi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), (int)((s + i) & 63)));
-        if (s + i < n && fi != 0.f)  // uniform
+    for (int i = 0; i < AHEAD; ++i) {
+      const float fi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), (int)((s + i) & 63)));
+      if (s + i < ns && fi != 0.f)  // uniform
 #pragma unroll
-          for (int r = 0; r < R; ++r) A[r] += fi * x[i][r];
-      }
+        for (int r = 0; r < R; ++r) A[r] += fi * x[i][r];
     }
   }
   L = wave_sum(L);
@@ -1756,7 +1826,7 @@ __device__ __forceinline__ void wide_rows(const Chunk& c, const RowTile& t, uint
       }
     if (LSE && c.lse && hf == 0) c.lse[orow] = lse_of(m, lx, kWeightLog2);
   } else {
-    const uint64_t p = orow * c.splits + (SHARE ? t.slot : 0) + sp;
+    const uint64_t p = part_of<SHARE>(c, t, orow, sp);
     if (hf == 0) *reinterpret_cast<float2s*>(c.ml + 2 * p) = float2s{m, l};
     if (LSE && hf == 0) c.lsum[p] = lx;
 #pragma unroll
@@ -1795,12 +1865,9 @@ __global__ NF_TWO_PER_CU void shared_kernel(Chunk c) {
   if (c.items) {
     if (!find_planned<C>(c, idx, t, sp)) return;
   } else {
-    uint2 keys;
+    Cuts keys;
     if (!find_few<C>(c, idx, t, sp, keys)) return;
-    if (idx == 0 && kvh == 0 && threadIdx.x == 0) {
-      c.keys[0] = keys.x;
-      c.keys[1] = keys.y;
-    }
+    if (idx == 0 && kvh == 0 && threadIdx.x == 0) store_cuts(c, keys);
   }
   const uint32_t ns = t.last == 0 && t.slot == 0 ? t.splits : t.splits + 1;
   if (!t.wide) narrow_tile<PT, DD, NT, UNI, kShared>(c, t, sp, ns, kvh, lds.narrow);
@@ -1833,12 +1900,12 @@ __device__ __forceinline__ float4v codes4_f32(uint32_t w, float d) {
 
 // One row's output or partial, from the layout above.
 template <int DD, Form FORM>
-__device__ __forceinline__ void store_f32(const Chunk& c, uint64_t orow, uint32_t sp, uint32_t ns, int g, float m, float l,
+__device__ __forceinline__ void store_f32(const Chunk& c, uint64_t orow, uint64_t part, uint32_t ns, int g, float m, float l,
                                           const float4v* ot) {
-  float* dst = ns == 1 ? static_cast<float*>(c.out) + orow * DD : c.acc + (orow * c.splits + sp) * DD;
+  float* dst = ns == 1 ? static_cast<float*>(c.out) + orow * DD : c.acc + part * DD;
   const float f = ns > 1 ? 1.0f : l == 0.f ? 0.f : 1.0f / l;
   if (FORM != kChunk && ns == 1 && c.lse && g == 0) c.lse[orow] = lse_of(m, l, 0.f);
-  if (ns > 1 && g == 0) *reinterpret_cast<float2s*>(c.ml + 2 * (orow * c.splits + sp)) = float2s{m, l};
+  if (ns > 1 && g == 0) *reinterpret_cast<float2s*>(c.ml + 2 * part) = float2s{m, l};
 #pragma unroll
   for (int h = 0; h < (DD + 63) / 64; ++h)
 #pragma unroll
@@ -2103,7 +2170,7 @@ __device__ __forceinline__ void narrow_f32_tile(const Chunk& c, const RowTile& t
       *reinterpret_cast<float4v*>(static_cast<float*>(c.out) + o * DD + d) = A * inv;
       if (FORM != kChunk && c.lse && d == 0) c.lse[o] = lse_of(M, L, 0.f);
     } else {
-      const uint64_t p = o * c.splits + (SHARE ? t.slot : 0) + sp;
+      const uint64_t p = part_of<SHARE>(c, t, o, sp);
       if (d == 0) *reinterpret_cast<float2s*>(c.ml + 2 * p) = float2s{M, L};
       *reinterpret_cast<float4v*>(c.acc + p * DD + d) = A;
     }
@@ -2352,7 +2419,7 @@ __device__ __forceinline__ void wide_f32_rows(const Chunk& c, const RowTile& t, 
     if (wave_live && rows.at(t0) <= w_hi) tile(t0, seen, par, std::false_type{});  // uniform
     next();
   }
-  if (wave_live && r0 + n < t.rows) store_f32<DD, FORM>(c, orow, (SHARE ? t.slot : 0) + sp, ns, g, m, l, ot);
+  if (wave_live && r0 + n < t.rows) store_f32<DD, FORM>(c, orow, part_of<SHARE>(c, t, orow, sp), ns, g, m, l, ot);
 }
 
 template <PoolType PT, int DD, bool UNI, Form FORM>
@@ -2379,12 +2446,9 @@ __global__ NF_TWO_PER_CU void shared_f32_kernel(Chunk c) {
   if (c.items) {
     if (!find_planned<C>(c, idx, t, sp)) return;
   } else {
-    uint2 keys;
+    Cuts keys;
     if (!find_few<C>(c, idx, t, sp, keys)) return;
-    if (idx == 0 && kvh == 0 && threadIdx.x == 0) {
-      c.keys[0] = keys.x;
-      c.keys[1] = keys.y;
-    }
+    if (idx == 0 && kvh == 0 && threadIdx.x == 0) store_cuts(c, keys);
   }
   const uint32_t ns = t.last == 0 && t.slot == 0 ? t.splits : t.splits + 1;
   if (!t.wide) narrow_f32_tile<PT, DD, UNI, kShared>(c, t, sp, ns, kvh, lds.narrow);
@@ -2410,8 +2474,7 @@ constexpr uint32_t kFewRows = 32;
 // Partials take this many floats for each split of a query row: its maximum, its sums and
 // the output row, and what aligns them.
 constexpr uint32_t kPartFloats = 4;
-inline void place_parts(Chunk& c, const nfhip::Workspace& ws, uint32_t dim) {
-  const uint64_t n = (uint64_t)c.b.rows * c.n_heads * c.splits;
+inline void place_parts(Chunk& c, const nfhip::Workspace& ws, uint32_t dim, uint64_t n) {  // for n of them
   c.ml = ws.part;
   c.acc = ws.part + (n * 2 + 3) / 4 * 4;
   c.lsum = c.acc + n * dim;
@@ -2473,7 +2536,7 @@ hipError_t chunk_mfma_at(const PagedBatch& b, uint32_t n_heads, const Operands& 
   c.keys_per_split = (uint32_t)keys;
   c.splits = (uint32_t)((b.limit + keys - 1) / keys);
   if (c.splits == 0) c.splits = 1;
-  place_parts(c, ws, DD);
+  place_parts(c, ws, DD, (uint64_t)b.rows * n_heads * c.splits);
   if (wide) {
     c.tiles = (uint32_t)most_tiles;
     c.lo = narrow ? kFewRows : 0;

@@ -40,7 +40,7 @@ hipError_t prefix_at(const PagedBatch& b, const PagedShared& sh, uint32_t n_head
   // The workspace's end: a few numbers, and the plan of a large batch.
   auto plan_floats = [&](bool apart) {
     const uint64_t n = b.n_seqs + (apart ? sh.n_groups : 0);
-    return n <= kFewParts && sh.n_groups <= kFewGroups ? 4 : 4 + n * (sizeof(Part) / 4) + items_of(apart) * 2;
+    return n <= kFewParts && sh.n_groups <= kFewGroups ? 8 : 8 + n * (sizeof(Part) / 4) + items_of(apart) * 2;
   };
   auto splits_in = [&](uint64_t used) {  // of all rows' keys
     return ws.part_floats > used ? (ws.part_floats - used) / ((uint64_t)b.rows * n_heads * (DD + kPartFloats)) : 0;
@@ -56,10 +56,12 @@ hipError_t prefix_at(const PagedBatch& b, const PagedShared& sh, uint32_t n_head
   keys = (keys + 127) / 128 * 128;
   c.keys_per_split = (uint32_t)keys;
   c.splits = (uint32_t)((limit + keys - 1) / keys + parts);
-  place_parts(c, ws, DD);
+  c.last_round = most < 2 && used == 8;
+  c.room = (ws.part_floats - used) / (DD + kPartFloats);
+  place_parts(c, ws, DD, c.last_round ? c.room : (uint64_t)b.rows * n_heads * c.splits);
   c.keys = reinterpret_cast<uint32_t*>(ws.part + (ws.part_floats - used) / 4 * 4);
-  if (used > 4) {
-    Part* const plan = reinterpret_cast<Part*>(c.keys + 4);
+  if (used > 8) {
+    Part* const plan = reinterpret_cast<Part*>(c.keys + 8);
     uint2* const list = reinterpret_cast<uint2*>(plan + b.n_seqs + (c.apart ? sh.n_groups : 0));
     if (nt == 2) plan_kernel<Cut<kFew, 32, kWideRows>><<<1, 1024, 0, s>>>(c, plan, list, (uint32_t)items);
     else plan_kernel<Cut<kFew, 16, kWideRows>><<<1, 1024, 0, s>>>(c, plan, list, (uint32_t)items);
@@ -71,9 +73,12 @@ hipError_t prefix_at(const PagedBatch& b, const PagedShared& sh, uint32_t n_head
   if constexpr (!F16) shared_f32_kernel<PT, DD, UNI><<<grid, 256, 0, s>>>(c);
   else if (nt == 2) shared_kernel<PT, DD, 2, UNI><<<grid, 256, 0, s>>>(c);
   else shared_kernel<PT, DD, 1, UNI><<<grid, 256, 0, s>>>(c);
-  if (c.splits > 1) {
-    const uint32_t outs = b.rows * n_heads;
-    if (c.splits <= kFewSplits) chunk_combine_few_kernel<T, DD, kShared><<<dim3((outs + 3) / 4), 256, 0, s>>>(c);
+  if (c.splits > 1 || c.last_round) {
+    // of the last sequences, where only they have partials: as many rows as those of two splits fit
+    const uint64_t all = (uint64_t)b.rows * n_heads;
+    const uint32_t outs = (uint32_t)(c.last_round && all > c.room / 2 ? c.room / 2 : all);
+    if (c.last_round) shared_combine_kernel<T, DD><<<dim3((outs + 3) / 4), 256, 0, s>>>(c);
+    else if (c.splits <= kFewSplits) chunk_combine_few_kernel<T, DD, kShared><<<dim3((outs + 3) / 4), 256, 0, s>>>(c);
     else if (outs >= kManyRows) shared_combine_kernel<T, DD><<<dim3((outs + 3) / 4), 256, 0, s>>>(c);
     else chunk_combine_kernel<T, DD, kShared><<<dim3(outs), 256, 0, s>>>(c);
   }

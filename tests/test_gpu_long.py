@@ -122,6 +122,19 @@ def test_prefix_past_the_rows(provider, act, pool, dim, bs):
 
 
 @pytest.mark.parametrize("act,pool", ACT_POOL)
+@pytest.mark.parametrize("dim,seqs,groups", [
+    (128, [(290 + 7 * i, 120) for i in range(7)] + [(60, 33), (333, 131)], [(0, 5, 200), (5, 9, 31)]),
+    (64, [(250 + i, 120) for i in range(16)] + [(70, 1), (0, 0), (310, 121)], [(0, 17, 100)]),
+    (96, [(400, 330), (390, 330), (300, 255), (420, 403)], [(0, 3, 48)]),
+])
+def test_prefix_more_rows_than_partials(provider, act, pool, dim, seqs, groups):
+    """So many query rows that the workspace does not hold two partials of each: the last sequences' keys alone are cut."""
+    rng = np.random.default_rng(38)
+    batch = ref.Batch(rng, seqs, 16, behind=3)
+    run_attention(provider, rng, batch, ref.Shared(batch, groups), act, pool, 32, 8, dim)
+
+
+@pytest.mark.parametrize("act,pool", ACT_POOL)
 def test_prefix_bad_groups(provider, act, pool):
     """Groups below zero, past the sequences or decreasing, and negative prefixes end in time and touch no other row."""
     rng = np.random.default_rng(32)
