@@ -682,6 +682,69 @@ def test_decode_evict_decode(provider, act, pool):
             assert np.array_equal(b.read(np.uint8, p.nbytes), p.view(np.uint8).ravel())
 
 
+@pytest.mark.parametrize("act,pool,rows", [("f16", "f16", 1), ("f16", "i8", 1), ("f32", "f32", 1), ("f16", "f16", 90)])
+def test_offsets_past_32_bits(provider, act, pool, rows):
+    """The blocks that are used lie past 2^32 bytes and elements of the pools, the last rows of the weights past as many."""
+    rng = np.random.default_rng(63)
+    heads, kv, dim, bs, top = 8, 8, 128, 16, 60
+    width = 3 << 26
+    batch = ref.Batch(rng, [(190, rows), (170, rows), (150, rows)], bs, spare=0)
+    shared = ref.Shared(batch, [(0, 3, 64)], named=True)
+    page = paged_ref.empty_pool(rng, pool, 1, 1, bs, dim).nbytes * kv
+    used, pages = batch.blocks, -(-top // bs)
+    batch.blocks += 3 * pages  # the evicted sequences' blocks
+    new = (used + rng.permutation(3 * pages).reshape(3, pages)).astype(np.uint32)
+    blocks = ((18 if pool == "f32" else 9) << 30) // page
+    first = blocks - batch.blocks
+    small = fill(rng, batch, shared, act, pool, kv, dim)
+    q = rows_of(rng, act, batch.rows, heads, dim)
+    limit = batch.width * bs
+    held = rng.random((3, kv, limit)).astype(np.float32)
+    budget = np.array([[60, 10], [50, 0], [33, 33]], np.int32)
+    with Bufs(provider) as m:
+        big = [provider.alloc(NF[pool], blocks * page) for _ in range(2)]
+        wb = provider.alloc(NF["f32"], 3 * kv * width * 4)
+        m.all += big + [wb]
+        for b, p in zip(big, small):
+            b.write(p, offset=first * page)
+        for i in range(3 * kv):
+            wb.write(held[i // kv, i % kv], offset=i * width * 4)
+        at = ref.Batch(rng, batch.seqs, bs)
+        far = lambda t: np.where(t == ref.NONE, t, t + np.uint32(first)).astype(np.uint32)  # noqa: E731
+        at.table = far(batch.table)
+        desc = m.batch(at)
+        out, lb = m.put(np.zeros_like(q)), m.put(np.zeros((batch.rows, heads), np.float32))
+        lens, kept = m.put(np.zeros(3, np.int32)), m.put(np.zeros((3, kv, top), np.int32))
+        pc = pc_of(batch, kv, dim, n_heads=heads, step_idx=1)
+        provider.dispatch("flash_attention_paged_prefix", [m.put(q)] + big + desc + [m.put(shared.first), m.put(shared.len)],
+                          [out, lb], pc=pc)
+        got = out.read(NP[act], q.size).reshape(q.shape)
+        provider.dispatch("flash_attention_paged_chunk", [m.put(q)] + big + desc, [out, lb], pc=pc_of(batch, kv, dim, n_heads=heads))
+        z = lb.read(np.float32, batch.rows * heads).reshape(batch.rows, heads)
+        provider.dispatch("paged_kv_weights", [m.put(q), big[0]] + desc + [lb, wb], [wb],
+                          pc=pc_of(batch, kv, dim, n_heads=heads, step_idx=width, theta=0.5))
+        row = lambda i: wb.read(np.float32, limit, offset=i * width * 4)  # noqa: E731
+        w = np.stack([row(i) for i in range(3 * kv)]).reshape(held.shape)
+        pc = push_constants(M=kv, N=batch.width, K=3, seq_len=top, head_dim=dim, window_size=bs, step_idx=width)
+        provider.dispatch("paged_kv_evict", big + [wb, desc[0], desc[2], m.put(budget), m.put(far(new))], big + [wb, lens, kept], pc=pc)
+        chosen = kept.read(np.int32, 3 * kv * top).reshape(3, kv, top)
+        after = [b.read(np.uint8, p.nbytes, offset=first * page).reshape(p.view(np.uint8).shape) for b, p in zip(big, small)]
+        left = np.stack([row(i) for i in range(3 * kv)]).reshape(held.shape)
+    want, err, wz, zerr = ref.attention(batch, shared, pool, dim, heads, kv, small, q, act)
+    check(got, want, err, (act, pool))
+    check(z, wz, zerr, (act, pool))
+    want, err = ref.weights(batch, pool, dim, heads, kv, small[0], q, act, z, held, 0.5, held)
+    check(w, want, err, (act, pool))
+    rows = ref.evict(batch, batch.lens, w, budget, top)
+    for s in range(3):
+        k = rows[s].shape[1]
+        assert np.array_equal(chosen[s, :, :k], rows[s])
+        assert np.array_equal(left[s, :, :k].view(np.uint32), np.take_along_axis(w[s], rows[s], 1).view(np.uint32))
+    ref.move(batch, pool, dim, [p.copy() for p in small], small, rows, new)
+    for a, p in zip(after, small):
+        assert np.array_equal(a, p.view(np.uint8))
+
+
 @pytest.mark.parametrize("act,pool", [("f16", "f16"), ("f16", "i8"), ("f32", "f32")])
 def test_captured_steps_replay(provider, act, pool):
     """Captured attention, weights and eviction follow lengths, groups and budgets that their buffers hold at each replay."""
