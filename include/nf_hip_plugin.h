@@ -106,8 +106,8 @@
  *     blocks of two sequences have to differ, and no block that the op reads may be among
  *     them (a block that several sequences share stays as it is); the other outputs may
  *     not overlap any operand.  Push constants: M, N, K, head_dim, window_size, max_seq_len,
- *     step_idx (the length of a row of weights, at least the positions a sequence may hold)
- *     and seq_len = most positions kept, at most 2^22.  Keys keep what position they were
+ *     step_idx (the length of a row of weights, at least the positions a sequence may hold,
+ *     which are 2^30 at most) and seq_len = most positions kept, at most 2^22.  Keys keep what position they were
  *     rotated for: a server counts positions for that by itself.
  *   sample_token        LOGITS, U, PARAMS, TOP_K -> TOKEN, PROB
  *     LOGITS [seq_len, N] F32 or F16; U f32[seq_len], random numbers of [0, 1);

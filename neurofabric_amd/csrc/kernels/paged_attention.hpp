@@ -246,7 +246,7 @@ struct Cuts {
 // no partials.)
 __device__ __forceinline__ uint32_t own_keys(const Chunk& c, const Cuts& k, uint32_t seq, uint32_t start, int n) {
   if (!c.last_round) return k.own;
-  return seq < k.seq || start * c.n_heads < k.row || n <= 0 ? 1u << 30 : ((uint32_t)n / k.pieces + 64) / 64 * 64;
+  return seq < k.seq || start * c.n_heads < k.row || n <= 0 ? c.keys_per_split : ((uint32_t)n / k.pieces + 64) / 64 * 64;
 }
 __device__ __forceinline__ Cuts load_cuts(const Chunk& c) { return {c.keys[0], c.keys[1], c.keys[2], c.keys[3], c.keys[4]}; }
 __device__ __forceinline__ void store_cuts(const Chunk& c, const Cuts& k) {

@@ -376,6 +376,7 @@ nf_status plan_paged_evict(const nf_tensor_desc* const* ins, uint32_t n_in, cons
   if (st != NF_OK) return st;
   LayerParams& lp = p->lp;
   lp.width = pc.step;
+  if (lp.max_seq > (1u << 30)) return fail(why, "more than 2^30 positions a sequence (max_seq_len bounds them)");
   const uint64_t S = lp.rows;
   if (outs[0]->dtype != ins[0]->dtype || outs[1]->dtype != ins[0]->dtype)
     return fail(why, "the pools that are read and written must have one dtype");

@@ -84,6 +84,9 @@ PREFIX = [  # sequences (positions, rows), groups (first, one past the last, sha
     ([(600, 40)] + [(530 + i, 1) for i in range(30)], [(0, 31, 512)], 8, 2, 128, 16),
     ([(130, 1)] * 40, [(0, 40, 128)], 4, 4, 64, 64),
     ([(150, 1)] * 12, [(0, 12, 144)], 64, 8, 128, 48),
+    ([(90, 1), (70, 2), (60, 1)], [(0, 2, 48)], 160, 1, 64, 16),   # many heads of one KV head
+    ([(300, 1), (290, 3)], [(0, 2, 256)], 66, 2, 96, 16),
+    ([(200 + i, 1) for i in range(6)], [(0, 4, 160), (4, 6, 96)], 40, 1, 128, 16),
     # more sequences, or groups, than a workgroup looks through by itself
     ([(140 + i % 9, 1 + i % 2) for i in range(150)], [(0, 70, 96), (70, 149, 130)], 4, 2, 64, 16),
     ([(60 + i % 7, 1) for i in range(160)], [(2 * i, 2 * i + 2, 16 + i % 33) for i in range(80)], 4, 1, 64, 16),
@@ -328,6 +331,8 @@ CHUNK = [  # sequences (positions, rows), heads, KV heads, head_dim, block size
     ([(64, 1), (65, 1), (63, 1), (128, 32), (32, 32)], 1, 1, 128, 16),
     ([(300, 140)], 16, 16, 64, 16),
     ([(130, 129), (40, 1), (9, 9)], 8, 2, 96, 64),
+    ([(90, 1), (70, 2), (200, 1)], 80, 2, 64, 16),       # many heads of one KV head
+    ([(90, 1), (300, 7)], 130, 1, 128, 16),
     ([(600, 500), (90, 2), (300, 260)], 8, 1, 64, 16),   # rows cut as well
     ([(1100, 900)], 4, 1, 96, 8),
 ]

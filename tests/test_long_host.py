@@ -143,3 +143,12 @@ def test_no_sizes_wrap(lib):
     big = dict(M=65535, K=65535, N=0xFFFFFFFF, window_size=65536, head_dim=256)
     refused(evict, lib, pc=args(**{**big, "seq_len": 1 << 22, "step_idx": 0xFFFFFFFF}))
     refused(weigh, lib, pc=args(**{**big, "seq_len": 1, "n_heads": 65535, "step_idx": 0xFFFFFFFF, "theta": 1.0}))
+
+
+def test_evict_of_too_many_positions(lib):
+    """A sequence may hold 2^30 positions at most, by its table or by max_seq_len."""
+    wide = dict(seq_len=TOP, N=16385, window_size=65536)
+    tables, blocks = desc(I32, S * 16385 * 4), [desc(F16, 1 << 40)] * 2
+    sized = dict(pools=blocks, to=blocks, tables=tables, rows=desc(F32, 1 << 50), rows_to=desc(F32, 1 << 50))
+    refused(evict, lib, pc=args(**wide, step_idx=0x7FFFFFFF), match="2\\^30", **sized)
+    assert evict(lib, pc=args(**wide, step_idx=1 << 30, max_seq_len=1 << 30), **sized)["count"] == S * KV * TOP
