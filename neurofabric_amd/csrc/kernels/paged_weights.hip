@@ -46,7 +46,9 @@ __device__ __forceinline__ bool find_span(const PagedBatch& b, uint32_t seq, Spa
 }
 
 // Any head_dim, head ratio and alignment: 64 keys a workgroup, as f32 in LDS; a lane
-// scores one key, the four waves take query rows in turn and add up at the end.
+// scores one key, the four waves take query rows in turn and add up at the end.  Bound by
+// LDS and the vector ALU (8 single tokens over 4096 positions, 32 heads over 8 KV heads of
+// 80, f16: 171 us, 0.3 TB/s).
 constexpr int kAnyDim = 256;
 template <typename T, PoolType PT>
 __global__ __launch_bounds__(256) void weights_any_kernel(Weigh w) {
@@ -264,7 +266,10 @@ struct Query16<float, PT, DD> {
 };
 
 // Single tokens and short chunks, up to 16 NT query rows, which stay in registers while
-// the waves take 32-key tiles in turn, the next one's loads in flight.
+// the waves take 32-key tiles in turn, the next one's loads in flight.  Bound by HBM: 64
+// single tokens over up to 8192 positions, 32 heads over 8 KV heads of 128, f16, 0.70 GB in
+// 155 us, 4.5 TB/s; 16 over up to 32768, I8, 0.38 GB in 100 us, 3.8 TB/s, the codes'
+// conversion beside it; one of 100 positions, f32, 4.9 us, by its latency.
 template <typename T, PoolType PT, int DD, int NT, bool UNI>
 __global__ __launch_bounds__(256) void weights_few_kernel(Weigh w) {
   Task k;
@@ -366,7 +371,10 @@ __global__ __launch_bounds__(256) void weights_join_kernel(Weigh w) {
 // Many query rows, f16: 64 keys a wave stay in registers as B operands, 32-row tiles of the
 // queries go through LDS for all four waves on v_mfma_f32_32x32x16_f16.  Per tile and wave
 // there are DD / 8 MFMAs and 32 exponentials a lane, about as long: those of the tile before
-// are issued between the MFMAs of the next one.
+// are issued between the MFMAs of the next one.  2048 rows of two sequences with 8192
+// positions, 32 heads of 128: 241 GFLOP in 314 us a pass, 766 TFLOP/s, where a product of
+// 8192 in each size reaches 1187; the MFMA pipes are 37 % busy, as the exponentials, the
+// subtractions before them and the sums take as many issue slots.
 template <PoolType PT, int DD, bool UNI>
 __global__ __launch_bounds__(256, 2) void weights_many_kernel(Weigh w) {
   constexpr int KS = DD / 16, QP = DD + 8, CPR = DD / 8, NU = (32 * CPR + 255) / 256;
@@ -567,9 +575,11 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Weigh w) {
 }
 
 // Many query rows, f32: 32 keys a wave stay in registers, 16-row tiles of the queries come
-// straight from the caches, the next one in flight; the f32 MFMA's time hides them.
+// straight from the caches, the next one in flight; the f32 MFMA's time hides them.  512
+// rows of two sequences with 2048 positions, 32 heads of 128: 15 GFLOP, 213 us, 71 TFLOP/s
+// of 153 (261 with one buffer of queries); the waits between a tile's few sums.
 template <PoolType PT, int DD, bool UNI>
-__global__ __launch_bounds__(256, 2) void weights_many_f32_kernel(Weigh w) {
+__global__ NF_TWO_PER_CU void weights_many_f32_kernel(Weigh w) {
   constexpr int DG = DD / 4;
   Task k;
   const uint32_t kvh = blockIdx.y, seq = find_many(w, blockIdx.z), cut = blockIdx.x % w.cuts;
@@ -597,42 +607,49 @@ __global__ __launch_bounds__(256, 2) void weights_many_f32_kernel(Weigh w) {
   const Rows2 mine_rows = cut_rows(w, k, skip <= 0 ? 0 : (uint32_t)skip * k.group / 16 * 16, 16, cut);
   uint32_t r0 = mine_rows.from;
   const uint32_t r_end = mine_rows.to;
-  Query16<float, PT, DD> qa;
-  float base[4];
-  auto fetch = [&](uint32_t r) {
-    qa.fetch(w.q, q_row(w, k, min(r + n, k.live - 1), kvh), g);
+  Query16<float, PT, DD> qa[2];
+  float lse[2][4];  // nothing is computed from a load before its turn, which would wait for it
+  auto fetch = [&](int buf, uint32_t r) {
+    qa[buf].fetch(w.q, q_row(w, k, min(r + n, k.live - 1), kvh), g);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t at = r + 4 * g + i;
-      base[i] = at < k.live ? base_of(w.lse[q_row(w, k, at, kvh)]) : INFINITY;
-    }
+    for (int i = 0; i < 4; ++i) lse[buf][i] = w.lse[q_row(w, k, min(r + 4 * g + i, k.live - 1), kvh)];
   };
   float x[2] = {0.f, 0.f};
-  if (r0 < r_end) fetch(r0);
-  for (; r0 < r_end; r0 += 16) {
-    float4v sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  if (r0 < r_end) fetch(0, r0);
+  while (r0 < r_end) {
 #pragma unroll
-    for (int s = 0; s < DG; ++s)
+    for (int h = 0; h < 2; ++h) {
+      if (r0 >= r_end) continue;  // uniform
+      // whether or not there is a next tile: behind a branch, the wait for this one's rows
+      // would be one for the next one's too
+      fetch(h ^ 1, r0 + 16);
+      __builtin_amdgcn_sched_barrier(0);
+      float4v sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-      for (int j = 0; j < 2; ++j) sc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(qa.x[s / 4][s % 4], kb[j][s], sc[j], 0, 0, 0);
-    const float4v bs = {base[0], base[1], base[2], base[3]};
-    if (r0 + 16 < r_end) fetch(r0 + 16);
-    const int64_t first = k.t.pos0 + r0 / k.group;
-    if (first >= (int64_t)t0 + 31) {  // uniform: all rows see all keys
+      for (int s = 0; s < DG; ++s)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < 2; ++j) sc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(qa[h].x[s / 4][s % 4], kb[j][s], sc[j], 0, 0, 0);
+      float base[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[j] += __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][i], scale_log2, -bs[i]));
-    } else {
+      for (int i = 0; i < 4; ++i) base[i] = r0 + 4 * g + i < k.live ? base_of(lse[h][i]) : INFINITY;
+      const int64_t first = k.t.pos0 + r0 / k.group;
+      if (first >= (int64_t)t0 + 31) {  // uniform: all rows see all keys
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t pos = k.t.pos0 + (r0 + 4 * g + i) / k.group;
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][i], scale_log2, -bs[i]));
-          x[j] += (int64_t)t0 + 16 * j + n <= pos ? e : 0.f;
+          for (int i = 0; i < 4; ++i) x[j] += __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][i], scale_log2, -base[i]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int64_t pos = k.t.pos0 + (r0 + 4 * g + i) / k.group;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][i], scale_log2, -base[i]));
+            x[j] += (int64_t)t0 + 16 * j + n <= pos ? e : 0.f;
+          }
         }
       }
+      r0 += 16;
     }
   }
 #pragma unroll
