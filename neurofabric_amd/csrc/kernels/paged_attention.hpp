@@ -390,7 +390,7 @@ struct Work {
 //   S k^2 + (S F - W - B) k - W F = 0.
 // Own keys are cut where their tile would take longer than that, into no more pieces than
 // there are workgroups left.  (32 sequences with own parts of up to 1024 positions behind
-// 32768 in I8: all keys cut alike 54.8 us, without the fifth 52.7, so {I8}.)
+// 32768 in I8, one head_dim of 128: all keys cut alike 54.8 us, without the fifth 52.7, so 49.6.)
 __device__ __forceinline__ Cuts keys_of(const Chunk& c, const Work& w) {
   const float S = (float)c.target, F = 200.f;
   float shared = 0.f, own = w.own / S;
@@ -1850,7 +1850,8 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
   if (sp < ns) wide_rows<PT, DD, UNI, FORM>(c, t, sp, ns, kvh, lds);
 }
 
-// kShared: narrow and wide tiles in one launch, whose workgroups find out which theirs is.
+// kShared: narrow and wide tiles in one launch, whose workgroups find out which theirs is, so
+// that the groups' parts and the sequences' run beside each other.
 // `ns` of a part: 1 says that no other has partials of its rows.
 template <PoolType PT, int DD, int NT, bool UNI>
 __global__ NF_TWO_PER_CU void shared_kernel(Chunk c) {

@@ -36,8 +36,10 @@ __device__ __forceinline__ Budget find_budget(const PagedBatch& b, const PagedEv
 // 2. Runs of the positions, of a wave each, are counted: what stays, and ties.
 // 3. With the sums of the runs before it, each wave writes its own.
 // A row of up to some thousand positions is one workgroup's, all in one launch; its
-// instructions bound it (1024 threads, 131072 positions 158 us).  Longer ones are cut into
-// chunks, and what the chunks have to know of each other is left between launches.
+// steps, one after the other, bound it (600 positions 10 us; 32 sequences of up to 4096, 8 KV
+// heads, 14.6; 131072 positions 158).  Longer ones are cut into chunks, and what the chunks
+// have to know of each other is left between launches (two sequences of 131072, 8 KV heads:
+// clearing 5 us, the histograms 7 each, counts 8, writing 10).
 constexpr int kBins = 2048, kPasses = 3;
 __device__ __forceinline__ int shift_of(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
 __device__ __forceinline__ uint32_t known_of(int pass) { return pass == 0 ? 0u : ~0u << (pass == 1 ? 21 : 10); }
@@ -380,7 +382,8 @@ __global__ __launch_bounds__(256) void move_any_kernel(PagedBatch b, PagedEvict 
 }
 
 // Rows of whole 16-byte pieces: a lane per piece, as many rows a wave as fit, kRows of them
-// in flight, K and V.  Bound by HBM.
+// in flight, K and V.  Bound by HBM: 1024 rows of 32 sequences, 8 KV heads of 128, f16, 0.27
+// GB in 60 us, 4.5 TB/s; 32768 of two, I8, 0.28 GB in 57 to 70 us, 4 to 4.9 TB/s.
 constexpr int kRows = 4;
 template <PoolType PT>
 __global__ __launch_bounds__(256) void move_kernel(PagedBatch b, PagedEvict e) {

@@ -8,14 +8,31 @@
 //   m = max m_i,  l = sum l_i 2^(m_i - m),  acc likewise.
 // Where they bring many, each sequence's tiles go through the shared keys and its own ones
 // after them: a tile's rows are then a sequence's anyway.
+//
+// The tiles are those of the chunk attention.  What bounds it, 32 heads over 8 KV heads of
+// 128 (kernel times):
+//   64 single tokens behind 8192 positions, up to 512 of their own, f16: 43 us, combination
+//   6; 119 MB, of which a copy takes 24 us (each sequence reading all: 2.2 GB, 440 us).  A
+//   workgroup takes 9 us for finding its rows, the first keys and the partials and 2.1 to 2.7
+//   for 64 keys, so that more splits would not help.
+//   32 behind 32768, up to 1024 of their own, I8: 50 + 8 us, the codes' conversion besides.
+//   Five tokens of 32 behind four prompts of 4096: 51 + 7 us.
+//   16 questions of up to 200 behind 8192: 517 us a pass, 630 TFLOP/s; the softmax between
+//   the products, and a last round of workgroups that does not fill the chip.
 #include "paged_attention.hpp"
 
 namespace nfk {
 namespace paged {
 
-// Query rows of a sequence, on average, up to which the shared keys are apart.
-constexpr uint32_t kApartRows = 64;
-// Workgroups that run at once, two on each CU, and the fewest keys that one takes.
+// Query rows of a sequence (and KV head), on average, up to which the shared keys are apart.
+// 16 sequences behind 4096 positions, f16, with the combination, apart and not: 32 rows 43
+// and 49 us, 64 rows 60 and 78, 96 rows 88 and 87; behind two prefixes of 2048, I8: 64 rows
+// 40 and 47, 96 rows 52 and 60 (each tile converts its keys).
+template <PoolType PT>
+constexpr uint32_t kApartRows = PT == PoolType::I8 ? 96 : 64;
+// Workgroups that run at once, two on each CU, and the fewest keys that one takes: 256 and
+// 128, three chunks of 154 tokens with 833 positions, I8, 42.8 and 38.7 us; six tokens of 53
+// sequences with up to 1260, I8, 24.3 and 25.5; one chunk of 493 with 1197, f16, 52 and 52.6.
 constexpr uint32_t kResident = 512;
 constexpr uint32_t kMinKeys = 256;
 
@@ -45,7 +62,7 @@ hipError_t prefix_at(const PagedBatch& b, const PagedShared& sh, uint32_t n_head
   auto splits_in = [&](uint64_t used) {  // of all rows' keys
     return ws.part_floats > used ? (ws.part_floats - used) / ((uint64_t)b.rows * n_heads * (DD + kPartFloats)) : 0;
   };
-  c.apart = sh.n_groups > 0 && sh.n_groups < b.n_seqs && mean <= kApartRows && splits_in(plan_floats(true)) >= 4;
+  c.apart = sh.n_groups > 0 && sh.n_groups < b.n_seqs && mean <= kApartRows<PT> && splits_in(plan_floats(true)) >= 4;
   const uint64_t used = plan_floats(c.apart), most = splits_in(used), items = items_of(c.apart);
   if (!ws.part || ws.part_floats < used) return hipErrorOutOfMemory;
   // The fewest keys of a split for which the partials fit (`limit` as Border counts); a row
