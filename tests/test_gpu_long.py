@@ -802,6 +802,56 @@ def test_captured_steps_replay(provider, act, pool):
             assert np.array_equal(wb.read(np.float32, held.size).reshape(held.shape), w)
 
 
+@pytest.mark.parametrize("act,pool", ACT_POOL)
+def test_captured_long_steps_share_the_workspace(provider, act, pool):
+    """Two captured graphs of one prompt's attention, weights and eviction, whose kernels all keep partials in the workspace, are
+    replayed in turn with new lengths, eager calls between them: every replay gives the eager calls' bits."""
+    rng = np.random.default_rng(65)
+    heads, kv, dim, bs, top, rows = 8, 1, 64, 16, 300, 200
+    batch = ref.Batch(rng, [(17000, rows)], bs, spare=2 * -(-top // bs))
+    free = [i for i in range(batch.blocks) if i not in batch.table]
+    new = np.array(free, np.uint32).reshape(2, 1, -1)
+    pools = fill(rng, batch, None, act, pool, kv, dim, 0.1)
+    q, width = rows_of(rng, act, batch.rows, heads, dim), batch.width * bs
+    held = rng.random((1, kv, width)).astype(np.float32)
+    z0, k0 = np.zeros((batch.rows, heads), np.float32), np.zeros((1, kv, top), np.int32)
+    with Bufs(provider) as m:
+        desc, qb, hb = m.batch(batch), m.put(q), m.put(held)
+        first, plen, budget = m.put(np.array([0, 1], np.int32)), m.put(np.array([9000], np.int32)), m.put(np.array([[top, 20]], np.int32))
+
+        def steps(table):
+            kb = [m.put(p) for p in pools]
+            out = [m.put(np.zeros_like(q)), m.put(z0), m.put(np.zeros_like(held)), m.put(held), m.put(np.zeros(1, np.int32)), m.put(k0)]
+            tasks = (abi.nf_task_desc * 3)(
+                provider.task("flash_attention_paged_prefix", [qb] + kb + desc + [first, plen], out[:2],
+                              pc=pc_of(batch, kv, dim, n_heads=heads, step_idx=1)),
+                provider.task("paged_kv_weights", [qb, kb[0]] + desc + [out[1], hb], [out[2]],
+                              pc=pc_of(batch, kv, dim, n_heads=heads, step_idx=width, theta=0.5)),
+                provider.task("paged_kv_evict", kb + [out[2], desc[0], desc[2], budget, m.put(table)], kb + out[3:],
+                              pc=push_constants(M=kv, N=batch.width, K=1, seq_len=top, head_dim=dim, window_size=bs, step_idx=width)))
+            return tasks, kb + out
+
+        all_steps = [steps(new[i]) for i in range(2)] + [steps(new[0])]
+        read = lambda bufs: [b.read(np.uint8) for b in bufs]  # noqa: E731
+        graphs = []
+        for tasks, _ in all_steps[:2]:
+            provider.run_tasks(tasks)
+            graphs.append(hiprt.Graph(provider.stream(), lambda t=tasks: provider.run_tasks(t)))
+        for n in (17000, 900, 16999, 300, 12345):
+            desc[2].write(np.array([n], np.int32))
+            plen.write(np.array([n // 2], np.int32))
+            provider.run_tasks(all_steps[2][0])
+            eager = read(all_steps[2][1][2:])
+            for i in (0, 1, 0):
+                graphs[i].launch()
+            for i in range(2):
+                got = read(all_steps[i][1][2:])
+                for j, (a, b) in enumerate(zip(got, eager)):
+                    assert np.array_equal(a, b), (n, i, j)
+            kept = eager[5].view(np.int32)
+            assert (np.diff(kept[:min(n, top)]) > 0).all() and kept[min(n, top) - 1] == n - 1
+
+
 def test_output_in_place_of_the_query(provider):
     rng = np.random.default_rng(64)
     for seqs, group, act, dim in (([(900, 1), (820, 1)] * 4, 800, "f16", 128), ([(200, 90), (250, 80)], 96, "f16", 64),
