@@ -409,7 +409,8 @@ __device__ __forceinline__ Cuts keys_of(const Chunk& c, const Work& w) {
 // With last_round: T tiles of a KV head are q rounds of the S workgroups at once and r more,
 // which would take a round of their own.  The last sequences with r tiles between them are
 // cut into as many pieces as still fit that round, which then takes 1 / pieces of one (16
-// questions of up to 200 tokens behind 8192, 88 tiles, S 64: uncut 700 us, so 608).
+// questions of up to 200 tokens behind 8192, 88 tiles, S 64: uncut 700 us, so 608, both before
+// wide_rows()'s HINT).
 constexpr uint32_t kMostPieces = 4;
 __device__ __forceinline__ uint32_t more_tiles(const Chunk& c, uint32_t tiles) {
   return tiles > c.target ? tiles % c.target : 0;
@@ -1486,7 +1487,10 @@ struct WideLds {
   __attribute__((aligned(16))) half_t lds[2 * BUF];
   int tile_bad[2];
 };
-template <PoolType PT, int DD, bool UNI, Form FORM>
+// HINT: the open loop's test of the end is a branch of its own, unlikely to be taken.  In
+// kShared 16 chunks of up to 200 tokens behind 8192 positions take 515 us without and 457
+// with it (474 on another card), five tokens of 32 sequences 58.1 and 52.6, but single tokens of 64 53.8 and 55.5.
+template <PoolType PT, int DD, bool UNI, Form FORM, bool HINT = false>
 __device__ __forceinline__ void wide_rows(const Chunk& c, const RowTile& t, uint32_t sp, uint32_t ns, uint32_t kvh,
                                           WideLds<DD>& mem) {
   constexpr bool SHARE = FORM == kShared, LSE = FORM != kChunk;
@@ -1783,7 +1787,10 @@ __device__ __forceinline__ void wide_rows(const Chunk& c, const RowTile& t, uint
   // the first that has a hole.  While one is computed from its buffer, the next is
   // staged into the other and the one after that is loaded.  Two loops, as one with
   // both kinds of tile does not fit the registers.
-  auto open = [&]() { return t0 < end && rows.have() == ~0ull && rows.at(t0) + 63 <= pos_lo; };  // uniform
+  auto open = [&]() {  // uniform
+    if (HINT && __builtin_expect(t0 >= end, 0)) return false;
+    return t0 < end && rows.have() == ~0ull && rows.at(t0) + 63 <= pos_lo;
+  };
   if (open()) {
     stage(~0ull, std::true_type{}, 0, 0);
     next();
@@ -1872,7 +1879,7 @@ __global__ NF_TWO_PER_CU void shared_kernel(Chunk c) {
   }
   const uint32_t ns = t.last == 0 && t.slot == 0 ? t.splits : t.splits + 1;
   if (!t.wide) narrow_tile<PT, DD, NT, UNI, kShared>(c, t, sp, ns, kvh, lds.narrow);
-  else wide_rows<PT, DD, UNI, kShared>(c, t, sp, ns, kvh, lds.wide);
+  else wide_rows<PT, DD, UNI, kShared, NT == 2>(c, t, sp, ns, kvh, lds.wide);
 }
 
 // ---- f32 rows -----------------------------------------------------------------------

@@ -16,8 +16,8 @@
 //   workgroup takes 9 us for finding its rows, the first keys and the partials and 2.1 to 2.7
 //   for 64 keys, so that more splits would not help.
 //   32 behind 32768, up to 1024 of their own, I8: 50 + 8 us, the codes' conversion besides.
-//   Five tokens of 32 behind four prompts of 4096: 51 + 7 us.
-//   16 questions of up to 200 behind 8192: 517 us a pass, 630 TFLOP/s; the softmax between
+//   Five tokens of 32 behind four prompts of 4096: 46 + 7 us.
+//   16 questions of up to 200 behind 8192: 457 to 474 us a pass, 700 TFLOP/s; the softmax between
 //   the products, and a last round of workgroups that does not fill the chip.
 #include "paged_attention.hpp"
 
@@ -25,7 +25,8 @@ namespace nfk {
 namespace paged {
 
 // Query rows of a sequence (and KV head), on average, up to which the shared keys are apart.
-// 16 sequences behind 4096 positions, f16, with the combination, apart and not: 32 rows 43
+// 16 sequences behind 4096 positions, f16, with the combination, apart and not, both
+// without wide_rows()'s HINT: 32 rows 43
 // and 49 us, 64 rows 60 and 78, 96 rows 88 and 87; behind two prefixes of 2048, I8: 64 rows
 // 40 and 47, 96 rows 52 and 60 (each tile converts its keys).
 template <PoolType PT>
