@@ -19,6 +19,7 @@
 //   Five tokens of 32 behind four prompts of 4096: 46 + 7 us.
 //   16 questions of up to 200 behind 8192: 457 to 474 us a pass, 700 TFLOP/s; the softmax between
 //   the products, and a last round of workgroups that does not fill the chip.
+#include "../paged_tiles.hpp"
 #include "paged_attention.hpp"
 
 namespace nfk {
@@ -47,13 +48,9 @@ hipError_t prefix_at(const PagedBatch& b, const PagedShared& sh, uint32_t n_head
   const uint64_t rows = (uint64_t)b.rows * c.group, mean = (rows + b.n_seqs - 1) / b.n_seqs;
   const uint32_t nt = F16 && mean > 16 ? 2 : 1;
   c.target = (kResident + b.n_kv - 1) / b.n_kv;
-  // At most so many tiles and splits of a KV head: a part's last tile and split may be short.
-  auto tiles = [&](uint64_t n) {  // of n parts that have all rows between them, `group` at least each
-    if (n > b.rows) n = b.rows;
-    const uint64_t few = rows < kFew * n ? rows : kFew * n, most = rows / kWideRows + few / (16 * nt) + n;
-    const uint64_t more = n + (rows - n * c.group) / (16 * nt);
-    return c.group <= 16 * nt && more < most ? more : most;
-  };
+  // At most so many tiles and splits of a KV head: those of all parts, and what keys_of() and
+  // cut_last() may add to them.
+  auto tiles = [&](uint64_t parts) { return nfhip::most_tiles(rows, parts, c.group, kFew, 16 * nt, kWideRows); };
   auto items_of = [&](bool apart) { return tiles(b.n_seqs) + (apart ? tiles(sh.n_groups) : 0) + c.target + 16; };
   // The workspace's end: a few numbers, and the plan of a large batch.
   auto plan_floats = [&](bool apart) {

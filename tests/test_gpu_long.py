@@ -889,3 +889,50 @@ def test_repeated_calls_give_the_same_bits(provider, act, pool):
                               pc=pc_of(batch, kv, dim, n_heads=heads, step_idx=width, theta=1.0))
             seen.add(b"".join(b.read(np.uint8).tobytes() for b in (out, lb, wb)))
     assert len(seen) == 1
+
+
+# ---- many sequences, padding, rows that count for nothing -------------------------------
+
+RAGGED_HEADS = [  # types, sequences (positions, rows), positions that all share, heads, KV heads, head_dim
+    ("f16", [(3 + i % 9, 3) for i in range(400)], 0, 96, 8, 64),
+    ("f32", [(2 + i % 9, 2) for i in range(400)], 0, 96, 8, 64),
+    ("f32", [(3 + i % 9, 3) for i in range(400)], 0, 48, 8, 64),
+    ("f16", [(1000 if i < 30 else 10, 3) for i in range(100)], 0, 96, 8, 64),  # with splits, each workgroup finds its tile itself
+    ("f16", [(35 + i % 3, 3) for i in range(700)], 32, 96, 8, 64),
+    ("f16", [(5 + i % 3, 5) for i in range(1300)], 0, 28, 4, 64),
+    ("f16", [(7 + i % 3, 7) for i in range(1400)], 0, 40, 8, 64),
+    ("f16", [(11 + i % 3, 11) for i in range(1400)], 0, 24, 8, 64),
+    ("f32", [(6 + i % 3, 6) for i in range(1400)], 0, 24, 8, 96),
+]
+
+
+@pytest.mark.parametrize("pool", ["rows", "i8"])
+@pytest.mark.parametrize("act,seqs,share,heads,kv,dim", RAGGED_HEADS)
+def test_prefix_heads_that_do_not_divide_a_tile(provider, act, pool, seqs, share, heads, kv, dim):
+    """Many sequences whose query rows fill their tiles badly: every row is written; the first, the last and some others are
+    held to the plain form."""
+    pool = act if pool == "rows" else pool
+    rng = np.random.default_rng(71)
+    batch = ref.Batch(rng, seqs, 16, behind=3)
+    shared = ref.Shared(batch, [(0, len(seqs), share)] if share else [])
+    pools = fill(rng, batch, shared, act, pool, kv, dim)
+    q = rows_of(rng, act, batch.rows, heads, dim)
+    was = np.full_like(q, np.nan)
+    with Bufs(provider) as m:
+        out, lb = m.put(was), m.put(np.full((batch.rows, heads), np.nan, np.float32))
+        provider.dispatch("flash_attention_paged_prefix", [m.put(q)] + [m.put(p) for p in pools] + m.batch(batch) +
+                          [m.put(shared.first), m.put(shared.len)], [out, lb],
+                          pc=pc_of(batch, kv, dim, n_heads=heads, step_idx=len(shared.groups)))
+        got = out.read(NP[act], q.size).reshape(q.shape)
+        z = lb.read(np.float32, batch.rows * heads).reshape(batch.rows, heads)
+    mine = mine_of(batch)
+    assert np.isfinite(got[mine]).all() and np.isfinite(z[mine]).all()
+    assert np.isnan(got[~mine]).all() and np.isnan(z[~mine]).all()
+    some = [0] + list(range(1, len(seqs) - 30, 37)) + list(range(len(seqs) - 30, len(seqs)))
+    part = ref.Batch(rng, [(0, seqs[s][1]) for s in some], 16)
+    part.lens, part.table, part.width, part.blocks = batch.lens[some], batch.table[some], batch.width, batch.blocks
+    rows = np.concatenate([np.arange(batch.starts[s], batch.starts[s + 1]) for s in some])
+    of = ref.Shared(part, [(0, len(some), share)] if share else [])
+    want, err, wz, zerr = ref.attention(part, of, pool, dim, heads, kv, pools, q[rows], act)
+    check(got[rows], want, err, (act, pool, heads, kv, seqs[:3]))
+    check(z[rows], wz, zerr, ("lse", act, pool, heads, kv, seqs[:3]))
