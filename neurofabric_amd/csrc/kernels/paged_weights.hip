@@ -666,11 +666,12 @@ hipError_t weights_mfma(Weigh& w, const nfhip::Workspace& ws, hipStream_t s) {
   const PagedBatch& b = w.b;
   const uint64_t rows = (uint64_t)b.rows * (w.n_heads / b.n_kv), pairs = (uint64_t)b.n_kv * b.n_seqs;
   // Rows of a sequence are known on the device only: each kernel leaves the sequences that
-  // are the other's.
+  // are the other's.  A lone sequence's are the kernel's for many, though it may have few of
+  // the batch's rows, the others padding.
   const uint32_t few_rows = rows > 16ull * b.n_seqs ? 32 : 16;
   const bool many = rows > few_rows, few = b.n_seqs > 1 || !many;
   if (many) {
-    w.lo = few_rows;
+    w.lo = few ? few_rows : 0;
     w.hi = ~0ull;
     w.keys = kManyKeys;
     const uint64_t most = rows / (few_rows + 1);  // such sequences

@@ -936,3 +936,48 @@ def test_prefix_heads_that_do_not_divide_a_tile(provider, act, pool, seqs, share
     want, err, wz, zerr = ref.attention(part, of, pool, dim, heads, kv, pools, q[rows], act)
     check(got[rows], want, err, (act, pool, heads, kv, seqs[:3]))
     check(z[rows], wz, zerr, ("lse", act, pool, heads, kv, seqs[:3]))
+
+
+@pytest.mark.parametrize("act,pool", ACT_POOL)
+@pytest.mark.parametrize("n,rows,heads,kv,dim,bs", [
+    (200, 1, 8, 1, 64, 16), (77, 2, 8, 2, 128, 16), (700, 5, 4, 2, 96, 8), (33, 8, 4, 1, 64, 32), (1, 1, 16, 16, 128, 16),
+    (5000, 3, 8, 1, 64, 16), (90, 0, 8, 2, 64, 16), (60, 4, 6, 4, 64, 16), (60, 2, 4, 2, 80, 16)])
+def test_weights_of_one_padded_sequence(provider, act, pool, n, rows, heads, kv, dim, bs):
+    """One sequence with few of the batch's rows, the others padding."""
+    if pool == "i8" and dim % 32:
+        pytest.skip("an 8-bit cache needs groups of 32")
+    rng = np.random.default_rng(72)
+    for behind in (7, 60, 300):
+        batch = ref.Batch(rng, [(n, rows)], bs, behind=behind, before=behind % 2)
+        q, pools, z = run_attention(provider, rng, batch, None, act, pool, heads, kv, dim, chunk=True)
+        run_weights(provider, rng, batch, act, pool, heads, kv, dim, z, q, pools, theta=0.5)
+
+
+@pytest.mark.parametrize("act,pool", ACT_POOL)
+def test_captured_drafts_of_one_sequence(provider, act, pool):
+    """A captured step of up to 16 drafts of one sequence is replayed with fewer of them, and with more again."""
+    rng = np.random.default_rng(73)
+    heads, kv, dim, bs, most = 8, 2, 64, 16, 16
+    batch = ref.Batch(rng, [(400, most)], bs)
+    pools, q, width = fill(rng, batch, None, act, pool, kv, dim), rows_of(rng, act, most, heads, dim), batch.width * bs
+    held = rng.random((1, kv, width)).astype(np.float32)
+    with Bufs(provider) as m:
+        kb, desc, qb, hb = [m.put(p) for p in pools], m.batch(batch), m.put(q), m.put(held)
+        out, lb, wb = m.put(np.zeros_like(q)), m.put(np.zeros((most, heads), np.float32)), m.put(held)
+        tasks = (abi.nf_task_desc * 2)(
+            provider.task("flash_attention_paged_chunk", [qb] + kb + desc, [out, lb], pc=pc_of(batch, kv, dim, n_heads=heads)),
+            provider.task("paged_kv_weights", [qb, kb[0]] + desc + [lb, hb], [wb],
+                          pc=pc_of(batch, kv, dim, n_heads=heads, step_idx=width, theta=0.5)))
+        graph = hiprt.Graph(provider.stream(), lambda: provider.run_tasks(tasks))
+        for n, rows in ((400, 16), (300, 1), (399, 8), (17, 9), (1, 1), (400, 16)):
+            batch.seqs, batch.lens, batch.starts = [(n, rows)], np.array([n], np.int32), np.array([0, rows], np.int32)
+            desc[1].write(batch.starts)
+            desc[2].write(batch.lens)
+            wb.write(np.full_like(held, 3.0))
+            graph.launch()
+            z, w = lb.read(np.float32, most * heads).reshape(most, heads), wb.read(np.float32, held.size).reshape(held.shape)
+            want, err = ref.weights(batch, pool, dim, heads, kv, pools[0], q, act, z, held, 0.5, np.full_like(held, 3.0))
+            check(w, want, err, (n, rows))
+            wb.write(np.full_like(held, 3.0))
+            provider.run_tasks(tasks)
+            assert np.array_equal(wb.read(np.float32, held.size).reshape(held.shape), w)
