@@ -981,3 +981,29 @@ def test_captured_drafts_of_one_sequence(provider, act, pool):
             wb.write(np.full_like(held, 3.0))
             provider.run_tasks(tasks)
             assert np.array_equal(wb.read(np.float32, held.size).reshape(held.shape), w)
+
+
+@pytest.mark.parametrize("act,pool", ACT_POOL)
+@pytest.mark.parametrize("n,dim,bs,width", [(4096, 64, 16, 8192), (4500, 128, 16, 8192), (4096, 96, 8, 16384), (4096, 80, 16, 300),
+                                            (4096, 64, 16, 0)])
+def test_weights_of_many_rows_keep_their_bits(provider, act, pool, n, dim, bs, width):
+    """Each of 4096 rows gives the same weight, so that every rounding of a long sum may go the same way: a sum may be off by
+    as many of them as there are tiles of 32 query rows, and some for what is within one, not by one for each row."""
+    if pool == "i8" and dim % 32:
+        pytest.skip("an 8-bit cache needs groups of 32")
+    rng = np.random.default_rng(74)
+    heads, kv, rows = 16, 2, 4096
+    batch = ref.Batch(rng, [(n, rows)], bs, width=width)
+    pools, q = fill(rng, batch, None, act, pool, kv, dim), np.zeros((rows, heads, dim), NP[act])  # all score 0
+    lse = np.tile(np.repeat(np.array([3.4887, 0.5843], np.float32), 8), (rows, 1))
+    held = np.zeros((1, kv, batch.width * bs), np.float32)
+    with Bufs(provider) as m:
+        wb = m.put(held)
+        provider.dispatch("paged_kv_weights", [m.put(q), m.put(pools[0])] + m.batch(batch) + [m.put(lse), m.put(held)], [wb],
+                          pc=pc_of(batch, kv, dim, n_heads=heads, step_idx=held.shape[2]))
+        got = wb.read(np.float32, held.size).reshape(held.shape)[0, :, :n].astype(np.float64)
+    # the weight as the kernel has it: the last position has one token's, a sum of 8, off by 8 roundings at most
+    one = got[:, -1] / 8
+    assert np.allclose(one, np.exp(-lse[0, ::8].astype(np.float64)), rtol=2e-6, atol=0)
+    want = one[:, None] * (8.0 * np.minimum(n - np.arange(n), rows))
+    check(got, want, (8 * rows / 32 + 32 + 8) * paged_ref.U * want, (act, pool, n, dim))
