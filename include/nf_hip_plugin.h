@@ -86,10 +86,11 @@
  *       WEIGHTS[s][g][j] = theta HELD[s][g][j] + sum of exp(score of j - LSE[r][h]) over the
  *     sequence's rows r at positions >= j and the query heads h that read KV head g.  theta
  *     (0 to 1) lets older weights fade; 0 does not read HELD.  The positions of the rows
- *     themselves start from 0.  A position without storage gets nothing, a row whose LSE is
- *     -inf gives nothing, nor does a score of -inf.  Positions past the length (or the bound)
- *     and sequences without rows are left as they are.  WEIGHTS may be HELD's buffer; other
- *     overlaps are not allowed.  Operands and limits are those of the attention.
+ *     themselves start from 0.  A position without storage gets nothing; a row whose LSE is
+ *     -inf gives nothing, whatever Q holds, nor does a score of -inf where LSE is a number.
+ *     Positions past the length (or the bound) and sequences without rows are left as they
+ *     are.  WEIGHTS may be HELD's buffer; other overlaps are not allowed.  Operands and limits
+ *     are those of the attention.
  *   paged_kv_evict      K_pool, V_pool, WEIGHTS, TABLES, LENS, BUDGET, NEW_TABLES
  *                       -> K_pool', V_pool', WEIGHTS', NEW_LENS, KEPT
  *     Of the L positions of a sequence every KV head keeps k = min(keep, L, seq_len), with

@@ -118,8 +118,14 @@ __global__ __launch_bounds__(256) void weights_any_kernel(Weigh w) {
 // rows of 8 heads that weigh 0.03 each: off by 39 half steps, by 3073 as one sum; 2048 rows of
 // two prompts of 8192: 1.8e-7 and 7.1e-7 from 64 bits, 319 us both).
 
-// What is taken off a row's score in base 2; a row that counts for nothing has infinity.
-__device__ __forceinline__ float base_of(float lse) { return lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f; }
+// What is taken off a row's score in base 2.
+__device__ __forceinline__ float base_of(float lse) { return lse * 1.4426950408889634f; }
+// The position up to which a row's weights count: a row that counts for nothing sees no
+// position, as its scores may be infinite or NaN.
+constexpr int kNowhere = -1;
+__device__ __forceinline__ int sees_up_to(bool live, float lse, int64_t pos) {
+  return live && lse != -INFINITY ? (int)pos : kNowhere;
+}
 
 // The sequence of a workgroup, its keys and query rows; false for none.
 struct Task {
@@ -278,7 +284,7 @@ struct Query16<float, PT, DD> {
 // Single tokens and short chunks, up to 16 NT query rows, which stay in registers while
 // the waves take 32-key tiles in turn, the next one's loads in flight.  Bound by HBM: 64
 // single tokens over up to 8192 positions, 32 heads over 8 KV heads of 128, f16, 0.70 GB in
-// 155 us, 4.5 TB/s; 16 over up to 32768, I8, 0.38 GB in 100 us, 3.8 TB/s, the codes'
+// 157 us, 4.4 TB/s; 16 over up to 32768, I8, 0.38 GB in 92 us, 4.1 TB/s, the codes'
 // conversion beside it; one of 100 positions, f32, 4.9 us, by its latency.
 template <typename T, PoolType PT, int DD, int NT, bool UNI>
 __global__ __launch_bounds__(256) void weights_few_kernel(Weigh w) {
@@ -302,8 +308,9 @@ __global__ __launch_bounds__(256) void weights_few_kernel(Weigh w) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t r = 16 * u + 4 * g + i, at = min(r, k.live - 1);
-      pos[u][i] = (int)k.t.pos0 + (int)(at / k.group);
-      base[u][i] = r < k.live ? base_of(w.lse[q_row(w, k, at, kvh)]) : INFINITY;
+      const float lse = w.lse[q_row(w, k, at, kvh)];
+      pos[u][i] = sees_up_to(r < k.live, lse, k.t.pos0 + at / k.group);
+      base[u][i] = base_of(lse);
     }
   }
   Keys16<T, PT, DD> keys[2];
@@ -382,7 +389,7 @@ __global__ __launch_bounds__(256) void weights_join_kernel(Weigh w) {
 // queries go through LDS for all four waves on v_mfma_f32_32x32x16_f16.  Per tile and wave
 // there are DD / 8 MFMAs and 32 exponentials a lane, about as long: those of the tile before
 // are issued between the MFMAs of the next one.  2048 rows of two sequences with 8192
-// positions, 32 heads of 128: 241 GFLOP in 314 us a pass, 766 TFLOP/s, where a product of
+// positions, 32 heads of 128: 241 GFLOP in 313 to 319 us a pass on several cards, 755 to 769 TFLOP/s, where a product of
 // 8192 in each size reaches 1187; the MFMA pipes are 37 % busy, as the exponentials, the
 // subtractions before them and the sums take as many issue slots.
 template <PoolType PT, int DD, bool UNI>
@@ -452,9 +459,15 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Weigh w) {
     const bool in = r.token < k.t.rows;
     return (uint64_t)(k.t.start + (in ? r.token : k.t.rows - 1)) * w.n_heads + kvh * k.group + (in ? r.head : k.group - 1);
   };
-  Row at[NU], mine = row_at(r0 + (tid & 31)), first = row_at(r0);
+  Row at[NU], mine, first;
+  auto begin = [&]() {
+    uint32_t from = r0;
+    asm volatile("" : "+s"(from));  // found anew in each pass, and not kept in registers for the next
+    mine = row_at(from + (tid & 31));
+    first = row_at(from);
 #pragma unroll
-  for (int u = 0; u < NU; ++u) at[u] = row_at(r0 + (tid + 256 * u < 32 * CPR ? tid + 256 * u : 32 * CPR - 1) / CPR);
+    for (int u = 0; u < NU; ++u) at[u] = row_at(from + (tid + 256 * u < 32 * CPR ? tid + 256 * u : 32 * CPR - 1) / CPR);
+  };
   auto fetch = [&]() {  // the next tile
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
@@ -463,8 +476,8 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Weigh w) {
       go_on(at[u]);
     }
     if (tid < 32) {
-      b0 = mine.token < k.t.rows ? base_of(w.lse[place_of(mine)]) : INFINITY;
-      p0 = (int)k.t.pos0 + (int)mine.token;
+      b0 = w.lse[place_of(mine)];
+      p0 = sees_up_to(mine.token < k.t.rows, b0, k.t.pos0 + mine.token);
       go_on(mine);
     }
   };
@@ -475,7 +488,7 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Weigh w) {
       if (32 * CPR % 256 == 0 || ch < 32 * CPR) *reinterpret_cast<u32x4*>(&qs[buf][ch / CPR * QP + 8 * (ch % CPR)]) = raw[u];
     }
     if (tid < 32) {
-      base[buf][tid] = b0;
+      base[buf][tid] = b0 == -INFINITY ? INFINITY : base_of(b0);
       place[buf][tid] = p0;
     }
   };
@@ -527,65 +540,76 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Weigh w) {
       t[j] = 0.f;
     }
   };
-  if (r0 < r_end) {  // uniform
-    // A first tile whose rows count for nothing stands before the first.
-    fetch();
-    stage(0);
-    if (tid < 32) {
-      base[2][tid] = INFINITY;
-      place[2][tid] = 0x7FFFFFFF;
-    }
-    if (r0 + 32 < r_end) fetch();
-    __syncthreads();
-    f32x16 sc[2][2];
+  // A row that counts for nothing weighs exp2(-inf) as well, unless its score is infinite or
+  // NaN: where a sum is, all tiles are gone through again with a test of each row's place
+  // (a look at each tile's rows took 331 us where this takes 319).
+  for (bool strict = false;; strict = true) {
+    if (r0 < r_end) {  // uniform
+      // A first tile whose rows weigh exp2(-inf) stands before the first.
+      begin();
+      fetch();
+      stage(0);
+      if (tid < 32) {
+        base[2][tid] = INFINITY;
+        place[2][tid] = 0x7FFFFFFF;
+      }
+      if (r0 + 32 < r_end) fetch();
+      __syncthreads();
+      f32x16 sc[2][2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sc[1][j][i] = 0.f;
-    int buf = 0, old = 2;
-    uint32_t r = r0;  // the tile in buf
-    bool open = true; // the one in old: all rows see all keys
-    // Two tiles a round, so that the scores' registers are known.
-    for (;;) {
-      bool done = false;
+        for (int i = 0; i < 16; ++i) sc[1][j][i] = 0.f;
+      int buf = 0, old = 2;
+      uint32_t r = r0;  // the tile in buf
+      bool open = true; // the one in old: all rows see all keys
+      // Two tiles a round, so that the scores' registers are known.
+      for (;;) {
+        bool done = false;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (done) break;
-        const int nb = 3 - buf - old;
-        const bool more = r + 32 < r_end;
-        if (more) {
-          stage(nb);  // its readers passed the last barrier
-          if (r + 64 < r_end) fetch();
-        }
-        if (t0 < k.end) {  // uniform
-          if (open) step(buf, sc[h], old, sc[h ^ 1], std::true_type{});
-          else step(buf, sc[h], old, sc[h ^ 1], std::false_type{});
-        }
-        open = (int64_t)k.t.pos0 + first.token >= (int64_t)t0 + 63;
-        go_on(first);
-        old = buf;
-        buf = nb;
-        r += 32;
-        __syncthreads();
-        if (!more) {
-          // the last tile's weights
-          if (t0 < k.end) {
+        for (int h = 0; h < 2; ++h) {
+          if (done) break;
+          const int nb = 3 - buf - old;
+          const bool more = r + 32 < r_end;
+          if (more) {
+            stage(nb);  // its readers passed the last barrier
+            if (r + 64 < r_end) fetch();
+          }
+          if (t0 < k.end) {  // uniform
+            if (open) step(buf, sc[h], old, sc[h ^ 1], std::true_type{});
+            else step(buf, sc[h], old, sc[h ^ 1], std::false_type{});
+          }
+          open = !strict && (int64_t)k.t.pos0 + first.token >= (int64_t)t0 + 63;
+          go_on(first);
+          old = buf;
+          buf = nb;
+          r += 32;
+          __syncthreads();
+          if (!more) {
+            // the last tile's weights
+            if (t0 < k.end) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int at = 8 * (i / 4) + 4 * hf + i % 4;
+              for (int i = 0; i < 16; ++i) {
+                const int at = 8 * (i / 4) + 4 * hf + i % 4;
 #pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[h][j][i], scale_log2, -base[old][at]));
-                t[j] += t0 + 32 * j + n <= place[old][at] ? v : 0.f;
+                for (int j = 0; j < 2; ++j) {
+                  const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[h][j][i], scale_log2, -base[old][at]));
+                  t[j] += t0 + 32 * j + n <= place[old][at] ? v : 0.f;
+                }
               }
             }
+            done = true;
           }
-          done = true;
         }
+        flush();
+        if (done) break;
       }
-      flush();
-      if (done) break;
     }
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) bad = bad || ((seen >> (32 * j + n)) & 1 && !(__builtin_fabsf(x[j]) < INFINITY));
+    if (strict || !__syncthreads_or(bad)) break;  // uniform
+    x[0] = x[1] = 0.f;
   }
 #pragma unroll
   for (int j = 0; j < 2; ++j) x[j] = sum2((seen >> (32 * j + n)) & 1 ? x[j] : 0.f);
@@ -594,8 +618,9 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Weigh w) {
 
 // Many query rows, f32: 32 keys a wave stay in registers, 16-row tiles of the queries come
 // straight from the caches, the next one in flight; the f32 MFMA's time hides them.  512
-// rows of two sequences with 2048 positions, 32 heads of 128: 15 GFLOP, 213 us, 71 TFLOP/s
-// of 153 (261 with one buffer of queries); the waits between a tile's few sums.
+// rows of two sequences with 2048 positions, 32 heads of 128: 15 GFLOP, 183 us, 82 TFLOP/s
+// of 153 (with one buffer of queries 261 where this took 213); the waits between a tile's few
+// sums.
 template <PoolType PT, int DD, bool UNI>
 __global__ NF_TWO_PER_CU void weights_many_f32_kernel(Weigh w) {
   constexpr int DG = DD / 4;
@@ -649,10 +674,14 @@ __global__ NF_TWO_PER_CU void weights_many_f32_kernel(Weigh w) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) sc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(qa[h].x[s / 4][s % 4], kb[j][s], sc[j], 0, 0, 0);
       float base[4];
+      bool count[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) base[i] = r0 + 4 * g + i < k.live ? base_of(lse[h][i]) : INFINITY;
+      for (int i = 0; i < 4; ++i) {
+        base[i] = base_of(lse[h][i]);
+        count[i] = sees_up_to(r0 + 4 * g + i < k.live, lse[h][i], 0) == 0;
+      }
       const int64_t first = k.t.pos0 + r0 / k.group;
-      if (first >= (int64_t)t0 + 31) {  // uniform: all rows see all keys
+      if (first >= (int64_t)t0 + 31 && __ballot(!(count[0] && count[1] && count[2] && count[3])) == 0) {  // uniform: all rows see all keys
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -664,7 +693,7 @@ __global__ NF_TWO_PER_CU void weights_many_f32_kernel(Weigh w) {
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][i], scale_log2, -base[i]));
-            t[j] += (int64_t)t0 + 16 * j + n <= pos ? e : 0.f;
+            t[j] += count[i] && (int64_t)t0 + 16 * j + n <= pos ? e : 0.f;
           }
         }
       }

@@ -1007,3 +1007,31 @@ def test_weights_of_many_rows_keep_their_bits(provider, act, pool, n, dim, bs, w
     assert np.allclose(one, np.exp(-lse[0, ::8].astype(np.float64)), rtol=2e-6, atol=0)
     want = one[:, None] * (8.0 * np.minimum(n - np.arange(n), rows))
     check(got, want, (8 * rows / 32 + 32 + 8) * paged_ref.U * want, (act, pool, n, dim))
+
+
+@pytest.mark.parametrize("act,pool", ACT_POOL)
+@pytest.mark.parametrize("seqs,heads,kv,dim", [
+    ([(300, 1), (90, 2), (64, 4)], 8, 2, 64), ([(300, 90), (200, 64), (33, 33)], 8, 2, 128), ([(400, 130)], 4, 1, 96),
+    ([(700, 40), (90, 2)], 16, 2, 64), ([(90, 20), (60, 1)], 4, 2, 40), ([(600, 500)], 8, 1, 64)])
+def test_weights_of_rows_that_count_for_nothing(provider, act, pool, seqs, heads, kv, dim):
+    """Rows whose log-sum-exp is -inf give nothing, whatever their queries hold."""
+    if pool == "i8" and dim % 32:
+        pytest.skip("an 8-bit cache needs groups of 32")
+    rng = np.random.default_rng(75)
+    batch = ref.Batch(rng, seqs, 16, behind=2)
+    q, pools, z = run_attention(provider, rng, batch, None, act, pool, heads, kv, dim, chunk=True)
+    none = rng.random(z.shape) < 0.15
+    none[batch.starts[1:] - 1] |= rng.random((len(seqs), heads)) < 0.5  # the last rows of the sequences among them
+    z = np.where(none, -np.inf, z).astype(np.float32)
+    bad = q.copy()
+    bad[none] = rng.choice([np.nan, np.inf, -np.inf, 6e4], (int(none.sum()), dim)).astype(NP[act])
+    plain = run_weights(provider, np.random.default_rng(5), batch, act, pool, heads, kv, dim, z, np.where(none[..., None], NP[act](0), q), pools)
+    width = batch.width * batch.bs
+    held = np.random.default_rng(5).random((len(seqs), kv, width)).astype(np.float32)
+    with Bufs(provider) as m:
+        wb = m.put(np.full_like(held, 9.0))
+        provider.dispatch("paged_kv_weights", [m.put(bad), m.put(pools[0])] + m.batch(batch) + [m.put(z), m.put(held)], [wb],
+                          pc=pc_of(batch, kv, dim, n_heads=heads, step_idx=width, theta=1.0))
+        got = wb.read(np.float32, held.size).reshape(held.shape)
+    assert np.isfinite(got).all()
+    assert np.array_equal(got, plain)
