@@ -78,7 +78,8 @@
  *     tables name for them is not read.  Sequences before GROUPS[0] and behind the last
  *     group, and groups with a prefix of 0 or less, share nothing.  A row attends to the
  *     positions 0 .. p as above, shared or not: a prefix may reach past new rows and past
- *     a sequence's end.  At most 65535 groups; their contents are read when the op runs.
+ *     a sequence's end.  At most 65535 groups, whose contents are read when the op runs, and
+ *     at most 2^30 positions a sequence (max_seq_len, where a table names more).
  *   paged_kv_weights    Q, K_pool, TABLES, STARTS, LENS, LSE, HELD -> WEIGHTS
  *     The attention weights that the rows give the cached positions, added up.  HELD and
  *     WEIGHTS are f32[n_seqs][M][step_idx], an element for each KV head and position, with

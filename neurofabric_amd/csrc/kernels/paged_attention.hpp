@@ -656,7 +656,8 @@ __global__ __launch_bounds__(1024) void plan_kernel(Chunk c, Part* parts, uint2*
   }
 }
 
-constexpr int kEverywhere = 0x3FFFFFFF;  // the position of a row that sees all keys
+// The position of a row that sees all keys, of which a sequence in kShared has at most 2^30.
+constexpr int kEverywhere = 0x3FFFFFFF;
 
 // Position of a query row's token: of a group's rows, that in whatever sequence it is.
 template <Form FORM>

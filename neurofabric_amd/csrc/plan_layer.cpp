@@ -310,6 +310,8 @@ nf_status plan_paged_chunk(bool prefix, const nf_tensor_desc* const* ins, uint32
     if (!ins[6] || !ins[7]) return fail(why, "null descriptor");
     lp.groups = pc.step;
     if (lp.groups > 65535) return fail(why, "more than 65535 groups");
+    // a row that sees all shared positions is at kEverywhere, the last of these
+    if (lp.max_seq > (1u << 30)) return fail(why, "more than 2^30 positions a sequence (max_seq_len bounds them)");
     if (!fits(ins[6], (uint64_t)lp.groups + 1, 4)) return fail(why, "groups hold fewer than step_idx + 1 entries");
     if (!fits(ins[7], lp.groups, 4)) return fail(why, "prefixes hold fewer than step_idx entries");
   }

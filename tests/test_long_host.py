@@ -145,6 +145,17 @@ def test_no_sizes_wrap(lib):
     refused(weigh, lib, pc=args(**{**big, "seq_len": 1, "n_heads": 65535, "step_idx": 0xFFFFFFFF, "theta": 1.0}))
 
 
+def test_prefix_of_too_many_positions(lib):
+    """A sequence may hold 2^30 positions at most, by its table or by max_seq_len: a row of a group that sees all of its shared
+    positions is at position 2^30 - 1 for the kernels."""
+    wide = dict(n_heads=H, step_idx=GROUPS, N=16385, window_size=65536)
+    sized = dict(pools=[desc(F16, 1 << 40)] * 2, bat=[desc(I32, S * 16385 * 4)] + batch()[1:])
+    refused(prefix, lib, pc=args(**wide), match="2\\^30", **sized)
+    refused(prefix, lib, pc=args(**wide, max_seq_len=(1 << 30) + 1), match="2\\^30", **sized)
+    assert prefix(lib, pc=args(**wide, max_seq_len=1 << 30), **sized)["count"] == T * H
+    assert prefix(lib, pc=args(**{**wide, "N": 16384}), **sized)["count"] == T * H
+
+
 def test_evict_of_too_many_positions(lib):
     """A sequence may hold 2^30 positions at most, by its table or by max_seq_len."""
     wide = dict(seq_len=TOP, N=16385, window_size=65536)
