@@ -686,6 +686,11 @@ __device__ __forceinline__ Keys find_keys(const Chunk& c, const RowTile& t, uint
   return {{0, 0, end}, lo, hi};
 }
 
+// Where the keys of a split from `begin` on end.  (begin + keys may not fit 31 bits.)
+__device__ __forceinline__ int cut_end(int begin, int end, uint32_t keys) {
+  return end > begin && (uint32_t)(end - begin) > keys ? begin + (int)keys : end;
+}
+
 // A query row's partial of split `sp` of a tile's part.
 template <bool SHARE>
 __device__ __forceinline__ uint64_t part_of(const Chunk& c, const RowTile& t, uint64_t orow, uint32_t sp) {
@@ -965,7 +970,7 @@ __device__ __forceinline__ void narrow_tile(const Chunk& c, const RowTile& t, ui
   const uint32_t cut_keys = SHARE ? t.keys : c.keys_per_split;
   const int pos_lo = keys.lo, begin = (int)(sp * cut_keys);
   int end = keys.at.end;  // keys below it
-  if (end > begin + (int)cut_keys) end = begin + (int)cut_keys;
+  end = cut_end(begin, end, cut_keys);
   end = __builtin_amdgcn_readfirstlane(end);
 
   half8 qb[NT][KSTEP];
@@ -1516,7 +1521,7 @@ __device__ __forceinline__ void wide_rows(const Chunk& c, const RowTile& t, uint
   const uint32_t cut_keys = SHARE ? t.keys : c.keys_per_split;
   const int pos_lo = keys.lo, begin = (int)(sp * cut_keys);
   int end = keys.at.end;
-  if (end > begin + (int)cut_keys) end = begin + (int)cut_keys;
+  end = cut_end(begin, end, cut_keys);
   end = __builtin_amdgcn_readfirstlane(end);
 
   const uint32_t r0 = t.first + 32 * w;
@@ -1952,7 +1957,7 @@ __device__ __forceinline__ void narrow_f32_tile(const Chunk& c, const RowTile& t
   const uint32_t cut_keys = SHARE ? t.keys : c.keys_per_split;
   const int pos_lo = keys.lo, begin = (int)(sp * cut_keys);
   int end = keys.at.end;
-  if (end > begin + (int)cut_keys) end = begin + (int)cut_keys;
+  end = cut_end(begin, end, cut_keys);
   end = __builtin_amdgcn_readfirstlane(end);
   const uint32_t row = t.first + n < t.rows ? t.first + n : t.rows - 1;
   const uint64_t orow = (uint64_t)(t.start + row / G) * H + kvh * G + row % G;
@@ -2232,7 +2237,7 @@ __device__ __forceinline__ void wide_f32_rows(const Chunk& c, const RowTile& t, 
   const uint32_t cut_keys = SHARE ? t.keys : c.keys_per_split;
   const int pos_lo = keys.lo, begin = (int)(sp * cut_keys);
   int end = keys.at.end;
-  if (end > begin + (int)cut_keys) end = begin + (int)cut_keys;
+  end = cut_end(begin, end, cut_keys);
   end = __builtin_amdgcn_readfirstlane(end);
   const uint32_t r0 = t.first + 16 * w;
   const bool wave_live = r0 < t.rows;

@@ -1035,3 +1035,37 @@ def test_weights_of_rows_that_count_for_nothing(provider, act, pool, seqs, heads
         got = wb.read(np.float32, held.size).reshape(held.shape)
     assert np.isfinite(got).all()
     assert np.array_equal(got, plain)
+
+
+@pytest.mark.parametrize("act,pool", [("f16", "f16"), ("f32", "f32"), ("f16", "i8")])
+@pytest.mark.parametrize("op,lens,share", [("chunk", [0x7FFFF000], 0), ("chunk", [0x7FFFEF81], 0), ("prefix", [1 << 30, (1 << 30) - 77], (1 << 30) - 200),
+                                           ("prefix", [1 << 30], (1 << 30) - 9)])
+def test_as_many_positions_as_there_may_be(provider, act, pool, op, lens, share):
+    """Sequences of the most positions, all in one block: keys of equal scores, of which none may be lost."""
+    rng = np.random.default_rng(76)
+    dim, bs, n = 64, 65536, len(lens)
+    pages = -(-max(lens) // bs)
+    batch = ref.Batch(rng, [(1, 1)] * n, bs)
+    batch.blocks, batch.width, batch.table = 1, pages, np.zeros((n, pages), np.uint32)
+    batch.lens = np.array(lens, np.int32)
+    value = rng.choice([-1.0, 1.0], dim).astype(NP[act])
+    pools = [paged_ref.empty_pool(rng, pool, 1, 1, bs, dim) for _ in range(2)]
+    if pool == "i8":
+        pools[1][0, 0, :bs * dim] = np.tile((64 * value).astype(np.int8).view(np.uint8), bs)
+        pools[1][0, 0, bs * dim:] = np.full(bs * dim // 32, 2.0 ** -6, np.float16).view(np.uint8)
+    else:
+        pools[1][:] = value
+    with Bufs(provider) as m:
+        out, lb = m.put(np.zeros((n, 1, dim), NP[act])), m.put(np.zeros((n, 1), np.float32))
+        ins = [m.put(np.zeros((n, 1, dim), NP[act]))] + [m.put(x) for x in pools] + m.batch(batch)
+        more = {}
+        if op == "prefix":
+            ins += [m.put(np.array([0, n], np.int32)), m.put(np.array([share], np.int32))]
+            more["step_idx"] = 1
+        provider.dispatch("flash_attention_paged_" + op, ins, [out, lb],
+                          pc=pc_of(batch, 1, dim, n_heads=1, max_seq_len=1 << 30 if op == "prefix" else 0, **more))
+        got, z = out.read(NP[act], n * dim).reshape(n, dim), lb.read(np.float32, n)
+    # Sums of weights of 1 or 2^7, 32 or more at a time, are exact; the combination of up to 512 splits may round each, and
+    # the logarithm its parts, of up to 32.
+    check(z, np.log(np.array(lens, np.float64)), (512 + 6 * 32 + 16) * paged_ref.U, (op, act, pool))
+    check(got, np.tile(value.astype(np.float64), (n, 1)), 600 * paged_ref.U + (0 if act == "f32" else paged_ref.H), (op, act, pool))
