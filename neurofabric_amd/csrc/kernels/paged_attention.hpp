@@ -289,8 +289,6 @@ struct Cut {
     const uint64_t rows = (uint64_t)p.n * c.group;
     return (uint32_t)(rows <= FEW ? (rows + NARROW - 1) / NARROW : (rows + WIDE - 1) / WIDE);
   }
-  // Tile and split k of a part.  All tiles of a split come after each other, so that they
-  // share its keys in the caches.
   // The time of a tile's key, that of a narrow one's being 2/5 of a wide one's.
   static __device__ __forceinline__ float cost(const Chunk& c, const Part& p) {
     return (uint64_t)p.n * c.group <= FEW ? 0.4f : 1.f;
@@ -300,6 +298,8 @@ struct Cut {
   static __device__ __forceinline__ float fixed(const Chunk& c, const Part& p) {
     return (uint64_t)p.n * c.group <= FEW && NARROW == 32 ? 500.f : 200.f;
   }
+  // Tile and split k of a part.  All tiles of a split come after each other, so that they
+  // share its keys in the caches.
   static __device__ __forceinline__ void tile(const Chunk& c, const Part& p, uint32_t nt, uint32_t k, const Cuts& keys, RowTile& t,
                                               uint32_t& sp) {
     t.keys = p.last ? keys.shared : own_keys(c, keys, p.seq, p.start, p.keys);
