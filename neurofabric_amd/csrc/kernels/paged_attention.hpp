@@ -1496,6 +1496,8 @@ struct WideLds {
 // HINT: the open loop's test of the end is a branch of its own, unlikely to be taken.  In
 // kShared 16 chunks of up to 200 tokens behind 8192 positions take 515 us without and 457
 // with it (474 on another card), five tokens of 32 sequences 58.1 and 52.6, but single tokens of 64 53.8 and 55.5.
+// In kChunk two chunks of 2048 tokens behind 6144, f16, 128 dims, 638 and 624, but four of up
+// to 512, 64 dims, 110 and 111.5; I8 and 96 dims alike within 0.5 %.
 template <PoolType PT, int DD, bool UNI, Form FORM, bool HINT = false>
 __device__ __forceinline__ void wide_rows(const Chunk& c, const RowTile& t, uint32_t sp, uint32_t ns, uint32_t kvh,
                                           WideLds<DD>& mem) {
@@ -1860,7 +1862,7 @@ __global__ __launch_bounds__(256, 2) void chunk_wide_kernel(Chunk c) {
   if (!find_tile(c.b, idx, c.group, 128, c.lo, c.hi, t)) return;
   const uint32_t ns = splits_of(c, t.len);
   __shared__ WideLds<DD> lds;
-  if (sp < ns) wide_rows<PT, DD, UNI, FORM>(c, t, sp, ns, kvh, lds);
+  if (sp < ns) wide_rows<PT, DD, UNI, FORM, FORM == kChunk && PT == PoolType::F16 && DD == 128>(c, t, sp, ns, kvh, lds);
 }
 
 // kShared: narrow and wide tiles in one launch, whose workgroups find out which theirs is, so
