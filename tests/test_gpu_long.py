@@ -1069,3 +1069,32 @@ def test_as_many_positions_as_there_may_be(provider, act, pool, op, lens, share)
     # the logarithm its parts, of up to 32.
     check(z, np.log(np.array(lens, np.float64)), (512 + 6 * 32 + 16) * paged_ref.U, (op, act, pool))
     check(got, np.tile(value.astype(np.float64), (n, 1)), 600 * paged_ref.U + (0 if act == "f32" else paged_ref.H), (op, act, pool))
+
+
+@pytest.mark.parametrize("act,pool", ACT_POOL)
+@pytest.mark.parametrize("seqs,heads,kv,dim", [([(300, 3), (90, 2)], 8, 2, 64), ([(300, 90), (200, 64), (33, 33)], 8, 2, 128),
+                                               ([(90, 20), (60, 1)], 4, 2, 40), ([(600, 500)], 8, 1, 64)])
+def test_weights_of_rows_without_a_number(provider, act, pool, seqs, heads, kv, dim):
+    """A row whose log-sum-exp is NaN leaves NaN at the positions that it sees, and its KV head's others as they are without it."""
+    if pool == "i8" and dim % 32:
+        pytest.skip("an 8-bit cache needs groups of 32")
+    rng = np.random.default_rng(77)
+    batch = ref.Batch(rng, seqs, 16, behind=2)
+    q, pools, z = run_attention(provider, rng, batch, None, act, pool, heads, kv, dim, chunk=True)
+    r, h = int(batch.starts[0]) + seqs[0][1] // 2, heads - 1
+    pos = seqs[0][0] - seqs[0][1] + seqs[0][1] // 2
+    width = batch.width * batch.bs
+    held = rng.random((len(seqs), kv, width)).astype(np.float32)
+    got = []
+    with Bufs(provider) as m:
+        base, wb, hb = [m.put(q), m.put(pools[0])] + m.batch(batch), m.put(held), m.put(held)
+        for x in (-np.inf, np.nan):
+            lse = z.copy()
+            lse[r, h] = x
+            wb.write(held)
+            provider.dispatch("paged_kv_weights", base + [m.put(lse), hb], [wb],
+                              pc=pc_of(batch, kv, dim, n_heads=heads, step_idx=width, theta=1.0))
+            got.append(wb.read(np.float32, held.size).reshape(held.shape))
+    want = got[0].copy()
+    want[0, kv - 1, :pos + 1] = np.nan
+    assert np.isfinite(got[0]).all() and np.array_equal(got[1], want, equal_nan=True)
