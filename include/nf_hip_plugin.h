@@ -87,7 +87,8 @@
  *       WEIGHTS[s][g][j] = theta HELD[s][g][j] + sum of exp(score of j - LSE[r][h]) over the
  *     sequence's rows r at positions >= j and the query heads h that read KV head g.  theta
  *     (0 to 1) lets older weights fade; 0 does not read HELD.  The positions of the rows
- *     themselves start from 0.  A position without storage gets nothing; a row whose LSE is
+ *     themselves start from 0.  Positions are looked up in their own sequence's table, shared
+ *     ones too.  A position without storage gets nothing; a row whose LSE is
  *     -inf gives nothing, whatever Q holds, nor does a score of -inf where LSE is a number.
  *     Positions past the length (or the bound) and sequences without rows are left as they
  *     are.  WEIGHTS may be HELD's buffer; other overlaps are not allowed.  Operands and limits

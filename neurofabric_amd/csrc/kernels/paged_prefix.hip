@@ -17,8 +17,8 @@
 //   for 64 keys, so that more splits would not help.
 //   32 behind 32768, up to 1024 of their own, I8: 50 + 8 us, the codes' conversion besides.
 //   Five tokens of 32 behind four prompts of 4096: 46 + 7 us.
-//   16 questions of up to 200 behind 8192: 457 to 474 us a pass, 700 TFLOP/s; the softmax between
-//   the products, and a last round of workgroups that does not fill the chip.
+//   16 questions of up to 200 behind 8192: 457 to 486 us a pass (four cards), 700 TFLOP/s; the
+//   softmax between the products, and a last round of workgroups that does not fill the chip.
 #include "../paged_tiles.hpp"
 #include "paged_attention.hpp"
 
@@ -33,8 +33,11 @@ namespace paged {
 template <PoolType PT>
 constexpr uint32_t kApartRows = PT == PoolType::I8 ? 96 : 64;
 // Workgroups that run at once, two on each CU, and the fewest keys that one takes: 256 and
-// 128, three chunks of 154 tokens with 833 positions, I8, 42.8 and 38.7 us; six tokens of 53
-// sequences with up to 1260, I8, 24.3 and 25.5; one chunk of 493 with 1197, f16, 52 and 52.6.
+// 128, the attention alone and the combination, three chunks of 154 tokens with 833 positions,
+// I8, 42.9 + 8.3 and 38.9 + 8.3 us; six tokens of 53 sequences with up to 1260, I8, 24.2 + 5.4
+// and 25.1 + 5.6; one chunk of 493 with 1197, f16, 47.8 + 8.6 and 48.0 + 8.6; single tokens of
+// 40 behind 700, 64 dims, 12.8 + 4.1 and 12.3 + 5.4; three of 24 behind 1000, f32, 64 dims, 22.9
+// + 5.2 and 20.5 + 5.2.
 constexpr uint32_t kResident = 512;
 constexpr uint32_t kMinKeys = 256;
 
